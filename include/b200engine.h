@@ -470,6 +470,109 @@ int b200_op_paged_attn_prefill_tc(const void* qkv, int32_t q_rows, int32_t ldq, 
  * most, softcap (0: none) on the scores, sink fp32 [heads] or NULL.  A wait that ran out is reported by the next operation (b200_op_kernel_mark). */
 int b200_op_prompt_attn(const void* q, const void* q2, const void* kv, const void* k2, const void* v2, void* out, int32_t T, int32_t heads, int32_t kv_heads,
                         const int32_t* seqs, int32_t nseq, int32_t window, float scale, float softcap, const float* sink, void* stream);
+/* ---- a verification step of drafted tokens (csrc/tree_step.h): from the requests' lengths to their new tokens without the host.
+ * S requests; request s owns rows starts[s] .. starts[s + 1] - 1 of the step's T rows and has ctx[s] tokens in the cache in front of them.
+ * Row 0 of a request is its last token, which is not in the cache yet, the others are drafts; a row's parent is the number of another row
+ * of its request in front of it, or -1.  Row i lies in the cache at position ctx + i, whatever its depth.  All integers int32 on the device.
+ * No argument that the device holds makes a kernel read or write outside the buffers: a request whose lengths do not fit (starts that
+ * descend or pass T, more rows than max_tree, a negative ctx, more tokens than its row of the block table holds) is left out and what
+ * it would have written stays as it was, rows that no request owns too.  Calls may run side by side on several streams and be captured; they keep nothing. */
+/* Block tables and slot maps from lengths.  Request s brings rows[s] tokens and holds held[s] pages, at least those of its ctx tokens; the pages it
+ * lacks are taken from free_pages[cursor ..], in the order of the requests, and written behind those in its row of block_tables.
+ * Out: starts [S + 1]; for each of the T rows positions (ctx + depth), slots (page * 16 + offset), seqs (optional: its request) and, with words > 0, masks
+ * [T, words]: bit i of a row is set where row i of its request leads to it, itself among them; held_out, cursor_out (may be held and cursor);
+ * status [S]: 0, or bits: 1 too few pages left (the request gets none), 2 its lengths do not fit (negative, beyond its row of the table, fewer pages held than
+ * ctx needs, more rows than 32 words or than T leaves), 4 a parent not in front of its child, which counts as -1.  Rows of a request with
+ * 1 or 2 have slot -1, which b200_op_rope_kvwrite skips, position 0 and no mask bits; rows behind the last request the same and seq -1.
+ * parents NULL: every row's parent is the one in front of it.  S <= 8192, words <= 8. */
+typedef struct {
+  int32_t S, T, max_blocks, ld_tables, num_free, words;
+  const int32_t* ctx;
+  const int32_t* rows;
+  const int32_t* held;
+  const int32_t* free_pages;
+  const int32_t* cursor;
+  const int32_t* parents;
+  int32_t* block_tables;
+  int32_t* held_out;
+  int32_t* cursor_out;
+  int32_t* starts;
+  int32_t* positions;
+  int32_t* slots;
+  int32_t* seqs;
+  int32_t* masks;
+  int32_t* status;
+} b200_step_maps_args;
+int b200_op_step_maps(const b200_step_maps_args* a, void* stream);
+/* Attention of the step's rows over the paged cache, their own K and V in it already: a row sees its request's ctx tokens and, of its rows, those
+ * that masks [T, words] names (NULL: itself and every row in front).  q: rows ldq apart, heads of 128 first; out rows ldo apart; kv_heads times 1, 2, 4 or 8
+ * heads; kv_layer [num_pages][2][kv_heads][16][128].  max_tree: most rows of a request; max_ctx: most tokens in front of them if known (0: what a row of the
+ * table holds), which only decides how the work is split.  A row that sees nothing is zero; what a row does not see has no part in it, NaN and infinities
+ * too.  A page that the cache does not have reads as zeros.  q 16-byte and kv_layer 256-byte aligned, ldq a multiple of 8, ldo of 8, out 16-byte aligned. */
+typedef struct {
+  int32_t S, T, q_heads, kv_heads, ldq, ldo, max_blocks, ld_tables, words, max_tree, max_ctx;
+  float scale;
+  int64_t num_pages;
+  const void* q;
+  void* out;
+  const void* kv_layer;
+  const int32_t* block_tables;
+  const int32_t* starts;
+  const int32_t* ctx;
+  const int32_t* masks;
+} b200_tree_attn_args;
+int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream);
+/* Penalties, biases and masks on logits [T, V], rows ld apart, bf16 or fp32 (logits_f32), and the greedy choice.  In fp32, each step rounded once:
+ *   y = x;  a token among the request's history or the row's drafts: y = y > 0 ? y / repetition : y * repetition;
+ *   y -= frequency * c, then y -= presence where c > 0, c = how often it stands in the history behind prompt_lens tokens and in the row's drafts;
+ *   y += bias, the last of the request's entries for the token;  a token that the row's mask does not allow: -inf.
+ * ids [T] (optional): the lowest allowed token of the largest y, NaN counting as -inf; -1 where none is allowed.  out (optional): y, fp32 or bf16 (out_f32), rows
+ * ld_out apart; may be logits itself where type and ld are the same.
+ * starts NULL: row r belongs to request r (S == T).  history: the requests' tokens one behind the other, hist_starts [S + 1], at most history_len; NULL: none.
+ * drafts [T] (NULL: none): the step's tokens; a row's are those that masks [T, words] names (NULL: itself and every row of its request in front).
+ * penalties fp32 [S][3]: repetition, presence, frequency (NULL: 1, 0, 0).  bias_starts [S + 1], bias_ids, bias_values, at most bias_len entries (NULL: none).
+ * allow [allow_count][ld_allow words], bit v of a row: token v is allowed; allow_rows [T]: each row's mask, -1 for none (NULL: mask r, allow_count == T).
+ * Tokens outside 0 .. V - 1 in any list count for nothing.  V <= 393216. */
+typedef struct {
+  int32_t S, T, V, ld, logits_f32, ld_out, out_f32, words, history_len, bias_len, allow_count, ld_allow;
+  const void* logits;
+  void* out;
+  int32_t* ids;
+  const int32_t* starts;
+  const int32_t* history;
+  const int32_t* hist_starts;
+  const int32_t* prompt_lens;
+  const int32_t* drafts;
+  const int32_t* masks;
+  const float* penalties;
+  const int32_t* bias_starts;
+  const int32_t* bias_ids;
+  const float* bias_values;
+  const int32_t* allow;
+  const int32_t* allow_rows;
+} b200_constrain_args;
+int b200_op_constrain(const b200_constrain_args* a, void* stream);
+/* The drafts that the choices confirm.  From row 0 of a request on, the path goes to the lowest row whose parent is the path's last row and whose draft is
+ * ids of that row, up to max_path rows; the paths' K and V rows move to positions ctx, ctx + 1, ... of the cache [layers][num_pages][2][kv_heads][16][128] (layers
+ * layer_stride elements apart).  Out: accepted [S] rows of the path, path [S, max_path] and tokens [S, max_path] = ids of the path's rows (-1 behind the
+ * last), new_ctx [S] = ctx + accepted (not ctx itself).  A request without rows, with more than 2048 or whose lengths do not fit accepts 0.  parents NULL: a chain.
+ * A move from or to a page that the cache does not have is left out. */
+typedef struct {
+  int32_t S, T, max_blocks, ld_tables, max_path, layers, kv_heads;
+  int64_t num_pages, layer_stride;
+  const int32_t* ids;
+  const int32_t* drafts;
+  const int32_t* parents;
+  const int32_t* starts;
+  const int32_t* ctx;
+  const int32_t* block_tables;
+  void* kv;
+  int32_t* accepted;
+  int32_t* path;
+  int32_t* tokens;
+  int32_t* new_ctx;
+} b200_tree_accept_args;
+int b200_op_tree_accept(const b200_tree_accept_args* a, void* stream);
 int b200_op_init_uniform(void* p, uint64_t n, uint32_t seed, float scale, float offset, void* stream);
 
 #ifdef __cplusplus

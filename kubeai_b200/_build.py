@@ -52,7 +52,12 @@ SOURCES = [
     "soselix.cu",
     "dabodra.cu",
     "model_registry.cc",
+    "step_maps.cu",
+    "tree_attention.cu",
+    "constrain.cu",
+    "tree_accept.cu",
     "abi_ops.cu",
+    "abi_tree.cu",
     "engine.cu",
     "router.cc",
     "loader.cc",

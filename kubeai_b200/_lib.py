@@ -41,6 +41,29 @@ class Gemm3Args(C.Structure):
                 ("argmax_out", C.c_void_p), ("n_valid", C.c_int32), ("normed_out", C.c_void_p), ("norm_w_out", C.c_void_p)]
 
 
+class StepMapsArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("S", "T", "max_blocks", "ld_tables", "num_free", "words")] + \
+        [(n, C.c_void_p) for n in ("ctx", "rows", "held", "free_pages", "cursor", "parents", "block_tables", "held_out", "cursor_out", "starts",
+                                   "positions", "slots", "seqs", "masks", "status")]
+
+
+class TreeAttnArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("S", "T", "q_heads", "kv_heads", "ldq", "ldo", "max_blocks", "ld_tables", "words", "max_tree", "max_ctx")] + \
+        [("scale", C.c_float), ("num_pages", C.c_int64)] + [(n, C.c_void_p) for n in ("q", "out", "kv_layer", "block_tables", "starts", "ctx", "masks")]
+
+
+class ConstrainArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("S", "T", "V", "ld", "logits_f32", "ld_out", "out_f32", "words", "history_len", "bias_len", "allow_count", "ld_allow")] + \
+        [(n, C.c_void_p) for n in ("logits", "out", "ids", "starts", "history", "hist_starts", "prompt_lens", "drafts", "masks", "penalties",
+                                   "bias_starts", "bias_ids", "bias_values", "allow", "allow_rows")]
+
+
+class TreeAcceptArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("S", "T", "max_blocks", "ld_tables", "max_path", "layers", "kv_heads")] + \
+        [(n, C.c_int64) for n in ("num_pages", "layer_stride")] + \
+        [(n, C.c_void_p) for n in ("ids", "drafts", "parents", "starts", "ctx", "block_tables", "kv", "accepted", "path", "tokens", "new_ctx")]
+
+
 class FeedEntry(C.Structure):
     _fields_ = [("req_id", C.c_uint64), ("tokens", C.POINTER(C.c_int32)), ("n_tokens", C.c_int32),
                 ("want", C.POINTER(C.c_int32)), ("n_want", C.c_int32)]
@@ -211,6 +234,10 @@ SYMBOLS = {
     "b200_op_paged_attn_decode_split": (C.c_int, [_vp, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _f, _i32, _vp]),
     "b200_op_paged_attn_prefill_tc": (C.c_int, [_vp, _i32, _i32, _vp, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _f, _vp]),
     "b200_op_prompt_attn": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _i32, _i32, _f, _f, _vp, _vp]),
+    "b200_op_step_maps": (C.c_int, [C.POINTER(StepMapsArgs), _vp]),
+    "b200_op_paged_attn_tree": (C.c_int, [C.POINTER(TreeAttnArgs), _vp]),
+    "b200_op_constrain": (C.c_int, [C.POINTER(ConstrainArgs), _vp]),
+    "b200_op_tree_accept": (C.c_int, [C.POINTER(TreeAcceptArgs), _vp]),
     "b200_op_init_uniform": (C.c_int, [_vp, _u64, C.c_uint32, _f, _f, _vp]),
 }
 

@@ -1,0 +1,87 @@
+// A verification step of drafted tokens: the arguments of its four operations (step_maps.cu, tree_attention.cu, constrain.cu,
+// tree_accept.cu) and the index arithmetic that their kernels share.  The latter compiles as plain C++ too, so that what a kernel would
+// read and write for given lengths and tables can be checked without a GPU.
+//
+// A step has T rows.  Request s owns rows starts[s] .. starts[s + 1] - 1, its tokens of this step, and has ctx[s] tokens in the paged cache
+// in front of them.  Row i of a request lies in the cache at position ctx + i; its place in the sequence is ctx + its depth in the tree.
+#pragma once
+#include <stdint.h>
+
+#ifdef __CUDACC__
+#include <cuda_runtime.h>
+#define B200_HD __host__ __device__ __forceinline__
+#else
+#define B200_HD inline
+#endif
+
+#include "../../include/b200engine.h"
+
+namespace b200 {
+namespace tree {
+
+constexpr int kPage = 16;             // tokens of a page
+constexpr int kMaxRequests = 8192;    // of a step_maps call: their offsets lie in shared memory
+constexpr int kMaxWords = 8;          // words of an ancestor mask: trees of up to 256 rows
+constexpr int kMaxTree = 2048;        // rows of a request that tree_accept walks
+
+struct Request {
+  int row0, rows, ctx;
+};
+
+// The rows of request s as the device's lengths have them; no rows where they do not describe one: lengths out of order, rows behind T, more
+// rows than `most`, or more tokens than its row of the block table has pages for.
+B200_HD Request request_of(const int* starts, const int* ctx, int s, int T, int max_blocks, int most) {
+  const int a = starts[s], b = starts[s + 1], c = ctx[s];
+  const bool ok = a >= 0 && b >= a && b <= T && b - a <= most && c >= 0 && static_cast<long long>(c) + (b - a) <= static_cast<long long>(max_blocks) * kPage;
+  Request r;
+  r.row0 = ok ? a : 0;
+  r.rows = ok ? b - a : 0;
+  r.ctx = ok ? c : 0;
+  return r;
+}
+
+// The cache row (page * 16 + offset) of a position, -1 where the table names a page that the cache does not have.
+B200_HD long long cache_row(const int* table, int pos, long long num_pages) {
+  const int page = table[pos >> 4];
+  return page >= 0 && page < num_pages ? static_cast<long long>(page) * kPage + (pos & 15) : -1;
+}
+
+// A parent counts where it lies in front of its child; every other number stands for the request's last token in the cache (-1).
+B200_HD int parent_of(const int* parents, int row0, int i) {
+  if (!parents) return i - 1;
+  const int p = parents[row0 + i];
+  return p >= 0 && p < i ? p : -1;
+}
+
+// The last index of the n + 1 ascending values v whose value is at most x; v[0] <= x.
+B200_HD int last_at_most(const int* v, int n, int x) {
+  int lo = 0, hi = n + 1;      // v[lo] <= x < v[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (v[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// What a request asks of step_maps: rows (never negative), and pages beyond those it holds; -1 pages where its lengths do not fit.
+B200_HD int rows_asked(int n) { return n > 0 ? n : 0; }
+B200_HD int pages_asked(int ctx, int n, int held, int max_blocks, int words) {
+  if (ctx < 0 || n < 0 || held < 0 || held > max_blocks) return -1;
+  if (static_cast<long long>(ctx) + n > static_cast<long long>(max_blocks) * kPage) return -1;
+  if (ctx > static_cast<long long>(held) * kPage) return -1;
+  if (words > 0 && n > 32 * words) return -1;
+  const int all = static_cast<int>((static_cast<long long>(ctx) + n + kPage - 1) / kPage);
+  return all > held ? all - held : 0;
+}
+
+}  // namespace tree
+
+#ifdef __CUDACC__
+int step_maps(const b200_step_maps_args& a, cudaStream_t st);
+int paged_attention_tree(const b200_tree_attn_args& a, cudaStream_t st);
+int constrain(const b200_constrain_args& a, cudaStream_t st);
+int tree_accept(const b200_tree_accept_args& a, cudaStream_t st);
+#endif
+
+}  // namespace b200
