@@ -476,7 +476,7 @@ int b200_op_prompt_attn(const void* q, const void* q2, const void* kv, const voi
  * of its request in front of it, or -1.  Row i lies in the cache at position ctx + i, whatever its depth.  All integers int32 on the device.
  * No argument that the device holds makes a kernel read or write outside the buffers: a request whose lengths do not fit (starts that
  * descend or pass T, more rows than max_tree, a negative ctx, more tokens than its row of the block table holds) is left out and what
- * it would have written stays as it was, rows that no request owns too.  Calls may run side by side on several streams and be captured; they keep nothing. */
+ * it would have written stays as it was, rows that no request owns too, but where an operation says what becomes of them.  Calls may run side by side on several streams and be captured; they keep nothing. */
 /* Block tables and slot maps from lengths.  Request s brings rows[s] tokens and holds held[s] pages, at least those of its ctx tokens; the pages it
  * lacks are taken from free_pages[cursor ..], in the order of the requests, and written behind those in its row of block_tables.
  * Out: starts [S + 1]; for each of the T rows positions (ctx + depth), slots (page * 16 + offset), seqs (optional: its request) and, with words > 0, masks
@@ -507,10 +507,11 @@ int b200_op_step_maps(const b200_step_maps_args* a, void* stream);
 /* Attention of the step's rows over the paged cache, their own K and V in it already: a row sees its request's ctx tokens and, of its rows, those
  * that masks [T, words] names (NULL: itself and every row in front).  q: rows ldq apart, heads of 128 first; out rows ldo apart; kv_heads times 1, 2, 4 or 8
  * heads; kv_layer [num_pages][2][kv_heads][16][128].  max_tree: most rows of a request; max_ctx: most tokens in front of them if known (0: what a row of the
- * table holds), which only decides how the work is split.  A row that sees nothing is zero; what a row does not see has no part in it, NaN and infinities
+ * table holds), which only decides how the work is split; zero_rest: rows of
+ * requests that are left out and rows that no request owns become zeros.  A row that sees nothing is zero; what a row does not see has no part in it, NaN and infinities
  * too.  A page that the cache does not have reads as zeros.  q 16-byte and kv_layer 256-byte aligned, ldq a multiple of 8, ldo of 8, out 16-byte aligned. */
 typedef struct {
-  int32_t S, T, q_heads, kv_heads, ldq, ldo, max_blocks, ld_tables, words, max_tree, max_ctx;
+  int32_t S, T, q_heads, kv_heads, ldq, ldo, max_blocks, ld_tables, words, max_tree, max_ctx, zero_rest;
   float scale;
   int64_t num_pages;
   const void* q;
@@ -526,7 +527,7 @@ int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream);
  *   y = x;  a token among the request's history or the row's drafts: y = y > 0 ? y / repetition : y * repetition;
  *   y -= frequency * c, then y -= presence where c > 0, c = how often it stands in the history behind prompt_lens tokens and in the row's drafts;
  *   y += bias, the last of the request's entries for the token;  a token that the row's mask does not allow: -inf.
- * ids [T] (optional): the lowest allowed token of the largest y, NaN counting as -inf; -1 where none is allowed.  out (optional): y, fp32 or bf16 (out_f32), rows
+ * ids [T] (optional): the lowest allowed token of the largest y, NaN counting as -inf; -1 where none is allowed and for rows that no request owns.  out (optional): y, fp32 or bf16 (out_f32), rows
  * ld_out apart; may be logits itself where type and ld are the same.
  * starts NULL: row r belongs to request r (S == T).  history: the requests' tokens one behind the other, hist_starts [S + 1], at most history_len; NULL: none.
  * drafts [T] (NULL: none): the step's tokens; a row's are those that masks [T, words] names (NULL: itself and every row of its request in front).

@@ -48,7 +48,7 @@ class StepMapsArgs(C.Structure):
 
 
 class TreeAttnArgs(C.Structure):
-    _fields_ = [(n, C.c_int32) for n in ("S", "T", "q_heads", "kv_heads", "ldq", "ldo", "max_blocks", "ld_tables", "words", "max_tree", "max_ctx")] + \
+    _fields_ = [(n, C.c_int32) for n in ("S", "T", "q_heads", "kv_heads", "ldq", "ldo", "max_blocks", "ld_tables", "words", "max_tree", "max_ctx", "zero_rest")] + \
         [("scale", C.c_float), ("num_pages", C.c_int64)] + [(n, C.c_void_p) for n in ("q", "out", "kv_layer", "block_tables", "starts", "ctx", "masks")]
 
 

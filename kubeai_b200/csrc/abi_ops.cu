@@ -62,8 +62,21 @@ StreamParts g_parts[kStreams];
 int g_nparts = 0;
 constexpr size_t kCounterBytes = (kCounterInts + static_cast<size_t>(kStreams) * kStreamCounters) * sizeof(int);   // for all calls, then the streams'
 
+// Pinned memory can be had while a stream is captured (by this thread or another) in relaxed mode only.
+int ensure_mark_locked() {
+  if (g_mark) return 0;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  const bool ok = cudaMallocHost(&g_mark, sizeof(int)) == cudaSuccess;
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  if (!ok) { cudaGetLastError(); g_mark = nullptr; return -1; }
+  *g_mark = 0;
+  return 0;
+}
+
 int ensure_scratch() {
   std::lock_guard<std::mutex> lk(g_mu);
+  if (ensure_mark_locked()) return -1;
   if (g_ws) return 0;
   int sms = 0, dev = 0;
   cudaGetDevice(&dev);
@@ -72,8 +85,6 @@ int ensure_scratch() {
   if (cudaMalloc(&g_ws, g_ws_bytes) != cudaSuccess) return -1;
   if (cudaMalloc(&g_counters, kCounterBytes) != cudaSuccess) return -1;
   if (cudaMemset(g_counters, 0, kCounterBytes) != cudaSuccess || cudaStreamSynchronize(nullptr) != cudaSuccess) return -1;   // a stream need not wait for the default one
-  if (cudaMallocHost(&g_mark, sizeof(int)) != cudaSuccess) return -1;
-  *g_mark = 0;
   return 0;
 }
 
@@ -116,13 +127,23 @@ int report_mark() {
   volatile int* mark = g_mark;
   if (!*mark) return 0;
   cudaDeviceSynchronize();
-  cudaMemset(g_counters, 0, kCounterBytes);
+  if (g_counters) cudaMemset(g_counters, 0, kCounterBytes);
   cudaDeviceSynchronize();      // the next kernel's stream need not wait for this one
   *mark = 0;
   set_error("a wait inside the kernel of an earlier product ran out: its output is not valid");
   return B200_ERR_CUDA;
 }
 }  // namespace
+
+int op_mark(int** mark) {
+  {
+    std::lock_guard<std::mutex> lk(g_mu);
+    if (ensure_mark_locked()) { set_error("no pinned memory for the mark of kernels"); return B200_ERR_OOM; }
+  }
+  *mark = g_mark;
+  return report_mark();
+}
+
 }  // namespace b200
 
 using namespace b200;

@@ -39,26 +39,33 @@ int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream) {
   if (!a || a->S < 0 || a->T < 0 || a->max_blocks < 0 || a->ld_tables < a->max_blocks || a->max_tree < 0 || a->max_ctx < 0 || a->num_pages < 0) return refuse(op, "bad sizes");
   const int group = a->kv_heads > 0 && a->q_heads > 0 && a->q_heads % a->kv_heads == 0 ? a->q_heads / a->kv_heads : 0;
   if (group != 1 && group != 2 && group != 4 && group != 8) return refuse(op, "a key head serves 1, 2, 4 or 8 heads");
-  if (a->S > 65535 || a->kv_heads > 4096) return refuse(op, "too many requests or heads for a launch");
+  if (a->S > 65534 || a->kv_heads > 4096) return refuse(op, "too many requests or heads for a launch");
   if (a->words < 0 || a->words > tree::kMaxWords || (a->masks && !a->words)) return refuse(op, "masks of 1 to 8 words");
   if (a->masks && a->max_tree > 32 * a->words) return refuse(op, "more rows of a request than its masks have bits");
-  if (a->max_blocks > INT_MAX / tree::kPage || a->num_pages > INT_MAX / (32ll * a->kv_heads)) return refuse(op, "positions or cache rows pass 32 bits");
+  if (a->max_blocks > INT_MAX / tree::kPage || a->num_pages >= INT_MAX / (32ll * a->kv_heads)) return refuse(op, "positions or cache rows pass 32 bits");
   if (static_cast<int64_t>(a->q_heads) * 128 > a->ldq || static_cast<int64_t>(a->q_heads) * 128 > a->ldo || a->ldq % 8 || a->ldo % 8) return refuse(op, "rows of q and out are whole heads, a multiple of 8 apart");
   if (!(a->scale == a->scale)) return refuse(op, "scale is no number");
-  if (!a->S || !a->T || !a->max_tree) return 0;
-  if (!a->q || !a->out || !a->kv_layer || !a->starts || !a->ctx || (a->max_blocks && !a->block_tables) || !a->num_pages) return refuse(op, "a buffer is missing");
-  if (!aligned(a->q, 16) || !aligned(a->out, 16) || !aligned(a->kv_layer, 256)) return refuse(op, "q and out are 16-byte aligned, the cache is 256-byte aligned");
+  if (!a->T || !a->q_heads) return 0;
+  if (!a->out || !aligned(a->out, 16)) return refuse(op, "out is missing or not 16-byte aligned");
+  if (!a->S || !a->max_tree) {      // no row is anybody's
+    if (!a->zero_rest) return 0;
+    if (int rc = require_device()) return rc;
+    return launched(op, cudaMemset2DAsync(a->out, a->ldo * 2ll, 0, a->q_heads * 256ll, a->T, static_cast<cudaStream_t>(stream)) == cudaSuccess ? 0 : -2);
+  }
+  if (!a->q || !a->kv_layer || !a->starts || !a->ctx || (a->max_blocks && !a->block_tables) || !a->num_pages) return refuse(op, "a buffer is missing");
+  if (!aligned(a->q, 16) || !aligned(a->kv_layer, 256)) return refuse(op, "q is 16-byte aligned, the cache is 256-byte aligned");
   if (int rc = require_device()) return rc;
-  return launched(op, paged_attention_tree(*a, static_cast<cudaStream_t>(stream)));
+  int* mark = nullptr;
+  if (int rc = op_mark(&mark)) return rc;
+  return launched(op, paged_attention_tree(*a, mark, static_cast<cudaStream_t>(stream)));
 }
 
 int b200_op_constrain(const b200_constrain_args* a, void* stream) {
   const char* op = "b200_op_constrain";
   if (!a || a->S < 0 || a->T < 0 || a->V < 1 || a->ld < a->V || (a->out && a->ld_out < a->V)) return refuse(op, "bad sizes");
   if (a->V > 393216) return refuse(op, "more than 393216 tokens");
-  if (a->S > 65535) return refuse(op, "more than 65535 requests");
+  if (a->S > 65534) return refuse(op, "more than 65534 requests");
   if (!a->starts && a->S != a->T) return refuse(op, "without starts every row is a request");
-  if (!a->ids && !a->out) return refuse(op, "neither choices nor logits asked for");
   if (a->words < 0 || a->words > tree::kMaxWords || (a->masks && !a->words)) return refuse(op, "masks of 1 to 8 words");
   if (a->masks && !a->drafts) return refuse(op, "masks without drafts");
   if (a->drafts && !a->starts) return refuse(op, "drafts without starts");
@@ -68,7 +75,13 @@ int b200_op_constrain(const b200_constrain_args* a, void* stream) {
   if (a->allow && (a->ld_allow < (a->V + 31) / 32 || a->allow_count < 0)) return refuse(op, "rows of allow are narrower than the vocabulary");
   if (a->allow && !a->allow_rows && a->allow_count < a->T) return refuse(op, "fewer masks than rows");
   if (a->allow_rows && !a->allow) return refuse(op, "rows of masks that are not there");
-  if (!a->S || !a->T) return 0;
+  if (!a->T) return 0;
+  if (!a->ids && !a->out) return refuse(op, "neither choices nor logits asked for");
+  if (!a->S) {
+    if (!a->ids) return 0;
+    if (int rc = require_device()) return rc;
+    return launched(op, cudaMemsetAsync(a->ids, 0xff, a->T * 4ll, static_cast<cudaStream_t>(stream)) == cudaSuccess ? 0 : -2);      // no row is anybody's: -1
+  }
   if (!a->logits) return refuse(op, "a buffer is missing");
   if (!aligned(a->logits, a->logits_f32 ? 4 : 2) || !aligned(a->out, a->out_f32 ? 4 : 2)) return refuse(op, "logits lie off their type's alignment");
   if (a->out == a->logits && (a->ld_out != a->ld || !a->out_f32 != !a->logits_f32)) return refuse(op, "logits kept in place have their type and rows");

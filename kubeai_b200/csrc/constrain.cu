@@ -81,6 +81,18 @@ constrain_kernel(const b200_constrain_args a, int slice) {
   const int s = blockIdx.z, group = blockIdx.y, groups = gridDim.y;
   // ids may be read by a kernel behind this one ahead of its dependency wait: none is let in before the end
   griddep_wait();
+  if (s == a.S) {      // rows that no request owns have no choice
+    if (group || rank) return;
+    bool plain = true;
+    for (int i = tid; i < a.S; i += kThreads) plain = plain && a.starts[i] >= 0 && a.starts[i] <= a.starts[i + 1] && a.starts[i + 1] <= a.T;
+    plain = __syncthreads_and(plain);
+    for (int t = tid; t < a.T; t += kThreads) {
+      bool owned = plain && t >= a.starts[0] && t < a.starts[a.S];
+      for (int i = 0; !plain && !owned && i < a.S; ++i) owned = a.starts[i] >= 0 && a.starts[i + 1] <= a.T && t >= a.starts[i] && t < a.starts[i + 1];
+      if (!owned) a.ids[t] = -1;
+    }
+    return;
+  }
   int row0 = s, rows = 1;
   if (a.starts) {
     row0 = a.starts[s];
@@ -246,7 +258,7 @@ int launch(const b200_constrain_args& a, cudaStream_t st) {
   const int groups = a.starts ? std::max((a.T + kRows - 1) / kRows, std::min((a.T + a.S - 1) / a.S, 32)) : 1;
   if (groups > 65535) return -1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(ctas, groups, a.S);
+  cfg.gridDim = dim3(ctas, groups, a.S + (a.starts && a.ids ? 1 : 0));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;

@@ -5,6 +5,8 @@ namespace b200 {
 void set_error(const char* fmt, ...);
 int require_device();            // B200_ERR_NO_DEVICE (+message) when no GPU is present
 int cuda_fail(const char* what, int rc);
+// Operations: where a kernel leaves a mark when a wait ran out.  An earlier operation's mark is reported first (and taken away).
+int op_mark(int** mark);
 }  // namespace b200
 struct b200_engine;
 namespace b200 {

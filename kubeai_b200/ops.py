@@ -189,19 +189,19 @@ def _refused(why):
     return B200Error(-1, why)
 
 
-def _ints(*tensors):
-    """int32, contiguous and on one GPU, the current one (the kernels run on its current stream)."""
-    for t in tensors:
-        if t is not None and not (t.is_cuda and t.dtype is torch.int32 and t.is_contiguous()):
-            raise _refused(f"needs contiguous int32 on the GPU, got {t.dtype} on {t.device}{'' if t.is_contiguous() else ', with strides'}")
-    _here(*tensors)
+def _gpu(t):
+    """The GPU that a call runs on: its first tensor's, which has to be the current one."""
+    at = t.get_device()
+    if at < 0 or at != torch._C._cuda_getDevice():
+        raise _refused(f"a tensor on {t.device} where the current GPU's are wanted")
+    return at
 
 
-def _here(*tensors):
-    at = torch.cuda.current_device()
+def _ints(at, *tensors):
+    """int32, contiguous and on the call's GPU."""
     for t in tensors:
-        if t is not None and t.get_device() != at:
-            raise _refused(f"a tensor on {t.device}, the current device is cuda:{at}")
+        if t is not None and not (t.dtype is torch.int32 and t.get_device() == at and t.is_contiguous()):
+            raise _refused(f"needs contiguous int32 on cuda:{at}, got {t.dtype} on {t.device}{'' if t.is_contiguous() else ', with strides'}")
 
 
 def _sized(t, n, what):
@@ -209,17 +209,21 @@ def _sized(t, n, what):
         raise _refused(f"{what}: {t.numel()} values, not {n}")
 
 
-def _table(t, requests):
-    """int32 [requests, pages] whose rows may be a wider buffer's leading columns."""
-    if not (t.is_cuda and t.dtype is torch.int32 and t.dim() == 2 and t.shape[0] == requests and
-            (not t.numel() or ((t.shape[1] == 1 or t.stride(1) == 1) and (t.shape[0] == 1 or t.stride(0) >= t.shape[1])))):
-        raise _refused(f"block tables: int32 [{requests}, pages] on the GPU, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    _here(t)
-    return t.shape[1], max(t.stride(0), t.shape[1])
+def _rows(at, t, kinds, what, columns=None, rows=None):
+    """Rows that may be a wider buffer's leading columns: how far apart they are."""
+    shape, stride = t.shape, t.stride()
+    if not (t.dtype in kinds and t.get_device() == at and len(shape) == 2 and (rows is None or shape[0] == rows) and (columns is None or shape[1] >= columns) and
+            (not t.numel() or ((shape[1] == 1 or stride[1] == 1) and (shape[0] == 1 or stride[0] >= shape[1])))):
+        raise _refused(f"{what}: rows [{'any' if rows is None else rows}, {'any' if columns is None else columns}] of {' or '.join(map(str, kinds))} on cuda:{at}, "
+                       f"got {t.dtype} {tuple(shape)}, strides {stride}, on {t.device}")
+    return stride[0] if shape[0] > 1 and stride[0] > shape[1] else shape[1]
 
 
 def _ptr(t):
     return None if t is None else t.data_ptr()
+
+
+_I32, _BF16, _LOGITS = (torch.int32,), (torch.bfloat16,), (torch.bfloat16, torch.float32)
 
 
 class StepMaps(NamedTuple):
@@ -237,49 +241,48 @@ def step_maps(ctx_lens, new_lens, held, block_tables, free_pages, cursor, rows, 
     """Slots, positions and, with words > 0, ancestor masks of a step's `rows` rows, from each request's cached tokens and its rows of this step; pages that
     requests lack come from free_pages[cursor:] and are entered in block_tables (b200_op_step_maps).  held and cursor are left as they are and returned
     anew, or updated themselves (inplace).  parents [rows]: the number of each row's parent in its request, -1 for none; without them a chain."""
-    _ints(ctx_lens, new_lens, held, free_pages, cursor, parents)
+    at = _gpu(ctx_lens)
+    _ints(at, ctx_lens, new_lens, held, free_pages, cursor, parents)
     S = ctx_lens.numel()
     _sized(new_lens, S, "new_lens"), _sized(held, S, "held"), _sized(cursor, 1, "cursor"), _sized(parents, rows, "parents")
     if rows < 0 or not 0 <= words <= 8:
         raise _refused(f"{rows} rows, masks of {words} words")
-    blocks, ld = _table(block_tables, S)
+    ld = _rows(at, block_tables, _I32, "block tables", rows=S)
     sizes = [S + 1, rows, rows, rows, S, 0 if inplace else S, 0 if inplace else 1, rows * words]
-    starts, positions, slots, seqs, status, held_out, cursor_out, masks = torch.empty(sum(sizes), dtype=torch.int32, device=ctx_lens.device).split(sizes)
+    starts, positions, slots, seqs, status, held_out, cursor_out, masks = torch.empty(sum(sizes), dtype=torch.int32, device=ctx_lens.device).split_with_sizes(sizes)
     if inplace:
         held_out, cursor_out = held, cursor
-    a = StepMapsArgs(S, rows, blocks, ld, free_pages.numel(), words, ctx_lens.data_ptr(), new_lens.data_ptr(), held.data_ptr(), free_pages.data_ptr(),
+    a = StepMapsArgs(S, rows, block_tables.shape[1], ld, free_pages.numel(), words, ctx_lens.data_ptr(), new_lens.data_ptr(), held.data_ptr(), free_pages.data_ptr(),
                      cursor.data_ptr(), _ptr(parents), block_tables.data_ptr(), held_out.data_ptr(), cursor_out.data_ptr(), starts.data_ptr(),
                      positions.data_ptr(), slots.data_ptr(), seqs.data_ptr(), masks.data_ptr(), status.data_ptr())
-    check(lib().b200_op_step_maps(C.byref(a), _stream()))
+    check(lib().b200_op_step_maps(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
     return StepMaps(starts, positions, slots, seqs, masks.view(rows, words) if words else None, held_out, cursor_out, status)
 
 
 def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_heads, kv_heads, max_tree, max_ctx=0, scale=128 ** -0.5, out=None):
     """Attention of a step's rows over the paged cache and those rows of their own request that masks [T, words] names, None: all in front and
     itself (b200_op_paged_attn_tree).  qkv: [T, at least q_heads * 128], q first; kv_layer: [pages, 2, kv_heads, 16, 128] with the step's K and V in it.
-    max_tree: the most rows of a request; max_ctx: the most tokens in front of them, if known.  Rows that no request owns are left as they were in `out`,
-    of which a new one is zeros."""
-    if not (qkv.is_cuda and qkv.dtype is torch.bfloat16 and qkv.dim() == 2 and qkv.stride(1) == 1):
-        raise _refused(f"qkv: bf16 rows on the GPU, got {qkv.dtype} {tuple(qkv.shape)} on {qkv.device}")
-    if not (kv_layer.is_cuda and kv_layer.dtype is torch.bfloat16 and kv_layer.is_contiguous()) or tuple(kv_layer.shape[1:]) != (2, kv_heads, 16, 128):
-        raise _refused(f"kv_layer: contiguous bf16 [pages, 2, {kv_heads}, 16, 128], got {kv_layer.dtype} {tuple(kv_layer.shape)}")
-    _ints(starts, ctx_lens, masks)
+    max_tree: the most rows of a request; max_ctx: the most tokens in front of them, if known.  Rows that no request owns are left as they were in `out`
+    and are zeros in a new one."""
+    at = _gpu(qkv)
+    ldq = _rows(at, qkv, _BF16, "qkv", columns=q_heads * 128)
+    if kv_layer.dtype is not torch.bfloat16 or kv_layer.get_device() != at or not kv_layer.is_contiguous() or kv_layer.shape[1:] != (2, kv_heads, 16, 128):
+        raise _refused(f"kv_layer: contiguous bf16 [pages, 2, {kv_heads}, 16, 128] on cuda:{at}, got {kv_layer.dtype} {tuple(kv_layer.shape)} on {kv_layer.device}")
+    _ints(at, starts, ctx_lens, masks)
     S, T = ctx_lens.numel(), qkv.shape[0]
     _sized(starts, S + 1, "starts")
     if masks is not None and (masks.dim() != 2 or masks.shape[0] != T):
         raise _refused(f"masks: [{T}, words], got {tuple(masks.shape)}")
-    if out is None:
-        out = torch.zeros(T, q_heads * 128, dtype=torch.bfloat16, device=qkv.device)
-    elif not (out.is_cuda and out.dtype is torch.bfloat16 and out.dim() == 2 and out.shape[0] >= T and out.shape[1] >= q_heads * 128 and out.stride(1) == 1):
-        raise _refused(f"out: bf16 [{T}, {q_heads * 128}], got {out.dtype} {tuple(out.shape)}")
-    if qkv.shape[1] < q_heads * 128:
-        raise _refused(f"qkv rows of {qkv.shape[1]} values hold no {q_heads} heads")
-    _here(qkv, kv_layer, out)
-    blocks, ld = _table(block_tables, S)
-    a = TreeAttnArgs(S, T, q_heads, kv_heads, qkv.stride(0) if T > 1 else qkv.shape[1], out.stride(0) if out.shape[0] > 1 else out.shape[1], blocks, ld,
-                     masks.shape[1] if masks is not None else 0, max_tree, max_ctx, scale, kv_layer.shape[0], qkv.data_ptr(), out.data_ptr(),
-                     kv_layer.data_ptr(), block_tables.data_ptr(), starts.data_ptr(), ctx_lens.data_ptr(), _ptr(masks))
-    check(lib().b200_op_paged_attn_tree(C.byref(a), _stream()))
+    fresh = out is None
+    if fresh:
+        out = torch.empty(T, q_heads * 128, dtype=torch.bfloat16, device=qkv.device)
+    ldo = _rows(at, out, _BF16, "out", columns=q_heads * 128)
+    if out.shape[0] < T:
+        raise _refused(f"out has {out.shape[0]} rows, not {T}")
+    ld = _rows(at, block_tables, _I32, "block tables", rows=S)
+    a = TreeAttnArgs(S, T, q_heads, kv_heads, ldq, ldo, block_tables.shape[1], ld, masks.shape[1] if masks is not None else 0, max_tree, max_ctx, fresh, scale,
+                     kv_layer.shape[0], qkv.data_ptr(), out.data_ptr(), kv_layer.data_ptr(), block_tables.data_ptr(), starts.data_ptr(), ctx_lens.data_ptr(), _ptr(masks))
+    check(lib().b200_op_paged_attn_tree(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
     return out
 
 
@@ -289,42 +292,41 @@ def constrain(logits, starts=None, history=None, hist_starts=None, prompt_lens=N
     choice; returns (ids [T] or None, the logits that it was made from or None).  b200_op_constrain has the formulas and the lists' meaning.
     penalties: fp32 [S, 3] = repetition, presence, frequency.  bias: (starts [S + 1], ids, fp32 values).  allow: int32 [masks, at least ceil(V / 32)].
     out: None, a type (torch.float32 or torch.bfloat16) for new logits, or a tensor for them, which may be `logits`.  ids of rows that no request owns
-    are -1, new logits there are not written."""
-    kinds = (torch.bfloat16, torch.float32)
-    if not (logits.is_cuda and logits.dtype in kinds and logits.dim() == 2 and (logits.shape[1] <= 1 or logits.stride(1) == 1)):
-        raise _refused(f"logits: bf16 or fp32 rows on the GPU, got {logits.dtype} {tuple(logits.shape)} on {logits.device}")
+    are -1, logits there are not written."""
+    at = _gpu(logits)
+    ld = _rows(at, logits, _LOGITS, "logits")
     T, V = logits.shape
-    _ints(starts, history, hist_starts, prompt_lens, drafts, masks, allow_rows)
+    _ints(at, starts, history, hist_starts, prompt_lens, drafts, masks, allow_rows)
     S = starts.numel() - 1 if starts is not None else T
     _sized(hist_starts, S + 1, "hist_starts"), _sized(prompt_lens, S, "prompt_lens"), _sized(drafts, T, "drafts"), _sized(allow_rows, T, "allow_rows")
-    if masks is not None and (masks.dim() != 2 or masks.shape[0] != T):
-        raise _refused(f"masks: [{T}, words], got {tuple(masks.shape)}")
-    if penalties is not None and not (penalties.is_cuda and penalties.dtype is torch.float32 and penalties.is_contiguous() and tuple(penalties.shape) == (S, 3)):
-        raise _refused(f"penalties: fp32 [{S}, 3], got {penalties.dtype} {tuple(penalties.shape)}")
-    b_starts, b_ids, b_values = bias if bias is not None else (None, None, None)
+    words = 0
+    if masks is not None:
+        if masks.dim() != 2 or masks.shape[0] != T:
+            raise _refused(f"masks: [{T}, words], got {tuple(masks.shape)}")
+        words = masks.shape[1]
+    if penalties is not None and not (penalties.dtype is torch.float32 and penalties.get_device() == at and penalties.is_contiguous() and penalties.shape == (S, 3)):
+        raise _refused(f"penalties: fp32 [{S}, 3] on cuda:{at}, got {penalties.dtype} {tuple(penalties.shape)} on {penalties.device}")
+    b_starts, b_ids, b_values, b_len = None, None, None, 0
     if bias is not None:
-        _ints(b_starts, b_ids), _sized(b_starts, S + 1, "bias starts"), _sized(b_values, b_ids.numel(), "bias values")
-        if not (b_values.is_cuda and b_values.dtype is torch.float32 and b_values.is_contiguous()):
-            raise _refused(f"bias values: fp32, got {b_values.dtype}")
-    if allow is not None and not (allow.is_cuda and allow.dtype is torch.int32 and allow.dim() == 2 and (allow.shape[1] <= 1 or allow.stride(1) == 1)):
-        raise _refused(f"allow: int32 [masks, words], got {allow.dtype} {tuple(allow.shape)}")
-    if isinstance(out, torch.dtype):
-        if out not in kinds:
-            raise _refused(f"logits are kept as bf16 or fp32, not {out}")
-        out = torch.empty(T, V, dtype=out, device=logits.device)
-    elif out is not None and not (out.is_cuda and out.dtype in kinds and tuple(out.shape) == (T, V) and (V <= 1 or out.stride(1) == 1)):
-        raise _refused(f"out: bf16 or fp32 [{T}, {V}], got {out.dtype} {tuple(out.shape)}")
-    _here(logits, penalties, b_values, allow, out)
+        b_starts, b_ids, b_values = bias
+        b_len = b_ids.numel()
+        _ints(at, b_starts, b_ids), _sized(b_starts, S + 1, "bias starts"), _sized(b_values, b_len, "bias values")
+        if not (b_values.dtype is torch.float32 and b_values.get_device() == at and b_values.is_contiguous()):
+            raise _refused(f"bias values: fp32 on cuda:{at}, got {b_values.dtype} on {b_values.device}")
+    allow_ld = _rows(at, allow, _I32, "allow") if allow is not None else 0
+    out_ld = 0
+    if out is not None:
+        if isinstance(out, torch.dtype):
+            if out not in _LOGITS:
+                raise _refused(f"logits are kept as bf16 or fp32, not {out}")
+            out = torch.empty(T, V, dtype=out, device=logits.device)
+        out_ld = _rows(at, out, _LOGITS, "out", rows=T, columns=V)
     ids = torch.empty(T, dtype=torch.int32, device=logits.device) if pick else None
-    if pick and starts is not None:
-        ids.fill_(-1)
-    f32 = torch.float32
-    a = ConstrainArgs(S, T, V, max(logits.stride(0), V), logits.dtype is f32, max(out.stride(0), V) if out is not None else 0, out is not None and out.dtype is f32,
-                      masks.shape[1] if masks is not None else 0, history.numel() if history is not None else 0, b_ids.numel() if bias is not None else 0,
-                      allow.shape[0] if allow is not None else 0, max(allow.stride(0), allow.shape[1]) if allow is not None else 0, logits.data_ptr(), _ptr(out), _ptr(ids),
+    a = ConstrainArgs(S, T, V, ld, logits.dtype is torch.float32, out_ld, out is not None and out.dtype is torch.float32, words,
+                      history.numel() if history is not None else 0, b_len, allow.shape[0] if allow is not None else 0, allow_ld, logits.data_ptr(), _ptr(out), _ptr(ids),
                       _ptr(starts), _ptr(history), _ptr(hist_starts), _ptr(prompt_lens), _ptr(drafts), _ptr(masks), _ptr(penalties), _ptr(b_starts), _ptr(b_ids),
                       _ptr(b_values), _ptr(allow), _ptr(allow_rows))
-    check(lib().b200_op_constrain(C.byref(a), _stream()))
+    check(lib().b200_op_constrain(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
     return ids, out
 
 
@@ -339,21 +341,25 @@ def tree_accept(ids, drafts, parents, starts, ctx_lens, block_tables, kv, max_pa
     """The path of drafts that the choices `ids` confirm in each request's tree (parents None: a chain), and its K and V moved to the positions behind the cached
     tokens in every layer of kv [layers, pages, 2, kv_heads, 16, 128], None: nowhere (b200_op_tree_accept).  Returns the paths' lengths, rows and chosen tokens (-1 behind
     the last) and the requests' new lengths."""
-    _ints(ids, drafts, parents, starts, ctx_lens)
+    at = _gpu(ids)
+    _ints(at, ids, drafts, parents, starts, ctx_lens)
     S, T = ctx_lens.numel(), ids.numel()
     _sized(starts, S + 1, "starts"), _sized(drafts, T, "drafts"), _sized(parents, T, "parents")
-    if kv is not None and not (kv.is_cuda and kv.dtype is torch.bfloat16 and kv.dim() == 6 and kv.shape[2] == 2 and tuple(kv.shape[4:]) == (16, 128) and (not len(kv) or kv[0].is_contiguous())):
-        raise _refused(f"kv: bf16 [layers, pages, 2, kv_heads, 16, 128], got {kv.dtype} {tuple(kv.shape)}")
+    layers, pages, heads, apart = 0, 0, 1, 0
+    if kv is not None:
+        shape = kv.shape
+        if not (kv.dtype is torch.bfloat16 and kv.get_device() == at and len(shape) == 6 and shape[2] == 2 and shape[4:] == (16, 128) and (kv.is_contiguous() or not len(kv) or kv[0].is_contiguous())):
+            raise _refused(f"kv: bf16 [layers, pages, 2, kv_heads, 16, 128] on cuda:{at}, got {kv.dtype} {tuple(shape)} on {kv.device}")
+        layers, pages, heads = shape[0], shape[1], shape[3]
+        apart = kv.stride(0) if layers > 1 else 0
     if not 1 <= max_path <= 256:
         raise _refused(f"paths of {max_path} rows")
-    _here(kv)
-    blocks, ld = _table(block_tables, S)
+    ld = _rows(at, block_tables, _I32, "block tables", rows=S)
     sizes = [S, S, S * max_path, S * max_path]
-    accepted, ctx, path, tokens = torch.empty(sum(sizes), dtype=torch.int32, device=ids.device).split(sizes)
-    layers, pages, _, heads = kv.shape[:4] if kv is not None else (0, 0, 2, 1)
-    a = TreeAcceptArgs(S, T, blocks, ld, max_path, layers, heads, pages, kv.stride(0) if layers > 1 else 0, ids.data_ptr(), drafts.data_ptr(), _ptr(parents),
+    accepted, ctx, path, tokens = torch.empty(sum(sizes), dtype=torch.int32, device=ids.device).split_with_sizes(sizes)
+    a = TreeAcceptArgs(S, T, block_tables.shape[1], ld, max_path, layers, heads, pages, apart, ids.data_ptr(), drafts.data_ptr(), _ptr(parents),
                        starts.data_ptr(), ctx_lens.data_ptr(), block_tables.data_ptr(), _ptr(kv), accepted.data_ptr(), path.data_ptr(), tokens.data_ptr(), ctx.data_ptr())
-    check(lib().b200_op_tree_accept(C.byref(a), _stream()))
+    check(lib().b200_op_tree_accept(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
     return TreeAccept(accepted, path.view(S, max_path), tokens.view(S, max_path), ctx)
 
 

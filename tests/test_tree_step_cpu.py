@@ -58,7 +58,7 @@ def attn(**kw):
 @pytest.mark.parametrize("kw,why", [
     (dict(S=-1), "bad sizes"), (dict(T=-2), "bad sizes"), (dict(ld_tables=2), "bad sizes"), (dict(max_tree=-1), "bad sizes"), (dict(max_ctx=-1), "bad sizes"), (dict(num_pages=-1), "bad sizes"),
     (dict(q_heads=6), "1, 2, 4 or 8"), (dict(q_heads=7), "1, 2, 4 or 8"), (dict(q_heads=32, ldq=8192, ldo=4096), "1, 2, 4 or 8"), (dict(kv_heads=0), "1, 2, 4 or 8"), (dict(q_heads=0), "1, 2, 4 or 8"),
-    (dict(words=0), "1 to 8 words"), (dict(words=9), "1 to 8 words"), (dict(max_tree=33), "than its masks have bits"), (dict(S=65536), "too many"),
+    (dict(words=0), "1 to 8 words"), (dict(words=9), "1 to 8 words"), (dict(max_tree=33), "than its masks have bits"), (dict(S=65535), "too many"),
     (dict(max_blocks=1 << 27, ld_tables=1 << 27), "32 bits"), (dict(num_pages=1 << 25), "32 bits"), (dict(ldq=1000), "whole heads"), (dict(ldo=1020), "whole heads"), (dict(ldq=1540), "whole heads"),
     (dict(scale=float("nan")), "no number"), (dict(q=P + 8), "aligned"), (dict(out=P + 2), "aligned"), (dict(kv_layer=P + 128), "aligned"), (dict(num_pages=0), "missing"),
     *((dict([(k, None)]), "missing") for k in ("q", "out", "kv_layer", "block_tables", "starts", "ctx"))])
@@ -74,7 +74,7 @@ def choose(**kw):
 
 @pytest.mark.parametrize("kw,why", [
     (dict(S=-1), "bad sizes"), (dict(T=-1), "bad sizes"), (dict(V=0), "bad sizes"), (dict(ld=99), "bad sizes"), (dict(ld_out=99), "bad sizes"), (dict(bias_len=-1), "bad sizes"),
-    (dict(V=393217, ld=393217, ld_out=393217), "393216"), (dict(S=65536), "65535"), (dict(starts=None), "every row is a request"), (dict(ids=None, out=None), "neither"),
+    (dict(V=393217, ld=393217, ld_out=393217), "393216"), (dict(S=65535), "65534"), (dict(starts=None), "every row is a request"), (dict(ids=None, out=None), "neither"),
     (dict(words=0), "1 to 8 words"), (dict(words=9), "1 to 8 words"), (dict(drafts=None), "masks without drafts"), (dict(starts=None, S=4, masks=None), "drafts without starts"),
     (dict(hist_starts=None), "without its starts"), (dict(history_len=-1), "without its starts"), (dict(bias_ids=None), "without their tokens"), (dict(bias_values=None), "without their tokens"),
     (dict(ld_allow=3), "narrower"), (dict(allow_count=-1), "narrower"), (dict(allow_rows=None, allow_count=3), "fewer masks"), (dict(allow=None), "that are not there"), (dict(logits=None), "missing"),

@@ -248,6 +248,21 @@ def test_attention_far_into_a_large_cache():
     assert torch.equal(got, run_attention(c))
 
 
+def test_calls_of_no_requests_or_rows():
+    from kubeai_b200 import ops
+    c = attention_case(12, [5], [3], 1, 4)
+    e, kv, none = ints([]), c["kv"].cuda(), ints(np.zeros((0, 4)))
+    assert (ops.paged_attn_tree(c["qkv"].cuda(), kv, none, ints([0]), e, None, 4, 1, 3) == 0).all()
+    assert (ops.paged_attn_tree(c["qkv"].cuda(), kv, ints(c["tables"]), ints([0, 3]), ints([5]), None, 4, 1, 0) == 0).all()
+    assert ops.paged_attn_tree(c["qkv"].cuda()[:0], kv, ints(c["tables"]), ints([0, 0]), ints([5]), None, 4, 1, 3).shape == (0, 512)
+    assert ops.constrain(torch.zeros(3, 9, device="cuda"), starts=ints([0]))[0].tolist() == [-1] * 3
+    assert ops.constrain(torch.zeros(0, 9, device="cuda"))[0].shape == (0,)
+    a = ops.tree_accept(e, e, None, ints([0]), e, none, None, 3)
+    assert a.path.shape == (0, 3)
+    a = ops.tree_accept(e, e, e, ints([0, 0]), ints([7]), ints([[1]]), None, 3)
+    assert a.accepted.tolist() == [0] and a.ctx_lens.tolist() == [7] and a.path.tolist() == [[-1] * 3]
+
+
 # ------------------------------------------------------------------ constrain
 def constrain_case(seed, rows, V, history, f32, bias=0, grammar=None, drafts="tree", penalties=True, ld=0, repeat=False):
     rng = np.random.default_rng(seed)
