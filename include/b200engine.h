@@ -521,7 +521,12 @@ typedef struct {
   const int32_t* starts;
   const int32_t* ctx;
   const int32_t* masks;
+  void* workspace;
+  int64_t workspace_bytes;
 } b200_tree_attn_args;
+/* Bytes of a call's workspace, which it uses until its kernels have run and which needs no preparation (a few tens of MB, by max_tree, T and heads alone).
+ * Calls that may run at once have one each. */
+int64_t b200_op_paged_attn_tree_workspace(const b200_tree_attn_args* a);
 int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream);
 /* Penalties, biases and masks on logits [T, V], rows ld apart, bf16 or fp32 (logits_f32), and the greedy choice.  In fp32, each step rounded once:
  *   y = x;  a token among the request's history or the row's drafts: y = y > 0 ? y / repetition : y * repetition;

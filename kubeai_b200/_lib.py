@@ -49,7 +49,7 @@ class StepMapsArgs(C.Structure):
 
 class TreeAttnArgs(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("S", "T", "q_heads", "kv_heads", "ldq", "ldo", "max_blocks", "ld_tables", "words", "max_tree", "max_ctx", "zero_rest")] + \
-        [("scale", C.c_float), ("num_pages", C.c_int64)] + [(n, C.c_void_p) for n in ("q", "out", "kv_layer", "block_tables", "starts", "ctx", "masks")]
+        [("scale", C.c_float), ("num_pages", C.c_int64)] + [(n, C.c_void_p) for n in ("q", "out", "kv_layer", "block_tables", "starts", "ctx", "masks", "workspace")] + [("workspace_bytes", C.c_int64)]
 
 
 class ConstrainArgs(C.Structure):
@@ -236,6 +236,7 @@ SYMBOLS = {
     "b200_op_prompt_attn": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _i32, _i32, _f, _f, _vp, _vp]),
     "b200_op_step_maps": (C.c_int, [C.POINTER(StepMapsArgs), _vp]),
     "b200_op_paged_attn_tree": (C.c_int, [C.POINTER(TreeAttnArgs), _vp]),
+    "b200_op_paged_attn_tree_workspace": (C.c_int64, [C.POINTER(TreeAttnArgs)]),
     "b200_op_constrain": (C.c_int, [C.POINTER(ConstrainArgs), _vp]),
     "b200_op_tree_accept": (C.c_int, [C.POINTER(TreeAcceptArgs), _vp]),
     "b200_op_init_uniform": (C.c_int, [_vp, _u64, C.c_uint32, _f, _f, _vp]),

@@ -34,8 +34,7 @@ int b200_op_step_maps(const b200_step_maps_args* a, void* stream) {
   return launched(op, step_maps(*a, static_cast<cudaStream_t>(stream)));
 }
 
-int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream) {
-  const char* op = "b200_op_paged_attn_tree";
+static int attn_sizes(const b200_tree_attn_args* a, const char* op) {
   if (!a || a->S < 0 || a->T < 0 || a->max_blocks < 0 || a->ld_tables < a->max_blocks || a->max_tree < 0 || a->max_ctx < 0 || a->num_pages < 0) return refuse(op, "bad sizes");
   const int group = a->kv_heads > 0 && a->q_heads > 0 && a->q_heads % a->kv_heads == 0 ? a->q_heads / a->kv_heads : 0;
   if (group != 1 && group != 2 && group != 4 && group != 8) return refuse(op, "a key head serves 1, 2, 4 or 8 heads");
@@ -45,6 +44,19 @@ int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream) {
   if (a->max_blocks > INT_MAX / tree::kPage || a->num_pages >= INT_MAX / (32ll * a->kv_heads)) return refuse(op, "positions or cache rows pass 32 bits");
   if (static_cast<int64_t>(a->q_heads) * 128 > a->ldq || static_cast<int64_t>(a->q_heads) * 128 > a->ldo || a->ldq % 8 || a->ldo % 8) return refuse(op, "rows of q and out are whole heads, a multiple of 8 apart");
   if (!(a->scale == a->scale)) return refuse(op, "scale is no number");
+  const long long rows = static_cast<long long>(a->max_tree < a->T ? a->max_tree : a->T) * group;
+  if ((rows + 127) / 128 * a->kv_heads > INT_MAX / (a->S + 1ll) / (a->max_blocks / 4 + 1)) return refuse(op, "the tiles of all requests pass 32 bits");
+  return 0;
+}
+
+int64_t b200_op_paged_attn_tree_workspace(const b200_tree_attn_args* a) {
+  if (int rc = attn_sizes(a, "b200_op_paged_attn_tree_workspace")) return rc;
+  return a->S && a->T && a->max_tree ? tree_attention_workspace(*a) : 0;
+}
+
+int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream) {
+  const char* op = "b200_op_paged_attn_tree";
+  if (int rc = attn_sizes(a, op)) return rc;
   if (!a->T || !a->q_heads) return 0;
   if (!a->out || !aligned(a->out, 16)) return refuse(op, "out is missing or not 16-byte aligned");
   if (!a->S || !a->max_tree) {      // no row is anybody's
@@ -54,6 +66,7 @@ int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream) {
   }
   if (!a->q || !a->kv_layer || !a->starts || !a->ctx || (a->max_blocks && !a->block_tables) || !a->num_pages) return refuse(op, "a buffer is missing");
   if (!aligned(a->q, 16) || !aligned(a->kv_layer, 256)) return refuse(op, "q is 16-byte aligned, the cache is 256-byte aligned");
+  if (!a->workspace || !aligned(a->workspace, 16) || a->workspace_bytes < tree_attention_workspace(*a)) return refuse(op, "the workspace is missing, too small or not 16-byte aligned");
   if (int rc = require_device()) return rc;
   int* mark = nullptr;
   if (int rc = op_mark(&mark)) return rc;

@@ -2,16 +2,20 @@
 //
 //   out_t = sum_j softmax_j(scale q_t . k_j) v_j   over j < ctx and those j = ctx + i whose bit i the row's mask has
 //
-// A request's rows share all keys but the last few, so what counts is that K and V pass once for all of a key head's rows: a CTA takes up to 128 * NT
-// of them (row = token * group + head), its share of the context in tiles of 64 keys, and works as the kernels of chunks and prompts do:
-//   one warp looks pages up (32 of the table at a time) and loads tiles by TMA, 128-byte swizzle, keys and values in rings of their own;
-//   one warp issues every tcgen05.mma:  S_i = Q_i K^T (M = 128, N = 64, two buffers in TMEM),  O_i += P_i V (M = 128, N = 128, P_i in TMEM over its scores);
-//   four warps a row tile (thread = row) do the softmax in fp32, base 2; warps whose rows nobody owns sleep.
-// The masks' bits are looked at only in tiles that reach behind the context.  There the products' warp also clears what must not meet a weight of zero:
-// values behind the last key, and infinities and NaN among the drafts' values, which the rows that see them add at the end by themselves.
-// Few requests: a cluster of CTAs shares a context, each leaves its unnormalised rows in its shared memory, and the rows are joined through
-// distributed shared memory in a fixed order; no workspace, one launch, the same bits every time.
-// Every wait has a limit; a CTA that gives up sets an error mark and still meets at the barriers.
+// A request's rows share all keys but the last few, so what counts is that K and V pass once for all rows of a key head and that nothing stops the stream
+// of pages.  An item is a request's key head and up to 128 * NT of its rows (row = token * group + head); its keys come in tiles of 64.  All items' tiles
+// one behind the other are cut into as many equal ranges as there are SMs, and a CTA an SM walks its range without a gap:
+//   two warps look pages up (32 of the table at a time, the next ones ahead) and load by TMA, 128-byte swizzle, into rings, one queries and keys, one
+//   values: a box of 2 KB takes its warp 85 cycles, and 16 of them for a tile left the memory waiting;
+//   two warps issue tcgen05.mma, one S = Q K^T (M = 128, N = 64), one O += P V (M = 128, N = 128, P in TMEM over its scores): a wait that is over costs
+//   its warp 100 cycles all the same, and one warp for both took 1500 a tile of which the tensor cores need 640;
+//   two groups of four warps (thread = row) do the softmax in fp32, base 2.  Up to 128 rows (NT = 1) the groups take tiles in turn, each with a maximum,
+//   sum and output of its own, and join them at the item's end; beyond (NT = 2) each has 128 rows and both take every tile.
+// The loads run into the next item while the groups finish one.  The masks' bits are looked at only in tiles that reach behind the context.  There the
+// products' warp also clears what must not meet a weight of zero: values behind the last key, and infinities and NaN among the drafts' values, which the
+// rows that see them add at the end by themselves.
+// An item that a range's end cuts leaves unnormalised rows in the workspace, which a second kernel joins in a fixed order: the same bits every time.
+// Every wait has a limit; a CTA that gives up sets an error mark and still meets at the end.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -25,7 +29,6 @@
 #include "launch.h"
 #include "ptx.cuh"
 #include "tree_step.h"
-#include "umma2.cuh"
 
 namespace b200 {
 namespace {
@@ -33,20 +36,20 @@ namespace {
 typedef __nv_bfloat16 bf16;
 constexpr int kD = 128, kRows = 128, kKeys = 64;
 constexpr int kQSlab = kRows * 128, kSlab = kKeys * 128, kTile = 2 * kSlab;      // bytes: 64 columns of a row tile, of a key tile, a key tile
-constexpr int kLd = kD + 4;                                                      // floats from row to row of what a cluster joins: no bank twice
+constexpr int kThreads = 384, kWarps = kThreads / 32;
+constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
+constexpr int kSnap = 2;                   // a range does not end within this many tiles of an item's ends
+constexpr int kLeast = 2;                  // tiles of a range at least
+constexpr float kSlack = 8.f;              // by which a row's maximum may pass what its weights are relative to, in units of log 2
 constexpr int kWaitLimit = 1 << 22;
-constexpr int kMostParts = 8;
 
 template <int NT>
 struct Shape {
-  static constexpr int kStages = NT == 1 ? 2 : 4;               // of keys and of values
-  static constexpr int kThreads = 32 * (4 * NT + 2);
-  static constexpr int kCtas = NT == 1 ? 2 : 1;                 // an SM
-  static constexpr int kRing = NT * 2 * kQSlab;                 // where the keys begin
-  static constexpr int kBars = kRing + 2 * kStages * kTile;
-  static constexpr int kSmem = 1024 + kBars + 512;
-  static_assert(NT * kRows * (kLd + 2) * 4 <= kBars, "rows to be joined lie over queries and tiles");
-  static_assert(kCtas * (kSmem + 1024) <= 228 * 1024, "");
+  static constexpr int kK = NT == 1 ? 4 : 3, kV = NT == 1 ? 5 : 3;      // tiles of keys and of values in flight
+  static constexpr int kKeysAt = 2 * NT * 2 * kQSlab, kValuesAt = kKeysAt + kK * kTile, kBars = kValuesAt + kV * kTile;
+  static constexpr int kStates = kBars + 512;                            // NT = 1: maximum and sum of each group's rows
+  static constexpr int kSmem = 1024 + kStates + (NT == 1 ? 2 * kRows * 8 : 0);
+  static_assert(kSmem <= 227 * 1024, "");
 };
 
 __device__ __forceinline__ uint32_t idesc_bf16(uint32_t m, uint32_t n, uint32_t b_mn) {
@@ -62,16 +65,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst_smem, const void* tmap,
   asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
                ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
                : "memory");
-}
-__device__ __forceinline__ float4 peer_float4(uint32_t at) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-  return v;
-}
-__device__ __forceinline__ float2 peer_float2(uint32_t at) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
-  return v;
 }
 __device__ __forceinline__ bool odd_pair(uint32_t u) { return (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u; }      // an infinity or NaN among two bf16
 __device__ __forceinline__ uint32_t without_odd(uint32_t u) { return ((u & 0x7f80u) == 0x7f80u ? 0u : u & 0xffffu) | ((u & 0x7f800000u) == 0x7f800000u ? 0u : u & 0xffff0000u); }
@@ -111,370 +104,593 @@ __device__ void zero_rest(const b200_tree_attn_args& a) {
   }
 }
 
+
+// ---- items and ranges
+struct Item {
+  int s, kvh, block;              // request, key head, which of its blocks of rows
+  tree::Request r;
+  int first, nb, kv_end, tiles;   // the block's tokens, keys that they may see
+};
+
+__device__ __forceinline__ int block_tokens(const b200_tree_attn_args& a, int NT) { return NT * kRows / (a.q_heads / a.kv_heads); }
+__device__ __forceinline__ int tiles_of(const b200_tree_attn_args& a, const tree::Request& r, int bt, int block) {
+  const int seen = a.masks ? r.rows : min(r.rows, (block + 1) * bt);
+  return (r.ctx + seen + kKeys - 1) / kKeys;
+}
+__device__ __forceinline__ int blocks_of(const tree::Request& r, int bt) { return (r.rows + bt - 1) / bt; }
+// tiles of all of a key head's blocks
+__device__ __forceinline__ int head_tiles(const b200_tree_attn_args& a, const tree::Request& r, int bt) {
+  const int blocks = blocks_of(r, bt);
+  if (a.masks || blocks <= 1) return blocks ? blocks * tiles_of(a, r, bt, 0) : 0;
+  int n = 0;
+  for (int b = 0; b < blocks; ++b) n += tiles_of(a, r, bt, b);
+  return n;
+}
+__device__ __forceinline__ tree::Request request(const b200_tree_attn_args& a, int s) { return tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, a.max_tree); }
+__device__ __forceinline__ void fill(const b200_tree_attn_args& a, int bt, Item* it) {
+  it->first = it->block * bt;
+  it->nb = min(bt, it->r.rows - it->first);
+  it->kv_end = it->r.ctx + (a.masks ? it->r.rows : it->first + it->nb);
+  it->tiles = tiles_of(a, it->r, bt, it->block);
+}
+// Range c of the N tiles begins at c * each + min(c, more).
+struct Ranges {
+  int n, each, more;
+  __device__ __forceinline__ Ranges(int N, int ctas) : n(min(ctas, max(N / kLeast, 1))), each(N / n), more(N - each * n) {}
+  __device__ __forceinline__ int at(int c) const { return c * each + min(c, more); }
+  // ranges but the first that begin at tile x or in front of it
+  __device__ __forceinline__ int up_to(int x) const {
+    if (x < 0) return 0;
+    const int c = x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each;
+    return min(n - 1, c);
+  }
+};
+// the cut b as it is moved within the item [g0, g1)
+__device__ __forceinline__ int snapped(int b, int g0, int g1) { return b - g0 <= kSnap ? g0 : g1 - b <= kSnap ? g1 : b; }
+// What a CTA leaves for the second kernel: the item that begins in its range and ends behind it, and in how many ranges it lies (0: no such item).
+struct Cut {
+  int row0, rows, kvh, parts;      // the item's first row of the step, rows (token * group + head)
+};
+
+// The workspace: a Cut and two parts' rows for every CTA
+__host__ __device__ __forceinline__ float* rows_of(void* workspace, int ctas) { return reinterpret_cast<float*>(static_cast<Cut*>(workspace) + ctas); }
+
+// A row's dimensions [c_begin, c_begin + columns) = w_a o_a + w_b o_b: normalised to the output where the item is whole, else to the workspace with its
+// maximum m (units of log 2) and sum.
 template <int NT>
-__global__ void __launch_bounds__(Shape<NT>::kThreads, Shape<NT>::kCtas)
+__device__ __forceinline__ void finish(const b200_tree_attn_args& a, const Item& it, uint32_t o_a, int has_a, float w_a, uint32_t o_b, int has_b, float w_b, int c_begin, int columns,
+                                       bool valid, int token, int head, float m, float sum, bool whole, int t0, int take, bool odd, int cta, int row) {
+  const int group = a.q_heads / a.kv_heads;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  bf16* dst = static_cast<bf16*>(a.out) + static_cast<size_t>(it.r.row0 + token) * a.ldo + (it.kvh * group + head) * kD;
+  float* part = rows_of(a.workspace, gridDim.x) + (static_cast<size_t>(2 * cta + (t0 == 0)) * (NT * kRows) + row) * kLd;      // a part without the item's beginning is the range's first
+  for (int c0 = c_begin; c0 < c_begin + columns; c0 += 32) {
+    uint32_t v[32];
+    if (has_a) {
+      tmem_ld_32x32(o_a + c0, v);
+      tmem_ld_wait();
+    } else {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) v[c] = 0u;
+    }
+    if (NT == 1) {
+#pragma unroll
+      for (int c = 0; c < 32; ++c) v[c] = w_a == 0.f ? 0u : __float_as_uint(__uint_as_float(v[c]) * w_a);
+      if (has_b) {
+        uint32_t x[32];
+        tmem_ld_32x32(o_b + c0, x);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 32; ++c) v[c] = w_b == 0.f ? v[c] : __float_as_uint(fmaf(__uint_as_float(x[c]), w_b, __uint_as_float(v[c])));
+      }
+    }
+    if (valid && odd) {
+      // infinities and NaN of the drafts that this row sees, which stayed out of the products
+      const int* table = a.block_tables + static_cast<size_t>(it.s) * a.ld_tables;
+      const int* mask = a.masks ? a.masks + static_cast<size_t>(it.r.row0 + token) * a.words : nullptr;
+      for (int p = max(it.r.ctx, t0 * kKeys); p < min(it.kv_end, (t0 + take) * kKeys); ++p) {
+        if (!(seen_bits(mask, a.words, token, it.r.rows, p - it.r.ctx) & 1)) continue;
+        const long long at = tree::cache_row(table, p, a.num_pages);
+        if (at < 0) continue;
+        const bf16* value = static_cast<const bf16*>(a.kv_layer) + ((((at >> 4) * 2 + 1) * a.kv_heads + it.kvh) * 16 + (at & 15)) * kD + c0;
+#pragma unroll
+        for (int c = 0; c < 32; ++c) {
+          const float x = __bfloat162float(value[c]);
+          if (!isfinite(x)) v[c] = __float_as_uint(__uint_as_float(v[c]) + x);
+        }
+      }
+    }
+    if (valid && whole) {
+#pragma unroll
+      for (int c = 0; c < 32; c += 8)
+        *reinterpret_cast<uint4*>(dst + c0 + c) =
+            make_uint4(pack_bf16x2(__uint_as_float(v[c]) * inv, __uint_as_float(v[c + 1]) * inv), pack_bf16x2(__uint_as_float(v[c + 2]) * inv, __uint_as_float(v[c + 3]) * inv),
+                       pack_bf16x2(__uint_as_float(v[c + 4]) * inv, __uint_as_float(v[c + 5]) * inv), pack_bf16x2(__uint_as_float(v[c + 6]) * inv, __uint_as_float(v[c + 7]) * inv));
+    } else if (valid) {
+#pragma unroll
+      for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(part + c0 + c) = make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]);
+    }
+    __syncwarp();
+  }
+  if (valid && !whole && c_begin == 0) *reinterpret_cast<float2*>(part + kD) = make_float2(m, sum);
+}
+
+template <int NT>
+__global__ void __launch_bounds__(kThreads, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ b200_tree_attn_args a, float scale_log2, int* error) {
-  constexpr int kStages = Shape<NT>::kStages, kWarps = Shape<NT>::kThreads / 32;
+  constexpr int kK = Shape<NT>::kK, kV = Shape<NT>::kV;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (sbase - smem_u32(smem_raw));
-  const uint32_t q_s = sbase, k_s = sbase + Shape<NT>::kRing, v_s = k_s + kStages * kTile, bars = sbase + Shape<NT>::kBars;
+  const uint32_t q_s = sbase, k_s = sbase + Shape<NT>::kKeysAt, v_s = sbase + Shape<NT>::kValuesAt, bars = sbase + Shape<NT>::kBars;
   auto k_full = [&](int s) { return bars + 8u * s; };
-  auto k_empty = [&](int s) { return bars + 8u * (kStages + s); };
-  auto v_full = [&](int s) { return bars + 8u * (2 * kStages + s); };
-  auto v_empty = [&](int s) { return bars + 8u * (3 * kStages + s); };
-  auto s_full = [&](int i, int b) { return bars + 8u * (4 * kStages + 2 * i + b); };
-  // of every other tile each, as the scores': a warp is up to two tiles ahead of the slowest one of its group
-  auto p_ready = [&](int i, int b) { return bars + 8u * (4 * kStages + 4 + 2 * i + b); };
-  auto pv_full = [&](int i, int b) { return bars + 8u * (4 * kStages + 8 + 2 * i + b); };
-  const uint32_t q_bar = bars + 8u * (4 * kStages + 12), slot = q_bar + 8;
+  auto k_empty = [&](int s) { return bars + 8u * (5 + s); };
+  auto v_full = [&](int s) { return bars + 8u * (10 + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (15 + s); };
+  auto q_full = [&](int b) { return bars + 8u * (20 + b); };
+  auto q_empty = [&](int b) { return bars + 8u * (22 + b); };
+  // of every other tile of a group each: a warp is up to two tiles ahead of the slowest one of its group
+  auto s_full = [&](int g, int b) { return bars + 8u * (24 + 2 * g + b); };
+  auto p_ready = [&](int g, int b) { return bars + 8u * (28 + 2 * g + b); };
+  auto pv_full = [&](int g, int b) { return bars + 8u * (32 + 2 * g + b); };
+  auto joined = [&](int k) { return bars + 8u * (36 + k); };      // NT = 1: both groups' eight warps, at an item's end: products landed, outputs read
+  const uint32_t slot = bars + 8u * 38;
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (slot - sbase));
-  volatile uint32_t* odd_values = tmem_slot + 1;
-  const int warp = warp_number(), lane = threadIdx.x & 31;
-
-  const int parts = static_cast<int>(gridDim.x), part = static_cast<int>(blockIdx.x);
-  const int kvh = blockIdx.y % a.kv_heads, block = blockIdx.y / a.kv_heads, s = blockIdx.z;
-  const int group = a.q_heads / a.kv_heads, block_rows = NT * kRows / group;      // tokens of a block
-  griddep_enter();
-  if (s == a.S) {
-    if (part == 0 && blockIdx.y == 0) zero_rest(a);
-    return;
-  }
-  const tree::Request r = tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, a.max_tree);
-  const int first = block * block_rows, nb = min(block_rows, r.rows - first);      // this block's tokens of the request
-  if (nb <= 0) return;
-  const int kv_end = r.ctx + (a.masks ? r.rows : first + nb), all_tiles = (kv_end + kKeys - 1) / kKeys;
-  // its part of the tiles; parts that find none leave (a cluster barrier does not wait for threads that have ended)
-  const int per = max((all_tiles + parts - 1) / parts, 2), active = (all_tiles + per - 1) / per;
-  if (part >= active) return;
-  const int t_begin = part * per, t_end = min(all_tiles, t_begin + per), tiles = t_end - t_begin;
-  const int tiles_q = NT == 2 && nb * group > kRows ? 2 : 1;
-  auto warps_of = [&](int i) { return (min(nb * group - i * kRows, kRows) + 31) / 32; };
+  volatile int* odd_item = reinterpret_cast<volatile int*>(tmem_slot + 2);      // [2]: the last item of each parity with infinities or NaN among its drafts' values
+  __shared__ int sums[kWarps];
+  __shared__ int s_range[3];        // begin, end, and the first tile of the begin's item
+  __shared__ int s_where[3];
+  const int warp = warp_number(), lane = threadIdx.x & 31, tid = threadIdx.x;
 
   if (warp == 0) {
     if (lane == 0) {
-      for (int st = 0; st < kStages; ++st) {
-        mbar_init(k_full(st), 1); mbar_init(k_empty(st), 1); mbar_init(v_full(st), 1); mbar_init(v_empty(st), 1);
+      for (int s = 0; s < 5; ++s) { mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1); mbar_init(v_full(s), 1); mbar_init(v_empty(s), 1); }
+      for (int g = 0; g < 2; ++g) {
+        mbar_init(q_full(g), 1); mbar_init(q_empty(g), 1);
+        for (int b = 0; b < 2; ++b) { mbar_init(s_full(g, b), 1); mbar_init(p_ready(g, b), 4); mbar_init(pv_full(g, b), 1); }
       }
-      for (int i = 0; i < tiles_q; ++i)
-        for (int b = 0; b < 2; ++b) { mbar_init(s_full(i, b), 1); mbar_init(p_ready(i, b), warps_of(i)); mbar_init(pv_full(i, b), 1); }
-      mbar_init(q_bar, 1);
+      mbar_init(joined(0), 8);
+      mbar_init(joined(1), 8);
       fence_mbar_init();
-      *odd_values = 0;
+      odd_item[0] = odd_item[1] = -1;
+      tma_prefetch_desc(&tm_q);
+      tma_prefetch_desc(&tm_kv);
     }
     __syncwarp();
-    tmem_alloc(slot, 256 * NT);
+    tmem_alloc(slot, 512);
     tmem_relinquish();
+  }
+  griddep_enter();
+  const int ctas = gridDim.x, cta = blockIdx.x, bt = block_tokens(a, NT);
+  // ---- this CTA's range, and where it begins: every thread sums some requests, one behind the other, and the sums of the threads in front of it
+  const int per_thread = (a.S + kThreads - 1) / kThreads, s_begin = min(a.S, tid * per_thread), s_end = min(a.S, s_begin + per_thread);
+  int before = 0, N = 0;
+  for (int s = s_begin; s < s_end; ++s) before += head_tiles(a, request(a, s), bt) * a.kv_heads;
+  const int own = before;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += y;
+  }
+  if (lane == 31) sums[warp] = before;
+  __syncthreads();
+  before -= own;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const int x = sums[w];
+    if (w < warp) before += x;
+    N += x;
+  }
+  const Ranges ranges(N, ctas);
+  bool ok = true;
+  if (N > 0 && cta < ranges.n) {
+    const int b[2] = {ranges.at(cta), ranges.at(cta + 1)};
+    if (tid == 0 && cta + 1 == ranges.n) s_range[1] = N;      // which lies in no item
+    if (b[0] < before + own && b[1] >= before)
+      for (int s = s_begin; s < s_end; ++s) {
+        const tree::Request r = request(a, s);
+        const int per_head = head_tiles(a, r, bt), mine = per_head * a.kv_heads;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (mine == 0 || b[e] < before || b[e] >= before + mine) continue;
+          const int kvh = (b[e] - before) / per_head;
+          int g0 = before + kvh * per_head, block = 0;
+          for (int n; b[e] >= g0 + (n = tiles_of(a, r, bt, block)); ++block) g0 += n;
+          s_range[e] = snapped(b[e], g0, g0 + tiles_of(a, r, bt, block));
+          if (e == 0) { s_where[0] = s; s_where[1] = kvh; s_where[2] = block; s_range[2] = g0; }
+        }
+        before += mine;
+      }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  auto tm_s = [&](int i, int b) { return tmem + 64u * (2 * i + b); };
-  auto tm_o = [&](int i) { return tmem + 128u * NT + 128u * i; };
-  bool ok = true;
-  float ref = -INFINITY, l = 0.f;      // of a softmax thread's row: what its weights are relative to, in units of log 2, and their sum
+  auto tm_s = [&](int g, int b) { return tmem + 64u * (2 * g + b); };
+  auto tm_o = [&](int g) { return tmem + 256u + 128u * g; };
+  Cut cut = {0, 0, 0, 0};
+  const int left = N > 0 && cta < ranges.n ? s_range[1] - s_range[0] : 0;
 
-  if (warp == 0) {
-    // ------------------------------------------------------------ loads
-    const bool one = elect_one();
-    if (one) mbar_arrive_expect_tx(q_bar, tiles_q * 2 * kQSlab);
-    for (int i = 0; i < tiles_q; ++i)
-      for (int h = 0; h < 2; ++h)
-        if (one) tma_load_3d(q_s + (2 * i + h) * kQSlab, &tm_q, q_bar, 64 * h, kvh * group, r.row0 + first + i * (kRows / group));
-    const int pages = (kv_end + 15) >> 4, p_begin = t_begin * 4;
-    const int* table = a.block_tables + static_cast<size_t>(s) * a.ld_tables;
-    // a page that the cache does not have lies behind its last row, where a load finds zeros
-    auto look_up = [&](int base) {
-      const int p = base + lane, page = p < pages ? table[p] : -1;
-      return page >= 0 && page < a.num_pages ? page : static_cast<int>(a.num_pages);
-    };
-    const uint64_t hint = gridDim.y > static_cast<unsigned>(a.kv_heads) ? kEvictNormal : kEvictFirst;
-    int mine = look_up(p_begin), next = look_up(p_begin + 32);
-    for (int it = 0; it < tiles; ++it) {
-      if (it && it % 8 == 0) {
-        mine = next;
-        next = look_up(p_begin + 4 * it + 32);
-      }
-      const int st = it % kStages, n = min(4, pages - p_begin - 4 * it);
-      const uint32_t parity = ((it / kStages) & 1) ^ 1u;
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {      // keys, then values
-        if (!(ok = warp_wait(w ? v_empty(st) : k_empty(st), parity))) break;
-        const uint32_t full = w ? v_full(st) : k_full(st), dst = (w ? v_s : k_s) + st * kTile;
-        if (one) mbar_arrive_expect_tx(full, n * 4096);
-#pragma unroll
-        for (int pg = 0; pg < 4; ++pg) {
-          const int page = __shfl_sync(0xffffffffu, mine, (4 * it + pg) & 31), row = ((page * 2 + w) * a.kv_heads + kvh) * 16;
-          if (pg >= n || !one) continue;
-          tma_load_2d(dst + pg * 2048, &tm_kv, full, 0, row, hint);
-          tma_load_2d(dst + kSlab + pg * 2048, &tm_kv, full, 64, row, hint);
+  if (left > 0) {
+    // every role walks the same items: item, its first tile here and how many
+    Item it;
+    it.s = s_where[0]; it.kvh = s_where[1]; it.block = s_where[2];
+    it.r = request(a, it.s);
+    fill(a, bt, &it);
+    int t0 = s_range[0] - s_range[2], rest = left;
+    auto next_item = [&] {
+      ++it.block;
+      if (it.block >= blocks_of(it.r, bt)) {
+        it.block = 0;
+        if (++it.kvh >= a.kv_heads) {
+          it.kvh = 0;
+          do it.r = request(a, ++it.s);
+          while (it.r.rows == 0);      // (a range's tiles are some request's: the walk ends in front of a.S)
         }
       }
-      if (!ok) {
-        // the copies in flight land before the CTA ends
-        for (int j = max(0, it - kStages); j <= it; ++j) { warp_wait(k_full(j % kStages), (j / kStages) & 1); warp_wait(v_full(j % kStages), (j / kStages) & 1); }
-        break;
-      }
+      fill(a, bt, &it);
+    };
+    if (t0 == it.tiles) {              // the range begins where the item in front of it ends
+      t0 = 0;
+      next_item();
     }
-    warp_wait(q_bar, 0);
-  } else if (warp == kWarps - 1) {
-    // ------------------------------------------------------------ products
-    const bool one = elect_one();
-    const uint32_t id_s = idesc_bf16(kRows, kKeys, 0), id_o = idesc_bf16(kRows, kD, 1);
-    const uint64_t q_d = desc_sw128(q_s, 16, 1024), k_d = desc_sw128(k_s, 16, 1024), v_d = desc_sw128(v_s, kSlab, 1024);
-    auto scores = [&](int it) {
-      const int st = it % kStages;
-      if (!warp_wait(k_full(st), (it / kStages) & 1)) return false;
-      tc_fence_after();
-      if (one) {
-        for (int i = 0; i < tiles_q; ++i) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) umma_bf16_k64(tm_s(i, it & 1), q_d + (2 * i + h) * (kQSlab >> 4), k_d + st * (kTile >> 4) + h * (kSlab >> 4), id_s, h);
-          umma_commit(s_full(i, it & 1));
+    const int group = a.q_heads / a.kv_heads;
+    int gt = 0, item = 0;              // tiles and items of this range so far
+
+    if (warp == 0 || warp == kWarps - 3) {
+      // ------------------------------------------------------------ loads: queries and keys, or values
+      const bool one = elect_one(), values = warp != 0;
+      const int depth = values ? kV : kK;
+      const uint32_t ring = values ? v_s : k_s, full0 = values ? v_full(0) : k_full(0), empty0 = values ? v_empty(0) : k_empty(0);
+      int st = 0, phase = 1;
+      for (; ok && rest > 0; ++item) {
+        const uint64_t hint = it.r.rows > bt ? kEvictNormal : kEvictFirst;
+        const int take = min(it.tiles - t0, rest), pages = (it.kv_end + 15) >> 4, p_begin = t0 * 4;
+        const int* table = a.block_tables + static_cast<size_t>(it.s) * a.ld_tables;
+        // the first row of a page's head; a page that the cache does not have lies behind its last row, where a load finds zeros
+        auto look_up = [&](int base) {
+          const int p = base + lane, page = p < pages ? table[p] : -1;
+          return ((page >= 0 && page < a.num_pages ? page : static_cast<int>(a.num_pages)) * 2 + values) * a.kv_heads * 16 + it.kvh * 16;
+        };
+        int mine = look_up(p_begin), next = look_up(p_begin + 32);
+        if (!values) {
+          const int qb = item & 1, tiles_q = NT == 2 && it.nb * group > kRows ? 2 : 1;
+          if (!(ok = warp_wait(q_empty(qb), ((item >> 1) & 1) ^ 1u))) break;
+          if (one) {
+            mbar_arrive_expect_tx(q_full(qb), tiles_q * 2 * kQSlab);
+            for (int i = 0; i < tiles_q; ++i)
+              for (int h = 0; h < 2; ++h) tma_load_3d(q_s + ((qb * NT + i) * 2 + h) * kQSlab, &tm_q, q_full(qb), 64 * h, it.kvh * group, it.r.row0 + it.first + i * (kRows / group));
+          }
         }
-        umma_commit(k_empty(st));
-      }
-      __syncwarp();
-      return true;
-    };
-    ok = warp_wait(q_bar, 0) && scores(0);
-    for (int it = 0; ok && it < tiles; ++it) {
-      // the next scores go to the other buffers, whose readers have handed in their P of the tile before this one
-      if (it + 1 < tiles && !(ok = scores(it + 1))) break;
-      const int st = it % kStages, kv0 = (t_begin + it) * kKeys;
-      if (!(ok = warp_wait(v_full(st), (it / kStages) & 1))) break;
-      if (kv0 + kKeys > r.ctx) {
-        bool odd = false;
-        for (int e = max(0, r.ctx - kv0) * 8 + lane; e < kKeys * 8; e += 32) {
+        for (int j = 0; j < take; ++j, ++gt) {
+          if (j && j % 8 == 0) {
+            mine = next;
+            next = look_up(p_begin + 4 * j + 32);
+          }
+          const int n = min(4, pages - p_begin - 4 * j);
+          int row[4];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            uint4* v = reinterpret_cast<uint4*>(smem + (v_s - sbase) + st * kTile + h * kSlab) + e;      // (a row's pieces in some order)
-            if (kv0 + (e >> 3) >= kv_end) *v = make_uint4(0, 0, 0, 0);
-            else if (const uint4 x = *v; odd_pair(x.x) || odd_pair(x.y) || odd_pair(x.z) || odd_pair(x.w)) {
-              *v = make_uint4(without_odd(x.x), without_odd(x.y), without_odd(x.z), without_odd(x.w));
-              odd = true;
+          for (int pg = 0; pg < 4; ++pg) row[pg] = __shfl_sync(0xffffffffu, mine, (4 * j + pg) & 31);
+          if (!(ok = warp_wait(empty0 + 8 * st, phase))) break;
+          const uint32_t full = full0 + 8 * st, dst = ring + st * kTile;
+          if (one) {
+            mbar_arrive_expect_tx(full, n * 4096);
+#pragma unroll
+            for (int pg = 0; pg < 4; ++pg) {
+              if (pg >= n) break;
+              tma_load_2d(dst + pg * 2048, &tm_kv, full, 0, row[pg], hint);
+              tma_load_2d(dst + kSlab + pg * 2048, &tm_kv, full, 64, row[pg], hint);
             }
           }
+          __syncwarp();
+          if (++st == depth) { st = 0; phase ^= 1; }
         }
-        if (odd) *odd_values = 1;
-        fence_proxy_async();
-        __syncwarp();
+        if (!ok) break;
+        rest -= take;
+        if (rest == 0 && t0 == 0 && take < it.tiles)
+          cut = {it.r.row0 + it.first, it.nb * group, it.kvh, ranges.up_to(s_range[1] - take + it.tiles - kSnap - 1) - cta + 1};
+        t0 = 0;
+        if (rest > 0) next_item();
       }
-      for (int i = 0; i < tiles_q; ++i) {
-        if (!(ok = warp_wait(p_ready(i, it & 1), (it >> 1) & 1))) break;
-        tc_fence_after();
-        if (one) {
-          umma_bf16_tmem_k64(tm_o(i), tm_s(i, it & 1), v_d + st * (kTile >> 4), id_o, it > 0);
-          umma_commit(pv_full(i, it & 1));
-        }
-        __syncwarp();
-      }
-      if (ok && one) umma_commit(v_empty(st));
-      __syncwarp();
-    }
-  } else {
-    // ------------------------------------------------------------ softmax: thread = row (token * group + head)
-    const int gi = (warp - 1) >> 2, q = warp & 3, row = gi * kRows + q * 32 + lane;
-    const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
-    const bool valid = row < nb * group;
-    const int token = first + row / group;
-    const int* mask = a.masks && valid ? a.masks + static_cast<size_t>(r.row0 + token) * a.words : nullptr;
-    if (gi < tiles_q && gi * kRows + q * 32 < nb * group) {
-      for (int it = 0; it < tiles; ++it) {
-        const int b = it & 1, kv0 = (t_begin + it) * kKeys;
-        if (!(ok = warp_wait(s_full(gi, b), (it >> 1) & 1))) break;
-        tc_fence_after();
-        uint32_t s0[32], s1[32];
-        tmem_ld_32x32(tm_s(gi, b) + lane_off, s0);
-        tmem_ld_32x32(tm_s(gi, b) + lane_off + 32, s1);
-        tmem_ld_wait();
-        if (kv0 + kKeys > r.ctx) {
-          const uint32_t m0 = valid ? seen_bits(mask, a.words, token, r.rows, kv0 - r.ctx) : 0u, m1 = valid ? seen_bits(mask, a.words, token, r.rows, kv0 + 32 - r.ctx) : 0u;
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            if (!(m0 >> c & 1)) s0[c] = 0xff800000u;
-            if (!(m1 >> c & 1)) s1[c] = 0xff800000u;
-          }
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int c = 0; c < 32; c += 2)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            mx[k] = fmaxf(mx[k], __uint_as_float(s0[c + k]));
-            mx[2 + k] = fmaxf(mx[2 + k], __uint_as_float(s1[c + k]));
-          }
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
-        float alpha = 1.f;
-        if (top > ref) {
-          alpha = exp2_ftz(ref - top);
-          ref = top;
-        }
-        const float mu = ref == -INFINITY ? 0.f : ref;
-        auto weight = [&](uint32_t u) { return exp2_ftz(fmaf(__uint_as_float(u), scale_log2, -mu)); };
-        float ps = 0.f;
-        uint32_t pk[32];
-#pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          const float p0 = weight(s0[c]), p1 = weight(s0[c + 1]), p2 = weight(s1[c]), p3 = weight(s1[c + 1]);
-          ps += (p0 + p1) + (p2 + p3);
-          pk[c >> 1] = pack_bf16x2(p0, p1);
-          pk[16 + (c >> 1)] = pack_bf16x2(p2, p3);
-        }
-        l = l * alpha + ps;
-        // P in place of the scores: what read this buffer's last P went ahead of them.  Where some row of the warp moved its maximum, its output so
-        // far is scaled once the previous tile's product has landed.
-        tmem_st_32x32(tm_s(gi, b) + lane_off, pk);
-        if (it > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-          if (!(ok = warp_wait(pv_full(gi, b ^ 1), ((it - 1) >> 1) & 1))) break;
+      // the copies in flight land before the CTA ends, also where it gives up
+      if (!values)
+        for (int k = max(0, item - 2); k < item + !ok; ++k) warp_wait(q_full(k & 1), (k >> 1) & 1);
+      for (int k = max(0, gt - depth); k < gt; ++k) warp_wait(full0 + 8 * (k % depth), (k / depth) & 1);
+    } else if (warp == kWarps - 2) {
+      // ------------------------------------------------------------ scores
+      const bool one = elect_one();
+      const uint32_t id_s = idesc_bf16(kRows, kKeys, 0);
+      const uint64_t q_d = desc_sw128(q_s, 16, 1024), k_d = desc_sw128(k_s, 16, 1024);
+      for (; ok && rest > 0; ++item) {
+        const int take = min(it.tiles - t0, rest), tiles_q = NT == 2 && it.nb * group > kRows ? 2 : 1, qb = item & 1;
+        if (!(ok = warp_wait(q_full(qb), (item >> 1) & 1))) break;
+        for (int j = 0; j < take; ++j, ++gt) {
+          const int st = gt % kK, u = NT == 1 ? gt >> 1 : gt, b = u & 1;
+          if (!(ok = warp_wait(k_full(st), (gt / kK) & 1))) break;
+          // the buffer's last P has been read by the products with its values
+          if (u >= 2)
+            for (int i = 0; ok && i < NT; ++i) ok = warp_wait(pv_full(NT == 1 ? gt & 1 : i, b), ((u - 2) >> 1) & 1);
+          if (!ok) break;
           tc_fence_after();
+          if (one) {
 #pragma unroll
-          for (int c0 = 0; c0 < kD; c0 += 32) {
-            uint32_t v[32];
-            tmem_ld_32x32(tm_o(gi) + lane_off + c0, v);
-            tmem_ld_wait();
+            for (int i = 0; i < NT; ++i) {
+              const int g = NT == 1 ? gt & 1 : i;
+              if (i < tiles_q) {
 #pragma unroll
-            for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * alpha);
-            tmem_st_32x32(tm_o(gi) + lane_off + c0, v);
-          }
-        }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready(gi, b));
-      }
-      if (ok) ok = warp_wait(pv_full(gi, (tiles - 1) & 1), ((tiles - 1) >> 1) & 1);
-    }
-  }
-  if (!ok) *reinterpret_cast<volatile int*>(error) = 1;
-  ok = __syncthreads_and(ok);      // every product and copy has landed: queries and tiles may be written over
-  tc_fence_after();
-
-  // ------------------------------------------------------------ results
-  const int rows = nb * group;
-  float* joined = reinterpret_cast<float*>(smem);                       // [rows][kLd], then [rows] of maximum and sum
-  float2* state = reinterpret_cast<float2*>(joined + NT * kRows * kLd);
-  if (ok && warp >= 1 && warp < kWarps - 1) {
-    const int gi = (warp - 1) >> 2, q = warp & 3, row = gi * kRows + q * 32 + lane, token = first + row / group;
-    if (gi * kRows + q * 32 < rows) {
-      const bool valid = row < rows;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      bf16* dst = static_cast<bf16*>(a.out) + static_cast<size_t>(r.row0 + token) * a.ldo + (kvh * group + row % group) * kD;
-      const int* mask = a.masks && valid ? a.masks + static_cast<size_t>(r.row0 + token) * a.words : nullptr;
-#pragma unroll
-      for (int c0 = 0; c0 < kD; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld_32x32(tm_o(gi) + (static_cast<uint32_t>(q * 32) << 16) + c0, v);
-        tmem_ld_wait();
-        if (!valid) continue;
-        if (*odd_values) {
-          // infinities and NaN of the drafts that this row sees, which stayed out of the products
-          const int* table = a.block_tables + static_cast<size_t>(s) * a.ld_tables;
-          for (int p = max(r.ctx, t_begin * kKeys); p < min(kv_end, t_end * kKeys); ++p) {
-            if (!(seen_bits(mask, a.words, token, r.rows, p - r.ctx) & 1)) continue;
-            const long long at = tree::cache_row(table, p, a.num_pages);
-            if (at < 0) continue;
-            const bf16* value = static_cast<const bf16*>(a.kv_layer) + ((((at >> 4) * 2 + 1) * a.kv_heads + kvh) * 16 + (at & 15)) * kD + c0;
-#pragma unroll
-            for (int c = 0; c < 32; ++c) {
-              const float x = __bfloat162float(value[c]);
-              if (!isfinite(x)) v[c] = __float_as_uint(__uint_as_float(v[c]) + x);
+                for (int h = 0; h < 2; ++h) umma_bf16_k64(tm_s(g, b), q_d + ((qb * NT + i) * 2 + h) * (kQSlab >> 4), k_d + st * (kTile >> 4) + h * (kSlab >> 4), id_s, h);
+              }
+              umma_commit(s_full(g, b));      // (a group without rows keeps step)
             }
+            umma_commit(k_empty(st));
+            if (j + 1 == take) umma_commit(q_empty(qb));
           }
+          __syncwarp();
         }
-        if (active == 1) {
-#pragma unroll
-          for (int c = 0; c < 32; c += 8)
-            *reinterpret_cast<uint4*>(dst + c0 + c) =
-                make_uint4(pack_bf16x2(__uint_as_float(v[c]) * inv, __uint_as_float(v[c + 1]) * inv), pack_bf16x2(__uint_as_float(v[c + 2]) * inv, __uint_as_float(v[c + 3]) * inv),
-                           pack_bf16x2(__uint_as_float(v[c + 4]) * inv, __uint_as_float(v[c + 5]) * inv), pack_bf16x2(__uint_as_float(v[c + 6]) * inv, __uint_as_float(v[c + 7]) * inv));
-        } else {
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(joined + row * kLd + c0 + c) = make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]);
-        }
+        if (!ok) break;
+        rest -= take;
+        t0 = 0;
+        if (rest > 0) next_item();
       }
-      if (active > 1 && valid) state[row] = make_float2(ref, l);
+    } else if (warp == kWarps - 1) {
+      // ------------------------------------------------------------ outputs
+      const bool one = elect_one();
+      const uint32_t id_o = idesc_bf16(kRows, kD, 1);
+      const uint64_t v_d = desc_sw128(v_s, kSlab, 1024);
+      for (; ok && rest > 0; ++item) {
+        const int take = min(it.tiles - t0, rest), tiles_q = NT == 2 && it.nb * group > kRows ? 2 : 1;
+        for (int j = 0; j < take; ++j, ++gt) {
+          const int st = gt % kV, kv0 = (t0 + j) * kKeys;
+          if (!(ok = warp_wait(v_full(st), (gt / kV) & 1))) break;
+          if (kv0 + kKeys > it.r.ctx) {
+            bool odd = false;
+            const int from = max(0, it.r.ctx - kv0), end = min(kKeys, it.kv_end - kv0);      // the drafts' rows of the tile
+            for (int h = 0; h < 2; ++h) {
+              uint4* v = reinterpret_cast<uint4*>(smem + (v_s - sbase) + st * kTile + h * kSlab);      // (a row's pieces in some order)
+              for (int e0 = from * 8; e0 < end * 8; e0 += 128) {
+                uint4 x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = v[min(e0 + 32 * k + lane, end * 8 - 1)];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                  if (odd_pair(x[k].x) || odd_pair(x[k].y) || odd_pair(x[k].z) || odd_pair(x[k].w)) {
+                    v[min(e0 + 32 * k + lane, end * 8 - 1)] = make_uint4(without_odd(x[k].x), without_odd(x[k].y), without_odd(x[k].z), without_odd(x[k].w));
+                    odd = true;
+                  }
+              }
+              for (int e = end * 8 + lane; e < kKeys * 8; e += 32) v[e] = make_uint4(0, 0, 0, 0);
+            }
+            if (odd) odd_item[item & 1] = item;
+            __threadfence_block();
+            fence_proxy_async();
+            __syncwarp();
+          }
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            const int g = NT == 1 ? gt & 1 : i, u = NT == 1 ? gt >> 1 : gt, b = u & 1;
+            if (ok) ok = warp_wait(p_ready(g, b), (u >> 1) & 1);
+            if (!ok) continue;
+            tc_fence_after();
+            if (one) {
+              if (i < tiles_q) umma_bf16_tmem_k64(tm_o(g), tm_s(g, b), v_d + st * (kTile >> 4), id_o, j >= (NT == 1 ? 2 : 1));
+              umma_commit(pv_full(g, b));
+            }
+            __syncwarp();
+          }
+          if (!ok) break;
+          if (one) umma_commit(v_empty(st));
+          __syncwarp();
+        }
+        if (!ok) break;
+        rest -= take;
+        t0 = 0;
+        if (rest > 0) next_item();
+      }
+    } else {
+      // ------------------------------------------------------------ softmax: thread = row (token * group + head)
+      const int g = (warp - 1) >> 2, q = warp & 3, in_tile = q * 32 + lane;
+      const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
+      const int row = (NT == 2 ? g * kRows : 0) + in_tile, token_of = row / group, head_of = row - token_of * group;
+      float2* states = reinterpret_cast<float2*>(smem + Shape<NT>::kStates);
+      for (; ok && rest > 0; ++item) {
+        const int take = min(it.tiles - t0, rest), rows = it.nb * group;
+        const bool valid = row < rows, some = row - lane < rows;      // this warp has rows
+        const int token = it.first + token_of;
+        const int* mask = a.masks && valid ? a.masks + static_cast<size_t>(it.r.row0 + token) * a.words : nullptr;
+        float ref = -INFINITY, l = 0.f;      // what the row's weights are relative to, in units of log 2, and their sum
+        int mine = 0;                        // tiles of this group
+        for (int j = 0; j < take; ++j, ++gt) {
+          if (NT == 1 && (gt & 1) != g) continue;
+          const int u = NT == 1 ? gt >> 1 : gt, b = u & 1, kv0 = (t0 + j) * kKeys;
+          if (!(ok = warp_wait(s_full(g, b), (u >> 1) & 1))) break;
+          if (some) {
+            tc_fence_after();
+            uint32_t s0[32], s1[32];
+            tmem_ld_32x32(tm_s(g, b) + lane_off, s0);
+            tmem_ld_32x32(tm_s(g, b) + lane_off + 32, s1);
+            tmem_ld_wait();
+            if (kv0 + kKeys > it.r.ctx) {
+              const uint32_t m0 = valid ? seen_bits(mask, a.words, token, it.r.rows, kv0 - it.r.ctx) : 0u, m1 = valid ? seen_bits(mask, a.words, token, it.r.rows, kv0 + 32 - it.r.ctx) : 0u;
+#pragma unroll
+              for (int c = 0; c < 32; ++c) {
+                if (!(m0 >> c & 1)) s0[c] = 0xff800000u;
+                if (!(m1 >> c & 1)) s1[c] = 0xff800000u;
+              }
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 32; c += 2)
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                mx[k] = fmaxf(mx[k], __uint_as_float(s0[c + k]));
+                mx[2 + k] = fmaxf(mx[2 + k], __uint_as_float(s1[c + k]));
+              }
+            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
+            float alpha = 1.f;
+            if (top > ref + kSlack) {
+              alpha = exp2_ftz(ref - top);
+              ref = top;
+            }
+            const float mu = ref == -INFINITY ? 0.f : ref;
+            auto weight = [&](uint32_t w) { return exp2_ftz(fmaf(__uint_as_float(w), scale_log2, -mu)); };
+            float ps = 0.f;
+            uint32_t pk[32];
+#pragma unroll
+            for (int c = 0; c < 32; c += 2) {
+              const uint32_t a0 = pack_bf16x2(weight(s0[c]), weight(s0[c + 1])), a1 = pack_bf16x2(weight(s1[c]), weight(s1[c + 1]));
+              // the sum is that of the rounded weights: where one weight outweighs the others, its rounding cancels
+              ps += (__uint_as_float(a0 << 16) + __uint_as_float(a0 & 0xffff0000u)) + (__uint_as_float(a1 << 16) + __uint_as_float(a1 & 0xffff0000u));
+              pk[c >> 1] = a0;
+              pk[16 + (c >> 1)] = a1;
+            }
+            l = l * alpha + ps;
+            // P in place of the scores: what read this buffer's last P went ahead of them.  Where some row of the warp moved its maximum, its output so
+            // far is scaled once the group's previous product has landed.
+            tmem_st_32x32(tm_s(g, b) + lane_off, pk);
+            if (mine > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+              if (!(ok = warp_wait(pv_full(g, b ^ 1), ((u - 1) >> 1) & 1))) break;
+              tc_fence_after();
+#pragma unroll
+              for (int c0 = 0; c0 < kD; c0 += 32) {
+                uint32_t v[32];
+                tmem_ld_32x32(tm_o(g) + lane_off + c0, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * alpha);
+                tmem_st_32x32(tm_o(g) + lane_off + c0, v);
+              }
+            }
+            tmem_st_wait();
+            tc_fence_before();
+          }
+          ++mine;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_ready(g, b));
+        }
+        if (!ok) break;
+        // ---- the item's rows: gt is the first tile behind them
+        const bool whole = t0 == 0 && take == it.tiles;
+        if (NT == 1) {
+          // both groups' outputs lie in the same lanes: each thread joins half of its row's dimensions
+          const int other = take - mine;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {      // the last one or two tiles' products
+            const int t = gt - 1 - k;
+            if (ok && k < take) ok = warp_wait(pv_full(t & 1, (t >> 1) & 1), (t >> 2) & 1);
+          }
+          if (!ok) break;
+          states[g * kRows + in_tile] = make_float2(ref, l);
+          auto together = [&](int k) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(joined(k));
+            ok = warp_wait(joined(k), item & 1);
+            tc_fence_after();
+          };
+          together(0);
+          if (!ok) break;
+          if (some) {
+            const float2 st = states[(g ^ 1) * kRows + in_tile];
+            const float m = fmaxf(ref, st.x), base = m == -INFINITY ? 0.f : m;
+            const float w_mine = mine ? exp2f(ref - base) : 0.f, w_other = other ? exp2f(st.x - base) : 0.f;
+            const float sum = (mine ? l * w_mine : 0.f) + (other ? st.y * w_other : 0.f);
+            finish<NT>(a, it, tm_o(g) + lane_off, mine, w_mine, tm_o(g ^ 1) + lane_off, other, w_other, 64 * g, 64, valid, token, head_of, m, sum, whole, t0, take, odd_item[item & 1] == item, cta, row);
+          }
+          together(1);             // the next item's products may write over the outputs
+          if (!ok) break;
+        } else {
+          if (!(ok = warp_wait(pv_full(g, (gt - 1) & 1), ((gt - 1) >> 1) & 1))) break;
+          tc_fence_after();
+          if (some) finish<NT>(a, it, tm_o(g) + lane_off, 1, 1.f, 0u, 0, 0.f, 0, kD, valid, token, head_of, ref, l, whole, t0, take, odd_item[item & 1] == item, cta, row);
+          tc_fence_before();
+        }
+        rest -= take;
+        t0 = 0;
+        if (rest > 0) next_item();
+      }
     }
   }
+  if (tid == 0) reinterpret_cast<Cut*>(a.workspace)[cta] = cut;
+  if (!ok) *reinterpret_cast<volatile int*>(error) = 1;
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256 * NT);
+    tmem_dealloc(tmem, 512);
   }
-  if (active == 1) return;
-  // the parts' rows, each by a warp of one of the CTAs: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p
-  __syncwarp();
-  cluster_sync_all();
-  if (ok) {
-    const uint32_t at_joined = smem_u32(joined), at_state = smem_u32(state);
-    for (int row = part + active * warp; row < rows; row += active * kWarps) {
-      float2 st[kMostParts];
-      float m = -INFINITY, sum = 0.f;
+}
+
+// Rows of items that ranges' ends cut: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts, in order.  A warp a row.
+template <int NT>
+__global__ void __launch_bounds__(256)
+tree_attn_join_kernel(const __grid_constant__ b200_tree_attn_args a, int ctas) {
+  griddep_enter();
+  if (static_cast<int>(blockIdx.x) == ctas) {
+    if (blockIdx.y == 0) zero_rest(a);
+    return;
+  }
+  const Cut cut = static_cast<const Cut*>(a.workspace)[blockIdx.x];
+  if (!cut.parts) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.q_heads / a.kv_heads;
+  const float* ws = rows_of(a.workspace, ctas);
+  for (int row = blockIdx.y * 8 + warp; row < cut.rows; row += gridDim.y * 8) {
+    // the item's beginning lies in its range's second place, each other part in its range's first
+    auto part = [&](int p) { return ws + (static_cast<size_t>(2 * (blockIdx.x + p) + (p == 0)) * (NT * kRows) + row) * kLd; };
+    float m = -INFINITY, sum = 0.f;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p0 = 0; p0 < cut.parts; p0 += 8) {
+      float2 st[8];
+      float4 x[8];
+      float top = m;
 #pragma unroll
-      for (int p = 0; p < kMostParts; ++p)
-        if (p < active) {
-          st[p] = peer_float2(mapa_u32(at_state + row * 8, p));
-          m = fmaxf(m, st[p].x);
-        }
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < 8; ++k) {
+        const bool there = p0 + k < cut.parts;
+        st[k] = there ? *reinterpret_cast<const float2*>(part(p0 + k) + kD) : make_float2(-INFINITY, 0.f);
+        x[k] = there ? *reinterpret_cast<const float4*>(part(p0 + k) + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
 #pragma unroll
-      for (int p = 0; p < kMostParts; ++p)
-        if (p < active) {
-          const float w = st[p].x == -INFINITY && st[p].y == 0.f ? 0.f : exp2f(st[p].x - m);      // (a row that sees nothing of this part)
-          const float4 x = peer_float4(mapa_u32(at_joined + (row * kLd + lane * 4) * 4, p));
-          sum = fmaf(st[p].y, w, sum);
-          if (w != 0.f) o = make_float4(fmaf(x.x, w, o.x), fmaf(x.y, w, o.y), fmaf(x.z, w, o.z), fmaf(x.w, w, o.w));
-        }
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      uint2 y;
-      y.x = pack_bf16x2(o.x * inv, o.y * inv);
-      y.y = pack_bf16x2(o.z * inv, o.w * inv);
-      *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + static_cast<size_t>(r.row0 + first + row / group) * a.ldo + (kvh * group + row % group) * kD + lane * 4) = y;
+      for (int k = 0; k < 8; ++k) top = fmaxf(top, st[k].x);
+      const float base = top == -INFINITY ? 0.f : top, old = exp2f(m - base);
+      m = top;
+      sum *= old;
+      y = make_float4(y.x * old, y.y * old, y.z * old, y.w * old);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float w = exp2f(st[k].x - base);
+        sum += w == 0.f && st[k].y == st[k].y ? 0.f : st[k].y * w;
+        if (w != 0.f) y = make_float4(fmaf(x[k].x, w, y.x), fmaf(x[k].y, w, y.y), fmaf(x[k].z, w, y.z), fmaf(x[k].w, w, y.w));
+      }
     }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int token = cut.row0 + row / group;
+    *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + static_cast<size_t>(token) * a.ldo + (cut.kvh * group + row % group) * kD + lane * 4) =
+        make_uint2(pack_bf16x2(y.x * inv, y.y * inv), pack_bf16x2(y.z * inv, y.w * inv));
   }
-  __syncwarp();
-  cluster_sync_all();      // no CTA leaves while its rows are read
 }
 
 template <int NT>
 int launch(const b200_tree_attn_args& a, int* error, cudaStream_t st) {
-  const int group = a.q_heads / a.kv_heads;
+  const int group = a.q_heads / a.kv_heads, ctas = sm_count();
   CUtensorMap tm_q, tm_kv;
   if (int rc = tmap_encode_bf16_3d(&tm_q, a.q, kD, a.q_heads, a.T, kD, a.ldq, 64, group, kRows / group)) return rc;
   if (int rc = tmap_encode_bf16_2d(&tm_kv, a.kv_layer, static_cast<uint64_t>(a.num_pages) * 2 * a.kv_heads * 16, kD, kD, 16, 64, 1)) return rc;
-  const auto kernel = tree_attn_kernel<NT>;
   static std::atomic<unsigned long long> attr_done{0};
-  if (!ensure_dynamic_smem(kernel, Shape<NT>::kSmem, &attr_done)) return -3;
-  const long long blocks = static_cast<long long>((std::min(a.max_tree, a.T) * static_cast<long long>(group) + NT * kRows - 1) / (NT * kRows)) * a.kv_heads;
-  if (blocks > 65535) return -1;
-  // parts of a context: enough CTAs for the SMs, each with four tiles at least where the contexts are as long as that
-  const int most = a.max_ctx > 0 ? std::min(a.max_ctx, a.max_blocks * tree::kPage) : a.max_blocks * tree::kPage;
-  const int tiles = most / kKeys + 1;
-  int parts = 1;
-  while (parts < kMostParts && parts * 8 <= tiles && blocks * a.S * parts < 4ll * Shape<NT>::kCtas * sm_count()) parts *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(parts, static_cast<unsigned>(blocks), a.S + (a.zero_rest ? 1 : 0));
-  cfg.blockDim = dim3(Shape<NT>::kThreads);
-  cfg.dynamicSmemBytes = Shape<NT>::kSmem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = parts;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, tm_q, tm_kv, a, a.scale * 1.4426950408889634f, error) == cudaSuccess ? 0 : -2;
+  if (!ensure_dynamic_smem(tree_attn_kernel<NT>, Shape<NT>::kSmem, &attr_done)) return -3;
+  launch_pdl(tree_attn_kernel<NT>, dim3(ctas), dim3(kThreads), Shape<NT>::kSmem, st, tm_q, tm_kv, a, a.scale * 1.4426950408889634f, error);
+  if (cudaGetLastError() != cudaSuccess) return -2;
+  const int rows = static_cast<int>(std::min(static_cast<long long>(NT * kRows), std::min(a.max_tree, a.T) * static_cast<long long>(group)));
+  launch_pdl(tree_attn_join_kernel<NT>, dim3(ctas + (a.zero_rest ? 1 : 0), (rows + 15) / 16), dim3(256), 0, st, a, ctas);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
+
+// up to 128 rows of a key head: both groups on the same rows
+bool one_tile(const b200_tree_attn_args& a) { return static_cast<long long>(std::min(a.max_tree, a.T)) * (a.q_heads / a.kv_heads) <= kRows; }
 
 }  // namespace
 
-int paged_attention_tree(const b200_tree_attn_args& a, int* error, cudaStream_t st) {
-  const int group = a.q_heads / a.kv_heads;
-  return static_cast<long long>(std::min(a.max_tree, a.T)) * group <= kRows ? launch<1>(a, error, st) : launch<2>(a, error, st);
-}
+int64_t tree_attention_workspace(const b200_tree_attn_args& a) { return sm_count() * (static_cast<int64_t>(sizeof(Cut)) + 2ll * (one_tile(a) ? 1 : 2) * kRows * kLd * sizeof(float)); }
+
+int paged_attention_tree(const b200_tree_attn_args& a, int* error, cudaStream_t st) { return one_tile(a) ? launch<1>(a, error, st) : launch<2>(a, error, st); }
 
 }  // namespace b200

@@ -282,6 +282,9 @@ def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_head
     ld = _rows(at, block_tables, _I32, "block tables", rows=S)
     a = TreeAttnArgs(S, T, q_heads, kv_heads, ldq, ldo, block_tables.shape[1], ld, masks.shape[1] if masks is not None else 0, max_tree, max_ctx, fresh, scale,
                      kv_layer.shape[0], qkv.data_ptr(), out.data_ptr(), kv_layer.data_ptr(), block_tables.data_ptr(), starts.data_ptr(), ctx_lens.data_ptr(), _ptr(masks))
+    a.workspace_bytes = check(lib().b200_op_paged_attn_tree_workspace(C.byref(a)))
+    workspace = torch.empty(a.workspace_bytes, dtype=torch.uint8, device=qkv.device)
+    a.workspace = workspace.data_ptr()
     check(lib().b200_op_paged_attn_tree(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
     return out
 

@@ -52,7 +52,7 @@ def test_maps_refuse(kw, why):
 def attn(**kw):
     from kubeai_b200._lib import TreeAttnArgs
     a = dict(S=2, T=4, q_heads=8, kv_heads=2, ldq=1536, ldo=1024, max_blocks=3, ld_tables=3, words=1, max_tree=4, max_ctx=0, scale=0.1, num_pages=6)
-    return TreeAttnArgs(**(a | {k: P for k in ("q", "out", "kv_layer", "block_tables", "starts", "ctx", "masks")} | kw))
+    return TreeAttnArgs(**(a | {k: P for k in ("q", "out", "kv_layer", "block_tables", "starts", "ctx", "masks", "workspace")} | dict(workspace_bytes=1 << 30) | kw))
 
 
 @pytest.mark.parametrize("kw,why", [
@@ -61,7 +61,8 @@ def attn(**kw):
     (dict(words=0), "1 to 8 words"), (dict(words=9), "1 to 8 words"), (dict(max_tree=33), "than its masks have bits"), (dict(S=65535), "too many"),
     (dict(max_blocks=1 << 27, ld_tables=1 << 27), "32 bits"), (dict(num_pages=1 << 25), "32 bits"), (dict(ldq=1000), "whole heads"), (dict(ldo=1020), "whole heads"), (dict(ldq=1540), "whole heads"),
     (dict(scale=float("nan")), "no number"), (dict(q=P + 8), "aligned"), (dict(out=P + 2), "aligned"), (dict(kv_layer=P + 128), "aligned"), (dict(num_pages=0), "missing"),
-    *((dict([(k, None)]), "missing") for k in ("q", "out", "kv_layer", "block_tables", "starts", "ctx"))])
+    (dict(S=60000, max_blocks=1 << 18, ld_tables=1 << 18), "the tiles of all requests"), (dict(workspace_bytes=1 << 20), "workspace"), (dict(workspace=P + 8), "workspace"),
+    *((dict([(k, None)]), "missing") for k in ("q", "out", "kv_layer", "block_tables", "starts", "ctx", "workspace"))])
 def test_attention_refuses(kw, why):
     refused("b200_op_paged_attn_tree", attn(**kw), why)
 
