@@ -99,7 +99,9 @@ int b200_op_constrain(const b200_constrain_args* a, void* stream) {
   if (!aligned(a->logits, a->logits_f32 ? 4 : 2) || !aligned(a->out, a->out_f32 ? 4 : 2)) return refuse(op, "logits lie off their type's alignment");
   if (a->out == a->logits && (a->ld_out != a->ld || !a->out_f32 != !a->logits_f32)) return refuse(op, "logits kept in place have their type and rows");
   if (int rc = require_device()) return rc;
-  return launched(op, constrain(*a, static_cast<cudaStream_t>(stream)));
+  int* mark = nullptr;
+  if (int rc = op_mark(&mark)) return rc;
+  return launched(op, constrain(*a, mark, static_cast<cudaStream_t>(stream)));
 }
 
 int b200_op_tree_accept(const b200_tree_accept_args* a, void* stream) {

@@ -81,7 +81,7 @@ B200_HD int pages_asked(int ctx, int n, int held, int max_blocks, int words) {
 int step_maps(const b200_step_maps_args& a, cudaStream_t st);
 int64_t tree_attention_workspace(const b200_tree_attn_args& a);
 int paged_attention_tree(const b200_tree_attn_args& a, int* error, cudaStream_t st);      // error: pinned, set where a wait ran out
-int constrain(const b200_constrain_args& a, cudaStream_t st);
+int constrain(const b200_constrain_args& a, int* error, cudaStream_t st);
 int tree_accept(const b200_tree_accept_args& a, cudaStream_t st);
 #endif
 
