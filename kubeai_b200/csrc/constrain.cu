@@ -2,15 +2,16 @@
 //
 //   y = x;  said anywhere: y = y > 0 ? y / rho : y rho;  y -= phi c;  y -= pi where c > 0;  y += bias;  not allowed: -inf;  id = argmax y
 //
-// A vocabulary's rows are long and what is said about single tokens is short.  So a cluster of CTAs shares a row, each with a slice of the vocabulary, and
-// a CTA marks the tokens of its slice that the request's lists name with a bit each.  The bits' running count gives every such token a slot, where its count,
-// its bias and its number lie: as much shared memory as there is to say, whatever the vocabulary.  More tokens than slots: the slice is worked on in pieces
-// that have no more.  All of this is done once for the rows of a request that the cluster takes, while the first rows are on their way: a row's part of the
-// slice comes as one bulk copy, the next row's behind it, so that neither registers nor a thread's order of loads decide what is in flight.
-// A row is then two passes side by side: its vectors from shared memory, of which eight tokens cost a maximum of pairs, marked tokens left out; and the slots,
-// a thread each, which alone need the formula.  A row's drafts are counted in ahead of it and out behind it.
-// The slices' best pairs (value, token) meet through distributed shared memory.  Ties go to the lowest token: every comparison prefers it.
-// Every wait for a copy has a limit; a CTA that gives up sets an error mark.
+// A vocabulary's rows are long and what is said about single tokens is short.  A CTA marks the tokens of its part of the vocabulary that the request's lists
+// name with a bit each.  The bits' running count gives every such token a slot, where its count, its bias and its number lie: as much shared memory as there
+// is to say, whatever the vocabulary.  More tokens than slots: the part is worked on in pieces that have no more.  All of this is done once for the rows of a
+// request that the CTA takes.  A row then comes in chunks of 16 KB by bulk copies, several ahead, from one row into the next; of its vectors eight tokens cost
+// a maximum of pairs, marked tokens left out, and the chunk's slots, a thread each, alone need the formula.  A row's drafts are counted in ahead of it and out
+// behind it.  Few rows: a cluster of CTAs shares the vocabulary, whose best pairs (value, token) meet through distributed shared memory.  Ties go to the lowest token:
+// every comparison prefers it.  Every wait for a copy has a limit; a CTA that gives up sets an error mark.
+//
+// What bounds it: for many rows the copies; for one row each the lists' chain of look-ups, marks and counts ahead of it.  With the formula inside the pass over the
+// vectors, where it ran in nearly every warp for a few of its lanes, and a row over 16 CTAs that all read the lists, 128 rows of 128256 tokens took 99 us.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <limits.h>
@@ -28,9 +29,11 @@
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 256, kMostCtas = 16, kRows = 256, kAhead = 8, kSlots = 2048, kList = 4096, kPlaces = 3;      // kPlaces: CTAs of an SM
-constexpr int kSliceBytes = 32 << 10, kWaitLimit = 1 << 22;
-constexpr int kSaid = 0x8000;      // of a place: not in the prompt
+constexpr int kThreads = 256, kPlaces = 2, kMostCtas = 16, kRows = 256, kAhead = 8, kSlots = 4096;      // kPlaces: CTAs of an SM
+constexpr int kGroup = 32, kTokens = kThreads * kGroup;      // tokens that a thread takes of a chunk, and a chunk's
+template <typename T>
+constexpr int kDepth = sizeof(T) == 2 ? 3 : 2;               // chunks on their way
+constexpr int kMostTokens = 393216, kWaitLimit = 1 << 22;
 constexpr unsigned kPrompt = 0x80000000u, kBiased = 0x40000000u;      // of a count: said in the prompt, which the repetition penalty alone counts; has a bias
 
 __device__ __forceinline__ unsigned long long peer_load(const void* p, unsigned rank) {
@@ -120,37 +123,33 @@ __device__ void no_choice(const b200_constrain_args& a) {
   }
 }
 
-// bytes of one of a row's buffers: a slice from its 16-byte boundary on
-__host__ __device__ constexpr int buffer_bytes(int slice, int size) { return (slice * size + 15) / 16 * 16 + 16; }
-
-// TIn: the logits; TOut: y kept, or None.  slice: tokens of a CTA, a multiple of 32; buffers: rows on their way, 1 or 2.
+// TIn: the logits; TOut: y kept, or None.  part: tokens of a CTA, a multiple of 32.
 template <typename TIn, typename TOut>
 __global__ void __launch_bounds__(kThreads, kPlaces)
-constrain_kernel(const __grid_constant__ b200_constrain_args a, int slice, int buffers, int* error) {
-  constexpr int N = Vec<TIn>::N;
+constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* error) {
+  constexpr int N = Vec<TIn>::N, kWarps = kThreads / 32, kChunk = kTokens * static_cast<int>(sizeof(TIn)), kRing = kDepth<TIn>;
   constexpr unsigned kAll = (1u << N) - 1;
   constexpr bool KEEP = !std::is_same<TOut, None>::value;
   extern __shared__ __align__(16) uint8_t smem[];
-  const int slice_words = slice / 32;
-  uint8_t* buffer = smem;
-  unsigned* known = reinterpret_cast<unsigned*>(smem + buffers * buffer_bytes(slice, sizeof(TIn)));      // [slice_words + 1] the slice's tokens that the lists name
-  unsigned* may = known + slice_words + 1;                             // [slice_words + 1] those that the row's mask allows
-  int* slot_of = reinterpret_cast<int*>(may + slice_words + 1);        // [slice_words] marked tokens in front of each word
+  const int part_words = part / 32;
+  unsigned* known = reinterpret_cast<unsigned*>(smem + kRing * kChunk) + 1;      // [-1 .. part_words] the part's tokens that the lists name
+  int* slot_of = reinterpret_cast<int*>(known + part_words + 1);                  // [part_words] marked tokens in front of each word
   __shared__ unsigned count[kSlots];               // how often the token was said, with the marks above
   __shared__ int entry[kSlots];                    // the last bias entry, then the bias
-  __shared__ uint16_t token[kSlots];               // places in the slice
-  __shared__ uint16_t list[kList];                 // the history's tokens that are the slice's, by their places, with kSaid
+  __shared__ uint16_t token[kSlots];               // places in the part, their low 16 bits: a chunk's first place tells the others
   __shared__ unsigned long long best_of[kRows];
   __shared__ uint4 keep_of[1 << N];                // Vec<TIn>::keep of every set of a vector's tokens
-  __shared__ int sums[kThreads / 32], s_end, listed;
-  __shared__ uint64_t bar[2];
+  __shared__ int sums[kWarps], s_end;
+  __shared__ uint64_t full[kRing], empty[kRing];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = static_cast<int>(cluster_ctarank()), ctas = gridDim.x;
-  const int lo = rank * slice, size = max(0, min(slice, a.V - lo));
+  const int lo = rank * part, size = max(0, min(part, a.V - lo));
   const int s = blockIdx.z, group = blockIdx.y, groups = gridDim.y;
   if (tid == 0) {
-    for (int b = 0; b < 2; ++b) mbar_init(smem_u32(bar + b), 1);
+    for (int b = 0; b < kRing; ++b) {
+      mbar_init(smem_u32(full + b), 1);
+      mbar_init(smem_u32(empty + b), kWarps);
+    }
     fence_mbar_init();
-    listed = 0;
   }
   // ids may be read by a kernel behind this one ahead of its dependency wait: none is let in before the end
   griddep_wait();
@@ -173,79 +172,87 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int slice, int b
   b0 = max(b0, 0), b1 = min(b1, a.bias_len);
   if (group >= rows) return;      // (the whole cluster)
   const int my_rows = (rows - group + groups - 1) / groups;
-  __syncthreads();
-
-  // ---- a row's part of the piece [from, from + tokens) of the slice: its whole 16 bytes by a copy, the others by threads (warp 0)
-  int from = 0, tokens = size, issued = 0;      // copies so far
-  auto skew_of = [&](const TIn* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) / sizeof(TIn) % N); };      // tokens between a 16-byte boundary and p
-  auto row_at = [&](int d) { return static_cast<const TIn*>(a.logits) + static_cast<size_t>(row0 + group + d * groups) * a.ld + lo + from; };
-  auto fetch = [&](int d) {
-    const TIn* p = row_at(d);
-    const int skew = skew_of(p), head = min(tokens, (N - skew) % N), whole = (tokens - head) / N, tail = tokens - head - whole * N;
-    TIn* dst = reinterpret_cast<TIn*>(buffer + (issued % buffers) * buffer_bytes(slice, sizeof(TIn))) + skew;      // of token 0
-    const uint32_t b = smem_u32(bar + issued % buffers);
-    if (lane < head) dst[lane] = p[lane];
-    if (lane < tail) dst[head + whole * N + lane] = p[head + whole * N + lane];
-    if (lane == 0) {
-      mbar_arrive_expect_tx(b, whole * 16);
-      if (whole) bulk_load_1d(smem_u32(dst + head), p + head, whole * 16, b);
-    }
-  };
-  auto fetch_next = [&](int d) {
-    if (warp == 0) fetch(d);
-    ++issued;
-  };
-  for (int d = 0; d < min(buffers, my_rows); ++d) fetch_next(d);
-
-  auto place = [&](int v) { return v >= lo && v < lo + size ? v - lo : -1; };      // in the slice
-
-  // ---- which tokens of the slice the lists name.  The history's are noted down on the way, so that counting them need not look at the others again.  What a
-  // thread takes first of the biases and drafts stays in its registers.
-  int bias_at = -1, draft_at = -1;
-  float bias_value = 0.f;
-  if (b0 + tid < b1) bias_at = a.bias_ids[b0 + tid], bias_value = a.bias_values[b0 + tid];
-  if (a.drafts && tid < rows) draft_at = a.drafts[row0 + tid];
-  int ahead[kAhead];
-  auto look = [&](int base) {
-#pragma unroll
-    for (int e = 0; e < kAhead; ++e) {
-      const int i = base + e * kThreads + tid;
-      ahead[e] = i < h1 ? a.history[i] : -1;
-    }
-  };
-  look(h0);
-  auto mask_word = [&](int d) -> unsigned {      // of the cluster's row d, the one with this thread's draft
-    const int i = group + d * groups;
-    return !a.drafts || i >= rows ? 0u : !a.masks ? (tid <= i ? ~0u : 0u) : (tid >> 5) < a.words ? static_cast<unsigned>(a.masks[static_cast<size_t>(row0 + i) * a.words + (tid >> 5)]) : 0u;
-  };
-  auto allow_of = [&](int d) -> const unsigned* {      // its mask's words of the slice
-    const int i = group + d * groups;
-    if (!a.allow || i >= rows) return nullptr;
-    const int m = a.allow_rows ? a.allow_rows[row0 + i] : row0 + i;
-    return m >= 0 && m < a.allow_count ? reinterpret_cast<const unsigned*>(a.allow) + static_cast<size_t>(m) * a.ld_allow + lo / 32 : nullptr;
-  };
-  for (int w = tid; w <= slice_words; w += kThreads) known[w] = 0, may[w] = ~0u;
+  for (int w = tid; w < part_words + 2; w += kThreads) known[w - 1] = 0;
   for (int d = tid; d < kRows; d += kThreads) best_of[d] = 0;
   for (int d = tid; d < 1 << N; d += kThreads) keep_of[d] = Vec<TIn>::keep(d);
-  bias_at = place(bias_at);
-  draft_at = place(draft_at);
   __syncthreads();
+
+  // ---- the rows' tokens [from, from + tokens) of the part, chunk by chunk: chunk c of a row holds its tokens c * kTokens - skew ..
+  int from = 0, tokens = size;
+  unsigned issued = 0, taken = 0;      // chunks
+  int f_row = 0, f_chunk = 0;          // the next one to be issued
+  auto skew_of = [&](const TIn* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) / sizeof(TIn) % N); };      // tokens between a 16-byte boundary and p
+  auto row_at = [&](int d) { return static_cast<const TIn*>(a.logits) + static_cast<size_t>(row0 + group + d * groups) * a.ld + lo + from; };
+  auto chunks_of = [&](int d) { return (tokens + skew_of(row_at(d)) + kTokens - 1) / (kTokens); };
+  bool ok = true;
+  // warp 0: whole 16 bytes by a copy, a row's ragged ends by threads
+  auto issue = [&] {
+    if (f_row >= my_rows || !tokens) return;
+    const int b = issued % kRing;
+    if (issued >= kRing) ok = mbar_wait_limited(smem_u32(empty + b), (issued / kRing + 1) & 1, kWaitLimit) && ok;
+    const TIn* p = row_at(f_row);
+    const int skew = skew_of(p), first = f_chunk * kTokens - skew;                              // of its tokens
+    const int head = first < 0 ? min(tokens, N - skew) : 0, begin = max(first, 0) + head, end = min(first + kTokens, tokens), whole = max(0, end - begin) / N;
+    TIn* dst = reinterpret_cast<TIn*>(smem + b * kChunk) - first;      // of token 0
+    if (lane < head) dst[lane] = p[lane];
+    if (begin + whole * N + lane < end) dst[begin + whole * N + lane] = p[begin + whole * N + lane];
+    __syncwarp();
+    if (lane == 0) {
+      __threadfence_block();
+      mbar_arrive_expect_tx(smem_u32(full + b), whole * 16);
+      if (whole) bulk_load_1d(smem_u32(dst + begin), p + begin, whole * 16, smem_u32(full + b));
+    }
+    ++issued;
+    if (++f_chunk >= chunks_of(f_row)) f_chunk = 0, ++f_row;
+  };
+  auto arrived = [&] {
+    const unsigned b = taken % kRing;
+    ok = mbar_wait_limited(smem_u32(full + b), taken / kRing & 1, kWaitLimit) && ok;
+    ++taken;
+  };
+  auto left = [&] {      // the warp has read the chunk that arrived last
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(empty + (taken - 1) % kRing));
+  };
+  int early = 0;
+  for (int d = 0; d < my_rows && early < kRing && tokens; ++d) early = min(kRing, early + chunks_of(d));
+  if (warp == 0)
+    for (int k = 0; k < kRing; ++k) issue();
+
+  // ---- which tokens of the part the lists name.  What a thread takes first of the biases and drafts stays in its registers.
+  auto place = [&](int v) { return v >= lo && v < lo + size ? v - lo : -1; };      // in the part
   auto know = [&](int k) {
     if (k >= 0) atomicOr(known + (k >> 5), 1u << (k & 31));
   };
   auto history = [&](auto f) {      // f(place, said in the prompt)
     for (int base = h0; base < h1; base += kAhead * kThreads) {
+      int v[kAhead];
 #pragma unroll
-      for (int e = 0; e < kAhead; ++e) f(place(ahead[e]), base + e * kThreads + tid - h0 < prompt);
-      if (base + kAhead * kThreads < h1) look(base + kAhead * kThreads);
+      for (int e = 0; e < kAhead; ++e) {
+        const int i = base + e * kThreads + tid;
+        v[e] = i < h1 ? a.history[i] : -1;
+      }
+#pragma unroll
+      for (int e = 0; e < kAhead; ++e) f(place(v[e]), base + e * kThreads + tid - h0 < prompt);
     }
   };
-  history([&](int k, bool in_prompt) {
-    if (k < 0) return;
-    const int at = atomicAdd(&listed, 1);
-    if (at < kList) list[at] = static_cast<uint16_t>(k | (in_prompt ? 0 : kSaid));
-    know(k);
-  });
+  int bias_at = -1, draft_at = -1;
+  float bias_value = 0.f;
+  if (b0 + tid < b1) bias_at = a.bias_ids[b0 + tid], bias_value = a.bias_values[b0 + tid];
+  if (a.drafts && tid < rows) draft_at = a.drafts[row0 + tid];
+  auto mask_word = [&](int d) -> unsigned {      // of row d of this CTA's, the one with this thread's draft
+    const int i = group + d * groups;
+    return !a.drafts || i >= rows ? 0u : !a.masks ? (tid <= i ? ~0u : 0u) : (tid >> 5) < a.words ? static_cast<unsigned>(a.masks[static_cast<size_t>(row0 + i) * a.words + (tid >> 5)]) : 0u;
+  };
+  auto allow_of = [&](int d) -> const unsigned* {      // its mask's words of the part
+    const int i = group + d * groups;
+    if (!a.allow || i >= rows) return nullptr;
+    const int m = a.allow_rows ? a.allow_rows[row0 + i] : row0 + i;
+    return m >= 0 && m < a.allow_count ? reinterpret_cast<const unsigned*>(a.allow) + static_cast<size_t>(m) * a.ld_allow + lo / 32 : nullptr;
+  };
+  history([&](int k, bool) { know(k); });
+  bias_at = place(bias_at);
+  draft_at = place(draft_at);
   know(bias_at);
   for (int i = b0 + kThreads + tid; i < b1; i += kThreads) know(place(a.bias_ids[i]));
   know(draft_at);
@@ -253,7 +260,7 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int slice, int b
     for (int i = kThreads + tid; i < rows; i += kThreads) know(place(a.drafts[row0 + i]));
   __syncthreads();
   // slots: a thread sums some words, one behind the other
-  const int per = (slice_words + kThreads - 1) / kThreads, w_begin = min(slice_words, tid * per), w_end = min(slice_words, w_begin + per);
+  const int per = (part_words + kThreads - 1) / kThreads, w_begin = min(part_words, tid * per), w_end = min(part_words, w_begin + per);
   int before = 0;
   for (int w = w_begin; w < w_end; ++w) before += __popc(known[w]);
   const int own = before;
@@ -267,7 +274,7 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int slice, int b
   int marked = 0;
   before -= own;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < kWarps; ++w) {
     if (w < warp) before += sums[w];
     marked += sums[w];
   }
@@ -277,35 +284,33 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int slice, int b
   }
   __syncthreads();
 
-  bool ok = true;
-  int taken = 0;                     // copies waited for
-  auto arrived = [&] {
-    const bool here = mbar_wait_limited(smem_u32(bar + taken % buffers), (taken / buffers) & 1, kWaitLimit);
-    ++taken;
-    ok = ok && here;
-  };
-  bool first_piece = true;
-  for (int word0 = 0; word0 < slice_words && 32 * word0 < size;) {
+  for (int word0 = 0; 32 * word0 < size;) {
     // ---- the next piece: words that mark kSlots tokens at most (a word marks 32)
-    int word1 = slice_words;
+    int word1 = part_words;
     const int slot0 = slot_of[word0];
     if (marked - slot0 > kSlots) {
       if (tid == 0) s_end = word0 + 1;
       __syncthreads();
-      for (int w = word0 + 1 + tid; w < slice_words; w += kThreads)
+      for (int w = word0 + 1 + tid; w < part_words; w += kThreads)
         if (slot_of[w] - slot0 <= kSlots) atomicMax(&s_end, w);      // it may end in front of word w
       __syncthreads();
       word1 = s_end;
     }
-    const int slots = (word1 < slice_words ? slot_of[word1] : marked) - slot0;
-    if (!first_piece || word1 < slice_words) {      // the rows' first copies were of a slice in one piece
-      while (taken < issued) arrived();
+    const int slots = (word1 < part_words ? slot_of[word1] : marked) - slot0;
+    if (word0 || word1 < part_words) {
+      // the first chunks on their way are those of a part in one piece: they are let by
+      if (!word0)
+        for (int k = 0; k < early; ++k) {
+          arrived();
+          left();
+        }
       __syncthreads();
       from = 32 * word0;
       tokens = min(32 * word1, size) - from;
-      for (int d = 0; d < min(buffers, my_rows); ++d) fetch_next(d);
+      f_row = f_chunk = 0;
+      if (warp == 0)
+        for (int k = 0; k < kRing; ++k) issue();
     }
-    first_piece = false;
     auto slot = [&](int k) {        // of a marked token's place; -1 where it is not this piece's
       const int w = k >> 5;
       return k >= 0 && w >= word0 && w < word1 ? slot_of[w] - slot0 + __popc(known[w] & ((1u << (k & 31)) - 1)) : -1;
@@ -316,18 +321,12 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int slice, int b
       for (unsigned bits = known[w]; bits; bits &= bits - 1) token[n++] = static_cast<uint16_t>(32 * w + __ffs(bits) - 1);
     }
     __syncthreads();
-    auto counted = [&](int k, bool in_prompt) {
+    history([&](int k, bool in_prompt) {
       const int i = slot(k);
       if (i < 0) return;
       if (in_prompt) atomicOr(count + i, kPrompt);
       else atomicAdd(count + i, 1u);
-    };
-    if (listed <= kList)
-      for (int i = tid; i < listed; i += kThreads) counted(list[i] & (kSaid - 1), !(list[i] & kSaid));
-    else {
-      look(h0);
-      history(counted);
-    }
+    });
     const int bias_slot = slot(bias_at), draft_slot = slot(draft_at);
     if (bias_slot >= 0) atomicMax(entry + bias_slot, b0 + tid);
     for (int e = b0 + kThreads + tid; e < b1; e += kThreads) {
@@ -359,134 +358,155 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int slice, int b
         if (k >= 0) atomicAdd(count + k, by);
       }
     };
+    __syncthreads();
 
     // ---- the rows
     const unsigned* allow = allow_of(0);
+    const int allow_words = (a.V - lo - from + 31) / 32;      // from the piece's first on
     for (int d = 0; d < my_rows; ++d) {
-      const int row = row0 + group + d * groups;
-      const TIn* x = row_at(d);
+      const int i = group + d * groups, skew = skew_of(row_at(d)), chunks = chunks_of(d);
       TOut* out = nullptr;
-      if constexpr (KEEP) out = static_cast<TOut*>(a.out) + static_cast<size_t>(row) * a.ld_out + lo;
-      const bool masked = allow != nullptr;
-      if (a.allow)
-        for (int w = word0 + tid; w < word1 && 32 * w < size; w += kThreads) may[w] = masked ? allow[w] : ~0u;
+      if constexpr (KEEP) out = static_cast<TOut*>(a.out) + static_cast<size_t>(row0 + i) * a.ld_out + lo + from;
+      const unsigned *may = allow ? allow + word0 : nullptr, *marks = known + word0;
       const unsigned next_leads = mask_word(d + 1);
       allow = allow_of(d + 1);
-      if (a.drafts) drafted(row - row0, 1u);
-      arrived();
-      __syncthreads();
-      // Vectors as they lie in memory: number n holds the piece's tokens n * N - skew ..  Of the best one so far only where it is and which of its tokens count is
-      // kept; which of them it was, is seen at the end.
-      const int skew = skew_of(x), vectors = (tokens + skew + N - 1) / N, shift_of = (N - skew) % N;
-      const uint4* row_vectors = reinterpret_cast<const uint4*>(buffer + ((taken - 1) % buffers) * buffer_bytes(slice, sizeof(TIn)));
-      const uint8_t *known_bytes = reinterpret_cast<const uint8_t*>(known + word0), *may_bytes = reinterpret_cast<const uint8_t*>(may + word0);
-      float best = -INFINITY;
-      int at = -1;
+      if (a.drafts) {
+        drafted(i, 1u);
+        __syncthreads();
+      }
+      float best = -INFINITY, at_best = -INFINITY;
+      int id = -1, at = 0;               // the best marked token; of the others the best one's vector: its first token's place in the piece, and which of them count
       unsigned at_plain = 0;
-      auto take = [&](int n, unsigned inside, unsigned allowed, unsigned marks) {
-        const uint4 u = row_vectors[n];
-        const unsigned fine = inside & allowed, plain = fine & ~marks;
-        if constexpr (KEEP) {
-          float z[N];
-#pragma unroll
-          for (int j = 0; j < N; ++j) z[j] = fine >> j & 1 ? Vec<TIn>::get(u, j) : -INFINITY;
-          store_all<N>(out + from + n * N - skew, z, inside & ~marks);
-        }
-        const float m = Vec<TIn>::largest(u, keep_of[plain]);
-        if (m > best || (at < 0 && plain)) {
-          best = m != m ? -INFINITY : m;
-          at = n;
-          at_plain = plain;
-        }
+      // the masks of a thread's group, looked up a chunk ahead
+      unsigned next0 = ~0u, next1 = ~0u;
+      auto look_ahead = [&](int k) {
+        const int w = k >> 5;              // (-1 where the first group begins ahead of the piece)
+        next0 = next1 = ~0u;
+        if (!may || k >= tokens) return;
+        if (w >= 0) next0 = may[w];
+        if (skew && w + 1 < allow_words) next1 = may[w + 1];
       };
-      if (!skew) {
-        const int whole = tokens / N;
-#pragma unroll 4
-        for (int n = tid; n < whole; n += kThreads) {
-          const int shift = n * N & 7;
-          take(n, kAll, may_bytes[n * N / 8] >> shift, known_bytes[n * N / 8] >> shift);
+      look_ahead(tid * kGroup - skew);
+      for (int c = 0; c < chunks; ++c) {
+        const int first = c * kTokens - skew, k0 = first + tid * kGroup;      // of the chunk's tokens; of this thread's
+        const unsigned may0 = next0, may1 = next1;
+        look_ahead(k0 + kTokens);
+        // the chunk's slots: those of its tokens, in order
+        const int t0 = max(first, 0), t1 = min(first + kTokens, tokens);
+        auto slots_ahead = [&](int k) { return k >= tokens ? slots : slot_of[word0 + (k >> 5)] - slot0 + __popc(marks[k >> 5] & ((1u << (k & 31)) - 1)); };
+        const int slot_begin = slots_ahead(t0), slot_end = slots_ahead(t1);
+        // a thread's first one, from the last warp on, as warp 0 has chunks to issue
+        const int mine = slot_begin + kThreads - 1 - tid;
+        auto place_of = [&](int n) { return t0 + ((token[n] - (from + t0)) & 0xffff); };      // in the piece
+        const int place0 = mine < slot_end ? place_of(mine) : 0;
+        unsigned may_first = ~0u;
+        if (may && mine < slot_end) may_first = may[place0 >> 5];
+        arrived();
+        const uint4* vectors = reinterpret_cast<const uint4*>(smem + (taken - 1) % kRing * kChunk);
+        // a thread's group's bits, then its warp's vectors in the order of memory, each with the bits of the group that it belongs to
+        unsigned fine = 0, own = 0, plain = 0;      // allowed ones, ones to be written here, ones that are neither marked nor forbidden
+        if (k0 < tokens) {
+          const int w = k0 >> 5, over = k0 + kGroup - tokens;
+          const unsigned inside = (k0 < 0 ? ~0u << -k0 : ~0u) & (over > 0 ? ~0u >> over : ~0u);
+          fine = inside & __funnelshift_r(may0, may1, k0 & 31);
+          own = inside & ~__funnelshift_r(marks[w], skew ? marks[w + 1] : 0u, k0 & 31);
+          plain = fine & own;
         }
-        if (whole < vectors && tid == kThreads - 1) take(whole, (1u << (tokens - whole * N)) - 1, may_bytes[whole * N / 8] >> (whole * N & 7), known_bytes[whole * N / 8] >> (whole * N & 7));
-      } else {
-        // the first vector begins ahead of the piece: bits from its token 0 on, moved up; the others N - skew + (n - 1) * N tokens in
-#pragma unroll 4
-        for (int n = tid; n < vectors; n += kThreads) {
-          const int k = n ? shift_of + (n - 1) * N : 0, w = word0 + (k >> 5);
-          const unsigned m = __funnelshift_r(may[w], may[w + 1], k & 31), b = __funnelshift_r(known[w], known[w + 1], k & 31);
-          const int up = n ? 0 : skew, over = n * N - skew + N - tokens;
-          take(n, kAll & kAll << up & (over > 0 ? kAll >> over : kAll), m << up, b << up);
-        }
-      }
-      int id = -1;
-      if (at >= 0) {
-        const uint4 u = row_vectors[at];
+        constexpr int kOwn = kGroup / N;
 #pragma unroll
-        for (int j = N - 1; j >= 0; --j)
-          if ((at_plain >> j & 1) && (Vec<TIn>::get(u, j) == best || best == -INFINITY)) id = lo + from + at * N - skew + j;      // (no value above -inf: the first token will do)
-      }
-      // marked tokens
-      const TIn* row_tokens = reinterpret_cast<const TIn*>(row_vectors) + skew - from;
-      for (int i = tid; i < slots; i += kThreads) {
-        const int k = token[i];
-        const bool allowed = may[k >> 5] >> (k & 31) & 1;
-        if (!KEEP && !allowed) continue;
-        const unsigned c = count[i], n = c & ~(kPrompt | kBiased);
-        float z = Vec<TIn>::value(row_tokens[k]);
-        if (c & ~kBiased) z = z > 0.f ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
-        z = __fsub_rn(z, __fmul_rn(phi, static_cast<float>(n)));
-        if (n) z = __fsub_rn(z, pi);
-        if (c & kBiased) z = __fadd_rn(z, __int_as_float(entry[i]));
-        if constexpr (KEEP) store_one(out + k, allowed ? z : -INFINITY);
-        if (z != z) z = -INFINITY;
-        if (allowed && (z > best || id < 0 || (z == best && lo + k < id))) {
-          best = z;
-          id = lo + k;
+        for (int e = 0; e < kOwn; ++e) {
+          const int v = e * 32 + lane, shift = v % kOwn * N, k = first + (warp * 32 * kOwn + v) * N;
+          const uint4 u = vectors[warp * 32 * kOwn + v];
+          const unsigned here = __shfl_sync(0xffffffffu, plain, v / kOwn) >> shift & kAll;
+          if constexpr (KEEP) {
+            const unsigned shown = __shfl_sync(0xffffffffu, fine, v / kOwn) >> shift, written = __shfl_sync(0xffffffffu, own, v / kOwn) >> shift & kAll;
+            float z[N];
+#pragma unroll
+            for (int j = 0; j < N; ++j) z[j] = shown >> j & 1 ? Vec<TIn>::get(u, j) : -INFINITY;
+            if (written) store_all<N>(out + k, z, written);
+          }
+          const float top = Vec<TIn>::largest(u, keep_of[here]);
+          if (top > at_best || (!at_plain && here)) {
+            at_best = top != top ? -INFINITY : top;
+            at = k;
+            at_plain = here;
+          }
         }
+        for (int n = mine; n < slot_end; n += kThreads) {
+          const int k = n == mine ? place0 : place_of(n), v = k + from;
+          const bool allowed = (n == mine || !may ? may_first : may[k >> 5]) >> (k & 31) & 1;
+          const unsigned said = count[n], times = said & ~(kPrompt | kBiased);
+          float z = Vec<TIn>::value(reinterpret_cast<const TIn*>(vectors)[k - first]);
+          if (said & ~kBiased) z = z > 0.f ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
+          z = __fsub_rn(z, __fmul_rn(phi, static_cast<float>(times)));
+          if (times) z = __fsub_rn(z, pi);
+          if (said & kBiased) z = __fadd_rn(z, __int_as_float(entry[n]));
+          if constexpr (KEEP) store_one(out + k, allowed ? z : -INFINITY);
+          if (z != z) z = -INFINITY;
+          if (allowed && (z > best || id < 0)) best = z, id = lo + v;      // (a thread's slots ascend)
+        }
+        left();
+        if (warp == 0) issue();
       }
+      // which token of its vector the best other one is: the first of that value, or the first at all where none is above -inf.  The warp's best ones look.
+      __syncwarp();
+      const unsigned other = at_plain ? ordered(at_best, 0) : 0u, most = __reduce_max_sync(0xffffffffu, other);
+      if (other && other == most && (id < 0 || at_best >= best)) {
+        const TIn* x = row_at(d) + at;
+        int found = 0;
+        for (unsigned bits = at_plain; bits; bits &= bits - 1) {
+          found = __ffs(bits) - 1;
+          if (at_best == -INFINITY || Vec<TIn>::value(x[found]) == at_best) break;
+        }
+        found += lo + from + at;
+        if (id < 0 || at_best > best || found < id) best = at_best, id = found;
+      }
+      __syncwarp();
       // the warp's best: the largest value, then its lowest token
       const unsigned value = ordered(best, id), top = __reduce_max_sync(0xffffffffu, value);
       const unsigned lowest = __reduce_min_sync(0xffffffffu, value == top ? static_cast<unsigned>(id) : ~0u);
       if (lane == 0 && top) atomicMax(best_of + d, static_cast<unsigned long long>(top) << 32 | (INT_MAX - lowest));
-      __syncthreads();      // the row and the counts have been read
-      if (d + buffers < my_rows) fetch_next(d + buffers);
-      if (a.drafts) drafted(row - row0, ~0u);
+      if (a.drafts) {
+        __syncthreads();      // the counts have been read
+        drafted(i, ~0u);
+      }
       leads = next_leads;
     }
     __syncthreads();
     word0 = word1;
   }
-  while (taken < issued) arrived();      // (a slice without tokens)
   if (!ok) *reinterpret_cast<volatile int*>(error) = 1;
 
-  // ---- the slices' best of each row
+  // ---- the parts' best of each row
   if (!a.ids) return;
-  __syncwarp();
-  cluster_sync_all();
+  __syncthreads();
+  if (ctas > 1) cluster_sync_all();
   for (int d = rank + ctas * tid; d < my_rows; d += ctas * kThreads) {
-    unsigned long long b = 0;
-    for (int c = 0; c < ctas; ++c) b = max(b, peer_load(best_of + d, c));
+    unsigned long long b = best_of[d];
+    for (int c = 0; c < ctas; ++c)
+      if (c != rank) b = max(b, peer_load(best_of + d, c));
     a.ids[row0 + group + d * groups] = b ? INT_MAX - static_cast<int>(static_cast<unsigned>(b)) : -1;
   }
   __syncwarp();
-  cluster_sync_all();      // no CTA leaves while its best are read
+  if (ctas > 1) cluster_sync_all();      // no CTA leaves while its best are read
 }
 
 template <typename TIn, typename TOut>
 int launch(const b200_constrain_args& a, int* error, cudaStream_t st) {
   const auto kernel = constrain_kernel<TIn, TOut>;
-  // CTAs of a row: slices of 32 KB; where few rows leave SMs idle, smaller ones.  Two rows on their way where a cluster takes several.
-  const long long sms = sm_count();
-  int ctas = 1;
-  while (ctas < kMostCtas && (static_cast<long long>(a.V) * sizeof(TIn) > static_cast<long long>(ctas) * kSliceBytes || (ctas * static_cast<long long>(a.S) < sms && a.V > 4096 * ctas))) ctas *= 2;
-  // groups of a request's rows: three CTAs for each of an SM's two places, or a row a group
-  const long long clusters = (6 * sms + ctas - 1) / ctas;
-  const int groups = !a.starts ? 1 : static_cast<int>(std::max<long long>((a.T + kRows - 1) / kRows, std::min<long long>((a.T + a.S - 1) / a.S, (clusters + a.S - 1) / a.S)));
+  // A request has one row: as many CTAs as the SMs have places, a row over several of them where that leaves some free (128 rows of 128256 tokens: 27.8 us
+  // over two, 37 over one, 38 over four; one row 8.5 us over 16, 27 over one).  Several rows: their numbers differ, and most groups of a row end at once, so four
+  // times that (16 trees of up to 32 rows of 99991 fp32 logits: 85 us over four CTAs, 99 over one, 104 over two).  More rows than that: groups of several,
+  // which read their request's lists once.
+  const long long places = static_cast<long long>(kPlaces) * sm_count(), each = a.starts ? (a.T + a.S - 1) / a.S : 1;
+  const int groups = static_cast<int>(std::max<long long>((a.T + kRows - 1) / kRows, a.S * each <= places ? each : std::min(each, (3 * places + a.S - 1) / a.S)));
   if (groups > 65535) return -1;
-  const int slice = ((a.V + ctas - 1) / ctas + 31) / 32 * 32;
-  const int buffers = a.starts && a.T > a.S && 2 * buffer_bytes(slice, sizeof(TIn)) <= 2 * kSliceBytes + 32 ? 2 : 1;
-  const size_t smem = static_cast<size_t>(buffers) * buffer_bytes(slice, sizeof(TIn)) + (3 * static_cast<size_t>(slice / 32) + 2) * 4;
+  int ctas = 1;
+  while (ctas < kMostCtas && 2ll * ctas * a.S * groups <= (each > 1 ? 4 : 1) * places && a.V > 4096 * ctas) ctas *= 2;
+  const int part = ((a.V + ctas - 1) / ctas + 31) / 32 * 32;
+  const size_t smem = kDepth<TIn> * kTokens * static_cast<int>(sizeof(TIn)) + (2 * static_cast<size_t>(part / 32) + 2) * 4;
   static std::atomic<unsigned long long> attr_done{0}, wide_done{0};
-  if (!ensure_dynamic_smem(kernel, 192 << 10, &attr_done)) return -3;
+  if (!ensure_dynamic_smem(kernel, kDepth<TIn> * kTokens * static_cast<int>(sizeof(TIn)) + (2 * (kMostTokens / 32) + 2) * 4, &attr_done)) return -3;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return -3;
   if (!(wide_done.load() >> (dev & 63) & 1)) {
@@ -499,14 +519,14 @@ int launch(const b200_constrain_args& a, int* error, cudaStream_t st) {
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = ctas;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = pdl_enabled() ? attr : attr + 1;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, kernel, a, slice, buffers, error) == cudaSuccess ? 0 : -2;
+  return cudaLaunchKernelEx(&cfg, kernel, a, part, error) == cudaSuccess ? 0 : -2;
 }
 
 }  // namespace
