@@ -45,7 +45,7 @@ static int attn_sizes(const b200_tree_attn_args* a, const char* op) {
   if (static_cast<int64_t>(a->q_heads) * 128 > a->ldq || static_cast<int64_t>(a->q_heads) * 128 > a->ldo || a->ldq % 8 || a->ldo % 8) return refuse(op, "rows of q and out are whole heads, a multiple of 8 apart");
   if (!(a->scale == a->scale)) return refuse(op, "scale is no number");
   const long long rows = static_cast<long long>(a->max_tree < a->T ? a->max_tree : a->T) * group;
-  if ((rows + 127) / 128 * a->kv_heads > INT_MAX / (a->S + 1ll) / (a->max_blocks / 4 + 1)) return refuse(op, "the tiles of all requests pass 32 bits");
+  if ((rows + 127) / 128 * a->kv_heads > INT_MAX / 4 / (a->S + 1ll) / (a->max_blocks / 4 + 1)) return refuse(op, "the tiles of all requests pass 32 bits");
   return 0;
 }
 

@@ -3,17 +3,17 @@
 //   out_t = sum_j softmax_j(scale q_t . k_j) v_j   over j < ctx and those j = ctx + i whose bit i the row's mask has
 //
 // A request's rows share all keys but the last few, so what counts is that K and V pass once for all rows of a key head and that nothing stops the stream
-// of pages.  An item is a request's key head and up to 128 * NT of its rows (row = token * group + head); its keys come in tiles of 64.  All items' tiles
-// one behind the other are cut into as many equal ranges as there are SMs, and a CTA an SM walks its range without a gap:
-//   two warps look pages up (32 of the table at a time, the next ones ahead) and load by TMA, 128-byte swizzle, into rings, one queries and keys, one
-//   values: a box of 2 KB takes its warp 85 cycles, and 16 of them for a tile left the memory waiting;
-//   two warps issue tcgen05.mma, one S = Q K^T (M = 128, N = 64), one O += P V (M = 128, N = 128, P in TMEM over its scores): a wait that is over costs
-//   its warp 100 cycles all the same, and one warp for both took 1500 a tile of which the tensor cores need 640;
-//   two groups of four warps (thread = row) do the softmax in fp32, base 2.  Up to 128 rows (NT = 1) the groups take tiles in turn, each with a maximum,
-//   sum and output of its own, and join them at the item's end; beyond (NT = 2) each has 128 rows and both take every tile.
-// The loads run into the next item while the groups finish one.  The masks' bits are looked at only in tiles that reach behind the context.  There the
-// products' warp also clears what must not meet a weight of zero: values behind the last key, and infinities and NaN among the drafts' values, which the
-// rows that see them add at the end by themselves.
+// of pages.  An item is a request's key head and up to 128 of its rows (row = token * group + head); its keys come in tiles of 64.  All items' tiles one behind the
+// other are cut into as many equal ranges as the SMs have places for CTAs, two each, and a CTA walks its range without a gap:
+//   one warp looks pages up (32 of the table at a time, the next ones ahead) and loads queries and tiles by TMA, 128-byte swizzle, into rings;
+//   two warps issue tcgen05.mma, one S = Q K^T (M = 128, N = 64, two buffers), one O += P V (M = 128, N = 128, P in TMEM over its scores): a wait that is over
+//   costs its warp 100 cycles all the same, and one warp for both took 1500 a tile of which the tensor cores need 640;
+//   four warps (thread = row) do the softmax in fp32, base 2; a warp whose rows nobody owns only keeps step.
+// While one CTA of an SM ends an item, the other one keeps the memory busy.  (One CTA an SM with two softmax groups that took a row tile's keys in turn, or a row
+// tile each, stopped for 3 us at each item: 64 x 2048 74.8 us, 48 x 1999 with 64 rows 90.)  More than 128 rows: items side by side, which find each other's
+// pages in L2.
+// The masks' bits are looked at only in tiles that reach behind the context.  There the products' warp also clears what must not meet a weight of zero:
+// values behind the last key, and infinities and NaN among the drafts' values, which the rows that see them add at the end by themselves.
 // An item that a range's end cuts leaves unnormalised rows in the workspace, which a second kernel joins in a fixed order: the same bits every time.
 // Every wait has a limit; a CTA that gives up sets an error mark and still meets at the end.
 #include <cuda.h>
@@ -36,21 +36,17 @@ namespace {
 typedef __nv_bfloat16 bf16;
 constexpr int kD = 128, kRows = 128, kKeys = 64;
 constexpr int kQSlab = kRows * 128, kSlab = kKeys * 128, kTile = 2 * kSlab;      // bytes: 64 columns of a row tile, of a key tile, a key tile
-constexpr int kThreads = 384, kWarps = kThreads / 32;
+constexpr int kThreads = 224, kWarps = kThreads / 32, kPlaces = 2;                // kPlaces: CTAs of an SM
+constexpr int kDepth = 2;                  // tiles of keys, and of values, on their way
 constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
 constexpr int kSnap = 2;                   // a range does not end within this many tiles of an item's ends
 constexpr int kLeast = 2;                  // tiles of a range at least
 constexpr float kSlack = 8.f;              // by which a row's maximum may pass what its weights are relative to, in units of log 2
 constexpr int kWaitLimit = 1 << 22;
 
-template <int NT>
-struct Shape {
-  static constexpr int kK = NT == 1 ? 4 : 3, kV = NT == 1 ? 5 : 3;      // tiles of keys and of values in flight
-  static constexpr int kKeysAt = 2 * NT * 2 * kQSlab, kValuesAt = kKeysAt + kK * kTile, kBars = kValuesAt + kV * kTile;
-  static constexpr int kStates = kBars + 512;                            // NT = 1: maximum and sum of each group's rows
-  static constexpr int kSmem = 1024 + kStates + (NT == 1 ? 2 * kRows * 8 : 0);
-  static_assert(kSmem <= 227 * 1024, "");
-};
+// shared memory: queries, keys, values, 2 KB a softmax warp for its way out, barriers
+constexpr int kKeysAt = 2 * kQSlab, kValuesAt = kKeysAt + kDepth * kTile, kStageAt = kValuesAt + kDepth * kTile, kBars = kStageAt + 4 * 2048, kSmem = 1024 + kBars + 256;
+static_assert(kPlaces * (kSmem + 1024 + 128) <= 228 * 1024, "");
 
 __device__ __forceinline__ uint32_t idesc_bf16(uint32_t m, uint32_t n, uint32_t b_mn) {
   return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
@@ -66,7 +62,7 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst_smem, const void* tmap,
                ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
                : "memory");
 }
-__device__ __forceinline__ bool odd_pair(uint32_t u) { return (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u; }      // an infinity or NaN among two bf16
+// two bf16 without infinities and NaN
 __device__ __forceinline__ uint32_t without_odd(uint32_t u) { return ((u & 0x7f80u) == 0x7f80u ? 0u : u & 0xffffu) | ((u & 0x7f800000u) == 0x7f800000u ? 0u : u & 0xffff0000u); }
 
 // Which of the rows j .. j + 31 of its request row i sees (j may be negative: tokens of the context, all seen)
@@ -112,13 +108,13 @@ struct Item {
   int first, nb, kv_end, tiles;   // the block's tokens, keys that they may see
 };
 
-__device__ __forceinline__ int block_tokens(const b200_tree_attn_args& a, int NT) { return NT * kRows / (a.q_heads / a.kv_heads); }
+__device__ __forceinline__ int block_tokens(const b200_tree_attn_args& a) { return kRows / (a.q_heads / a.kv_heads); }
 __device__ __forceinline__ int tiles_of(const b200_tree_attn_args& a, const tree::Request& r, int bt, int block) {
   const int seen = a.masks ? r.rows : min(r.rows, (block + 1) * bt);
   return (r.ctx + seen + kKeys - 1) / kKeys;
 }
 __device__ __forceinline__ int blocks_of(const tree::Request& r, int bt) { return (r.rows + bt - 1) / bt; }
-// tiles of all of a key head's blocks
+// of all blocks of a key head
 __device__ __forceinline__ int head_tiles(const b200_tree_attn_args& a, const tree::Request& r, int bt) {
   const int blocks = blocks_of(r, bt);
   if (a.masks || blocks <= 1) return blocks ? blocks * tiles_of(a, r, bt, 0) : 0;
@@ -155,86 +151,101 @@ struct Cut {
 // The workspace: a Cut and two parts' rows for every CTA
 __host__ __device__ __forceinline__ float* rows_of(void* workspace, int ctas) { return reinterpret_cast<float*>(static_cast<Cut*>(workspace) + ctas); }
 
-// A row's dimensions [c_begin, c_begin + columns) = w_a o_a + w_b o_b: normalised to the output where the item is whole, else to the workspace with its
-// maximum m (units of log 2) and sum.
-template <int NT>
-__device__ __forceinline__ void finish(const b200_tree_attn_args& a, const Item& it, uint32_t o_a, int has_a, float w_a, uint32_t o_b, int has_b, float w_b, int c_begin, int columns,
-                                       bool valid, int token, int head, float m, float sum, bool whole, int t0, int take, bool odd, int cta, int row) {
-  const int group = a.q_heads / a.kv_heads;
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  bf16* dst = static_cast<bf16*>(a.out) + static_cast<size_t>(it.r.row0 + token) * a.ldo + (it.kvh * group + head) * kD;
-  float* part = rows_of(a.workspace, gridDim.x) + (static_cast<size_t>(2 * cta + (t0 == 0)) * (NT * kRows) + row) * kLd;      // a part without the item's beginning is the range's first
-  for (int c0 = c_begin; c0 < c_begin + columns; c0 += 32) {
-    uint32_t v[32];
-    if (has_a) {
-      tmem_ld_32x32(o_a + c0, v);
+// Infinities and NaN of the drafts that a row sees, which stayed out of the products, to its dimensions c1 ..
+__device__ __noinline__ void add_odd(const b200_tree_attn_args& a, const Item it, int t0, int take, int c1, int token, uint32_t* v) {
+  const int* table = a.block_tables + static_cast<size_t>(it.s) * a.ld_tables;
+  const int* mask = a.masks ? a.masks + static_cast<size_t>(it.r.row0 + it.first + token) * a.words : nullptr;
+  for (int p = max(it.r.ctx, t0 * kKeys); p < min(it.kv_end, (t0 + take) * kKeys); ++p) {
+    if (!(seen_bits(mask, a.words, it.first + token, it.r.rows, p - it.r.ctx) & 1)) continue;
+    const long long at = tree::cache_row(table, p, a.num_pages);
+    if (at < 0) continue;
+    const bf16* value = static_cast<const bf16*>(a.kv_layer) + ((((at >> 4) * 2 + 1) * a.kv_heads + it.kvh) * 16 + (at & 15)) * kD + c1;
+    for (int c = 0; c < 32; ++c) {
+      const float x = __bfloat162float(value[c]);
+      if (!isfinite(x)) v[c] = __float_as_uint(__uint_as_float(v[c]) + x);
+    }
+  }
+}
+
+// A warp's rows of an item on their way out: 32 rows of 64 bytes at a time lie in shared memory and leave it as whole sectors (a lane's own 16 bytes of 32
+// rows would be 32 lines a store).
+struct Rows {
+  const b200_tree_attn_args* a;
+  const Item* it;
+  uint8_t* stage;
+  int row0, rows, lane;           // the warp's first row, the item's rows
+  bool whole;                     // the item's tiles were all this range's: normalised rows to the output, else fp32 ones to `part` with their maximum and sum
+  int t0, take;
+  bool odd;                       // infinities or NaN among its drafts' values
+  float* part;
+
+  // the output at o in TMEM; m in units of log 2
+  __device__ __forceinline__ void write(uint32_t o, float m, float sum) const {
+    const int group = a->q_heads / a->kv_heads, shift = __ffs(group) - 1, row = row0 + lane;
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    // two rows are a line of 128 bytes, pieces of 16 bytes in an order that leaves no bank twice
+    auto piece = [&](int r, int k) { return reinterpret_cast<uint4*>(stage + (r >> 1) * 128 + ((((r & 1) * 4 + k) ^ ((r >> 1) & 7)) << 4)); };
+#pragma unroll
+    for (int c1 = 0; c1 < kD; c1 += 32) {
+      uint32_t v[32];
+      tmem_ld_32x32(o + c1, v);
       tmem_ld_wait();
-    } else {
-#pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = 0u;
-    }
-    if (NT == 1) {
-#pragma unroll
-      for (int c = 0; c < 32; ++c) v[c] = w_a == 0.f ? 0u : __float_as_uint(__uint_as_float(v[c]) * w_a);
-      if (has_b) {
-        uint32_t x[32];
-        tmem_ld_32x32(o_b + c0, x);
-        tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < 32; ++c) v[c] = w_b == 0.f ? v[c] : __float_as_uint(fmaf(__uint_as_float(x[c]), w_b, __uint_as_float(v[c])));
+      if (odd && row < rows) {
+        uint32_t y[32];
+        for (int c = 0; c < 32; ++c) y[c] = v[c];
+        add_odd(*a, *it, t0, take, c1, row >> shift, y);
+        for (int c = 0; c < 32; ++c) v[c] = y[c];
       }
-    }
-    if (valid && odd) {
-      // infinities and NaN of the drafts that this row sees, which stayed out of the products
-      const int* table = a.block_tables + static_cast<size_t>(it.s) * a.ld_tables;
-      const int* mask = a.masks ? a.masks + static_cast<size_t>(it.r.row0 + token) * a.words : nullptr;
-      for (int p = max(it.r.ctx, t0 * kKeys); p < min(it.kv_end, (t0 + take) * kKeys); ++p) {
-        if (!(seen_bits(mask, a.words, token, it.r.rows, p - it.r.ctx) & 1)) continue;
-        const long long at = tree::cache_row(table, p, a.num_pages);
-        if (at < 0) continue;
-        const bf16* value = static_cast<const bf16*>(a.kv_layer) + ((((at >> 4) * 2 + 1) * a.kv_heads + it.kvh) * 16 + (at & 15)) * kD + c0;
+      auto leave = [&](int to_column, int bytes_a_value) {      // what lies there, 64 bytes a row
+        __syncwarp();
 #pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          const float x = __bfloat162float(value[c]);
-          if (!isfinite(x)) v[c] = __float_as_uint(__uint_as_float(v[c]) + x);
+        for (int i = 0; i < 4; ++i) {
+          const int r = 8 * i + (lane >> 2), k = lane & 3, to = row0 + r;
+          const uint4 x = *piece(r, k);
+          if (to >= rows) continue;
+          if (bytes_a_value == 2)
+            *reinterpret_cast<uint4*>(static_cast<bf16*>(a->out) + static_cast<size_t>(it->r.row0 + it->first + (to >> shift)) * a->ldo + (it->kvh * group + (to & (group - 1))) * kD + to_column + 8 * k) = x;
+          else
+            *reinterpret_cast<uint4*>(part + static_cast<size_t>(to) * kLd + to_column + 4 * k) = x;
+        }
+        __syncwarp();
+      };
+      if (whole) {
+#pragma unroll
+        for (int c = 0; c < 32; c += 8)
+          *piece(lane, c / 8) =
+              make_uint4(pack_bf16x2(__uint_as_float(v[c]) * inv, __uint_as_float(v[c + 1]) * inv), pack_bf16x2(__uint_as_float(v[c + 2]) * inv, __uint_as_float(v[c + 3]) * inv),
+                         pack_bf16x2(__uint_as_float(v[c + 4]) * inv, __uint_as_float(v[c + 5]) * inv), pack_bf16x2(__uint_as_float(v[c + 6]) * inv, __uint_as_float(v[c + 7]) * inv));
+        leave(c1, 2);
+      } else {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int c = 0; c < 16; c += 4) *piece(lane, c / 4) = make_uint4(v[16 * h + c], v[16 * h + c + 1], v[16 * h + c + 2], v[16 * h + c + 3]);
+          leave(c1 + 16 * h, 4);
         }
       }
     }
-    if (valid && whole) {
-#pragma unroll
-      for (int c = 0; c < 32; c += 8)
-        *reinterpret_cast<uint4*>(dst + c0 + c) =
-            make_uint4(pack_bf16x2(__uint_as_float(v[c]) * inv, __uint_as_float(v[c + 1]) * inv), pack_bf16x2(__uint_as_float(v[c + 2]) * inv, __uint_as_float(v[c + 3]) * inv),
-                       pack_bf16x2(__uint_as_float(v[c + 4]) * inv, __uint_as_float(v[c + 5]) * inv), pack_bf16x2(__uint_as_float(v[c + 6]) * inv, __uint_as_float(v[c + 7]) * inv));
-    } else if (valid) {
-#pragma unroll
-      for (int c = 0; c < 32; c += 4) *reinterpret_cast<uint4*>(part + c0 + c) = make_uint4(v[c], v[c + 1], v[c + 2], v[c + 3]);
-    }
-    __syncwarp();
+    if (!whole && row < rows) *reinterpret_cast<float2*>(part + static_cast<size_t>(row) * kLd + kD) = make_float2(m, sum);
   }
-  if (valid && !whole && c_begin == 0) *reinterpret_cast<float2*>(part + kD) = make_float2(m, sum);
-}
+};
 
-template <int NT>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kThreads, kPlaces)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ b200_tree_attn_args a, float scale_log2, int* error) {
-  constexpr int kK = Shape<NT>::kK, kV = Shape<NT>::kV;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (sbase - smem_u32(smem_raw));
-  const uint32_t q_s = sbase, k_s = sbase + Shape<NT>::kKeysAt, v_s = sbase + Shape<NT>::kValuesAt, bars = sbase + Shape<NT>::kBars;
+  const uint32_t q_s = sbase, k_s = sbase + kKeysAt, v_s = sbase + kValuesAt, bars = sbase + kBars;
   auto k_full = [&](int s) { return bars + 8u * s; };
-  auto k_empty = [&](int s) { return bars + 8u * (5 + s); };
-  auto v_full = [&](int s) { return bars + 8u * (10 + s); };
-  auto v_empty = [&](int s) { return bars + 8u * (15 + s); };
-  auto q_full = [&](int b) { return bars + 8u * (20 + b); };
-  auto q_empty = [&](int b) { return bars + 8u * (22 + b); };
-  // of every other tile of a group each: a warp is up to two tiles ahead of the slowest one of its group
-  auto s_full = [&](int g, int b) { return bars + 8u * (24 + 2 * g + b); };
-  auto p_ready = [&](int g, int b) { return bars + 8u * (28 + 2 * g + b); };
-  auto pv_full = [&](int g, int b) { return bars + 8u * (32 + 2 * g + b); };
-  auto joined = [&](int k) { return bars + 8u * (36 + k); };      // NT = 1: both groups' eight warps, at an item's end: products landed, outputs read
-  const uint32_t slot = bars + 8u * 38;
+  auto k_empty = [&](int s) { return bars + 8u * (2 + s); };
+  auto v_full = [&](int s) { return bars + 8u * (4 + s); };
+  auto v_empty = [&](int s) { return bars + 8u * (6 + s); };
+  // of every other tile each: a softmax warp is up to two tiles ahead of the slowest one
+  auto s_full = [&](int b) { return bars + 8u * (8 + b); };
+  auto p_ready = [&](int b) { return bars + 8u * (10 + b); };
+  auto pv_full = [&](int b) { return bars + 8u * (12 + b); };
+  const uint32_t q_full = bars + 8u * 14, q_empty = bars + 8u * 15, slot = bars + 8u * 16;
+  static_assert(kDepth == 2, "");
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (slot - sbase));
   volatile int* odd_item = reinterpret_cast<volatile int*>(tmem_slot + 2);      // [2]: the last item of each parity with infinities or NaN among its drafts' values
   __shared__ int sums[kWarps];
@@ -244,24 +255,23 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
 
   if (warp == 0) {
     if (lane == 0) {
-      for (int s = 0; s < 5; ++s) { mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1); mbar_init(v_full(s), 1); mbar_init(v_empty(s), 1); }
-      for (int g = 0; g < 2; ++g) {
-        mbar_init(q_full(g), 1); mbar_init(q_empty(g), 1);
-        for (int b = 0; b < 2; ++b) { mbar_init(s_full(g, b), 1); mbar_init(p_ready(g, b), 4); mbar_init(pv_full(g, b), 1); }
+      for (int s = 0; s < 2; ++s) {
+        mbar_init(k_full(s), 1); mbar_init(k_empty(s), 1); mbar_init(v_full(s), 1); mbar_init(v_empty(s), 1);
+        mbar_init(s_full(s), 1); mbar_init(p_ready(s), 4); mbar_init(pv_full(s), 1);
       }
-      mbar_init(joined(0), 8);
-      mbar_init(joined(1), 8);
+      mbar_init(q_full, 1);
+      mbar_init(q_empty, 1);
       fence_mbar_init();
       odd_item[0] = odd_item[1] = -1;
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_kv);
     }
     __syncwarp();
-    tmem_alloc(slot, 512);
+    tmem_alloc(slot, 256);
     tmem_relinquish();
   }
   griddep_enter();
-  const int ctas = gridDim.x, cta = blockIdx.x, bt = block_tokens(a, NT);
+  const int ctas = gridDim.x, cta = blockIdx.x, bt = block_tokens(a);
   // ---- this CTA's range, and where it begins: every thread sums some requests, one behind the other, and the sums of the threads in front of it
   const int per_thread = (a.S + kThreads - 1) / kThreads, s_begin = min(a.S, tid * per_thread), s_end = min(a.S, s_begin + per_thread);
   int before = 0, N = 0;
@@ -289,14 +299,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     if (b[0] < before + own && b[1] >= before)
       for (int s = s_begin; s < s_end; ++s) {
         const tree::Request r = request(a, s);
-        const int per_head = head_tiles(a, r, bt), mine = per_head * a.kv_heads;
+        const int mine = head_tiles(a, r, bt) * a.kv_heads;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           if (mine == 0 || b[e] < before || b[e] >= before + mine) continue;
-          const int kvh = (b[e] - before) / per_head;
-          int g0 = before + kvh * per_head, block = 0;
-          for (int n; b[e] >= g0 + (n = tiles_of(a, r, bt, block)); ++block) g0 += n;
-          s_range[e] = snapped(b[e], g0, g0 + tiles_of(a, r, bt, block));
+          int g0 = before, block = 0, tiles = tiles_of(a, r, bt, 0);
+          while (b[e] >= g0 + tiles * a.kv_heads) g0 += tiles * a.kv_heads, tiles = tiles_of(a, r, bt, ++block);
+          const int kvh = (b[e] - g0) / tiles;
+          g0 += kvh * tiles;
+          s_range[e] = snapped(b[e], g0, g0 + tiles);
           if (e == 0) { s_where[0] = s; s_where[1] = kvh; s_where[2] = block; s_range[2] = g0; }
         }
         before += mine;
@@ -305,9 +316,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-  auto tm_s = [&](int g, int b) { return tmem + 64u * (2 * g + b); };
-  auto tm_o = [&](int g) { return tmem + 256u + 128u * g; };
+  const uint32_t tmem = *tmem_slot, tm_o = tmem + 128;
+  auto tm_s = [&](int b) { return tmem + 64u * b; };
   Cut cut = {0, 0, 0, 0};
   const int left = N > 0 && cta < ranges.n ? s_range[1] - s_range[0] : 0;
 
@@ -319,11 +329,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     fill(a, bt, &it);
     int t0 = s_range[0] - s_range[2], rest = left;
     auto next_item = [&] {
-      ++it.block;
-      if (it.block >= blocks_of(it.r, bt)) {
-        it.block = 0;
-        if (++it.kvh >= a.kv_heads) {
-          it.kvh = 0;
+      if (++it.kvh >= a.kv_heads) {
+        it.kvh = 0;
+        if (++it.block >= blocks_of(it.r, bt)) {
+          it.block = 0;
           do it.r = request(a, ++it.s);
           while (it.r.rows == 0);      // (a range's tiles are some request's: the walk ends in front of a.S)
         }
@@ -337,12 +346,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     const int group = a.q_heads / a.kv_heads;
     int gt = 0, item = 0;              // tiles and items of this range so far
 
-    if (warp == 0 || warp == kWarps - 3) {
-      // ------------------------------------------------------------ loads: queries and keys, or values
-      const bool one = elect_one(), values = warp != 0;
-      const int depth = values ? kV : kK;
-      const uint32_t ring = values ? v_s : k_s, full0 = values ? v_full(0) : k_full(0), empty0 = values ? v_empty(0) : k_empty(0);
-      int st = 0, phase = 1;
+    if (warp == 0) {
+      // ------------------------------------------------------------ loads
+      const bool one = elect_one();
+      int nk = 0, nv = 0;              // on their way
       for (; ok && rest > 0; ++item) {
         const uint64_t hint = it.r.rows > bt ? kEvictNormal : kEvictFirst;
         const int take = min(it.tiles - t0, rest), pages = (it.kv_end + 15) >> 4, p_begin = t0 * 4;
@@ -350,80 +357,71 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         // the first row of a page's head; a page that the cache does not have lies behind its last row, where a load finds zeros
         auto look_up = [&](int base) {
           const int p = base + lane, page = p < pages ? table[p] : -1;
-          return ((page >= 0 && page < a.num_pages ? page : static_cast<int>(a.num_pages)) * 2 + values) * a.kv_heads * 16 + it.kvh * 16;
+          return ((page >= 0 && page < a.num_pages ? page : static_cast<int>(a.num_pages)) * 2 * a.kv_heads + it.kvh) * 16;
         };
         int mine = look_up(p_begin), next = look_up(p_begin + 32);
-        if (!values) {
-          const int qb = item & 1, tiles_q = NT == 2 && it.nb * group > kRows ? 2 : 1;
-          if (!(ok = warp_wait(q_empty(qb), ((item >> 1) & 1) ^ 1u))) break;
-          if (one) {
-            mbar_arrive_expect_tx(q_full(qb), tiles_q * 2 * kQSlab);
-            for (int i = 0; i < tiles_q; ++i)
-              for (int h = 0; h < 2; ++h) tma_load_3d(q_s + ((qb * NT + i) * 2 + h) * kQSlab, &tm_q, q_full(qb), 64 * h, it.kvh * group, it.r.row0 + it.first + i * (kRows / group));
-          }
+        if (!(ok = warp_wait(q_empty, (item & 1) ^ 1u))) break;
+        if (one) {
+          mbar_arrive_expect_tx(q_full, 2 * kQSlab);
+          for (int h = 0; h < 2; ++h) tma_load_3d(q_s + h * kQSlab, &tm_q, q_full, 64 * h, it.kvh * group, it.r.row0 + it.first);
         }
         for (int j = 0; j < take; ++j, ++gt) {
           if (j && j % 8 == 0) {
             mine = next;
             next = look_up(p_begin + 4 * j + 32);
           }
-          const int n = min(4, pages - p_begin - 4 * j);
+          const int n = min(4, pages - p_begin - 4 * j), st = gt & 1;
+          const uint32_t parity = ((gt >> 1) & 1) ^ 1u;
           int row[4];
 #pragma unroll
           for (int pg = 0; pg < 4; ++pg) row[pg] = __shfl_sync(0xffffffffu, mine, (4 * j + pg) & 31);
-          if (!(ok = warp_wait(empty0 + 8 * st, phase))) break;
-          const uint32_t full = full0 + 8 * st, dst = ring + st * kTile;
-          if (one) {
-            mbar_arrive_expect_tx(full, n * 4096);
 #pragma unroll
-            for (int pg = 0; pg < 4; ++pg) {
-              if (pg >= n) break;
-              tma_load_2d(dst + pg * 2048, &tm_kv, full, 0, row[pg], hint);
-              tma_load_2d(dst + kSlab + pg * 2048, &tm_kv, full, 64, row[pg], hint);
+          for (int w = 0; w < 2; ++w) {      // keys, then values
+            if (!(ok = warp_wait(w ? v_empty(st) : k_empty(st), parity))) break;
+            const uint32_t full = w ? v_full(st) : k_full(st), dst = (w ? v_s : k_s) + st * kTile;
+            if (one) {
+              mbar_arrive_expect_tx(full, n * 4096);
+#pragma unroll
+              for (int pg = 0; pg < 4; ++pg) {
+                if (pg >= n) break;
+                tma_load_2d(dst + pg * 2048, &tm_kv, full, 0, row[pg] + w * a.kv_heads * 16, hint);
+                tma_load_2d(dst + kSlab + pg * 2048, &tm_kv, full, 64, row[pg] + w * a.kv_heads * 16, hint);
+              }
             }
+            __syncwarp();
+            w ? ++nv : ++nk;
           }
-          __syncwarp();
-          if (++st == depth) { st = 0; phase ^= 1; }
+          if (!ok) break;
         }
         if (!ok) break;
         rest -= take;
-        if (rest == 0 && t0 == 0 && take < it.tiles)
-          cut = {it.r.row0 + it.first, it.nb * group, it.kvh, ranges.up_to(s_range[1] - take + it.tiles - kSnap - 1) - cta + 1};
+        if (rest == 0 && t0 == 0 && take < it.tiles) cut = {it.r.row0 + it.first, it.nb * group, it.kvh, ranges.up_to(s_range[1] - take + it.tiles - kSnap - 1) - cta + 1};
         t0 = 0;
         if (rest > 0) next_item();
       }
       // the copies in flight land before the CTA ends, also where it gives up
-      if (!values)
-        for (int k = max(0, item - 2); k < item + !ok; ++k) warp_wait(q_full(k & 1), (k >> 1) & 1);
-      for (int k = max(0, gt - depth); k < gt; ++k) warp_wait(full0 + 8 * (k % depth), (k / depth) & 1);
+      if (item + !ok > 0) warp_wait(q_full, (item - ok) & 1);
+      for (int k = max(0, nk - kDepth); k < nk; ++k) warp_wait(k_full(k & 1), (k >> 1) & 1);
+      for (int k = max(0, nv - kDepth); k < nv; ++k) warp_wait(v_full(k & 1), (k >> 1) & 1);
     } else if (warp == kWarps - 2) {
       // ------------------------------------------------------------ scores
       const bool one = elect_one();
       const uint32_t id_s = idesc_bf16(kRows, kKeys, 0);
       const uint64_t q_d = desc_sw128(q_s, 16, 1024), k_d = desc_sw128(k_s, 16, 1024);
       for (; ok && rest > 0; ++item) {
-        const int take = min(it.tiles - t0, rest), tiles_q = NT == 2 && it.nb * group > kRows ? 2 : 1, qb = item & 1;
-        if (!(ok = warp_wait(q_full(qb), (item >> 1) & 1))) break;
+        const int take = min(it.tiles - t0, rest);
+        if (!(ok = warp_wait(q_full, item & 1))) break;
         for (int j = 0; j < take; ++j, ++gt) {
-          const int st = gt % kK, u = NT == 1 ? gt >> 1 : gt, b = u & 1;
-          if (!(ok = warp_wait(k_full(st), (gt / kK) & 1))) break;
-          // the buffer's last P has been read by the products with its values
-          if (u >= 2)
-            for (int i = 0; ok && i < NT; ++i) ok = warp_wait(pv_full(NT == 1 ? gt & 1 : i, b), ((u - 2) >> 1) & 1);
-          if (!ok) break;
+          const int b = gt & 1;
+          // the keys are there, and the buffer's last P has been read by the products with its values
+          if (!(ok = warp_wait(k_full(b), (gt >> 1) & 1) && (gt < 2 || warp_wait(pv_full(b), ((gt - 2) >> 1) & 1)))) break;
           tc_fence_after();
           if (one) {
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-              const int g = NT == 1 ? gt & 1 : i;
-              if (i < tiles_q) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) umma_bf16_k64(tm_s(g, b), q_d + ((qb * NT + i) * 2 + h) * (kQSlab >> 4), k_d + st * (kTile >> 4) + h * (kSlab >> 4), id_s, h);
-              }
-              umma_commit(s_full(g, b));      // (a group without rows keeps step)
-            }
-            umma_commit(k_empty(st));
-            if (j + 1 == take) umma_commit(q_empty(qb));
+            for (int h = 0; h < 2; ++h) umma_bf16_k64(tm_s(b), q_d + h * (kQSlab >> 4), k_d + b * (kTile >> 4) + h * (kSlab >> 4), id_s, h);
+            umma_commit(s_full(b));
+            umma_commit(k_empty(b));
+            if (j + 1 == take) umma_commit(q_empty);
           }
           __syncwarp();
         }
@@ -438,25 +436,28 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const uint32_t id_o = idesc_bf16(kRows, kD, 1);
       const uint64_t v_d = desc_sw128(v_s, kSlab, 1024);
       for (; ok && rest > 0; ++item) {
-        const int take = min(it.tiles - t0, rest), tiles_q = NT == 2 && it.nb * group > kRows ? 2 : 1;
+        const int take = min(it.tiles - t0, rest);
         for (int j = 0; j < take; ++j, ++gt) {
-          const int st = gt % kV, kv0 = (t0 + j) * kKeys;
-          if (!(ok = warp_wait(v_full(st), (gt / kV) & 1))) break;
+          const int b = gt & 1, kv0 = (t0 + j) * kKeys;
+          if (!(ok = warp_wait(v_full(b), (gt >> 1) & 1))) break;
           if (kv0 + kKeys > it.r.ctx) {
             bool odd = false;
             const int from = max(0, it.r.ctx - kv0), end = min(kKeys, it.kv_end - kv0);      // the drafts' rows of the tile
             for (int h = 0; h < 2; ++h) {
-              uint4* v = reinterpret_cast<uint4*>(smem + (v_s - sbase) + st * kTile + h * kSlab);      // (a row's pieces in some order)
-              for (int e0 = from * 8; e0 < end * 8; e0 += 128) {
-                uint4 x[4];
+              uint4* v = reinterpret_cast<uint4*>(smem + (v_s - sbase) + b * kTile + h * kSlab);      // (a row's pieces in some order)
+              for (int e0 = from * 8; e0 < end * 8; e0 += 256) {
+                uint4 x[8];
+                uint32_t any = 0;      // bit 15 or 31: an exponent of all ones
 #pragma unroll
-                for (int k = 0; k < 4; ++k) x[k] = v[min(e0 + 32 * k + lane, end * 8 - 1)];
+                for (int k = 0; k < 8; ++k) x[k] = v[min(e0 + 32 * k + lane, end * 8 - 1)];
+                auto carry = [](uint32_t w) { return (w & 0x7f807f80u) + 0x00800080u; };
 #pragma unroll
-                for (int k = 0; k < 4; ++k)
-                  if (odd_pair(x[k].x) || odd_pair(x[k].y) || odd_pair(x[k].z) || odd_pair(x[k].w)) {
-                    v[min(e0 + 32 * k + lane, end * 8 - 1)] = make_uint4(without_odd(x[k].x), without_odd(x[k].y), without_odd(x[k].z), without_odd(x[k].w));
-                    odd = true;
-                  }
+                for (int k = 0; k < 8; ++k) any |= carry(x[k].x) | carry(x[k].y) | carry(x[k].z) | carry(x[k].w);
+                if (any & 0x80008000u) {
+                  odd = true;
+#pragma unroll
+                  for (int k = 0; k < 8; ++k) v[min(e0 + 32 * k + lane, end * 8 - 1)] = make_uint4(without_odd(x[k].x), without_odd(x[k].y), without_odd(x[k].z), without_odd(x[k].w));
+                }
               }
               for (int e = end * 8 + lane; e < kKeys * 8; e += 32) v[e] = make_uint4(0, 0, 0, 0);
             }
@@ -465,20 +466,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             fence_proxy_async();
             __syncwarp();
           }
-#pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            const int g = NT == 1 ? gt & 1 : i, u = NT == 1 ? gt >> 1 : gt, b = u & 1;
-            if (ok) ok = warp_wait(p_ready(g, b), (u >> 1) & 1);
-            if (!ok) continue;
-            tc_fence_after();
-            if (one) {
-              if (i < tiles_q) umma_bf16_tmem_k64(tm_o(g), tm_s(g, b), v_d + st * (kTile >> 4), id_o, j >= (NT == 1 ? 2 : 1));
-              umma_commit(pv_full(g, b));
-            }
-            __syncwarp();
+          if (!(ok = warp_wait(p_ready(b), (gt >> 1) & 1))) break;
+          tc_fence_after();
+          if (one) {
+            umma_bf16_tmem_k64(tm_o, tm_s(b), v_d + b * (kTile >> 4), id_o, j > 0);
+            umma_commit(pv_full(b));
+            umma_commit(v_empty(b));
           }
-          if (!ok) break;
-          if (one) umma_commit(v_empty(st));
           __syncwarp();
         }
         if (!ok) break;
@@ -488,26 +482,22 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       }
     } else {
       // ------------------------------------------------------------ softmax: thread = row (token * group + head)
-      const int g = (warp - 1) >> 2, q = warp & 3, in_tile = q * 32 + lane;
+      const int q = warp & 3, row = q * 32 + lane;      // the quarter of the lanes that this warp may access
       const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
-      const int row = (NT == 2 ? g * kRows : 0) + in_tile, token_of = row / group, head_of = row - token_of * group;
-      float2* states = reinterpret_cast<float2*>(smem + Shape<NT>::kStates);
       for (; ok && rest > 0; ++item) {
         const int take = min(it.tiles - t0, rest), rows = it.nb * group;
         const bool valid = row < rows, some = row - lane < rows;      // this warp has rows
-        const int token = it.first + token_of;
+        const int token = it.first + row / group;
         const int* mask = a.masks && valid ? a.masks + static_cast<size_t>(it.r.row0 + token) * a.words : nullptr;
         float ref = -INFINITY, l = 0.f;      // what the row's weights are relative to, in units of log 2, and their sum
-        int mine = 0;                        // tiles of this group
         for (int j = 0; j < take; ++j, ++gt) {
-          if (NT == 1 && (gt & 1) != g) continue;
-          const int u = NT == 1 ? gt >> 1 : gt, b = u & 1, kv0 = (t0 + j) * kKeys;
-          if (!(ok = warp_wait(s_full(g, b), (u >> 1) & 1))) break;
+          const int b = gt & 1, kv0 = (t0 + j) * kKeys;
+          if (!(ok = warp_wait(s_full(b), (gt >> 1) & 1))) break;
           if (some) {
             tc_fence_after();
             uint32_t s0[32], s1[32];
-            tmem_ld_32x32(tm_s(g, b) + lane_off, s0);
-            tmem_ld_32x32(tm_s(g, b) + lane_off + 32, s1);
+            tmem_ld_32x32(tm_s(b) + lane_off, s0);
+            tmem_ld_32x32(tm_s(b) + lane_off + 32, s1);
             tmem_ld_wait();
             if (kv0 + kKeys > it.r.ctx) {
               const uint32_t m0 = valid ? seen_bits(mask, a.words, token, it.r.rows, kv0 - it.r.ctx) : 0u, m1 = valid ? seen_bits(mask, a.words, token, it.r.rows, kv0 + 32 - it.r.ctx) : 0u;
@@ -545,65 +535,37 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             }
             l = l * alpha + ps;
             // P in place of the scores: what read this buffer's last P went ahead of them.  Where some row of the warp moved its maximum, its output so
-            // far is scaled once the group's previous product has landed.
-            tmem_st_32x32(tm_s(g, b) + lane_off, pk);
-            if (mine > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-              if (!(ok = warp_wait(pv_full(g, b ^ 1), ((u - 1) >> 1) & 1))) break;
+            // far is scaled once the previous product has landed.
+            tmem_st_32x32(tm_s(b) + lane_off, pk);
+            if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+              if (!(ok = warp_wait(pv_full(b ^ 1), ((gt - 1) >> 1) & 1))) break;
               tc_fence_after();
 #pragma unroll
               for (int c0 = 0; c0 < kD; c0 += 32) {
                 uint32_t v[32];
-                tmem_ld_32x32(tm_o(g) + lane_off + c0, v);
+                tmem_ld_32x32(tm_o + lane_off + c0, v);
                 tmem_ld_wait();
 #pragma unroll
                 for (int c = 0; c < 32; ++c) v[c] = __float_as_uint(__uint_as_float(v[c]) * alpha);
-                tmem_st_32x32(tm_o(g) + lane_off + c0, v);
+                tmem_st_32x32(tm_o + lane_off + c0, v);
               }
             }
             tmem_st_wait();
             tc_fence_before();
           }
-          ++mine;
           __syncwarp();
-          if (lane == 0) mbar_arrive(p_ready(g, b));
+          if (lane == 0) mbar_arrive(p_ready(b));
         }
         if (!ok) break;
-        // ---- the item's rows: gt is the first tile behind them
-        const bool whole = t0 == 0 && take == it.tiles;
-        if (NT == 1) {
-          // both groups' outputs lie in the same lanes: each thread joins half of its row's dimensions
-          const int other = take - mine;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {      // the last one or two tiles' products
-            const int t = gt - 1 - k;
-            if (ok && k < take) ok = warp_wait(pv_full(t & 1, (t >> 1) & 1), (t >> 2) & 1);
-          }
-          if (!ok) break;
-          states[g * kRows + in_tile] = make_float2(ref, l);
-          auto together = [&](int k) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(joined(k));
-            ok = warp_wait(joined(k), item & 1);
-            tc_fence_after();
-          };
-          together(0);
-          if (!ok) break;
-          if (some) {
-            const float2 st = states[(g ^ 1) * kRows + in_tile];
-            const float m = fmaxf(ref, st.x), base = m == -INFINITY ? 0.f : m;
-            const float w_mine = mine ? exp2f(ref - base) : 0.f, w_other = other ? exp2f(st.x - base) : 0.f;
-            const float sum = (mine ? l * w_mine : 0.f) + (other ? st.y * w_other : 0.f);
-            finish<NT>(a, it, tm_o(g) + lane_off, mine, w_mine, tm_o(g ^ 1) + lane_off, other, w_other, 64 * g, 64, valid, token, head_of, m, sum, whole, t0, take, odd_item[item & 1] == item, cta, row);
-          }
-          together(1);             // the next item's products may write over the outputs
-          if (!ok) break;
-        } else {
-          if (!(ok = warp_wait(pv_full(g, (gt - 1) & 1), ((gt - 1) >> 1) & 1))) break;
-          tc_fence_after();
-          if (some) finish<NT>(a, it, tm_o(g) + lane_off, 1, 1.f, 0u, 0, 0.f, 0, kD, valid, token, head_of, ref, l, whole, t0, take, odd_item[item & 1] == item, cta, row);
-          tc_fence_before();
+        // ---- the item's rows
+        if (!(ok = warp_wait(pv_full((gt - 1) & 1), ((gt - 1) >> 1) & 1))) break;
+        tc_fence_after();
+        if (some) {
+          Rows out{&a, &it, smem + kStageAt + q * 2048, q * 32, rows, lane, t0 == 0 && take == it.tiles, t0, take, odd_item[item & 1] == item, nullptr};
+          out.part = rows_of(a.workspace, ctas) + static_cast<size_t>(2 * cta + (t0 == 0)) * kRows * kLd;      // a part without the item's beginning is the range's first
+          out.write(tm_o + lane_off, ref, l);
         }
+        tc_fence_before();
         rest -= take;
         t0 = 0;
         if (rest > 0) next_item();
@@ -617,14 +579,14 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   __syncthreads();
   if (warp == 0) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc(tmem, 256);
   }
 }
 
 // Rows of items that ranges' ends cut: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts, in order.  A warp a row.
-template <int NT>
 __global__ void __launch_bounds__(256)
 tree_attn_join_kernel(const __grid_constant__ b200_tree_attn_args a, int ctas) {
+  constexpr int kAtOnce = 12;
   griddep_enter();
   if (static_cast<int>(blockIdx.x) == ctas) {
     if (blockIdx.y == 0) zero_rest(a);
@@ -636,27 +598,27 @@ tree_attn_join_kernel(const __grid_constant__ b200_tree_attn_args a, int ctas) {
   const float* ws = rows_of(a.workspace, ctas);
   for (int row = blockIdx.y * 8 + warp; row < cut.rows; row += gridDim.y * 8) {
     // the item's beginning lies in its range's second place, each other part in its range's first
-    auto part = [&](int p) { return ws + (static_cast<size_t>(2 * (blockIdx.x + p) + (p == 0)) * (NT * kRows) + row) * kLd; };
+    auto part = [&](int p) { return ws + (static_cast<size_t>(2 * (blockIdx.x + p) + (p == 0)) * kRows + row) * kLd; };
     float m = -INFINITY, sum = 0.f;
     float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = 0; p0 < cut.parts; p0 += 8) {
-      float2 st[8];
-      float4 x[8];
+    for (int p0 = 0; p0 < cut.parts; p0 += kAtOnce) {
+      float2 st[kAtOnce];
+      float4 x[kAtOnce];
       float top = m;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < kAtOnce; ++k) {
         const bool there = p0 + k < cut.parts;
         st[k] = there ? *reinterpret_cast<const float2*>(part(p0 + k) + kD) : make_float2(-INFINITY, 0.f);
         x[k] = there ? *reinterpret_cast<const float4*>(part(p0 + k) + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
       }
 #pragma unroll
-      for (int k = 0; k < 8; ++k) top = fmaxf(top, st[k].x);
+      for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, st[k].x);
       const float base = top == -INFINITY ? 0.f : top, old = exp2f(m - base);
       m = top;
       sum *= old;
       y = make_float4(y.x * old, y.y * old, y.z * old, y.w * old);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
+      for (int k = 0; k < kAtOnce; ++k) {
         const float w = exp2f(st[k].x - base);
         sum += w == 0.f && st[k].y == st[k].y ? 0.f : st[k].y * w;
         if (w != 0.f) y = make_float4(fmaf(x[k].x, w, y.x), fmaf(x[k].y, w, y.y), fmaf(x[k].z, w, y.z), fmaf(x[k].w, w, y.w));
@@ -669,28 +631,22 @@ tree_attn_join_kernel(const __grid_constant__ b200_tree_attn_args a, int ctas) {
   }
 }
 
-template <int NT>
-int launch(const b200_tree_attn_args& a, int* error, cudaStream_t st) {
-  const int group = a.q_heads / a.kv_heads, ctas = sm_count();
+}  // namespace
+
+int64_t tree_attention_workspace(const b200_tree_attn_args&) { return static_cast<int64_t>(kPlaces) * sm_count() * (static_cast<int64_t>(sizeof(Cut)) + 2ll * kRows * kLd * sizeof(float)); }
+
+int paged_attention_tree(const b200_tree_attn_args& a, int* error, cudaStream_t st) {
+  const int group = a.q_heads / a.kv_heads, ctas = kPlaces * sm_count();
   CUtensorMap tm_q, tm_kv;
   if (int rc = tmap_encode_bf16_3d(&tm_q, a.q, kD, a.q_heads, a.T, kD, a.ldq, 64, group, kRows / group)) return rc;
   if (int rc = tmap_encode_bf16_2d(&tm_kv, a.kv_layer, static_cast<uint64_t>(a.num_pages) * 2 * a.kv_heads * 16, kD, kD, 16, 64, 1)) return rc;
   static std::atomic<unsigned long long> attr_done{0};
-  if (!ensure_dynamic_smem(tree_attn_kernel<NT>, Shape<NT>::kSmem, &attr_done)) return -3;
-  launch_pdl(tree_attn_kernel<NT>, dim3(ctas), dim3(kThreads), Shape<NT>::kSmem, st, tm_q, tm_kv, a, a.scale * 1.4426950408889634f, error);
+  if (!ensure_dynamic_smem(tree_attn_kernel, kSmem, &attr_done)) return -3;
+  launch_pdl(tree_attn_kernel, dim3(ctas), dim3(kThreads), kSmem, st, tm_q, tm_kv, a, a.scale * 1.4426950408889634f, error);
   if (cudaGetLastError() != cudaSuccess) return -2;
-  const int rows = static_cast<int>(std::min(static_cast<long long>(NT * kRows), std::min(a.max_tree, a.T) * static_cast<long long>(group)));
-  launch_pdl(tree_attn_join_kernel<NT>, dim3(ctas + (a.zero_rest ? 1 : 0), (rows + 15) / 16), dim3(256), 0, st, a, ctas);
+  const int rows = static_cast<int>(std::min(static_cast<long long>(kRows), std::min(a.max_tree, a.T) * static_cast<long long>(group)));
+  launch_pdl(tree_attn_join_kernel, dim3(ctas + (a.zero_rest ? 1 : 0), (rows + 7) / 8), dim3(256), 0, st, a, ctas);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
-
-// up to 128 rows of a key head: both groups on the same rows
-bool one_tile(const b200_tree_attn_args& a) { return static_cast<long long>(std::min(a.max_tree, a.T)) * (a.q_heads / a.kv_heads) <= kRows; }
-
-}  // namespace
-
-int64_t tree_attention_workspace(const b200_tree_attn_args& a) { return sm_count() * (static_cast<int64_t>(sizeof(Cut)) + 2ll * (one_tile(a) ? 1 : 2) * kRows * kLd * sizeof(float)); }
-
-int paged_attention_tree(const b200_tree_attn_args& a, int* error, cudaStream_t st) { return one_tile(a) ? launch<1>(a, error, st) : launch<2>(a, error, st); }
 
 }  // namespace b200
