@@ -5,7 +5,7 @@
 // A request's rows share all keys but the last few, so what counts is that K and V pass once for all rows of a key head and that nothing stops the stream
 // of pages.  An item is a request's key head and up to 128 of its rows (row = token * group + head); its keys come in tiles of 64.  All items' tiles one behind the
 // other are cut into as many equal ranges as the SMs have places for CTAs, two each, and a CTA walks its range without a gap:
-//   one warp looks pages up (32 of the table at a time, the next ones ahead) and loads queries and tiles by TMA, 128-byte swizzle, into rings;
+//   two warps look pages up (32 of the table at a time, the next ones ahead) and load by TMA, 128-byte swizzle, into rings, one queries and keys, one values;
 //   two warps issue tcgen05.mma, one S = Q K^T (M = 128, N = 64, two buffers), one O += P V (M = 128, N = 128, P in TMEM over its scores): a wait that is over
 //   costs its warp 100 cycles all the same, and one warp for both took 1500 a tile of which the tensor cores need 640;
 //   four warps (thread = row) do the softmax in fp32, base 2; a warp whose rows nobody owns only keeps step.
@@ -36,11 +36,12 @@ namespace {
 typedef __nv_bfloat16 bf16;
 constexpr int kD = 128, kRows = 128, kKeys = 64;
 constexpr int kQSlab = kRows * 128, kSlab = kKeys * 128, kTile = 2 * kSlab;      // bytes: 64 columns of a row tile, of a key tile, a key tile
-constexpr int kThreads = 224, kWarps = kThreads / 32, kPlaces = 2;                // kPlaces: CTAs of an SM
+constexpr int kThreads = 256, kWarps = kThreads / 32, kPlaces = 2;                // kPlaces: CTAs of an SM
 constexpr int kDepth = 2;                  // tiles of keys, and of values, on their way
 constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
-constexpr int kSnap = 2;                   // a range does not end within this many tiles of an item's ends
-constexpr int kLeast = 2;                  // tiles of a range at least
+constexpr int kItem = 2;                   // what an item costs besides its tiles, in tiles: its queries' trip and its rows' way out
+constexpr int kSnap = 3;                   // a range does not end within this many tiles of an item's ends, or an eighth of its length
+constexpr int kLeast = 2;                  // a range's cost at least, in tiles
 constexpr float kSlack = 8.f;              // by which a row's maximum may pass what its weights are relative to, in units of log 2
 constexpr int kWaitLimit = 1 << 22;
 
@@ -114,12 +115,12 @@ __device__ __forceinline__ int tiles_of(const b200_tree_attn_args& a, const tree
   return (r.ctx + seen + kKeys - 1) / kKeys;
 }
 __device__ __forceinline__ int blocks_of(const tree::Request& r, int bt) { return (r.rows + bt - 1) / bt; }
-// of all blocks of a key head
-__device__ __forceinline__ int head_tiles(const b200_tree_attn_args& a, const tree::Request& r, int bt) {
+// what all blocks of a key head cost
+__device__ __forceinline__ int head_cost(const b200_tree_attn_args& a, const tree::Request& r, int bt) {
   const int blocks = blocks_of(r, bt);
-  if (a.masks || blocks <= 1) return blocks ? blocks * tiles_of(a, r, bt, 0) : 0;
+  if (a.masks || blocks <= 1) return blocks ? blocks * (tiles_of(a, r, bt, 0) + kItem) : 0;
   int n = 0;
-  for (int b = 0; b < blocks; ++b) n += tiles_of(a, r, bt, b);
+  for (int b = 0; b < blocks; ++b) n += tiles_of(a, r, bt, b) + kItem;
   return n;
 }
 __device__ __forceinline__ tree::Request request(const b200_tree_attn_args& a, int s) { return tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, a.max_tree); }
@@ -129,20 +130,23 @@ __device__ __forceinline__ void fill(const b200_tree_attn_args& a, int bt, Item*
   it->kv_end = it->r.ctx + (a.masks ? it->r.rows : it->first + it->nb);
   it->tiles = tiles_of(a, it->r, bt, it->block);
 }
-// Range c of the N tiles begins at c * each + min(c, more).
+// Range c of all items' cost N begins at c * each + min(c, more).  An item that begins at g0 has its tile t at g0 + kItem + t.
 struct Ranges {
-  int n, each, more;
-  __device__ __forceinline__ Ranges(int N, int ctas) : n(min(ctas, max(N / kLeast, 1))), each(N / n), more(N - each * n) {}
+  int n, each, more, snap;
+  __device__ __forceinline__ Ranges(int N, int ctas) : n(min(ctas, max(N / kLeast, 1))), each(N / n), more(N - each * n), snap(min(kSnap, each / 8)) {}
   __device__ __forceinline__ int at(int c) const { return c * each + min(c, more); }
-  // ranges but the first that begin at tile x or in front of it
+  // ranges but the first that begin at x or in front of it
   __device__ __forceinline__ int up_to(int x) const {
     if (x < 0) return 0;
     const int c = x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each;
     return min(n - 1, c);
   }
 };
-// the cut b as it is moved within the item [g0, g1)
-__device__ __forceinline__ int snapped(int b, int g0, int g1) { return b - g0 <= kSnap ? g0 : g1 - b <= kSnap ? g1 : b; }
+// the cut b as it is moved to a tile of the item that begins at g0, its ends among them
+__device__ __forceinline__ int snapped(int b, int g0, int tiles, int snap) {
+  const int t = b - g0 - kItem;
+  return t <= snap ? g0 : g0 + kItem + (tiles - t <= snap ? tiles : t);
+}
 // What a CTA leaves for the second kernel: the item that begins in its range and ends behind it, and in how many ranges it lies (0: no such item).
 struct Cut {
   int row0, rows, kvh, parts;      // the item's first row of the step, rows (token * group + head)
@@ -275,7 +279,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   // ---- this CTA's range, and where it begins: every thread sums some requests, one behind the other, and the sums of the threads in front of it
   const int per_thread = (a.S + kThreads - 1) / kThreads, s_begin = min(a.S, tid * per_thread), s_end = min(a.S, s_begin + per_thread);
   int before = 0, N = 0;
-  for (int s = s_begin; s < s_end; ++s) before += head_tiles(a, request(a, s), bt) * a.kv_heads;
+  for (int s = s_begin; s < s_end; ++s) before += head_cost(a, request(a, s), bt) * a.kv_heads;
   const int own = before;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -299,15 +303,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     if (b[0] < before + own && b[1] >= before)
       for (int s = s_begin; s < s_end; ++s) {
         const tree::Request r = request(a, s);
-        const int mine = head_tiles(a, r, bt) * a.kv_heads;
+        const int mine = head_cost(a, r, bt) * a.kv_heads;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           if (mine == 0 || b[e] < before || b[e] >= before + mine) continue;
           int g0 = before, block = 0, tiles = tiles_of(a, r, bt, 0);
-          while (b[e] >= g0 + tiles * a.kv_heads) g0 += tiles * a.kv_heads, tiles = tiles_of(a, r, bt, ++block);
-          const int kvh = (b[e] - g0) / tiles;
-          g0 += kvh * tiles;
-          s_range[e] = snapped(b[e], g0, g0 + tiles);
+          while (b[e] >= g0 + (tiles + kItem) * a.kv_heads) g0 += (tiles + kItem) * a.kv_heads, tiles = tiles_of(a, r, bt, ++block);
+          const int kvh = (b[e] - g0) / (tiles + kItem);
+          g0 += kvh * (tiles + kItem);
+          s_range[e] = snapped(b[e], g0, tiles, ranges.snap);
           if (e == 0) { s_where[0] = s; s_where[1] = kvh; s_where[2] = block; s_range[2] = g0; }
         }
         before += mine;
@@ -322,12 +326,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   const int left = N > 0 && cta < ranges.n ? s_range[1] - s_range[0] : 0;
 
   if (left > 0) {
-    // every role walks the same items: item, its first tile here and how many
+    // every role walks the same items: item, its first tile here, and the range's cost to go
     Item it;
     it.s = s_where[0]; it.kvh = s_where[1]; it.block = s_where[2];
     it.r = request(a, it.s);
     fill(a, bt, &it);
-    int t0 = s_range[0] - s_range[2], rest = left;
+    int t0 = max(0, s_range[0] - s_range[2] - kItem), rest = left;
     auto next_item = [&] {
       if (++it.kvh >= a.kv_heads) {
         it.kvh = 0;
@@ -343,27 +347,35 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       t0 = 0;
       next_item();
     }
+    // the item's tiles of this range, and the cost that is left behind them
+    auto take_of = [&] {
+      const int start = t0 ? 0 : kItem, all = start + it.tiles - t0, take = rest >= all ? it.tiles - t0 : rest - start;
+      rest -= min(rest, all);
+      return take;
+    };
     const int group = a.q_heads / a.kv_heads;
     int gt = 0, item = 0;              // tiles and items of this range so far
 
-    if (warp == 0) {
-      // ------------------------------------------------------------ loads
-      const bool one = elect_one();
-      int nk = 0, nv = 0;              // on their way
-      for (; ok && rest > 0; ++item) {
+    if (warp == 0 || warp == kWarps - 3) {
+      // ------------------------------------------------------------ loads: queries and keys, or values
+      const bool one = elect_one(), values = warp != 0;
+      const uint32_t ring = values ? v_s : k_s, full0 = values ? v_full(0) : k_full(0), empty0 = values ? v_empty(0) : k_empty(0);
+      for (bool more = true; ok && more; ++item) {
         const uint64_t hint = it.r.rows > bt ? kEvictNormal : kEvictFirst;
-        const int take = min(it.tiles - t0, rest), pages = (it.kv_end + 15) >> 4, p_begin = t0 * 4;
+        const int take = take_of(), pages = (it.kv_end + 15) >> 4, p_begin = t0 * 4;
         const int* table = a.block_tables + static_cast<size_t>(it.s) * a.ld_tables;
         // the first row of a page's head; a page that the cache does not have lies behind its last row, where a load finds zeros
         auto look_up = [&](int base) {
           const int p = base + lane, page = p < pages ? table[p] : -1;
-          return ((page >= 0 && page < a.num_pages ? page : static_cast<int>(a.num_pages)) * 2 * a.kv_heads + it.kvh) * 16;
+          return (((page >= 0 && page < a.num_pages ? page : static_cast<int>(a.num_pages)) * 2 + values) * a.kv_heads + it.kvh) * 16;
         };
         int mine = look_up(p_begin), next = look_up(p_begin + 32);
-        if (!(ok = warp_wait(q_empty, (item & 1) ^ 1u))) break;
-        if (one) {
-          mbar_arrive_expect_tx(q_full, 2 * kQSlab);
-          for (int h = 0; h < 2; ++h) tma_load_3d(q_s + h * kQSlab, &tm_q, q_full, 64 * h, it.kvh * group, it.r.row0 + it.first);
+        if (!values) {
+          if (!(ok = warp_wait(q_empty, (item & 1) ^ 1u))) break;
+          if (one) {
+            mbar_arrive_expect_tx(q_full, 2 * kQSlab);
+            for (int h = 0; h < 2; ++h) tma_load_3d(q_s + h * kQSlab, &tm_q, q_full, 64 * h, it.kvh * group, it.r.row0 + it.first);
+          }
         }
         for (int j = 0; j < take; ++j, ++gt) {
           if (j && j % 8 == 0) {
@@ -371,45 +383,37 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
             next = look_up(p_begin + 4 * j + 32);
           }
           const int n = min(4, pages - p_begin - 4 * j), st = gt & 1;
-          const uint32_t parity = ((gt >> 1) & 1) ^ 1u;
           int row[4];
 #pragma unroll
           for (int pg = 0; pg < 4; ++pg) row[pg] = __shfl_sync(0xffffffffu, mine, (4 * j + pg) & 31);
+          if (!(ok = warp_wait(empty0 + 8 * st, ((gt >> 1) & 1) ^ 1u))) break;
+          const uint32_t full = full0 + 8 * st, dst = ring + st * kTile;
+          if (one) {
+            mbar_arrive_expect_tx(full, n * 4096);
 #pragma unroll
-          for (int w = 0; w < 2; ++w) {      // keys, then values
-            if (!(ok = warp_wait(w ? v_empty(st) : k_empty(st), parity))) break;
-            const uint32_t full = w ? v_full(st) : k_full(st), dst = (w ? v_s : k_s) + st * kTile;
-            if (one) {
-              mbar_arrive_expect_tx(full, n * 4096);
-#pragma unroll
-              for (int pg = 0; pg < 4; ++pg) {
-                if (pg >= n) break;
-                tma_load_2d(dst + pg * 2048, &tm_kv, full, 0, row[pg] + w * a.kv_heads * 16, hint);
-                tma_load_2d(dst + kSlab + pg * 2048, &tm_kv, full, 64, row[pg] + w * a.kv_heads * 16, hint);
-              }
+            for (int pg = 0; pg < 4; ++pg) {
+              if (pg >= n) break;
+              tma_load_2d(dst + pg * 2048, &tm_kv, full, 0, row[pg], hint);
+              tma_load_2d(dst + kSlab + pg * 2048, &tm_kv, full, 64, row[pg], hint);
             }
-            __syncwarp();
-            w ? ++nv : ++nk;
           }
-          if (!ok) break;
+          __syncwarp();
         }
         if (!ok) break;
-        rest -= take;
-        if (rest == 0 && t0 == 0 && take < it.tiles) cut = {it.r.row0 + it.first, it.nb * group, it.kvh, ranges.up_to(s_range[1] - take + it.tiles - kSnap - 1) - cta + 1};
+        if (rest == 0 && t0 == 0 && take < it.tiles) cut = {it.r.row0 + it.first, it.nb * group, it.kvh, ranges.up_to(s_range[1] - take + it.tiles - ranges.snap - 1) - cta + 1};
         t0 = 0;
-        if (rest > 0) next_item();
+        if ((more = rest > 0)) next_item();
       }
       // the copies in flight land before the CTA ends, also where it gives up
-      if (item + !ok > 0) warp_wait(q_full, (item - ok) & 1);
-      for (int k = max(0, nk - kDepth); k < nk; ++k) warp_wait(k_full(k & 1), (k >> 1) & 1);
-      for (int k = max(0, nv - kDepth); k < nv; ++k) warp_wait(v_full(k & 1), (k >> 1) & 1);
+      if (!values && item + !ok > 0) warp_wait(q_full, (item - ok) & 1);
+      for (int k = max(0, gt - kDepth); k < gt; ++k) warp_wait(full0 + 8 * (k & 1), (k >> 1) & 1);
     } else if (warp == kWarps - 2) {
       // ------------------------------------------------------------ scores
       const bool one = elect_one();
       const uint32_t id_s = idesc_bf16(kRows, kKeys, 0);
       const uint64_t q_d = desc_sw128(q_s, 16, 1024), k_d = desc_sw128(k_s, 16, 1024);
-      for (; ok && rest > 0; ++item) {
-        const int take = min(it.tiles - t0, rest);
+      for (bool more = true; ok && more; ++item) {
+        const int take = take_of();
         if (!(ok = warp_wait(q_full, item & 1))) break;
         for (int j = 0; j < take; ++j, ++gt) {
           const int b = gt & 1;
@@ -426,17 +430,16 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           __syncwarp();
         }
         if (!ok) break;
-        rest -= take;
         t0 = 0;
-        if (rest > 0) next_item();
+        if ((more = rest > 0)) next_item();
       }
     } else if (warp == kWarps - 1) {
       // ------------------------------------------------------------ outputs
       const bool one = elect_one();
       const uint32_t id_o = idesc_bf16(kRows, kD, 1);
       const uint64_t v_d = desc_sw128(v_s, kSlab, 1024);
-      for (; ok && rest > 0; ++item) {
-        const int take = min(it.tiles - t0, rest);
+      for (bool more = true; ok && more; ++item) {
+        const int take = take_of();
         for (int j = 0; j < take; ++j, ++gt) {
           const int b = gt & 1, kv0 = (t0 + j) * kKeys;
           if (!(ok = warp_wait(v_full(b), (gt >> 1) & 1))) break;
@@ -476,16 +479,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           __syncwarp();
         }
         if (!ok) break;
-        rest -= take;
         t0 = 0;
-        if (rest > 0) next_item();
+        if ((more = rest > 0)) next_item();
       }
     } else {
       // ------------------------------------------------------------ softmax: thread = row (token * group + head)
       const int q = warp & 3, row = q * 32 + lane;      // the quarter of the lanes that this warp may access
       const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
-      for (; ok && rest > 0; ++item) {
-        const int take = min(it.tiles - t0, rest), rows = it.nb * group;
+      for (bool more = true; ok && more; ++item) {
+        const int take = take_of(), rows = it.nb * group;
         const bool valid = row < rows, some = row - lane < rows;      // this warp has rows
         const int token = it.first + row / group;
         const int* mask = a.masks && valid ? a.masks + static_cast<size_t>(it.r.row0 + token) * a.words : nullptr;
@@ -566,9 +568,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           out.write(tm_o + lane_off, ref, l);
         }
         tc_fence_before();
-        rest -= take;
         t0 = 0;
-        if (rest > 0) next_item();
+        if ((more = rest > 0)) next_item();
       }
     }
   }
