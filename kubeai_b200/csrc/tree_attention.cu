@@ -39,9 +39,6 @@ constexpr int kQSlab = kRows * 128, kSlab = kKeys * 128, kTile = 2 * kSlab;     
 constexpr int kThreads = 256, kWarps = kThreads / 32, kPlaces = 2;                // kPlaces: CTAs of an SM
 constexpr int kDepth = 2;                  // tiles of keys, and of values, on their way
 constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
-constexpr int kItem = 2;                   // what an item costs besides its tiles, in tiles: its queries' trip and its rows' way out
-constexpr int kSnap = 3;                   // a range does not end within this many tiles of an item's ends, or an eighth of its length
-constexpr int kLeast = 2;                  // a range's cost at least, in tiles
 constexpr float kSlack = 8.f;              // by which a row's maximum may pass what its weights are relative to, in units of log 2
 constexpr int kWaitLimit = 1 << 22;
 
@@ -118,9 +115,9 @@ __device__ __forceinline__ int blocks_of(const tree::Request& r, int bt) { retur
 // what all blocks of a key head cost
 __device__ __forceinline__ int head_cost(const b200_tree_attn_args& a, const tree::Request& r, int bt) {
   const int blocks = blocks_of(r, bt);
-  if (a.masks || blocks <= 1) return blocks ? blocks * (tiles_of(a, r, bt, 0) + kItem) : 0;
+  if (a.masks || blocks <= 1) return blocks ? blocks * (tiles_of(a, r, bt, 0) + tree::kItem) : 0;
   int n = 0;
-  for (int b = 0; b < blocks; ++b) n += tiles_of(a, r, bt, b) + kItem;
+  for (int b = 0; b < blocks; ++b) n += tiles_of(a, r, bt, b) + tree::kItem;
   return n;
 }
 __device__ __forceinline__ tree::Request request(const b200_tree_attn_args& a, int s) { return tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, a.max_tree); }
@@ -129,23 +126,6 @@ __device__ __forceinline__ void fill(const b200_tree_attn_args& a, int bt, Item*
   it->nb = min(bt, it->r.rows - it->first);
   it->kv_end = it->r.ctx + (a.masks ? it->r.rows : it->first + it->nb);
   it->tiles = tiles_of(a, it->r, bt, it->block);
-}
-// Range c of all items' cost N begins at c * each + min(c, more).  An item that begins at g0 has its tile t at g0 + kItem + t.
-struct Ranges {
-  int n, each, more, snap;
-  __device__ __forceinline__ Ranges(int N, int ctas) : n(min(ctas, max(N / kLeast, 1))), each(N / n), more(N - each * n), snap(min(kSnap, each / 8)) {}
-  __device__ __forceinline__ int at(int c) const { return c * each + min(c, more); }
-  // ranges but the first that begin at x or in front of it
-  __device__ __forceinline__ int up_to(int x) const {
-    if (x < 0) return 0;
-    const int c = x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each;
-    return min(n - 1, c);
-  }
-};
-// the cut b as it is moved to a tile of the item that begins at g0, its ends among them
-__device__ __forceinline__ int snapped(int b, int g0, int tiles, int snap) {
-  const int t = b - g0 - kItem;
-  return t <= snap ? g0 : g0 + kItem + (tiles - t <= snap ? tiles : t);
 }
 // What a CTA leaves for the second kernel: the item that begins in its range and ends behind it, and in how many ranges it lies (0: no such item).
 struct Cut {
@@ -295,7 +275,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     if (w < warp) before += x;
     N += x;
   }
-  const Ranges ranges(N, ctas);
+  const tree::Ranges ranges = tree::ranges_of(N, ctas);
   bool ok = true;
   if (N > 0 && cta < ranges.n) {
     const int b[2] = {ranges.at(cta), ranges.at(cta + 1)};
@@ -308,10 +288,10 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         for (int e = 0; e < 2; ++e) {
           if (mine == 0 || b[e] < before || b[e] >= before + mine) continue;
           int g0 = before, block = 0, tiles = tiles_of(a, r, bt, 0);
-          while (b[e] >= g0 + (tiles + kItem) * a.kv_heads) g0 += (tiles + kItem) * a.kv_heads, tiles = tiles_of(a, r, bt, ++block);
-          const int kvh = (b[e] - g0) / (tiles + kItem);
-          g0 += kvh * (tiles + kItem);
-          s_range[e] = snapped(b[e], g0, tiles, ranges.snap);
+          while (b[e] >= g0 + (tiles + tree::kItem) * a.kv_heads) g0 += (tiles + tree::kItem) * a.kv_heads, tiles = tiles_of(a, r, bt, ++block);
+          const int kvh = (b[e] - g0) / (tiles + tree::kItem);
+          g0 += kvh * (tiles + tree::kItem);
+          s_range[e] = tree::snapped(b[e], g0, tiles, ranges.snap);
           if (e == 0) { s_where[0] = s; s_where[1] = kvh; s_where[2] = block; s_range[2] = g0; }
         }
         before += mine;
@@ -331,7 +311,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
     it.s = s_where[0]; it.kvh = s_where[1]; it.block = s_where[2];
     it.r = request(a, it.s);
     fill(a, bt, &it);
-    int t0 = max(0, s_range[0] - s_range[2] - kItem), rest = left;
+    int t0 = max(0, s_range[0] - s_range[2] - tree::kItem), rest = left;
     auto next_item = [&] {
       if (++it.kvh >= a.kv_heads) {
         it.kvh = 0;
@@ -347,12 +327,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       t0 = 0;
       next_item();
     }
-    // the item's tiles of this range, and the cost that is left behind them
-    auto take_of = [&] {
-      const int start = t0 ? 0 : kItem, all = start + it.tiles - t0, take = rest >= all ? it.tiles - t0 : rest - start;
-      rest -= min(rest, all);
-      return take;
-    };
     const int group = a.q_heads / a.kv_heads;
     int gt = 0, item = 0;              // tiles and items of this range so far
 
@@ -362,7 +336,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const uint32_t ring = values ? v_s : k_s, full0 = values ? v_full(0) : k_full(0), empty0 = values ? v_empty(0) : k_empty(0);
       for (bool more = true; ok && more; ++item) {
         const uint64_t hint = it.r.rows > bt ? kEvictNormal : kEvictFirst;
-        const int take = take_of(), pages = (it.kv_end + 15) >> 4, p_begin = t0 * 4;
+        const int take = tree::take_of(t0, it.tiles, &rest), pages = (it.kv_end + 15) >> 4, p_begin = t0 * 4;
         const int* table = a.block_tables + static_cast<size_t>(it.s) * a.ld_tables;
         // the first row of a page's head; a page that the cache does not have lies behind its last row, where a load finds zeros
         auto look_up = [&](int base) {
@@ -400,7 +374,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
           __syncwarp();
         }
         if (!ok) break;
-        if (rest == 0 && t0 == 0 && take < it.tiles) cut = {it.r.row0 + it.first, it.nb * group, it.kvh, ranges.up_to(s_range[1] - take + it.tiles - ranges.snap - 1) - cta + 1};
+        if (rest == 0 && t0 == 0 && take < it.tiles) cut = {it.r.row0 + it.first, it.nb * group, it.kvh, ranges.parts(cta, s_range[1] - take, it.tiles)};
         t0 = 0;
         if ((more = rest > 0)) next_item();
       }
@@ -413,7 +387,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const uint32_t id_s = idesc_bf16(kRows, kKeys, 0);
       const uint64_t q_d = desc_sw128(q_s, 16, 1024), k_d = desc_sw128(k_s, 16, 1024);
       for (bool more = true; ok && more; ++item) {
-        const int take = take_of();
+        const int take = tree::take_of(t0, it.tiles, &rest);
         if (!(ok = warp_wait(q_full, item & 1))) break;
         for (int j = 0; j < take; ++j, ++gt) {
           const int b = gt & 1;
@@ -439,7 +413,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const uint32_t id_o = idesc_bf16(kRows, kD, 1);
       const uint64_t v_d = desc_sw128(v_s, kSlab, 1024);
       for (bool more = true; ok && more; ++item) {
-        const int take = take_of();
+        const int take = tree::take_of(t0, it.tiles, &rest);
         for (int j = 0; j < take; ++j, ++gt) {
           const int b = gt & 1, kv0 = (t0 + j) * kKeys;
           if (!(ok = warp_wait(v_full(b), (gt >> 1) & 1))) break;
@@ -487,7 +461,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
       const int q = warp & 3, row = q * 32 + lane;      // the quarter of the lanes that this warp may access
       const uint32_t lane_off = static_cast<uint32_t>(q * 32) << 16;
       for (bool more = true; ok && more; ++item) {
-        const int take = take_of(), rows = it.nb * group;
+        const int take = tree::take_of(t0, it.tiles, &rest), rows = it.nb * group;
         const bool valid = row < rows, some = row - lane < rows;      // this warp has rows
         const int token = it.first + row / group;
         const int* mask = a.masks && valid ? a.masks + static_cast<size_t>(it.r.row0 + token) * a.words : nullptr;

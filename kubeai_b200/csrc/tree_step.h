@@ -64,6 +64,41 @@ B200_HD int last_at_most(const int* v, int n, int x) {
   return lo;
 }
 
+// ---- the ranges that the work of an attention call is cut into.  All items' costs, in tiles of keys, lie one behind the other; range c begins at c * each + min(c, more).  An
+// item that begins at g0 has its tile t at g0 + kItem + t.
+constexpr int kItem = 2;      // what an item costs besides its tiles: its queries' trip and its rows' way out
+constexpr int kSnap = 3;      // a range does not end within this many tiles of an item's ends, or an eighth of its length
+constexpr int kLeast = 2;     // a range's cost at least
+struct Ranges {
+  int n, each, more, snap;
+  B200_HD int at(int c) const { return c * each + (c < more ? c : more); }
+  // in how many ranges from c on lies an item of which c has the beginning, but not all: the first tile at g, and how many tiles
+  B200_HD int parts(int c, int g, int tiles) const {
+    const int x = g + tiles - snap - 1;      // a range that begins in front of it, or there, has the last tiles
+    const int last = x < more * (each + 1) ? x / (each + 1) : more + (x - more * (each + 1)) / each;
+    return (last < n - 1 ? last : n - 1) - c + 1;
+  }
+};
+B200_HD Ranges ranges_of(int cost, int most) {
+  Ranges r;
+  r.n = cost / kLeast < 1 ? 1 : cost / kLeast < most ? cost / kLeast : most;
+  r.each = cost / r.n;
+  r.more = cost - r.each * r.n;
+  r.snap = r.each / 8 < kSnap ? r.each / 8 : kSnap;
+  return r;
+}
+// the beginning b of a range as it is moved to a tile of the item that begins at g0, its ends among them
+B200_HD int snapped(int b, int g0, int tiles, int snap) {
+  const int t = b - g0 - kItem;
+  return t <= snap ? g0 : g0 + kItem + (tiles - t <= snap ? tiles : t);
+}
+// The tiles from t0 on of an item that a range takes, which has *rest left, and what is left behind them
+B200_HD int take_of(int t0, int tiles, int* rest) {
+  const int start = t0 ? 0 : kItem, all = start + tiles - t0, take = *rest >= all ? tiles - t0 : *rest - start;
+  *rest -= *rest < all ? *rest : all;
+  return take;
+}
+
 // What a request asks of step_maps: rows (never negative), and pages beyond those it holds; -1 pages where its lengths do not fit.
 B200_HD int rows_asked(int n) { return n > 0 ? n : 0; }
 B200_HD int pages_asked(int ctx, int n, int held, int max_blocks, int words) {
