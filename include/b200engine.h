@@ -484,7 +484,7 @@ int b200_op_prompt_attn(const void* q, const void* q2, const void* kv, const voi
  * status [S]: 0, or bits: 1 too few pages left (the request gets none), 2 its lengths do not fit (negative, beyond its row of the table, fewer pages held than
  * ctx needs, more rows than 32 words or than T leaves), 4 a parent not in front of its child, which counts as -1.  Rows of a request with
  * 1 or 2 have slot -1, which b200_op_rope_kvwrite skips, position 0 and no mask bits; rows behind the last request the same and seq -1.
- * parents NULL: every row's parent is the one in front of it.  S <= 8192, words <= 8. */
+ * parents NULL: every row's parent is the one in front of it.  S <= 8192, T and num_free <= 2^30, words <= 8. */
 typedef struct {
   int32_t S, T, max_blocks, ld_tables, num_free, words;
   const int32_t* ctx;
@@ -509,7 +509,8 @@ int b200_op_step_maps(const b200_step_maps_args* a, void* stream);
  * heads; kv_layer [num_pages][2][kv_heads][16][128].  max_tree: most rows of a request; max_ctx: most tokens in front of them if known (0: what a row of the
  * table holds), which only decides how the work is split; zero_rest: rows of
  * requests that are left out and rows that no request owns become zeros.  A row that sees nothing is zero; what a row does not see has no part in it, NaN and infinities
- * too.  A page that the cache does not have reads as zeros.  q 16-byte and kv_layer 256-byte aligned, ldq a multiple of 8, ldo of 8, out 16-byte aligned. */
+ * too.  A page that the cache does not have reads as zeros.  q 16-byte and kv_layer 256-byte aligned, ldq a multiple of 8, ldo of 8, out 16-byte aligned.
+ * 0 < scale < 1e30, S <= 65534. */
 typedef struct {
   int32_t S, T, q_heads, kv_heads, ldq, ldo, max_blocks, ld_tables, words, max_tree, max_ctx, zero_rest;
   float scale;
@@ -524,7 +525,7 @@ typedef struct {
   void* workspace;
   int64_t workspace_bytes;
 } b200_tree_attn_args;
-/* Bytes of a call's workspace, which it uses until its kernels have run and which needs no preparation (a few tens of MB, by max_tree, T and heads alone).
+/* Bytes of a call's workspace, which it uses until its kernels have run and which needs no preparation: a few tens of MB, by the GPU alone (0 where nothing is to be done).
  * Calls that may run at once have one each. */
 int64_t b200_op_paged_attn_tree_workspace(const b200_tree_attn_args* a);
 int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream);
@@ -538,7 +539,7 @@ int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream);
  * drafts [T] (NULL: none): the step's tokens; a row's are those that masks [T, words] names (NULL: itself and every row of its request in front).
  * penalties fp32 [S][3]: repetition, presence, frequency (NULL: 1, 0, 0).  bias_starts [S + 1], bias_ids, bias_values, at most bias_len entries (NULL: none).
  * allow [allow_count][ld_allow words], bit v of a row: token v is allowed; allow_rows [T]: each row's mask, -1 for none (NULL: mask r, allow_count == T).
- * Tokens outside 0 .. V - 1 in any list count for nothing.  V <= 393216. */
+ * Tokens outside 0 .. V - 1 in any list count for nothing.  V <= 393216, S <= 65534, T and bias_len <= 2^30, history_len <= 2^29. */
 typedef struct {
   int32_t S, T, V, ld, logits_f32, ld_out, out_f32, words, history_len, bias_len, allow_count, ld_allow;
   const void* logits;

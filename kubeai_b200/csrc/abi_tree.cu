@@ -25,6 +25,7 @@ int b200_op_step_maps(const b200_step_maps_args* a, void* stream) {
   const char* op = "b200_op_step_maps";
   if (!a || a->S < 0 || a->T < 0 || a->max_blocks < 0 || a->num_free < 0 || a->ld_tables < a->max_blocks) return refuse(op, "bad sizes");
   if (a->S > tree::kMaxRequests) return refuse(op, "more than 8192 requests");
+  if (a->T > tree::kMaxRows || a->num_free > tree::kMaxRows) return refuse(op, "more than 2^30 rows or pages");
   if (a->words < 0 || a->words > tree::kMaxWords) return refuse(op, "masks of more than 8 words");
   if (a->max_blocks > INT_MAX / tree::kPage) return refuse(op, "positions pass 32 bits");
   if (!a->starts || !a->cursor || !a->cursor_out || (a->S && (!a->ctx || !a->rows || !a->held || !a->held_out || !a->status)) || (a->T && (!a->positions || !a->slots || (a->words && !a->masks))) ||
@@ -43,7 +44,7 @@ static int attn_sizes(const b200_tree_attn_args* a, const char* op) {
   if (a->masks && a->max_tree > 32 * a->words) return refuse(op, "more rows of a request than its masks have bits");
   if (a->max_blocks > INT_MAX / tree::kPage || a->num_pages >= INT_MAX / (32ll * a->kv_heads)) return refuse(op, "positions or cache rows pass 32 bits");
   if (static_cast<int64_t>(a->q_heads) * 128 > a->ldq || static_cast<int64_t>(a->q_heads) * 128 > a->ldo || a->ldq % 8 || a->ldo % 8) return refuse(op, "rows of q and out are whole heads, a multiple of 8 apart");
-  if (!(a->scale == a->scale)) return refuse(op, "scale is no number");
+  if (!(a->scale > 0.f && a->scale < 1e30f)) return refuse(op, "scale is no number above 0 and below 1e30");      // a row's maximum is looked for ahead of the scale
   const long long rows = static_cast<long long>(a->max_tree < a->T ? a->max_tree : a->T) * group;
   if ((rows + 127) / 128 * a->kv_heads > INT_MAX / 4 / (a->S + 1ll) / (a->max_blocks / 4 + 1)) return refuse(op, "the tiles of all requests pass 32 bits");
   return 0;
@@ -78,6 +79,7 @@ int b200_op_constrain(const b200_constrain_args* a, void* stream) {
   if (!a || a->S < 0 || a->T < 0 || a->V < 1 || a->ld < a->V || (a->out && a->ld_out < a->V)) return refuse(op, "bad sizes");
   if (a->V > 393216) return refuse(op, "more than 393216 tokens");
   if (a->S > 65534) return refuse(op, "more than 65534 requests");
+  if (a->T > tree::kMaxRows || a->history_len > tree::kMaxSaid || a->bias_len > tree::kMaxRows) return refuse(op, "more than 2^30 rows or biases or 2^29 tokens of histories");
   if (!a->starts && a->S != a->T) return refuse(op, "without starts every row is a request");
   if (a->words < 0 || a->words > tree::kMaxWords || (a->masks && !a->words)) return refuse(op, "masks of 1 to 8 words");
   if (a->masks && !a->drafts) return refuse(op, "masks without drafts");

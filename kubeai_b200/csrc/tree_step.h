@@ -23,6 +23,8 @@ constexpr int kPage = 16;             // tokens of a page
 constexpr int kMaxRequests = 8192;    // of a step_maps call: their offsets lie in shared memory
 constexpr int kMaxWords = 8;          // words of an ancestor mask: trees of up to 256 rows
 constexpr int kMaxTree = 2048;        // rows of a request that tree_accept walks
+constexpr int kMaxRows = 1 << 30;     // of a step, or entries of a list: an index may run past the end by the threads of a launch
+constexpr int kMaxSaid = 1 << 29;     // tokens of all histories: a count shares its word with two marks
 
 struct Request {
   int row0, rows, ctx;
