@@ -483,7 +483,7 @@ int b200_op_prompt_attn(const void* q, const void* q2, const void* kv, const voi
  * [T, words]: bit i of a row is set where row i of its request leads to it, itself among them; held_out, cursor_out (may be held and cursor);
  * status [S]: 0, or bits: 1 too few pages left (the request gets none), 2 its lengths do not fit (negative, beyond its row of the table, fewer pages held than
  * ctx needs, more rows than 32 words or than T leaves), 4 a parent not in front of its child, which counts as -1.  Rows of a request with
- * 1 or 2 have slot -1, which b200_op_rope_kvwrite skips, position 0 and no mask bits; rows behind the last request the same and seq -1.
+ * 1 or 2, and those on a page whose number is negative or passes 2^27 - 2, have slot -1, which b200_op_rope_kvwrite skips, position 0 and no mask bits; rows behind the last request the same and seq -1.
  * parents NULL: every row's parent is the one in front of it.  S <= 8192, T and num_free <= 2^30, words <= 8. */
 typedef struct {
   int32_t S, T, max_blocks, ld_tables, num_free, words;

@@ -2,7 +2,7 @@
 //
 //   starts = running sum of rows;  need_s = pages(ctx + rows) - held;  off = running sum of need
 //   a request is served while off + need <= pages left;  page(p) = p / 16 < held ? table[p / 16] : free[cursor + off + p / 16 - held]
-//   slot(i) = page(ctx + i) * 16 + (ctx + i) % 16;  ancestors(i) = {i} + ancestors(parent(i));  position(i) = ctx + |ancestors(i)| - 1
+//   slot(i) = page(ctx + i) * 16 + (ctx + i) % 16, -1 where the page's number is none;  ancestors(i) = {i} + ancestors(parent(i));  position(i) = ctx + |ancestors(i)| - 1
 //
 // What bounds it: the latency of a handful of dependent steps (lengths, two sums, a search, the stores), not bytes.  So one launch: every CTA
 // of one cluster sums all requests' lengths for itself, which is cheaper than handing sums on, and then works on its share of rows
@@ -131,7 +131,7 @@ step_maps_kernel(const b200_step_maps_args a) {
       if (!s_flags[seq]) {
         const int i = t - s_start[seq], ctx = a.ctx[seq], p = ctx + i, page = p >> 4, held = s_held[seq];
         const int number = page < held ? a.block_tables[static_cast<size_t>(seq) * a.ld_tables + page] : a.free_pages[first + s_off[seq] + page - held];
-        slot = number * tree::kPage + (p & 15);
+        slot = tree::slot_on(number, p);
         int depth = i;
         bool odd = false;
         if (a.parents) {

@@ -48,6 +48,9 @@ B200_HD long long cache_row(const int* table, int pos, long long num_pages) {
   return page >= 0 && page < num_pages ? static_cast<long long>(page) * kPage + (pos & 15) : -1;
 }
 
+// The slot of a position on a page of this number; -1, which is written nowhere, where the number is no page's.
+B200_HD int slot_on(int page, int pos) { return page >= 0 && page <= INT32_MAX / kPage - 1 ? page * kPage + (pos & 15) : -1; }
+
 // A parent counts where it lies in front of its child; every other number stands for the request's last token in the cache (-1).
 B200_HD int parent_of(const int* parents, int row0, int i) {
   if (!parents) return i - 1;
