@@ -611,7 +611,12 @@ tree_attn_join_kernel(const __grid_constant__ b200_tree_attn_args a, int ctas) {
 int64_t tree_attention_workspace(const b200_tree_attn_args&) { return static_cast<int64_t>(kPlaces) * sm_count() * (static_cast<int64_t>(sizeof(Cut)) + 2ll * kRows * kLd * sizeof(float)); }
 
 int paged_attention_tree(const b200_tree_attn_args& a, int* error, cudaStream_t st) {
-  const int group = a.q_heads / a.kv_heads, ctas = kPlaces * sm_count();
+  const int group = a.q_heads / a.kv_heads;
+  const int rows = static_cast<int>(std::min(static_cast<long long>(kRows), std::min(a.max_tree, a.T) * static_cast<long long>(group)));
+  // as many CTAs as there are places, or as the most work that the call may have feeds: 11.4 us for 1 x 450, over all places 12.0
+  const long long seen = std::min(a.max_ctx ? a.max_ctx : INT_MAX, a.max_blocks * tree::kPage) + static_cast<long long>(std::min(a.max_tree, a.T));
+  const long long items = (static_cast<long long>(std::min(a.max_tree, a.T)) * group + kRows - 1) / kRows * a.kv_heads * a.S, cost = items * ((seen + kKeys - 1) / kKeys + tree::kItem);
+  const int ctas = static_cast<int>(std::min<long long>(kPlaces * sm_count(), std::max<long long>(1, cost / tree::kLeast)));
   CUtensorMap tm_q, tm_kv;
   if (int rc = tmap_encode_bf16_3d(&tm_q, a.q, kD, a.q_heads, a.T, kD, a.ldq, 64, group, kRows / group)) return rc;
   if (int rc = tmap_encode_bf16_2d(&tm_kv, a.kv_layer, static_cast<uint64_t>(a.num_pages) * 2 * a.kv_heads * 16, kD, kD, 16, 64, 1)) return rc;
@@ -619,7 +624,6 @@ int paged_attention_tree(const b200_tree_attn_args& a, int* error, cudaStream_t 
   if (!ensure_dynamic_smem(tree_attn_kernel, kSmem, &attr_done)) return -3;
   launch_pdl(tree_attn_kernel, dim3(ctas), dim3(kThreads), kSmem, st, tm_q, tm_kv, a, a.scale * 1.4426950408889634f, error);
   if (cudaGetLastError() != cudaSuccess) return -2;
-  const int rows = static_cast<int>(std::min(static_cast<long long>(kRows), std::min(a.max_tree, a.T) * static_cast<long long>(group)));
   launch_pdl(tree_attn_join_kernel, dim3(ctas + (a.zero_rest ? 1 : 0), (rows + 7) / 8), dim3(256), 0, st, a, ctas);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
