@@ -5,13 +5,16 @@
 // A vocabulary's rows are long and what is said about single tokens is short.  A CTA marks the tokens of its part of the vocabulary that the request's lists
 // name with a bit each.  The bits' running count gives every such token a slot, where its count, its bias and its number lie: as much shared memory as there
 // is to say, whatever the vocabulary.  More tokens than slots: the part is worked on in pieces that have no more.  All of this is done once for the rows of a
-// request that the CTA takes.  A row then comes in chunks of 16 KB by bulk copies, several ahead, from one row into the next; of its vectors eight tokens cost
+// request that the CTA takes.  A row then comes in chunks of 8192 tokens by bulk copies, two or three ahead, from one row into the next; of its vectors eight tokens cost
 // a maximum of pairs, marked tokens left out, and the chunk's slots, a thread each, alone need the formula.  A row's drafts are counted in ahead of it and out
 // behind it.  Few rows: a cluster of CTAs shares the vocabulary, whose best pairs (value, token) meet through distributed shared memory.  Ties go to the lowest token:
 // every comparison prefers it.  Every wait for a copy has a limit; a CTA that gives up sets an error mark.
 //
-// What bounds it: for many rows the copies; for one row each the lists' chain of look-ups, marks and counts ahead of it.  With the formula inside the pass over the
-// vectors, where it ran in nearly every warp for a few of its lanes, and a row over 16 CTAs that all read the lists, 128 rows of 128256 tokens took 99 us.
+// What bounds it: the lists' chain of look-ups, marks, slots and counts ahead of the rows, which is half of a CTA's time where it has one or two rows (128 rows of 128256
+// bf16 logits, 4000 tokens of history each: 25 us, of which the copies need 5; one row 8.2), and for trees the copies in and out behind it (264 rows of 99991 fp32
+// logits, kept: 82 us, 2.6 TB/s).  With the formula inside the pass over the vectors, where it ran in nearly every warp for a few of its lanes, and a row over 16 CTAs
+// that all read the lists, the 128 rows took 99 us; a thread that takes the marked tokens of its own 32 of a chunk in place of a slot, 34 (and the trees 112); slots' tokens
+// found by walking the words in place of being written by who counts them, 28.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <limits.h>
@@ -316,23 +319,26 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
       return k >= 0 && w >= word0 && w < word1 ? slot_of[w] - slot0 + __popc(known[w] & ((1u << (k & 31)) - 1)) : -1;
     };
     for (int i = tid; i < slots; i += kThreads) count[i] = 0, entry[i] = -1;
-    for (int w = word0 + tid; w < word1; w += kThreads) {
-      int n = slot_of[w] - slot0;
-      for (unsigned bits = known[w]; bits; bits &= bits - 1) token[n++] = static_cast<uint16_t>(32 * w + __ffs(bits) - 1);
-    }
     __syncthreads();
     history([&](int k, bool in_prompt) {
       const int i = slot(k);
       if (i < 0) return;
+      token[i] = static_cast<uint16_t>(k);      // (whoever else names it writes the same)
       if (in_prompt) atomicOr(count + i, kPrompt);
       else atomicAdd(count + i, 1u);
     });
     const int bias_slot = slot(bias_at), draft_slot = slot(draft_at);
-    if (bias_slot >= 0) atomicMax(entry + bias_slot, b0 + tid);
+    if (bias_slot >= 0) token[bias_slot] = static_cast<uint16_t>(bias_at), atomicMax(entry + bias_slot, b0 + tid);
     for (int e = b0 + kThreads + tid; e < b1; e += kThreads) {
-      const int i = slot(place(a.bias_ids[e]));
-      if (i >= 0) atomicMax(entry + i, e);
+      const int k = place(a.bias_ids[e]), i = slot(k);
+      if (i >= 0) token[i] = static_cast<uint16_t>(k), atomicMax(entry + i, e);
     }
+    if (draft_slot >= 0) token[draft_slot] = static_cast<uint16_t>(draft_at);
+    if (a.drafts)
+      for (int e = kThreads + tid; e < rows; e += kThreads) {
+        const int k = place(a.drafts[row0 + e]), i = slot(k);
+        if (i >= 0) token[i] = static_cast<uint16_t>(k);
+      }
     __syncthreads();
     // an entry becomes its bias, by the thread that has the last one of its token
     if (b1 - b0 <= kThreads) {
@@ -494,9 +500,9 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
 template <typename TIn, typename TOut>
 int launch(const b200_constrain_args& a, int* error, cudaStream_t st) {
   const auto kernel = constrain_kernel<TIn, TOut>;
-  // A request has one row: as many CTAs as the SMs have places, a row over several of them where that leaves some free (128 rows of 128256 tokens: 27.8 us
-  // over two, 37 over one, 38 over four; one row 8.5 us over 16, 27 over one).  Several rows: their numbers differ, and most groups of a row end at once, so four
-  // times that (16 trees of up to 32 rows of 99991 fp32 logits: 85 us over four CTAs, 99 over one, 104 over two).  More rows than that: groups of several,
+  // A request has one row: as many CTAs as the SMs have places, a row over several of them where that leaves some free (128 rows of 128256 tokens: 28 us
+  // over two, 37 over one, 38 over four; one row 8.5 us over 16, 27 over one; with the tables as they were then; now 25 and 8.2).  Several rows: their numbers differ, and most groups of a row end at once, so four
+  // times that (16 trees of up to 32 rows of 99991 fp32 logits: 82 us over four CTAs, 96 over one, 100 over two).  More rows than that: groups of several,
   // which read their request's lists once.
   const long long places = static_cast<long long>(kPlaces) * sm_count(), each = a.starts ? (a.T + a.S - 1) / a.S : 1;
   const int groups = static_cast<int>(std::max<long long>((a.T + kRows - 1) / kRows, a.S * each <= places ? each : std::min(each, (3 * places + a.S - 1) / a.S)));
