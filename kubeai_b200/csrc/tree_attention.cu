@@ -10,8 +10,9 @@
 //   costs its warp 100 cycles all the same, and one warp for both took 1500 a tile of which the tensor cores need 640;
 //   four warps (thread = row) do the softmax in fp32, base 2; a warp whose rows nobody owns only keeps step.
 // While one CTA of an SM ends an item, the other one keeps the memory busy.  (One CTA an SM with two softmax groups that took a row tile's keys in turn, or a row
-// tile each, stopped for 3 us at each item: 64 x 2048 74.8 us, 48 x 1999 with 64 rows 90.)  More than 128 rows: items side by side, which find each other's
-// pages in L2.
+// tile each, stopped for 3 us at each item: 64 x 2048 74.8 us.)  More than 128 rows: items side by side, which find each other's pages in L2.
+// What bounds it: K and V's bytes to three quarters (64 requests of 2048 tokens, 32 heads on 8: 62 us, 320 MB, 5.1 TB/s; two of 32001: 55 us, 4.7 TB/s), the rest is
+// ranges' first loads and the join; with 256 rows of a key head (48 x 1999 tokens, 64 rows, 83 us) the softmax, whose 1450 cycles a tile of 128 x 64 two CTAs share an SM for.
 // The masks' bits are looked at only in tiles that reach behind the context.  There the products' warp also clears what must not meet a weight of zero:
 // values behind the last key, and infinities and NaN among the drafts' values, which the rows that see them add at the end by themselves.
 // An item that a range's end cuts leaves unnormalised rows in the workspace, which a second kernel joins in a fixed order: the same bits every time.
@@ -40,6 +41,7 @@ constexpr int kThreads = 256, kWarps = kThreads / 32, kPlaces = 2;              
 constexpr int kDepth = 2;                  // tiles of keys, and of values, on their way
 constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
 constexpr float kSlack = 8.f;              // by which a row's maximum may pass what its weights are relative to, in units of log 2
+constexpr int kJoinThreads = 256, kJoinPlaces = 3, kJoinAtOnce = 8, kFew = 4;      // kJoinPlaces: CTAs of an SM; kJoinAtOnce: parts on their way
 constexpr int kWaitLimit = 1 << 22;
 
 // shared memory: queries, keys, values, 2 KB a softmax warp for its way out, barriers
@@ -127,6 +129,7 @@ __device__ __forceinline__ void fill(const b200_tree_attn_args& a, int bt, Item*
   it->kv_end = it->r.ctx + (a.masks ? it->r.rows : it->first + it->nb);
   it->tiles = tiles_of(a, it->r, bt, it->block);
 }
+
 // What a CTA leaves for the second kernel: the item that begins in its range and ends behind it, and in how many ranges it lies (0: no such item).
 struct Cut {
   int row0, rows, kvh, parts;      // the item's first row of the step, rows (token * group + head)
@@ -558,51 +561,119 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
   }
 }
 
-// Rows of items that ranges' ends cut: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts, in order.  A warp a row.
-__global__ void __launch_bounds__(256)
-tree_attn_join_kernel(const __grid_constant__ b200_tree_attn_args a, int ctas) {
-  constexpr int kAtOnce = 12;
-  griddep_enter();
-  if (static_cast<int>(blockIdx.x) == ctas) {
-    if (blockIdx.y == 0) zero_rest(a);
-    return;
+// A row of an item that ranges' ends cut: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts, in order, four dimensions a lane: the form for few parts.
+template <typename Part>
+__device__ __forceinline__ void join_few(int parts, Part part, int lane, uint2* out) {
+  float m = -INFINITY, sum = 0.f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < parts; p0 += kFew) {
+    float2 st[kFew];
+    float4 x[kFew];
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < kFew; ++k) {
+      const bool there = p0 + k < parts;
+      st[k] = there ? *reinterpret_cast<const float2*>(part(p0 + k) + kD) : make_float2(-INFINITY, 0.f);
+      x[k] = there ? *reinterpret_cast<const float4*>(part(p0 + k) + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < kFew; ++k) top = fmaxf(top, st[k].x);
+    const float base = top == -INFINITY ? 0.f : top, old = exp2f(m - base);
+    m = top;
+    sum *= old;
+    y = make_float4(y.x * old, y.y * old, y.z * old, y.w * old);
+#pragma unroll
+    for (int k = 0; k < kFew; ++k) {
+      const float w = exp2f(st[k].x - base);
+      sum += w == 0.f && st[k].y == st[k].y ? 0.f : st[k].y * w;
+      if (w != 0.f) y = make_float4(fmaf(x[k].x, w, y.x), fmaf(x[k].y, w, y.y), fmaf(x[k].z, w, y.z), fmaf(x[k].w, w, y.w));
+    }
   }
-  const Cut cut = static_cast<const Cut*>(a.workspace)[blockIdx.x];
-  if (!cut.parts) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.q_heads / a.kv_heads;
-  const float* ws = rows_of(a.workspace, ctas);
-  for (int row = blockIdx.y * 8 + warp; row < cut.rows; row += gridDim.y * 8) {
-    // the item's beginning lies in its range's second place, each other part in its range's first
-    auto part = [&](int p) { return ws + (static_cast<size_t>(2 * (blockIdx.x + p) + (p == 0)) * kRows + row) * kLd; };
-    float m = -INFINITY, sum = 0.f;
-    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p0 = 0; p0 < cut.parts; p0 += kAtOnce) {
-      float2 st[kAtOnce];
-      float4 x[kAtOnce];
-      float top = m;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *out = make_uint2(pack_bf16x2(y.x * inv, y.y * inv), pack_bf16x2(y.z * inv, y.w * inv));
+}
+
+// The form for many: a lane has the maximum, sum and weight of one part in 32.
+template <typename Part>
+__device__ __forceinline__ void join_row(int parts, Part part, int lane, uint2* out) {
+  float m = -INFINITY, sum = 0.f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < parts; p0 += 32) {
+    const int n = min(32, parts - p0);
+    const float2 st = lane < n ? *reinterpret_cast<const float2*>(part(p0 + lane) + kD) : make_float2(-INFINITY, 0.f);
+    float4 x[kJoinAtOnce];
+    auto load = [&](int k0) {
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        const bool there = p0 + k < cut.parts;
-        st[k] = there ? *reinterpret_cast<const float2*>(part(p0 + k) + kD) : make_float2(-INFINITY, 0.f);
-        x[k] = there ? *reinterpret_cast<const float4*>(part(p0 + k) + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+      for (int k = 0; k < kJoinAtOnce; ++k)
+        if (k0 + k < n) x[k] = *reinterpret_cast<const float4*>(part(p0 + k0 + k) + lane * 4);
+    };
+    load(0);
+    float top = fmaxf(m, st.x);
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) top = fmaxf(top, st[k].x);
-      const float base = top == -INFINITY ? 0.f : top, old = exp2f(m - base);
-      m = top;
-      sum *= old;
-      y = make_float4(y.x * old, y.y * old, y.z * old, y.w * old);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.f : top, old = exp2f(m - base), w = exp2f(st.x - base);
+    m = top;
+    float l = w == 0.f && st.y == st.y ? 0.f : st.y * w;
 #pragma unroll
-      for (int k = 0; k < kAtOnce; ++k) {
-        const float w = exp2f(st[k].x - base);
-        sum += w == 0.f && st[k].y == st[k].y ? 0.f : st[k].y * w;
-        if (w != 0.f) y = make_float4(fmaf(x[k].x, w, y.x), fmaf(x[k].y, w, y.y), fmaf(x[k].z, w, y.z), fmaf(x[k].w, w, y.w));
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    sum = sum * old + l;
+    y = make_float4(y.x * old, y.y * old, y.z * old, y.w * old);
+    for (int k0 = 0; k0 < n; k0 += kJoinAtOnce) {
+      if (k0) load(k0);
+#pragma unroll
+      for (int k = 0; k < kJoinAtOnce; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, w, (k0 + k) & 31);
+        if (k0 + k < n && wk != 0.f) y = make_float4(fmaf(x[k].x, wk, y.x), fmaf(x[k].y, wk, y.y), fmaf(x[k].z, wk, y.z), fmaf(x[k].w, wk, y.w));
       }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int token = cut.row0 + row / group;
-    *reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + static_cast<size_t>(token) * a.ldo + (cut.kvh * group + row % group) * kD + lane * 4) =
-        make_uint2(pack_bf16x2(y.x * inv, y.y * inv), pack_bf16x2(y.z * inv, y.w * inv));
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  *out = make_uint2(pack_bf16x2(y.x * inv, y.y * inv), pack_bf16x2(y.z * inv, y.w * inv));
+}
+
+// All such rows, a warp each: every block sums the cut items' rows for itself and takes its share.  What bounds it is the chain from the first kernel's end (the cuts,
+// a search, statistics, parts), some 5 us of a call.  A block for eight rows of each CTA's item, of which most had none, came in eleven waves and with the form of
+// twelve parts at once for every row: 64 x 2048 64.6 us a call in place of 62.4, 2 x 32001 59.9 in place of 55.4, 48 x 1999 with 64 rows 91.4 in place of 83.5.
+__global__ void __launch_bounds__(kJoinThreads, kJoinPlaces)
+tree_attn_join_kernel(const __grid_constant__ b200_tree_attn_args a, int ctas, int blocks) {
+  extern __shared__ int rows_before[];      // [ctas + 1] of each CTA's cut item
+  __shared__ int sums[kJoinThreads / 32];
+  griddep_enter();
+  if (static_cast<int>(blockIdx.x) == blocks) return zero_rest(a);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = a.q_heads / a.kv_heads;
+  const Cut* cuts = static_cast<const Cut*>(a.workspace);
+  const int per = (ctas + kJoinThreads - 1) / kJoinThreads, begin = min(ctas, tid * per), end = min(ctas, begin + per);
+  int before = 0, all = 0;
+  for (int c = begin; c < end; ++c) before += cuts[c].parts ? cuts[c].rows : 0;
+  const int own = before;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += y;
+  }
+  if (lane == 31) sums[warp] = before;
+  __syncthreads();
+  before -= own;
+#pragma unroll
+  for (int w = 0; w < kJoinThreads / 32; ++w) {
+    if (w < warp) before += sums[w];
+    all += sums[w];
+  }
+  for (int c = begin; c < end; ++c) {
+    rows_before[c] = before;
+    before += cuts[c].parts ? cuts[c].rows : 0;
+  }
+  if (tid == 0) rows_before[ctas] = all;
+  __syncthreads();
+  const float* ws = rows_of(a.workspace, ctas);
+  for (int n = blockIdx.x * (kJoinThreads / 32) + warp; n < all; n += blocks * (kJoinThreads / 32)) {
+    const int c = tree::last_at_most(rows_before, ctas, n), row = n - rows_before[c];
+    const Cut cut = cuts[c];
+    // the item's beginning lies in its range's second place, each other part in its range's first
+    auto part = [&](int p) { return ws + (static_cast<size_t>(2 * (c + p) + (p == 0)) * kRows + row) * kLd; };
+    uint2* out = reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + static_cast<size_t>(cut.row0 + row / group) * a.ldo + (cut.kvh * group + row % group) * kD + lane * 4);
+    if (cut.parts <= kFew) join_few(cut.parts, part, lane, out);
+    else join_row(cut.parts, part, lane, out);
   }
 }
 
@@ -624,7 +695,8 @@ int paged_attention_tree(const b200_tree_attn_args& a, int* error, cudaStream_t 
   if (!ensure_dynamic_smem(tree_attn_kernel, kSmem, &attr_done)) return -3;
   launch_pdl(tree_attn_kernel, dim3(ctas), dim3(kThreads), kSmem, st, tm_q, tm_kv, a, a.scale * 1.4426950408889634f, error);
   if (cudaGetLastError() != cudaSuccess) return -2;
-  launch_pdl(tree_attn_join_kernel, dim3(ctas + (a.zero_rest ? 1 : 0), (rows + 7) / 8), dim3(256), 0, st, a, ctas);
+  const int blocks = std::min(kJoinPlaces * sm_count(), (ctas * rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
+  launch_pdl(tree_attn_join_kernel, dim3(blocks + (a.zero_rest ? 1 : 0)), dim3(kJoinThreads), (ctas + 1) * sizeof(int), st, a, ctas, blocks);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
