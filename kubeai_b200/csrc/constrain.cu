@@ -11,8 +11,8 @@
 // every comparison prefers it.  Every wait for a copy has a limit; a CTA that gives up sets an error mark.
 //
 // What bounds it: the lists' chain of look-ups, marks, slots and counts ahead of the rows, which is half of a CTA's time where it has one or two rows (128 rows of 128256
-// bf16 logits, 4000 tokens of history each: 25 us, of which the copies need 5; one row 8.2), and for trees the copies in and out behind it (264 rows of 99991 fp32
-// logits, kept: 82 us, 2.6 TB/s).  With the formula inside the pass over the vectors, where it ran in nearly every warp for a few of its lanes, and a row over 16 CTAs
+// bf16 logits, 4000 tokens of history each: 25 us, of which the copies need 5; one row 8.2), and for trees the copies in and out behind it (288 rows of 99991 fp32
+// logits, kept: 82 us, 2.8 TB/s).  With the formula inside the pass over the vectors, where it ran in nearly every warp for a few of its lanes, and a row over 16 CTAs
 // that all read the lists, the 128 rows took 99 us; a thread that takes the marked tokens of its own 32 of a chunk in place of a slot, 34 (and the trees 112); slots' tokens
 // found by walking the words in place of being written by who counts them, 28.
 #include <cuda_bf16.h>
