@@ -78,8 +78,8 @@ __device__ __forceinline__ uint32_t seen_bits(const int* mask, int words, int i,
   return __funnelshift_r(word(j >> 5), word((j >> 5) + 1), j & 31);
 }
 
-// Rows that no request owns, and those of requests that are left out, become zeros (one block).
-__device__ void zero_rest(const b200_tree_attn_args& a) {
+// Of the rows that no request owns, and those of requests that are left out, every parts-th one becomes zeros (one block).
+__device__ void zero_rest(const b200_tree_attn_args& a, int part, int parts) {
   bool plain = true;
   for (int s = threadIdx.x; s < a.S; s += blockDim.x) {
     const int rows = a.starts[s + 1] - a.starts[s];
@@ -87,9 +87,9 @@ __device__ void zero_rest(const b200_tree_attn_args& a) {
   }
   plain = __syncthreads_and(plain);
   const int from = plain && a.S ? a.starts[0] : 0, to = plain && a.S ? a.starts[a.S] : 0;
-  for (int t = 0; t < a.T; ++t) {
+  for (int t = part; t < a.T; t += parts) {
     bool owned = plain && t >= from && t < to;
-    if (owned) { t = to - 1; continue; }
+    if (owned) { t += (to - 1 - t) / parts * parts; continue; }
     for (int s = 0; !plain && s < a.S && !owned; ++s) {
       const tree::Request r = tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, a.max_tree);
       owned = t >= r.row0 && t < r.row0 + r.rows;
@@ -639,7 +639,7 @@ tree_attn_join_kernel(const __grid_constant__ b200_tree_attn_args a, int ctas, i
   extern __shared__ int rows_before[];      // [ctas + 1] of each CTA's cut item
   __shared__ int sums[kJoinThreads / 32];
   griddep_enter();
-  if (static_cast<int>(blockIdx.x) == blocks) return zero_rest(a);
+  if (static_cast<int>(blockIdx.x) >= blocks) return zero_rest(a, blockIdx.x - blocks, gridDim.x - blocks);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, group = a.q_heads / a.kv_heads;
   const Cut* cuts = static_cast<const Cut*>(a.workspace);
   const int per = (ctas + kJoinThreads - 1) / kJoinThreads, begin = min(ctas, tid * per), end = min(ctas, begin + per);
@@ -696,7 +696,8 @@ int paged_attention_tree(const b200_tree_attn_args& a, int* error, cudaStream_t 
   launch_pdl(tree_attn_kernel, dim3(ctas), dim3(kThreads), kSmem, st, tm_q, tm_kv, a, a.scale * 1.4426950408889634f, error);
   if (cudaGetLastError() != cudaSuccess) return -2;
   const int blocks = std::min(kJoinPlaces * sm_count(), (ctas * rows + kJoinThreads / 32 - 1) / (kJoinThreads / 32));
-  launch_pdl(tree_attn_join_kernel, dim3(blocks + (a.zero_rest ? 1 : 0)), dim3(kJoinThreads), (ctas + 1) * sizeof(int), st, a, ctas, blocks);
+  const int zeros = a.zero_rest ? std::min(64, a.T / 16 + 1) : 0;      // blocks behind those
+  launch_pdl(tree_attn_join_kernel, dim3(blocks + zeros), dim3(kJoinThreads), (ctas + 1) * sizeof(int), st, a, ctas, blocks);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 

@@ -76,6 +76,24 @@ def test_attention_of_large_scores():
     check_attention(c, run_attention(c))
 
 
+@pytest.mark.parametrize("extra,ctx", [(1, [40, 70, 3]), (700, [40, 70, 3]), (2900, [40, 1 << 20, 3]), (15, [-1, 70, 3])])
+def test_attention_of_a_padded_batch_is_zero_in_rows_that_nobody_owns(extra, ctx):
+    """Behind the last request, and those of requests whose lengths are none, in a new output over memory that held something else."""
+    from kubeai_b200 import ops
+    c = attention_case(50, [40, 70, 3], [10, 21, 30], 2, 4, extra=extra)
+    torch.full((c["T"] + extra, c["heads"] * 128), float("nan"), dtype=torch.bfloat16, device="cuda")      # given back at once: what the output is likely to lie on
+    got = ops.paged_attn_tree(c["qkv"].cuda(), c["kv"].cuda(), ints(c["tables"]), ints(c["starts"]), ints(ctx), ints(c["bits"]), c["heads"], c["kv_heads"], 30)
+    whole = run_attention(c)
+    assert (got[c["T"]:] == 0).all() and (whole[c["T"]:] == 0).all()
+    for s in range(3):
+        rows = slice(c["starts"][s], c["starts"][s + 1])
+        if ctx[s] == c["ctx"][s]:
+            whole[rows] = got[rows]
+        else:
+            assert (got[rows] == 0).all()
+    check_attention(c, whole)
+
+
 # ------------------------------------------------------------------ constrain
 @pytest.mark.parametrize("rows,V,history,f32", [([1], 128256, 60000, False), ([1], 393216, 200000, True), ([3, 9], 50021, 30000, True), ([70, 70], 20011, 9000, False)])
 def test_constrain_with_more_marked_tokens_than_slots(rows, V, history, f32):
