@@ -152,6 +152,34 @@ def test_accept_of_more_requests_than_places():
     assert np.array_equal(kv.cpu().view(torch.int16).numpy(), want["kv"])
 
 
+def test_accept_far_into_a_large_cache():
+    """Layers and pages behind 2^31 values and 2^32 bytes."""
+    from kubeai_b200 import ops
+    c = accept_case(12, [10, 3], [30, 30], 2, 2)
+    want = U.accepted(c["ids"], c["drafts"], c["parents"], c["starts"], c["ctx"], c["tables"], c["kv"].view(torch.int16).numpy(), 16)
+    assert max(want["accepted"]) > 1
+    big = torch.zeros(2, 140000, 2, 2, 16, 128, dtype=torch.bfloat16, device="cuda")
+    at = np.array([139999 - 37 * i for i in range(c["kv"].shape[1])])
+    big[:, torch.tensor(at).cuda()] = c["kv"].cuda()
+    got = ops.tree_accept(ints(c["ids"]), ints(c["drafts"]), ints(c["parents"]), ints(c["starts"]), ints(c["ctx"]), ints(at[np.maximum(c["tables"], 0)]), big, 16)
+    assert got.path.tolist() == want["path"]
+    assert np.array_equal(big[:, torch.tensor(at).cuda()].cpu().view(torch.int16).numpy(), want["kv"])
+
+
+def test_constrain_far_into_many_rows():
+    """Rows behind 2^31 values and 2^32 bytes, in place."""
+    from kubeai_b200 import ops
+    T, V = 17000, 128256
+    x = torch.zeros(T, V, dtype=torch.bfloat16, device="cuda")
+    x[T - 1, 100000], x[T - 1, 77], x[T - 2, 128255], x[0, 5] = 2.0, 1.0, 1.0, 1.0
+    starts = np.zeros(T + 1, dtype=np.int64)
+    starts[T] = 1
+    ids, y = ops.constrain(x, bias=(ints(starts), ints([77]), torch.tensor([5.0]).cuda()), out=x)
+    ids = ids.tolist()
+    assert y is x and ids[T - 1] == 77 and ids[T - 2] == 128255 and ids[0] == 5 and not any(ids[1:T - 2])
+    assert x[T - 1, 77] == 6 and x[T - 1, 100000] == 2 and x[T - 2].sum() == 1 and x[T // 2].abs().sum() == 0
+
+
 # ------------------------------------------------------------------ graphs, streams, devices
 def test_two_graphs_replayed_at_once():
     """Each graph has its own workspace: side by side they give what they give alone."""
