@@ -476,7 +476,9 @@ int b200_op_prompt_attn(const void* q, const void* q2, const void* kv, const voi
  * of its request in front of it, or -1.  Row i lies in the cache at position ctx + i, whatever its depth.  All integers int32 on the device.
  * No argument that the device holds makes a kernel read or write outside the buffers: a request whose lengths do not fit (starts that
  * descend or pass T, more rows than max_tree, a negative ctx, more tokens than its row of the block table holds) is left out and what
- * it would have written stays as it was, rows that no request owns too, but where an operation says what becomes of them.  Calls may run side by side on several streams and be captured; they keep nothing. */
+ * it would have written stays as it was, rows that no request owns too, but where an operation says what becomes of them.
+ * A request that step_maps turned away (status 1 or 2) has lengths that fit all the same, but no K and V for its rows, and its table behind the pages that it holds
+ * names anybody's: the three operations behind step_maps take its status [S] and leave such requests out.  NULL says that there is none.  Calls may run side by side on several streams and be captured; they keep nothing. */
 /* Block tables and slot maps from lengths.  Request s brings rows[s] tokens and holds held[s] pages, at least those of its ctx tokens; the pages it
  * lacks are taken from free_pages[cursor ..], in the order of the requests, and written behind those in its row of block_tables.
  * Out: starts [S + 1]; for each of the T rows positions (ctx + depth), slots (page * 16 + offset), seqs (optional: its request) and, with words > 0, masks
@@ -524,6 +526,7 @@ typedef struct {
   const int32_t* masks;
   void* workspace;
   int64_t workspace_bytes;
+  const int32_t* status;
 } b200_tree_attn_args;
 /* Bytes of a call's workspace, which it uses until its kernels have run and which needs no preparation: a few tens of MB, by the GPU alone (0 where nothing is to be done).
  * Calls that may run at once have one each. */
@@ -533,7 +536,7 @@ int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream);
  *   y = x;  a token among the request's history or the row's drafts: y = y > 0 ? y / repetition : y * repetition;
  *   y -= frequency * c, then y -= presence where c > 0, c = how often it stands in the history behind prompt_lens tokens and in the row's drafts;
  *   y += bias, the last of the request's entries for the token;  a token that the row's mask does not allow: -inf.
- * ids [T] (optional): the lowest allowed token of the largest y, NaN counting as -inf; -1 where none is allowed and for rows that no request owns.  out (optional): y, fp32 or bf16 (out_f32), rows
+ * ids [T] (optional): the lowest allowed token of the largest y, NaN counting as -inf; -1 where none is allowed, for rows that no request owns and for those of requests that are left out.  out (optional): y, fp32 or bf16 (out_f32), rows
  * ld_out apart; may be logits itself where type and ld are the same.
  * starts NULL: row r belongs to request r (S == T).  history: the requests' tokens one behind the other, hist_starts [S + 1], at most history_len; NULL: none.
  * drafts [T] (NULL: none): the step's tokens; a row's are those that masks [T, words] names (NULL: itself and every row of its request in front).
@@ -557,12 +560,13 @@ typedef struct {
   const float* bias_values;
   const int32_t* allow;
   const int32_t* allow_rows;
+  const int32_t* status;
 } b200_constrain_args;
 int b200_op_constrain(const b200_constrain_args* a, void* stream);
 /* The drafts that the choices confirm.  From row 0 of a request on, the path goes to the lowest row whose parent is the path's last row and whose draft is
  * ids of that row, up to max_path rows; the paths' K and V rows move to positions ctx, ctx + 1, ... of the cache [layers][num_pages][2][kv_heads][16][128] (layers
  * layer_stride elements apart).  Out: accepted [S] rows of the path, path [S, max_path] and tokens [S, max_path] = ids of the path's rows (-1 behind the
- * last), new_ctx [S] = ctx + accepted (not ctx itself).  A request without rows, with more than 2048 or whose lengths do not fit accepts 0.  parents NULL: a chain.
+ * last), new_ctx [S] = ctx + accepted (not ctx itself).  A request without rows, with more than 2048, whose lengths do not fit or that step_maps turned away accepts 0.  parents NULL: a chain.
  * A move from or to a page that the cache does not have is left out. */
 typedef struct {
   int32_t S, T, max_blocks, ld_tables, max_path, layers, kv_heads;
@@ -578,6 +582,7 @@ typedef struct {
   int32_t* path;
   int32_t* tokens;
   int32_t* new_ctx;
+  const int32_t* status;
 } b200_tree_accept_args;
 int b200_op_tree_accept(const b200_tree_accept_args* a, void* stream);
 int b200_op_init_uniform(void* p, uint64_t n, uint32_t seed, float scale, float offset, void* stream);

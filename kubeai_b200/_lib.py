@@ -49,19 +49,20 @@ class StepMapsArgs(C.Structure):
 
 class TreeAttnArgs(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("S", "T", "q_heads", "kv_heads", "ldq", "ldo", "max_blocks", "ld_tables", "words", "max_tree", "max_ctx", "zero_rest")] + \
-        [("scale", C.c_float), ("num_pages", C.c_int64)] + [(n, C.c_void_p) for n in ("q", "out", "kv_layer", "block_tables", "starts", "ctx", "masks", "workspace")] + [("workspace_bytes", C.c_int64)]
+        [("scale", C.c_float), ("num_pages", C.c_int64)] + [(n, C.c_void_p) for n in ("q", "out", "kv_layer", "block_tables", "starts", "ctx", "masks", "workspace")] + \
+        [("workspace_bytes", C.c_int64), ("status", C.c_void_p)]
 
 
 class ConstrainArgs(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("S", "T", "V", "ld", "logits_f32", "ld_out", "out_f32", "words", "history_len", "bias_len", "allow_count", "ld_allow")] + \
         [(n, C.c_void_p) for n in ("logits", "out", "ids", "starts", "history", "hist_starts", "prompt_lens", "drafts", "masks", "penalties",
-                                   "bias_starts", "bias_ids", "bias_values", "allow", "allow_rows")]
+                                   "bias_starts", "bias_ids", "bias_values", "allow", "allow_rows", "status")]
 
 
 class TreeAcceptArgs(C.Structure):
     _fields_ = [(n, C.c_int32) for n in ("S", "T", "max_blocks", "ld_tables", "max_path", "layers", "kv_heads")] + \
         [(n, C.c_int64) for n in ("num_pages", "layer_stride")] + \
-        [(n, C.c_void_p) for n in ("ids", "drafts", "parents", "starts", "ctx", "block_tables", "kv", "accepted", "path", "tokens", "new_ctx")]
+        [(n, C.c_void_p) for n in ("ids", "drafts", "parents", "starts", "ctx", "block_tables", "kv", "accepted", "path", "tokens", "new_ctx", "status")]
 
 
 class FeedEntry(C.Structure):

@@ -173,7 +173,12 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
   if (a.starts) rows = row0 >= 0 && rows >= row0 && rows <= a.T ? rows - row0 : 0;
   h0 = max(h0, 0), h1 = min(h1, a.history_len);
   b0 = max(b0, 0), b1 = min(b1, a.bias_len);
-  if (group >= rows) return;      // (the whole cluster)
+  if (tree::turned_away(a.status, s)) {      // its rows have no choice
+    if (!group && a.ids)
+      for (int i = rank * kThreads + tid; i < rows; i += ctas * kThreads) a.ids[row0 + i] = -1;
+    return;      // (the whole cluster)
+  }
+  if (group >= rows) return;
   const int my_rows = (rows - group + groups - 1) / groups;
   for (int w = tid; w < part_words + 2; w += kThreads) known[w - 1] = 0;
   for (int d = tid; d < kRows; d += kThreads) best_of[d] = 0;

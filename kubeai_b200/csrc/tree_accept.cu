@@ -32,7 +32,7 @@ tree_accept_kernel(const b200_tree_accept_args a) {
   const int s = blockIdx.x, tid = threadIdx.x;
   // new lengths and tokens may be read by a kernel behind this one ahead of its dependency wait: none is let in before the end
   griddep_wait();
-  const tree::Request r = tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, tree::kMaxTree);
+  const tree::Request r = tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, tree::kMaxTree, a.status);
   for (int i = tid; i < r.rows; i += kThreads) child[i] = INT_MAX;
   __syncthreads();
   for (int i = tid; i < r.rows; i += kThreads) {

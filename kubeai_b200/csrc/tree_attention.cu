@@ -78,23 +78,33 @@ __device__ __forceinline__ uint32_t seen_bits(const int* mask, int words, int i,
   return __funnelshift_r(word(j >> 5), word((j >> 5) + 1), j & 31);
 }
 
+__device__ __forceinline__ tree::Request request(const b200_tree_attn_args& a, int s) { return tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, a.max_tree, a.status); }
+
 // Of the rows that no request owns, and those of requests that are left out, every parts-th one becomes zeros (one block).
 __device__ void zero_rest(const b200_tree_attn_args& a, int part, int parts) {
-  bool plain = true;
+  bool ordered = true, all = true;      // rows one behind the other; of requests that are all served
   for (int s = threadIdx.x; s < a.S; s += blockDim.x) {
-    const int rows = a.starts[s + 1] - a.starts[s];
-    plain = plain && a.starts[s] >= 0 && rows >= 0 && tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, a.max_tree).rows == rows;
+    const int begin = a.starts[s], end = a.starts[s + 1];
+    ordered = ordered && begin >= 0 && begin <= end && end <= a.T;
+    all = all && request(a, s).rows == end - begin;
   }
-  plain = __syncthreads_and(plain);
-  const int from = plain && a.S ? a.starts[0] : 0, to = plain && a.S ? a.starts[a.S] : 0;
+  ordered = __syncthreads_and(ordered);
+  all = __syncthreads_and(all);
+  const int from = ordered && a.S ? a.starts[0] : 0, to = ordered && a.S ? a.starts[a.S] : 0;
   for (int t = part; t < a.T; t += parts) {
-    bool owned = plain && t >= from && t < to;
-    if (owned) { t += (to - 1 - t) / parts * parts; continue; }
-    for (int s = 0; !plain && s < a.S && !owned; ++s) {
-      const tree::Request r = tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, a.max_tree);
-      owned = t >= r.row0 && t < r.row0 + r.rows;
+    int end = 0;      // of the rows that are somebody's from t on
+    if (ordered && t >= from && t < to) {
+      if (all) end = to;
+      else {
+        const int s = tree::last_at_most(a.starts, a.S, t);
+        if (request(a, s).rows) end = a.starts[s + 1];
+      }
     }
-    if (owned) continue;
+    for (int s = 0; !ordered && s < a.S && !end; ++s) {
+      const tree::Request r = request(a, s);
+      if (t >= r.row0 && t < r.row0 + r.rows) end = t + 1;
+    }
+    if (end) { t += (end - 1 - t) / parts * parts; continue; }
     uint4* out = reinterpret_cast<uint4*>(static_cast<bf16*>(a.out) + static_cast<size_t>(t) * a.ldo);
     for (int c = threadIdx.x; c < a.q_heads * (kD / 8); c += blockDim.x) out[c] = make_uint4(0, 0, 0, 0);
   }
@@ -122,7 +132,6 @@ __device__ __forceinline__ int head_cost(const b200_tree_attn_args& a, const tre
   for (int b = 0; b < blocks; ++b) n += tiles_of(a, r, bt, b) + tree::kItem;
   return n;
 }
-__device__ __forceinline__ tree::Request request(const b200_tree_attn_args& a, int s) { return tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, a.max_tree); }
 __device__ __forceinline__ void fill(const b200_tree_attn_args& a, int bt, Item* it) {
   it->first = it->block * bt;
   it->nb = min(bt, it->r.rows - it->first);

@@ -30,11 +30,14 @@ struct Request {
   int row0, rows, ctx;
 };
 
+// Whether step_maps gave request s no slots, so that its rows have no K and V in the cache and its table behind the pages it holds names anybody's.
+B200_HD bool turned_away(const int* status, int s) { return status && (status[s] & 3); }
+
 // The rows of request s as the device's lengths have them; no rows where they do not describe one: lengths out of order, rows behind T, more
-// rows than `most`, or more tokens than its row of the block table has pages for.
-B200_HD Request request_of(const int* starts, const int* ctx, int s, int T, int max_blocks, int most) {
+// rows than `most`, or more tokens than its row of the block table has pages for; nor where step_maps turned it away.
+B200_HD Request request_of(const int* starts, const int* ctx, int s, int T, int max_blocks, int most, const int* status = nullptr) {
   const int a = starts[s], b = starts[s + 1], c = ctx[s];
-  const bool ok = a >= 0 && b >= a && b <= T && b - a <= most && c >= 0 && static_cast<long long>(c) + (b - a) <= static_cast<long long>(max_blocks) * kPage;
+  const bool ok = !turned_away(status, s) && a >= 0 && b >= a && b <= T && b - a <= most && c >= 0 && static_cast<long long>(c) + (b - a) <= static_cast<long long>(max_blocks) * kPage;
   Request r;
   r.row0 = ok ? a : 0;
   r.rows = ok ? b - a : 0;

@@ -245,7 +245,8 @@ class StepMaps(NamedTuple):
 def step_maps(ctx_lens, new_lens, held, block_tables, free_pages, cursor, rows, parents=None, words=0, inplace=False) -> StepMaps:
     """Slots, positions and, with words > 0, ancestor masks of a step's `rows` rows, from each request's cached tokens and its rows of this step; pages that
     requests lack come from free_pages[cursor:] and are entered in block_tables (b200_op_step_maps).  held and cursor are left as they are and returned
-    anew, or updated themselves (inplace).  parents [rows]: the number of each row's parent in its request, -1 for none; without them a chain."""
+    anew, or updated themselves (inplace).  parents [rows]: the number of each row's parent in its request, -1 for none; without them a chain.  A request that pages or
+    lengths do not serve (status 1 or 2) keeps its rows, without slots: the operations behind this one leave it out where they are given `status`."""
     at = _gpu(ctx_lens)
     _ints(at, ctx_lens, new_lens, held, free_pages, cursor, parents)
     S = ctx_lens.numel()
@@ -264,18 +265,18 @@ def step_maps(ctx_lens, new_lens, held, block_tables, free_pages, cursor, rows, 
     return StepMaps(starts, positions, slots, seqs, masks.view(rows, words) if words else None, held_out, cursor_out, status)
 
 
-def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_heads, kv_heads, max_tree, max_ctx=0, scale=128 ** -0.5, out=None):
+def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_heads, kv_heads, max_tree, max_ctx=0, scale=128 ** -0.5, out=None, status=None):
     """Attention of a step's rows over the paged cache and those rows of their own request that masks [T, words] names, None: all in front and
     itself (b200_op_paged_attn_tree).  qkv: [T, at least q_heads * 128], q first; kv_layer: [pages, 2, kv_heads, 16, 128] with the step's K and V in it.
-    max_tree: the most rows of a request; max_ctx: the most tokens in front of them, if known.  Rows that no request owns are left as they were in `out`
-    and are zeros in a new one."""
+    max_tree: the most rows of a request; max_ctx: the most tokens in front of them, if known.  status [S]: step_maps' own, whose requests with 1 or 2 are left out.
+    Rows that no request owns, and those of one that is left out, are left as they were in `out` and are zeros in a new one."""
     at = _gpu(qkv)
     ldq = _rows(at, qkv, _BF16, "qkv", columns=q_heads * 128)
     if kv_layer.dtype is not torch.bfloat16 or kv_layer.get_device() != at or not kv_layer.is_contiguous() or kv_layer.shape[1:] != (2, kv_heads, 16, 128):
         raise _refused(f"kv_layer: contiguous bf16 [pages, 2, {kv_heads}, 16, 128] on cuda:{at}, got {kv_layer.dtype} {tuple(kv_layer.shape)} on {kv_layer.device}")
-    _ints(at, starts, ctx_lens, masks)
+    _ints(at, starts, ctx_lens, masks, status)
     S, T = ctx_lens.numel(), qkv.shape[0]
-    _sized(starts, S + 1, "starts")
+    _sized(starts, S + 1, "starts"), _sized(status, S, "status")
     if masks is not None and (masks.dim() != 2 or masks.shape[0] != T):
         raise _refused(f"masks: [{T}, words], got {tuple(masks.shape)}")
     fresh = out is None
@@ -289,6 +290,7 @@ def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_head
     ld = _rows(at, block_tables, _I32, "block tables", rows=S)
     a = TreeAttnArgs(S, T, q_heads, kv_heads, ldq, ldo, block_tables.shape[1], ld, masks.shape[1] if masks is not None else 0, max_tree, max_ctx, fresh, scale,
                      kv_layer.shape[0], qkv.data_ptr(), out.data_ptr(), kv_layer.data_ptr(), block_tables.data_ptr(), starts.data_ptr(), ctx_lens.data_ptr(), _ptr(masks))
+    a.status = _ptr(status)
     a.workspace_bytes = check(lib().b200_op_paged_attn_tree_workspace(C.byref(a)))
     workspace = starts.new_empty((a.workspace_bytes + 3) // 4)
     a.workspace = workspace.data_ptr()
@@ -297,18 +299,19 @@ def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_head
 
 
 def constrain(logits, starts=None, history=None, hist_starts=None, prompt_lens=None, drafts=None, masks=None, penalties=None, bias=None, allow=None,
-              allow_rows=None, out=None, pick=True):
+              allow_rows=None, out=None, pick=True, status=None):
     """Penalties for repeated tokens, biases and grammar masks on logits [T, V] (bf16 or fp32, rows may be a wider buffer's leading columns) and the greedy
     choice; returns (ids [T] or None, the logits that it was made from or None).  b200_op_constrain has the formulas and the lists' meaning.
     penalties: fp32 [S, 3] = repetition, presence, frequency.  bias: (starts [S + 1], ids, fp32 values).  allow: int32 [masks, at least ceil(V / 32)].
-    out: None, a type (torch.float32 or torch.bfloat16) for new logits, or a tensor for them, which may be `logits`.  ids of rows that no request owns
-    are -1, logits there are not written."""
+    out: None, a type (torch.float32 or torch.bfloat16) for new logits, or a tensor for them, which may be `logits`.  status [S]: step_maps' own.
+    ids of rows that no request owns, or one with status 1 or 2, are -1, logits there are not written."""
     at = _gpu(logits)
     ld = _rows(at, logits, _LOGITS, "logits")
     T, V = logits.shape
-    _ints(at, starts, history, hist_starts, prompt_lens, drafts, masks, allow_rows)
+    _ints(at, starts, history, hist_starts, prompt_lens, drafts, masks, allow_rows, status)
     S = starts.numel() - 1 if starts is not None else T
     _sized(hist_starts, S + 1, "hist_starts"), _sized(prompt_lens, S, "prompt_lens"), _sized(drafts, T, "drafts"), _sized(allow_rows, T, "allow_rows")
+    _sized(status, S, "status")
     words = 0
     if masks is not None:
         if masks.dim() != 2 or masks.shape[0] != T:
@@ -335,7 +338,7 @@ def constrain(logits, starts=None, history=None, hist_starts=None, prompt_lens=N
     a = ConstrainArgs(S, T, V, ld, logits.dtype is torch.float32, out_ld, out is not None and out.dtype is torch.float32, words,
                       history.numel() if history is not None else 0, b_len, allow.shape[0] if allow is not None else 0, allow_ld, logits.data_ptr(), _ptr(out), _ptr(ids),
                       _ptr(starts), _ptr(history), _ptr(hist_starts), _ptr(prompt_lens), _ptr(drafts), _ptr(masks), _ptr(penalties), _ptr(b_starts), _ptr(b_ids),
-                      _ptr(b_values), _ptr(allow), _ptr(allow_rows))
+                      _ptr(b_values), _ptr(allow), _ptr(allow_rows), _ptr(status))
     check(lib().b200_op_constrain(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
     return ids, out
 
@@ -347,14 +350,14 @@ class TreeAccept(NamedTuple):
     ctx_lens: torch.Tensor
 
 
-def tree_accept(ids, drafts, parents, starts, ctx_lens, block_tables, kv, max_path) -> TreeAccept:
+def tree_accept(ids, drafts, parents, starts, ctx_lens, block_tables, kv, max_path, status=None) -> TreeAccept:
     """The path of drafts that the choices `ids` confirm in each request's tree (parents None: a chain), and its K and V moved to the positions behind the cached
     tokens in every layer of kv [layers, pages, 2, kv_heads, 16, 128], None: nowhere (b200_op_tree_accept).  Returns the paths' lengths, rows and chosen tokens (-1 behind
-    the last) and the requests' new lengths."""
+    the last) and the requests' new lengths.  status [S]: step_maps' own, whose requests with 1 or 2 accept nothing."""
     at = _gpu(ids)
-    _ints(at, ids, drafts, parents, starts, ctx_lens)
+    _ints(at, ids, drafts, parents, starts, ctx_lens, status)
     S, T = ctx_lens.numel(), ids.numel()
-    _sized(starts, S + 1, "starts"), _sized(drafts, T, "drafts"), _sized(parents, T, "parents")
+    _sized(starts, S + 1, "starts"), _sized(drafts, T, "drafts"), _sized(parents, T, "parents"), _sized(status, S, "status")
     layers, pages, heads, apart = 0, 0, 1, 0
     if kv is not None:
         shape = kv.shape
@@ -368,7 +371,7 @@ def tree_accept(ids, drafts, parents, starts, ctx_lens, block_tables, kv, max_pa
     sizes = [S, S, S * max_path, S * max_path]
     accepted, ctx, path, tokens = _pieces(ids, sizes)
     a = TreeAcceptArgs(S, T, block_tables.shape[1], ld, max_path, layers, heads, pages, apart, ids.data_ptr(), drafts.data_ptr(), _ptr(parents),
-                       starts.data_ptr(), ctx_lens.data_ptr(), block_tables.data_ptr(), _ptr(kv), accepted.data_ptr(), path.data_ptr(), tokens.data_ptr(), ctx.data_ptr())
+                       starts.data_ptr(), ctx_lens.data_ptr(), block_tables.data_ptr(), _ptr(kv), accepted.data_ptr(), path.data_ptr(), tokens.data_ptr(), ctx.data_ptr(), _ptr(status))
     check(lib().b200_op_tree_accept(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
     return TreeAccept(accepted, path.view(S, max_path), tokens.view(S, max_path), ctx)
 
