@@ -326,7 +326,7 @@ def constrain(logits, starts=None, history=None, hist_starts=None, prompt_lens=N
         _ints(at, b_starts, b_ids), _sized(b_starts, S + 1, "bias starts"), _sized(b_values, b_len, "bias values")
         if not (b_values.dtype is torch.float32 and b_values.get_device() == at and b_values.is_contiguous()):
             raise _refused(f"bias values: fp32 on cuda:{at}, got {b_values.dtype} on {b_values.device}")
-    allow_ld = _rows(at, allow, _I32, "allow") if allow is not None else 0
+    allow_ld = _rows(at, allow, _I32, "allow", columns=(V + 31) // 32) if allow is not None else 0
     out_ld = 0
     if out is not None:
         if isinstance(out, torch.dtype):
