@@ -534,12 +534,14 @@ int64_t b200_op_paged_attn_tree_workspace(const b200_tree_attn_args* a);
 int b200_op_paged_attn_tree(const b200_tree_attn_args* a, void* stream);
 /* Penalties, biases and masks on logits [T, V], rows ld apart, bf16 or fp32 (logits_f32), and the greedy choice.  In fp32, each step rounded once:
  *   y = x;  a token among the request's history or the row's drafts: y = y > 0 ? y / repetition : y * repetition;
- *   y -= frequency * c, then y -= presence where c > 0, c = how often it stands in the history behind prompt_lens tokens and in the row's drafts;
+ *   y -= frequency * c, then y -= presence where c > 0, c = how often it stands in the row's text behind its first prompt_lens tokens;
  *   y += bias, the last of the request's entries for the token;  a token that the row's mask does not allow: -inf.
  * ids [T] (optional): the lowest allowed token of the largest y, NaN counting as -inf; -1 where none is allowed, for rows that no request owns and for those of requests that are left out.  out (optional): y, fp32 or bf16 (out_f32), rows
  * ld_out apart; may be logits itself where type and ld are the same.
  * starts NULL: row r belongs to request r (S == T).  history: the requests' tokens one behind the other, hist_starts [S + 1], at most history_len; NULL: none.
- * drafts [T] (NULL: none): the step's tokens; a row's are those that masks [T, words] names (NULL: itself and every row of its request in front).
+ * drafts [T] (NULL: none): the step's tokens; a row's are those that masks [T, words] names (NULL: itself and every row of its request in front).  A row's text is its
+ * request's history and behind it the row's drafts, row j of the request as its token number history + j: the history therefore ends in front of row 0's token, and rows that carry a part
+ * of the prompt count as prompt where prompt_lens (NULL: 0) reaches over them.
  * penalties fp32 [S][3]: repetition, presence, frequency (NULL: 1, 0, 0).  bias_starts [S + 1], bias_ids, bias_values, at most bias_len entries (NULL: none).
  * allow [allow_count][ld_allow words], bit v of a row: token v is allowed; allow_rows [T]: each row's mask, -1 for none (NULL: mask r, allow_count == T).
  * Tokens outside 0 .. V - 1 in any list count for nothing.  V <= 393216, S <= 65534, T and bias_len <= 2^30, history_len <= 2^29. */

@@ -38,6 +38,7 @@ template <typename T>
 constexpr int kDepth = sizeof(T) == 2 ? 3 : 2;               // chunks on their way
 constexpr int kMostTokens = 393216, kWaitLimit = 1 << 22;
 constexpr unsigned kPrompt = 0x80000000u, kBiased = 0x40000000u;      // of a count: said in the prompt, which the repetition penalty alone counts; has a bias
+constexpr unsigned kPromptDraft = 1u << 16;      // of a count: one of a tree's drafts that are of the prompt
 
 __device__ __forceinline__ unsigned long long peer_load(const void* p, unsigned rank) {
   unsigned long long v;
@@ -165,14 +166,16 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
   float rho = 1.f, pi = 0.f, phi = 0.f;
   if (a.starts) row0 = a.starts[s], rows = a.starts[s + 1];
   if (a.penalties) rho = a.penalties[3 * s], pi = a.penalties[3 * s + 1], phi = a.penalties[3 * s + 2];
-  if (a.history) {
-    h0 = a.hist_starts[s], h1 = a.hist_starts[s + 1];
-    if (a.prompt_lens) prompt = a.prompt_lens[s];
-  }
+  if (a.history) h0 = a.hist_starts[s], h1 = a.hist_starts[s + 1];
+  if (a.prompt_lens) prompt = a.prompt_lens[s];
   if (a.bias_starts) b0 = a.bias_starts[s], b1 = a.bias_starts[s + 1];
   if (a.starts) rows = row0 >= 0 && rows >= row0 && rows <= a.T ? rows - row0 : 0;
   h0 = max(h0, 0), h1 = min(h1, a.history_len);
   b0 = max(b0, 0), b1 = min(b1, a.bias_len);
+  // The request's rows follow its history: rows in front of this one are of the prompt.  Where there are any, so is all of the history, which leaves the low
+  // bits of a count to at most 256 drafts of a tree and those above them to the prompt's; a chain's prompt rows are seen by all rows behind them.
+  const int prompt_rows = static_cast<int>(max(0ll, static_cast<long long>(prompt) - max(0, h1 - h0)));
+  const bool prompt_apart = a.masks && prompt_rows;
   if (tree::turned_away(a.status, s)) {      // its rows have no choice
     if (!group && a.ids)
       for (int i = rank * kThreads + tid; i < rows; i += ctas * kThreads) a.ids[row0 + i] = -1;
@@ -362,11 +365,16 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
     }
     // the drafts that lead to row i, counted in or out: one a thread, whose mask is looked up a row ahead, and those behind them
     unsigned leads = mask_word(0);
+    auto count_draft = [&](int slot, int j, unsigned by) {
+      if (j >= prompt_rows) atomicAdd(count + slot, by);
+      else if (prompt_apart) atomicAdd(count + slot, by * kPromptDraft);
+      else atomicOr(count + slot, kPrompt);
+    };
     auto drafted = [&](int i, unsigned by) {
-      if (draft_slot >= 0 && leads >> (tid & 31) & 1) atomicAdd(count + draft_slot, by);
+      if (draft_slot >= 0 && leads >> (tid & 31) & 1) count_draft(draft_slot, tid, by);
       for (int j = kThreads + tid; j < (a.masks ? 0 : i + 1); j += kThreads) {
         const int k = slot(place(a.drafts[row0 + j]));
-        if (k >= 0) atomicAdd(count + k, by);
+        if (k >= 0) count_draft(k, j, by);
       }
     };
     __syncthreads();
@@ -446,7 +454,7 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
         for (int n = mine; n < slot_end; n += kThreads) {
           const int k = n == mine ? place0 : place_of(n), v = k + from;
           const bool allowed = (n == mine || !may ? may_first : may[k >> 5]) >> (k & 31) & 1;
-          const unsigned said = count[n], times = said & ~(kPrompt | kBiased);
+          const unsigned said = count[n], times = said & (prompt_apart ? kPromptDraft - 1 : ~(kPrompt | kBiased));
           float z = Vec<TIn>::value(reinterpret_cast<const TIn*>(vectors)[k - first]);
           if (said & ~kBiased) z = z > 0.f ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
           z = __fsub_rn(z, __fmul_rn(phi, static_cast<float>(times)));

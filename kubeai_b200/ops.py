@@ -302,7 +302,8 @@ def constrain(logits, starts=None, history=None, hist_starts=None, prompt_lens=N
               allow_rows=None, out=None, pick=True, status=None):
     """Penalties for repeated tokens, biases and grammar masks on logits [T, V] (bf16 or fp32, rows may be a wider buffer's leading columns) and the greedy
     choice; returns (ids [T] or None, the logits that it was made from or None).  b200_op_constrain has the formulas and the lists' meaning.
-    penalties: fp32 [S, 3] = repetition, presence, frequency.  bias: (starts [S + 1], ids, fp32 values).  allow: int32 [masks, at least ceil(V / 32)].
+    history: the requests' texts in front of this step's rows (not row 0's token, which drafts has); prompt_lens [S]: how many tokens of a text are its prompt, rows that carry a part of
+    it among them.  penalties: fp32 [S, 3] = repetition, presence, frequency.  bias: (starts [S + 1], ids, fp32 values).  allow: int32 [masks, at least ceil(V / 32)].
     out: None, a type (torch.float32 or torch.bfloat16) for new logits, or a tensor for them, which may be `logits`.  status [S]: step_maps' own.
     ids of rows that no request owns, or one with status 1 or 2, are -1, logits there are not written."""
     at = _gpu(logits)
