@@ -8,7 +8,7 @@
 // request that the CTA takes.  A row then comes in chunks of 8192 tokens by bulk copies, two or three ahead, from one row into the next; of its vectors eight tokens cost
 // a maximum of pairs, marked tokens left out, and the chunk's slots, a thread each, alone need the formula.  A row's drafts are counted in ahead of it and out
 // behind it.  Few rows: a cluster of CTAs shares the vocabulary, whose best pairs (value, token) meet through distributed shared memory.  Ties go to the lowest token:
-// every comparison prefers it.  Every wait for a copy has a limit; a CTA that gives up sets an error mark.
+// every comparison prefers it.  Every wait for a copy has a limit, and a warp that gave up makes no other: its CTA has no more copied, sets an error mark and still meets the others.
 //
 // What bounds it: the lists' chain of look-ups, marks, slots and counts ahead of the rows, which is half of a CTA's time where it has one or two rows (128 rows of 128256
 // bf16 logits, 4000 tokens of history each: 25 us, of which the copies need 5; one row 8.2), and for trees the copies in and out behind it (288 rows of 99991 fp32
@@ -190,17 +190,18 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
 
   // ---- the rows' tokens [from, from + tokens) of the part, chunk by chunk: chunk c of a row holds its tokens c * kTokens - skew ..
   int from = 0, tokens = size;
-  unsigned issued = 0, taken = 0;      // chunks
+  tree::Ring<kRing> ring;              // chunks (every warp takes them all, warp 0 has them copied)
   int f_row = 0, f_chunk = 0;          // the next one to be issued
   auto skew_of = [&](const TIn* p) { return static_cast<int>(reinterpret_cast<uintptr_t>(p) / sizeof(TIn) % N); };      // tokens between a 16-byte boundary and p
   auto row_at = [&](int d) { return static_cast<const TIn*>(a.logits) + static_cast<size_t>(row0 + group + d * groups) * a.ld + lo + from; };
   auto chunks_of = [&](int d) { return (tokens + skew_of(row_at(d)) + kTokens - 1) / (kTokens); };
-  bool ok = true;
+  auto wait_full = [&](unsigned b, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait_limited(smem_u32(full + b), parity, kWaitLimit)) != 0; };
+  auto wait_empty = [&](unsigned b, unsigned parity) { return __all_sync(0xffffffffu, mbar_wait_limited(smem_u32(empty + b), parity, kWaitLimit)) != 0; };
   // warp 0: whole 16 bytes by a copy, a row's ragged ends by threads
   auto issue = [&] {
     if (f_row >= my_rows || !tokens) return;
-    const int b = issued % kRing;
-    if (issued >= kRing) ok = mbar_wait_limited(smem_u32(empty + b), (issued / kRing + 1) & 1, kWaitLimit) && ok;
+    if (!ring.may_issue(wait_empty)) return;
+    const int b = ring.issued % kRing;
     const TIn* p = row_at(f_row);
     const int skew = skew_of(p), first = f_chunk * kTokens - skew;                              // of its tokens
     const int head = first < 0 ? min(tokens, N - skew) : 0, begin = max(first, 0) + head, end = min(first + kTokens, tokens), whole = max(0, end - begin) / N;
@@ -213,17 +214,12 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
       mbar_arrive_expect_tx(smem_u32(full + b), whole * 16);
       if (whole) bulk_load_1d(smem_u32(dst + begin), p + begin, whole * 16, smem_u32(full + b));
     }
-    ++issued;
+    ++ring.issued;
     if (++f_chunk >= chunks_of(f_row)) f_chunk = 0, ++f_row;
-  };
-  auto arrived = [&] {
-    const unsigned b = taken % kRing;
-    ok = mbar_wait_limited(smem_u32(full + b), taken / kRing & 1, kWaitLimit) && ok;
-    ++taken;
   };
   auto left = [&] {      // the warp has read the chunk that arrived last
     __syncwarp();
-    if (lane == 0) mbar_arrive(smem_u32(empty + (taken - 1) % kRing));
+    if (lane == 0) mbar_arrive(smem_u32(empty + ring.last()));
   };
   int early = 0;
   for (int d = 0; d < my_rows && early < kRing && tokens; ++d) early = min(kRing, early + chunks_of(d));
@@ -311,10 +307,7 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
     if (word0 || word1 < part_words) {
       // the first chunks on their way are those of a part in one piece: they are let by
       if (!word0)
-        for (int k = 0; k < early; ++k) {
-          arrived();
-          left();
-        }
+        for (int k = 0; k < early && ring.arrived(wait_full); ++k) left();
       __syncthreads();
       from = 32 * word0;
       tokens = min(32 * word1, size) - from;
@@ -420,8 +413,8 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
         const int place0 = mine < slot_end ? place_of(mine) : 0;
         unsigned may_first = ~0u;
         if (may && mine < slot_end) may_first = may[place0 >> 5];
-        arrived();
-        const uint4* vectors = reinterpret_cast<const uint4*>(smem + (taken - 1) % kRing * kChunk);
+        if (!ring.arrived(wait_full)) break;
+        const uint4* vectors = reinterpret_cast<const uint4*>(smem + ring.last() * kChunk);
         // a thread's group's bits, then its warp's vectors in the order of memory, each with the bits of the group that it belongs to
         unsigned fine = 0, own = 0, plain = 0;      // allowed ones, ones to be written here, ones that are neither marked nor forbidden
         if (k0 < tokens) {
@@ -494,7 +487,8 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
     __syncthreads();
     word0 = word1;
   }
-  if (!ok) *reinterpret_cast<volatile int*>(error) = 1;
+  if (warp == 0) ring.drain(wait_full);      // no copy is on its way when the CTA ends, where it gave up either
+  if (!ring.ok) *reinterpret_cast<volatile int*>(error) = 1;
 
   // ---- the parts' best of each row
   if (!a.ids) return;

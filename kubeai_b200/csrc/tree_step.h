@@ -107,6 +107,33 @@ B200_HD int take_of(int t0, int tiles, int* rest) {
   return take;
 }
 
+// The chunks of a ring of `kRing` buffers, in order: which buffer and phase each one's waits are for.  wait(buffer, parity) says whether it came; one that did not
+// ends the ring: no buffer is filled again, no chunk behind it is taken, and no other wait is made but those of drain.
+template <int kRing>
+struct Ring {
+  unsigned issued = 0, taken = 0;
+  bool ok = true;
+  // whether the next chunk's buffer may be filled: what lay there has been read
+  template <typename Wait>
+  B200_HD bool may_issue(Wait wait) {
+    if (ok && issued >= kRing) ok = wait(issued % kRing, (issued / kRing + 1) & 1);
+    return ok;
+  }
+  // whether the next chunk has come
+  template <typename Wait>
+  B200_HD bool arrived(Wait wait) {
+    if (ok) ok = wait(taken % kRing, taken / kRing & 1);
+    taken += ok;
+    return ok;
+  }
+  B200_HD int last() const { return static_cast<int>((taken - 1) % kRing); }      // buffer of the chunk that came last
+  // a bounded wait more for every chunk still on its way
+  template <typename Wait>
+  B200_HD void drain(Wait wait) const {
+    for (unsigned k = taken; k != issued; ++k) wait(k % kRing, k / kRing & 1);
+  }
+};
+
 // What a request asks of step_maps: rows (never negative), and pages beyond those it holds; -1 pages where its lengths do not fit.
 B200_HD int rows_asked(int n) { return n > 0 ? n : 0; }
 B200_HD int pages_asked(int ctx, int n, int held, int max_blocks, int words) {
