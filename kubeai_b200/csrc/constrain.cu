@@ -206,8 +206,10 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
     const int skew = skew_of(p), first = f_chunk * kTokens - skew;                              // of its tokens
     const int head = first < 0 ? min(tokens, N - skew) : 0, begin = max(first, 0) + head, end = min(first + kTokens, tokens), whole = max(0, end - begin) / N;
     TIn* dst = reinterpret_cast<TIn*>(smem + b * kChunk) - first;      // of token 0
+    const bool tail = begin + whole * N + lane < end;
     if (lane < head) dst[lane] = p[lane];
-    if (begin + whole * N + lane < end) dst[begin + whole * N + lane] = p[begin + whole * N + lane];
+    if (tail) dst[begin + whole * N + lane] = p[begin + whole * N + lane];
+    if (lane < head || tail) fence_proxy_async();      // a later copy into this buffer comes behind these stores
     __syncwarp();
     if (lane == 0) {
       __threadfence_block();
