@@ -127,8 +127,8 @@ __device__ void no_choice(const b200_constrain_args& a) {
   }
 }
 
-// TIn: the logits; TOut: y kept, or None.  part: tokens of a CTA, a multiple of 32.
-template <typename TIn, typename TOut>
+// TIn: the logits; TOut: y kept, or None; LONG: a CTA may have more than kRows rows (the loop for them costs one row 0.3 us of 8.1).  part: tokens of a CTA, a multiple of 32.
+template <typename TIn, typename TOut, bool LONG>
 __global__ void __launch_bounds__(kThreads, kPlaces)
 constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* error) {
   constexpr int N = Vec<TIn>::N, kWarps = kThreads / 32, kChunk = kTokens * static_cast<int>(sizeof(TIn)), kRing = kDepth<TIn>;
@@ -147,7 +147,8 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
   __shared__ uint64_t full[kRing], empty[kRing];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rank = static_cast<int>(cluster_ctarank()), ctas = gridDim.x;
   const int lo = rank * part, size = max(0, min(part, a.V - lo));
-  const int s = blockIdx.z, group = blockIdx.y, groups = gridDim.y;
+  const int s = blockIdx.z, groups = gridDim.y;
+  int group = blockIdx.y;      // the first of this CTA's rows, then of its next kRows
   if (tid == 0) {
     for (int b = 0; b < kRing; ++b) {
       mbar_init(smem_u32(full + b), 1);
@@ -182,7 +183,8 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
     return;      // (the whole cluster)
   }
   if (group >= rows) return;
-  const int my_rows = (rows - group + groups - 1) / groups;
+  auto rows_from_group = [&] { return min(kRows, (rows - group + groups - 1) / groups); };
+  int my_rows = rows_from_group();
   for (int w = tid; w < part_words + 2; w += kThreads) known[w - 1] = 0;
   for (int d = tid; d < kRows; d += kThreads) best_of[d] = 0;
   for (int d = tid; d < 1 << N; d += kThreads) keep_of[d] = Vec<TIn>::keep(d);
@@ -293,229 +295,232 @@ constrain_kernel(const __grid_constant__ b200_constrain_args a, int part, int* e
   }
   __syncthreads();
 
-  for (int word0 = 0; 32 * word0 < size;) {
-    // ---- the next piece: words that mark kSlots tokens at most (a word marks 32)
-    int word1 = part_words;
-    const int slot0 = slot_of[word0];
-    if (marked - slot0 > kSlots) {
-      if (tid == 0) s_end = word0 + 1;
-      __syncthreads();
-      for (int w = word0 + 1 + tid; w < part_words; w += kThreads)
-        if (slot_of[w] - slot0 <= kSlots) atomicMax(&s_end, w);      // it may end in front of word w
-      __syncthreads();
-      word1 = s_end;
-    }
-    const int slots = (word1 < part_words ? slot_of[word1] : marked) - slot0;
-    if (word0 || word1 < part_words) {
-      // the first chunks on their way are those of a part in one piece: they are let by
-      if (!word0)
-        for (int k = 0; k < early && ring.arrived(wait_full); ++k) left();
-      __syncthreads();
-      from = 32 * word0;
-      tokens = min(32 * word1, size) - from;
-      f_row = f_chunk = 0;
-      if (warp == 0)
-        for (int k = 0; k < kRing; ++k) issue();
-    }
-    auto slot = [&](int k) {        // of a marked token's place; -1 where it is not this piece's
-      const int w = k >> 5;
-      return k >= 0 && w >= word0 && w < word1 ? slot_of[w] - slot0 + __popc(known[w] & ((1u << (k & 31)) - 1)) : -1;
-    };
-    for (int i = tid; i < slots; i += kThreads) count[i] = 0, entry[i] = -1;
-    __syncthreads();
-    history([&](int k, bool in_prompt) {
-      const int i = slot(k);
-      if (i < 0) return;
-      token[i] = static_cast<uint16_t>(k);      // (whoever else names it writes the same)
-      if (in_prompt) atomicOr(count + i, kPrompt);
-      else atomicAdd(count + i, 1u);
-    });
-    const int bias_slot = slot(bias_at), draft_slot = slot(draft_at);
-    if (bias_slot >= 0) token[bias_slot] = static_cast<uint16_t>(bias_at), atomicMax(entry + bias_slot, b0 + tid);
-    for (int e = b0 + kThreads + tid; e < b1; e += kThreads) {
-      const int k = place(a.bias_ids[e]), i = slot(k);
-      if (i >= 0) token[i] = static_cast<uint16_t>(k), atomicMax(entry + i, e);
-    }
-    if (draft_slot >= 0) token[draft_slot] = static_cast<uint16_t>(draft_at);
-    if (a.drafts)
-      for (int e = kThreads + tid; e < rows; e += kThreads) {
-        const int k = place(a.drafts[row0 + e]), i = slot(k);
-        if (i >= 0) token[i] = static_cast<uint16_t>(k);
-      }
-    __syncthreads();
-    // an entry becomes its bias, by the thread that has the last one of its token
-    if (b1 - b0 <= kThreads) {
-      const bool last = bias_slot >= 0 && entry[bias_slot] == b0 + tid;
-      __syncthreads();
-      if (last) {
-        entry[bias_slot] = __float_as_int(bias_value);
-        atomicOr(count + bias_slot, kBiased);
-      }
-    } else {
-      for (int i = tid; i < slots; i += kThreads)
-        if (entry[i] >= 0) {
-          entry[i] = __float_as_int(a.bias_values[entry[i]]);
-          atomicOr(count + i, kBiased);
-        }
-    }
-    // the drafts that lead to row i, counted in or out: one a thread, whose mask is looked up a row ahead, and those behind them
-    unsigned leads = mask_word(0);
-    auto count_draft = [&](int slot, int j, unsigned by) {
-      if (j >= prompt_rows) atomicAdd(count + slot, by);
-      else if (prompt_apart) atomicAdd(count + slot, by * kPromptDraft);
-      else atomicOr(count + slot, kPrompt);
-    };
-    auto drafted = [&](int i, unsigned by) {
-      if (draft_slot >= 0 && leads >> (tid & 31) & 1) count_draft(draft_slot, tid, by);
-      for (int j = kThreads + tid; j < (a.masks ? 0 : i + 1); j += kThreads) {
-        const int k = slot(place(a.drafts[row0 + j]));
-        if (k >= 0) count_draft(k, j, by);
-      }
-    };
-    __syncthreads();
-
-    // ---- the rows
-    const unsigned* allow = allow_of(0);
-    const int allow_words = (a.V - lo - from + 31) / 32;      // from the piece's first on
-    for (int d = 0; d < my_rows; ++d) {
-      const int i = group + d * groups, skew = skew_of(row_at(d)), chunks = chunks_of(d);
-      TOut* out = nullptr;
-      if constexpr (KEEP) out = static_cast<TOut*>(a.out) + static_cast<size_t>(row0 + i) * a.ld_out + lo + from;
-      const unsigned *may = allow ? allow + word0 : nullptr, *marks = known + word0;
-      const unsigned next_leads = mask_word(d + 1);
-      allow = allow_of(d + 1);
-      if (a.drafts) {
-        drafted(i, 1u);
+  for (;;) {      // kRows rows at a time
+    for (int word0 = 0; 32 * word0 < size;) {
+      // ---- the next piece: words that mark kSlots tokens at most (a word marks 32)
+      int word1 = part_words;
+      const int slot0 = slot_of[word0];
+      if (marked - slot0 > kSlots) {
+        if (tid == 0) s_end = word0 + 1;
         __syncthreads();
+        for (int w = word0 + 1 + tid; w < part_words; w += kThreads)
+          if (slot_of[w] - slot0 <= kSlots) atomicMax(&s_end, w);      // it may end in front of word w
+        __syncthreads();
+        word1 = s_end;
       }
-      float best = -INFINITY, at_best = -INFINITY;
-      int id = -1, at = 0;               // the best marked token; of the others the best one's vector: its first token's place in the piece, and which of them count
-      unsigned at_plain = 0;
-      // the masks of a thread's group, looked up a chunk ahead
-      unsigned next0 = ~0u, next1 = ~0u;
-      auto look_ahead = [&](int k) {
-        const int w = k >> 5;              // (-1 where the first group begins ahead of the piece)
-        next0 = next1 = ~0u;
-        if (!may || k >= tokens) return;
-        if (w >= 0) next0 = may[w];
-        if (skew && w + 1 < allow_words) next1 = may[w + 1];
+      const int slots = (word1 < part_words ? slot_of[word1] : marked) - slot0;
+      const bool again = LONG && group != static_cast<int>(blockIdx.y);
+      if (word0 || word1 < part_words || again) {
+        // the first chunks on their way are those of a part in one piece: they are let by
+        if (!word0 && !again)
+          for (int k = 0; k < early && ring.arrived(wait_full); ++k) left();
+        __syncthreads();
+        from = 32 * word0;
+        tokens = min(32 * word1, size) - from;
+        f_row = f_chunk = 0;
+        if (warp == 0)
+          for (int k = 0; k < kRing; ++k) issue();
+      }
+      auto slot = [&](int k) {        // of a marked token's place; -1 where it is not this piece's
+        const int w = k >> 5;
+        return k >= 0 && w >= word0 && w < word1 ? slot_of[w] - slot0 + __popc(known[w] & ((1u << (k & 31)) - 1)) : -1;
       };
-      look_ahead(tid * kGroup - skew);
-      for (int c = 0; c < chunks; ++c) {
-        const int first = c * kTokens - skew, k0 = first + tid * kGroup;      // of the chunk's tokens; of this thread's
-        const unsigned may0 = next0, may1 = next1;
-        look_ahead(k0 + kTokens);
-        // the chunk's slots: those of its tokens, in order
-        const int t0 = max(first, 0), t1 = min(first + kTokens, tokens);
-        auto slots_ahead = [&](int k) { return k >= tokens ? slots : slot_of[word0 + (k >> 5)] - slot0 + __popc(marks[k >> 5] & ((1u << (k & 31)) - 1)); };
-        const int slot_begin = slots_ahead(t0), slot_end = slots_ahead(t1);
-        // a thread's first one, from the last warp on, as warp 0 has chunks to issue
-        const int mine = slot_begin + kThreads - 1 - tid;
-        auto place_of = [&](int n) { return t0 + ((token[n] - (from + t0)) & 0xffff); };      // in the piece
-        const int place0 = mine < slot_end ? place_of(mine) : 0;
-        unsigned may_first = ~0u;
-        if (may && mine < slot_end) may_first = may[place0 >> 5];
-        if (!ring.arrived(wait_full)) break;
-        const uint4* vectors = reinterpret_cast<const uint4*>(smem + ring.last() * kChunk);
-        // a thread's group's bits, then its warp's vectors in the order of memory, each with the bits of the group that it belongs to
-        unsigned fine = 0, own = 0, plain = 0;      // allowed ones, ones to be written here, ones that are neither marked nor forbidden
-        if (k0 < tokens) {
-          const int w = k0 >> 5, over = k0 + kGroup - tokens;
-          const unsigned inside = (k0 < 0 ? ~0u << -k0 : ~0u) & (over > 0 ? ~0u >> over : ~0u);
-          fine = inside & __funnelshift_r(may0, may1, k0 & 31);
-          own = inside & ~__funnelshift_r(marks[w], skew ? marks[w + 1] : 0u, k0 & 31);
-          plain = fine & own;
+      for (int i = tid; i < slots; i += kThreads) count[i] = 0, entry[i] = -1;
+      __syncthreads();
+      history([&](int k, bool in_prompt) {
+        const int i = slot(k);
+        if (i < 0) return;
+        token[i] = static_cast<uint16_t>(k);      // (whoever else names it writes the same)
+        if (in_prompt) atomicOr(count + i, kPrompt);
+        else atomicAdd(count + i, 1u);
+      });
+      const int bias_slot = slot(bias_at), draft_slot = slot(draft_at);
+      if (bias_slot >= 0) token[bias_slot] = static_cast<uint16_t>(bias_at), atomicMax(entry + bias_slot, b0 + tid);
+      for (int e = b0 + kThreads + tid; e < b1; e += kThreads) {
+        const int k = place(a.bias_ids[e]), i = slot(k);
+        if (i >= 0) token[i] = static_cast<uint16_t>(k), atomicMax(entry + i, e);
+      }
+      if (draft_slot >= 0) token[draft_slot] = static_cast<uint16_t>(draft_at);
+      if (a.drafts)
+        for (int e = kThreads + tid; e < rows; e += kThreads) {
+          const int k = place(a.drafts[row0 + e]), i = slot(k);
+          if (i >= 0) token[i] = static_cast<uint16_t>(k);
         }
-        constexpr int kOwn = kGroup / N;
-#pragma unroll
-        for (int e = 0; e < kOwn; ++e) {
-          const int v = e * 32 + lane, shift = v % kOwn * N, k = first + (warp * 32 * kOwn + v) * N;
-          const uint4 u = vectors[warp * 32 * kOwn + v];
-          const unsigned here = __shfl_sync(0xffffffffu, plain, v / kOwn) >> shift & kAll;
-          if constexpr (KEEP) {
-            const unsigned shown = __shfl_sync(0xffffffffu, fine, v / kOwn) >> shift, written = __shfl_sync(0xffffffffu, own, v / kOwn) >> shift & kAll;
-            float z[N];
-#pragma unroll
-            for (int j = 0; j < N; ++j) z[j] = shown >> j & 1 ? Vec<TIn>::get(u, j) : -INFINITY;
-            if (written) store_all<N>(out + k, z, written);
+      __syncthreads();
+      // an entry becomes its bias, by the thread that has the last one of its token
+      if (b1 - b0 <= kThreads) {
+        const bool last = bias_slot >= 0 && entry[bias_slot] == b0 + tid;
+        __syncthreads();
+        if (last) {
+          entry[bias_slot] = __float_as_int(bias_value);
+          atomicOr(count + bias_slot, kBiased);
+        }
+      } else {
+        for (int i = tid; i < slots; i += kThreads)
+          if (entry[i] >= 0) {
+            entry[i] = __float_as_int(a.bias_values[entry[i]]);
+            atomicOr(count + i, kBiased);
           }
-          const float top = Vec<TIn>::largest(u, keep_of[here]);
-          if (top > at_best || (!at_plain && here)) {
-            at_best = top != top ? -INFINITY : top;
-            at = k;
-            at_plain = here;
-          }
-        }
-        for (int n = mine; n < slot_end; n += kThreads) {
-          const int k = n == mine ? place0 : place_of(n), v = k + from;
-          const bool allowed = (n == mine || !may ? may_first : may[k >> 5]) >> (k & 31) & 1;
-          const unsigned said = count[n], times = said & (prompt_apart ? kPromptDraft - 1 : ~(kPrompt | kBiased));
-          float z = Vec<TIn>::value(reinterpret_cast<const TIn*>(vectors)[k - first]);
-          if (said & ~kBiased) z = z > 0.f ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
-          z = __fsub_rn(z, __fmul_rn(phi, static_cast<float>(times)));
-          if (times) z = __fsub_rn(z, pi);
-          if (said & kBiased) z = __fadd_rn(z, __int_as_float(entry[n]));
-          if constexpr (KEEP) store_one(out + k, allowed ? z : -INFINITY);
-          if (z != z) z = -INFINITY;
-          if (allowed && (z > best || id < 0)) best = z, id = lo + v;      // (a thread's slots ascend)
-        }
-        left();
-        if (warp == 0) issue();
       }
-      // which token of its vector the best other one is: the first of that value, or the first at all where none is above -inf.  The warp's best ones look.
-      __syncwarp();
-      const unsigned other = at_plain ? ordered(at_best, 0) : 0u, most = __reduce_max_sync(0xffffffffu, other);
-      if (other && other == most && (id < 0 || at_best >= best)) {
-        const TIn* x = row_at(d) + at;
-        int found = 0;
-        for (unsigned bits = at_plain; bits; bits &= bits - 1) {
-          found = __ffs(bits) - 1;
-          if (at_best == -INFINITY || Vec<TIn>::value(x[found]) == at_best) break;
+      // the drafts that lead to row i, counted in or out: one a thread, whose mask is looked up a row ahead, and those behind them
+      unsigned leads = mask_word(0);
+      auto count_draft = [&](int slot, int j, unsigned by) {
+        if (j >= prompt_rows) atomicAdd(count + slot, by);
+        else if (prompt_apart) atomicAdd(count + slot, by * kPromptDraft);
+        else atomicOr(count + slot, kPrompt);
+      };
+      auto drafted = [&](int i, unsigned by) {
+        if (draft_slot >= 0 && leads >> (tid & 31) & 1) count_draft(draft_slot, tid, by);
+        for (int j = kThreads + tid; j < (a.masks ? 0 : i + 1); j += kThreads) {
+          const int k = slot(place(a.drafts[row0 + j]));
+          if (k >= 0) count_draft(k, j, by);
         }
-        found += lo + from + at;
-        if (id < 0 || at_best > best || found < id) best = at_best, id = found;
-      }
-      __syncwarp();
-      // the warp's best: the largest value, then its lowest token
-      const unsigned value = ordered(best, id), top = __reduce_max_sync(0xffffffffu, value);
-      const unsigned lowest = __reduce_min_sync(0xffffffffu, value == top ? static_cast<unsigned>(id) : ~0u);
-      if (lane == 0 && top) atomicMax(best_of + d, static_cast<unsigned long long>(top) << 32 | (INT_MAX - lowest));
-      if (a.drafts) {
-        __syncthreads();      // the counts have been read
-        drafted(i, ~0u);
-      }
-      leads = next_leads;
-    }
-    __syncthreads();
-    word0 = word1;
-  }
-  if (warp == 0) ring.drain(wait_full);      // no copy is on its way when the CTA ends, where it gave up either
-  if (!ring.ok) *reinterpret_cast<volatile int*>(error) = 1;
+      };
+      __syncthreads();
 
-  // ---- the parts' best of each row
-  if (!a.ids) return;
-  __syncthreads();
-  if (ctas > 1) cluster_sync_all();
-  for (int d = rank + ctas * tid; d < my_rows; d += ctas * kThreads) {
-    unsigned long long b = best_of[d];
-    for (int c = 0; c < ctas; ++c)
-      if (c != rank) b = max(b, peer_load(best_of + d, c));
-    a.ids[row0 + group + d * groups] = b ? INT_MAX - static_cast<int>(static_cast<unsigned>(b)) : -1;
+      // ---- the rows
+      const unsigned* allow = allow_of(0);
+      const int allow_words = (a.V - lo - from + 31) / 32;      // from the piece's first on
+      for (int d = 0; d < my_rows; ++d) {
+        const int i = group + d * groups, skew = skew_of(row_at(d)), chunks = chunks_of(d);
+        TOut* out = nullptr;
+        if constexpr (KEEP) out = static_cast<TOut*>(a.out) + static_cast<size_t>(row0 + i) * a.ld_out + lo + from;
+        const unsigned *may = allow ? allow + word0 : nullptr, *marks = known + word0;
+        const unsigned next_leads = mask_word(d + 1);
+        allow = allow_of(d + 1);
+        if (a.drafts) {
+          drafted(i, 1u);
+          __syncthreads();
+        }
+        float best = -INFINITY, at_best = -INFINITY;
+        int id = -1, at = 0;               // the best marked token; of the others the best one's vector: its first token's place in the piece, and which of them count
+        unsigned at_plain = 0;
+        // the masks of a thread's group, looked up a chunk ahead
+        unsigned next0 = ~0u, next1 = ~0u;
+        auto look_ahead = [&](int k) {
+          const int w = k >> 5;              // (-1 where the first group begins ahead of the piece)
+          next0 = next1 = ~0u;
+          if (!may || k >= tokens) return;
+          if (w >= 0) next0 = may[w];
+          if (skew && w + 1 < allow_words) next1 = may[w + 1];
+        };
+        look_ahead(tid * kGroup - skew);
+        for (int c = 0; c < chunks; ++c) {
+          const int first = c * kTokens - skew, k0 = first + tid * kGroup;      // of the chunk's tokens; of this thread's
+          const unsigned may0 = next0, may1 = next1;
+          look_ahead(k0 + kTokens);
+          // the chunk's slots: those of its tokens, in order
+          const int t0 = max(first, 0), t1 = min(first + kTokens, tokens);
+          auto slots_ahead = [&](int k) { return k >= tokens ? slots : slot_of[word0 + (k >> 5)] - slot0 + __popc(marks[k >> 5] & ((1u << (k & 31)) - 1)); };
+          const int slot_begin = slots_ahead(t0), slot_end = slots_ahead(t1);
+          // a thread's first one, from the last warp on, as warp 0 has chunks to issue
+          const int mine = slot_begin + kThreads - 1 - tid;
+          auto place_of = [&](int n) { return t0 + ((token[n] - (from + t0)) & 0xffff); };      // in the piece
+          const int place0 = mine < slot_end ? place_of(mine) : 0;
+          unsigned may_first = ~0u;
+          if (may && mine < slot_end) may_first = may[place0 >> 5];
+          if (!ring.arrived(wait_full)) break;
+          const uint4* vectors = reinterpret_cast<const uint4*>(smem + ring.last() * kChunk);
+          // a thread's group's bits, then its warp's vectors in the order of memory, each with the bits of the group that it belongs to
+          unsigned fine = 0, own = 0, plain = 0;      // allowed ones, ones to be written here, ones that are neither marked nor forbidden
+          if (k0 < tokens) {
+            const int w = k0 >> 5, over = k0 + kGroup - tokens;
+            const unsigned inside = (k0 < 0 ? ~0u << -k0 : ~0u) & (over > 0 ? ~0u >> over : ~0u);
+            fine = inside & __funnelshift_r(may0, may1, k0 & 31);
+            own = inside & ~__funnelshift_r(marks[w], skew ? marks[w + 1] : 0u, k0 & 31);
+            plain = fine & own;
+          }
+          constexpr int kOwn = kGroup / N;
+#pragma unroll
+          for (int e = 0; e < kOwn; ++e) {
+            const int v = e * 32 + lane, shift = v % kOwn * N, k = first + (warp * 32 * kOwn + v) * N;
+            const uint4 u = vectors[warp * 32 * kOwn + v];
+            const unsigned here = __shfl_sync(0xffffffffu, plain, v / kOwn) >> shift & kAll;
+            if constexpr (KEEP) {
+              const unsigned shown = __shfl_sync(0xffffffffu, fine, v / kOwn) >> shift, written = __shfl_sync(0xffffffffu, own, v / kOwn) >> shift & kAll;
+              float z[N];
+#pragma unroll
+              for (int j = 0; j < N; ++j) z[j] = shown >> j & 1 ? Vec<TIn>::get(u, j) : -INFINITY;
+              if (written) store_all<N>(out + k, z, written);
+            }
+            const float top = Vec<TIn>::largest(u, keep_of[here]);
+            if (top > at_best || (!at_plain && here)) {
+              at_best = top != top ? -INFINITY : top;
+              at = k;
+              at_plain = here;
+            }
+          }
+          for (int n = mine; n < slot_end; n += kThreads) {
+            const int k = n == mine ? place0 : place_of(n), v = k + from;
+            const bool allowed = (n == mine || !may ? may_first : may[k >> 5]) >> (k & 31) & 1;
+            const unsigned said = count[n], times = said & (prompt_apart ? kPromptDraft - 1 : ~(kPrompt | kBiased));
+            float z = Vec<TIn>::value(reinterpret_cast<const TIn*>(vectors)[k - first]);
+            if (said & ~kBiased) z = z > 0.f ? __fdiv_rn(z, rho) : __fmul_rn(z, rho);
+            z = __fsub_rn(z, __fmul_rn(phi, static_cast<float>(times)));
+            if (times) z = __fsub_rn(z, pi);
+            if (said & kBiased) z = __fadd_rn(z, __int_as_float(entry[n]));
+            if constexpr (KEEP) store_one(out + k, allowed ? z : -INFINITY);
+            if (z != z) z = -INFINITY;
+            if (allowed && (z > best || id < 0)) best = z, id = lo + v;      // (a thread's slots ascend)
+          }
+          left();
+          if (warp == 0) issue();
+        }
+        // which token of its vector the best other one is: the first of that value, or the first at all where none is above -inf.  The warp's best ones look.
+        __syncwarp();
+        const unsigned other = at_plain ? ordered(at_best, 0) : 0u, most = __reduce_max_sync(0xffffffffu, other);
+        if (other && other == most && (id < 0 || at_best >= best)) {
+          const TIn* x = row_at(d) + at;
+          int found = 0;
+          for (unsigned bits = at_plain; bits; bits &= bits - 1) {
+            found = __ffs(bits) - 1;
+            if (at_best == -INFINITY || Vec<TIn>::value(x[found]) == at_best) break;
+          }
+          found += lo + from + at;
+          if (id < 0 || at_best > best || found < id) best = at_best, id = found;
+        }
+        __syncwarp();
+        // the warp's best: the largest value, then its lowest token
+        const unsigned value = ordered(best, id), top = __reduce_max_sync(0xffffffffu, value);
+        const unsigned lowest = __reduce_min_sync(0xffffffffu, value == top ? static_cast<unsigned>(id) : ~0u);
+        if (lane == 0 && top) atomicMax(best_of + d, static_cast<unsigned long long>(top) << 32 | (INT_MAX - lowest));
+        if (a.drafts) {
+          __syncthreads();      // the counts have been read
+          drafted(i, ~0u);
+        }
+        leads = next_leads;
+      }
+      __syncthreads();
+      word0 = word1;
+    }
+    if (warp == 0) ring.drain(wait_full);      // no copy is on its way when the CTA ends, where it gave up either
+    if (!ring.ok) *reinterpret_cast<volatile int*>(error) = 1;
+    // ---- the parts' best of each row
+    __syncthreads();
+    if (a.ids) {
+      if (ctas > 1) cluster_sync_all();
+      for (int d = rank + ctas * tid; d < my_rows; d += ctas * kThreads) {
+        unsigned long long b = best_of[d];
+        for (int c = 0; c < ctas; ++c)
+          if (c != rank) b = max(b, peer_load(best_of + d, c));
+        a.ids[row0 + group + d * groups] = b ? INT_MAX - static_cast<int>(static_cast<unsigned>(b)) : -1;
+      }
+      __syncwarp();
+      if (ctas > 1) cluster_sync_all();      // no CTA leaves while its best are read
+    }
+    if (!LONG || rows - group <= kRows * groups) break;
+    group += kRows * groups;
+    my_rows = rows_from_group();
+    __syncthreads();
+    for (int d = tid; d < kRows; d += kThreads) best_of[d] = 0;
+    __syncthreads();
   }
-  __syncwarp();
-  if (ctas > 1) cluster_sync_all();      // no CTA leaves while its best are read
 }
 
-template <typename TIn, typename TOut>
-int launch(const b200_constrain_args& a, int* error, cudaStream_t st) {
-  const auto kernel = constrain_kernel<TIn, TOut>;
-  // A request has one row: as many CTAs as the SMs have places, a row over several of them where that leaves some free (128 rows of 128256 tokens: 28 us
-  // over two, 37 over one, 38 over four; one row 8.5 us over 16, 27 over one; with the tables as they were then; now 25 and 8.2).  Several rows: their numbers differ, and most groups of a row end at once, so four
-  // times that (16 trees of up to 32 rows of 99991 fp32 logits: 82 us over four CTAs, 96 over one, 100 over two).  More rows than that: groups of several,
-  // which read their request's lists once.
+template <typename TIn, typename TOut, bool LONG>
+int launch_with(const b200_constrain_args& a, int groups, int* error, cudaStream_t st) {
+  const auto kernel = constrain_kernel<TIn, TOut, LONG>;
   const long long places = static_cast<long long>(kPlaces) * sm_count(), each = a.starts ? (a.T + a.S - 1) / a.S : 1;
-  const int groups = static_cast<int>(std::max<long long>((a.T + kRows - 1) / kRows, a.S * each <= places ? each : std::min(each, (3 * places + a.S - 1) / a.S)));
-  if (groups > 65535) return -1;
   int ctas = 1;
   while (ctas < kMostCtas && 2ll * ctas * a.S * groups <= (each > 1 ? 4 : 1) * places && a.V > 4096 * ctas) ctas *= 2;
   const int part = ((a.V + ctas - 1) / ctas + 31) / 32 * 32;
@@ -542,6 +547,19 @@ int launch(const b200_constrain_args& a, int* error, cudaStream_t st) {
   cfg.attrs = pdl_enabled() ? attr : attr + 1;
   cfg.numAttrs = pdl_enabled() ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, a, part, error) == cudaSuccess ? 0 : -2;
+}
+
+template <typename TIn, typename TOut>
+int launch(const b200_constrain_args& a, int* error, cudaStream_t st) {
+  // A request has one row: as many CTAs as the SMs have places, a row over several of them where that leaves some free (128 rows of 128256 tokens: 28 us
+  // over two, 37 over one, 38 over four; one row 8.5 us over 16, 27 over one; with the tables as they were then; now 25 and 8.2).  Several rows: their numbers differ, and most groups of a row end at once, so four
+  // times that (16 trees of up to 32 rows of 99991 fp32 logits: 82 us over four CTAs, 96 over one, 100 over two).  More rows than that: groups of several,
+  // which read their request's lists once.
+  const long long places = static_cast<long long>(kPlaces) * sm_count(), each = a.starts ? (a.T + a.S - 1) / a.S : 1;
+  // (and, where requests differ, groups for the longest one there may be, of kRows rows each, as far as a launch has room for so many of every request)
+  const long long longest = std::min<long long>((a.T + kRows - 1) / kRows, 65535 / a.S);
+  const int groups = static_cast<int>(std::max<long long>(longest, a.S * each <= places ? each : std::min(each, (3 * places + a.S - 1) / a.S)));
+  return static_cast<long long>(groups) * kRows < (a.starts ? a.T : 1) ? launch_with<TIn, TOut, true>(a, groups, error, st) : launch_with<TIn, TOut, false>(a, groups, error, st);
 }
 
 }  // namespace

@@ -129,8 +129,8 @@ struct Ring {
   B200_HD int last() const { return static_cast<int>((taken - 1) % kRing); }      // buffer of the chunk that came last
   // a bounded wait more for every chunk still on its way
   template <typename Wait>
-  B200_HD void drain(Wait wait) const {
-    for (unsigned k = taken; k != issued; ++k) wait(k % kRing, k / kRing & 1);
+  B200_HD void drain(Wait wait) {
+    for (; taken != issued; ++taken) wait(taken % kRing, taken / kRing & 1);
   }
 };
 

@@ -51,8 +51,9 @@ void walk(int chunks, int stops) {      // chunk `stops` never comes
   }
   CHECK(filler.ok == (stops >= chunks) && filler.ok == other.ok);
   CHECK(waits_after == 0);
+  const int under_way = static_cast<int>(filler.issued - filler.taken);
   filler.drain([&](unsigned b, unsigned) { return ++drained, lies[b] >= 0; });
-  CHECK(drained == static_cast<int>(filler.issued - filler.taken) && drained <= kRing && (filler.ok ? drained == 0 : drained > 0));
+  CHECK(drained == under_way && filler.taken == filler.issued && drained <= kRing && (filler.ok ? drained == 0 : drained > 0));
 }
 
 int main() {
