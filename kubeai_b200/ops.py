@@ -219,6 +219,15 @@ def _rows(at, t, kinds, what, columns=None, rows=None):
     return stride[0] if shape[0] > 1 and stride[0] > shape[1] else shape[1]
 
 
+def _mask_words(masks, T):
+    """Words of a row of ancestor masks [T, 1 to 8]; 0 where there are none.  (A tensor without words has no address either, which would stand for no masks.)"""
+    if masks is None:
+        return 0
+    if masks.dim() != 2 or masks.shape[0] != T or not 1 <= masks.shape[1] <= 8:
+        raise _refused(f"masks: [{T}, 1 to 8 words], got {tuple(masks.shape)}")
+    return masks.shape[1]
+
+
 def _pieces(like, sizes):
     """New int32 tensors of these sizes, one behind the other.  (Not views to autograd, which integers have no part in: 2.8 us for eight in place of 3.7.)"""
     return like.new_empty(sum(sizes)).unsafe_split_with_sizes(sizes)
@@ -277,8 +286,7 @@ def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_head
     _ints(at, starts, ctx_lens, masks, status)
     S, T = ctx_lens.numel(), qkv.shape[0]
     _sized(starts, S + 1, "starts"), _sized(status, S, "status")
-    if masks is not None and (masks.dim() != 2 or masks.shape[0] != T):
-        raise _refused(f"masks: [{T}, words], got {tuple(masks.shape)}")
+    words = _mask_words(masks, T)
     fresh = out is None
     if fresh:
         out = qkv.new_empty((T, q_heads * 128))
@@ -288,7 +296,7 @@ def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_head
         if out.shape[0] < T:
             raise _refused(f"out has {out.shape[0]} rows, not {T}")
     ld = _rows(at, block_tables, _I32, "block tables", rows=S)
-    a = TreeAttnArgs(S, T, q_heads, kv_heads, ldq, ldo, block_tables.shape[1], ld, masks.shape[1] if masks is not None else 0, max_tree, max_ctx, fresh, scale,
+    a = TreeAttnArgs(S, T, q_heads, kv_heads, ldq, ldo, block_tables.shape[1], ld, words, max_tree, max_ctx, fresh, scale,
                      kv_layer.shape[0], qkv.data_ptr(), out.data_ptr(), kv_layer.data_ptr(), block_tables.data_ptr(), starts.data_ptr(), ctx_lens.data_ptr(), _ptr(masks))
     a.status = _ptr(status)
     a.workspace_bytes = check(lib().b200_op_paged_attn_tree_workspace(C.byref(a)))
@@ -313,11 +321,7 @@ def constrain(logits, starts=None, history=None, hist_starts=None, prompt_lens=N
     S = starts.numel() - 1 if starts is not None else T
     _sized(hist_starts, S + 1, "hist_starts"), _sized(prompt_lens, S, "prompt_lens"), _sized(drafts, T, "drafts"), _sized(allow_rows, T, "allow_rows")
     _sized(status, S, "status")
-    words = 0
-    if masks is not None:
-        if masks.dim() != 2 or masks.shape[0] != T:
-            raise _refused(f"masks: [{T}, words], got {tuple(masks.shape)}")
-        words = masks.shape[1]
+    words = _mask_words(masks, T)
     if penalties is not None and not (penalties.dtype is torch.float32 and penalties.get_device() == at and penalties.is_contiguous() and penalties.shape == (S, 3)):
         raise _refused(f"penalties: fp32 [{S}, 3] on cuda:{at}, got {penalties.dtype} {tuple(penalties.shape)} on {penalties.device}")
     b_starts, b_ids, b_values, b_len = None, None, None, 0

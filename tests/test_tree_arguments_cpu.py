@@ -17,3 +17,17 @@ def test_masks_narrower_than_the_vocabulary_are_refused_however_far_apart_they_l
     allow = torch.zeros(4, 4010, dtype=torch.int32)[:rows, 4:]
     with pytest.raises(B200Error, match="allow"):
         ops.constrain(torch.zeros(1, 128256), allow=allow, allow_rows=torch.zeros(1, dtype=torch.int32))
+
+
+def ints(*shape):
+    return torch.zeros(*shape, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("shape", [(2, 0), (2, 9), (1, 1), (2,), (2, 1, 1)])
+def test_masks_without_words_are_not_no_masks(ops, shape):
+    """A tensor of no values has no address, which the library would take for a chain."""
+    from kubeai_b200 import B200Error
+    with pytest.raises(B200Error, match="masks: "):
+        ops.paged_attn_tree(torch.zeros(2, 512).bfloat16(), torch.zeros(1, 2, 1, 16, 128).bfloat16(), ints(1, 1), ints(2), ints(1), ints(*shape), 4, 1, 2)
+    with pytest.raises(B200Error, match="masks: "):
+        ops.constrain(torch.zeros(2, 10), starts=ints(2), drafts=ints(2), masks=ints(*shape))
