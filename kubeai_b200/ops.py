@@ -332,6 +332,10 @@ def constrain(logits, starts=None, history=None, hist_starts=None, prompt_lens=N
         if not (b_values.dtype is torch.float32 and b_values.get_device() == at and b_values.is_contiguous()):
             raise _refused(f"bias values: fp32 on cuda:{at}, got {b_values.dtype} on {b_values.device}")
     allow_ld = _rows(at, allow, _I32, "allow", columns=(V + 31) // 32) if allow is not None else 0
+    if allow is not None and not len(allow):      # no request has a grammar: every row's mask is one that is not there
+        if allow_rows is None and T:
+            raise _refused(f"allow: no masks for {T} rows")
+        allow = allow_rows = None
     out_ld = 0
     if out is not None:
         if isinstance(out, torch.dtype):

@@ -31,3 +31,27 @@ def test_masks_without_words_are_not_no_masks(ops, shape):
         ops.paged_attn_tree(torch.zeros(2, 512).bfloat16(), torch.zeros(1, 2, 1, 16, 128).bfloat16(), ints(1, 1), ints(2), ints(1), ints(*shape), 4, 1, 2)
     with pytest.raises(B200Error, match="masks: "):
         ops.constrain(torch.zeros(2, 10), starts=ints(2), drafts=ints(2), masks=ints(*shape))
+
+
+def test_rows_may_name_no_mask_where_there_are_none(ops, monkeypatch):
+    """A step in which no request has a grammar: no masks, and -1 for every row."""
+    from kubeai_b200 import B200Error
+    calls = []
+
+    class Library:
+        @staticmethod
+        def b200_op_constrain(a, stream):
+            calls.append(a._obj)
+            return 0
+
+    monkeypatch.setattr(ops, "lib", lambda: Library)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda at: 0)
+    x = torch.zeros(2, 70)
+    ops.constrain(x, allow=ints(0, 3), allow_rows=ints(2) - 1)
+    ops.constrain(x, allow=ints(4, 3), allow_rows=ints(2) - 1)
+    without, with_masks = calls
+    assert not without.allow and not without.allow_rows and with_masks.allow and with_masks.allow_rows and with_masks.allow_count == 4
+    for bad in (dict(allow=ints(0, 3)), dict(allow=ints(0, 2), allow_rows=ints(2) - 1), dict(allow=ints(0, 3), allow_rows=ints(1))):
+        with pytest.raises(B200Error, match="allow"):
+            ops.constrain(x, **bad)
+    assert len(calls) == 2
