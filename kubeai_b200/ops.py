@@ -228,6 +228,12 @@ def _mask_words(masks, T):
     return masks.shape[1]
 
 
+def _within(*sizes):
+    """Sizes go to the library as 32 bits, and one that does not fit would lose its upper ones."""
+    if max(sizes) >= 1 << 31:
+        raise _refused(f"{max(sizes)}: a size that passes 32 bits")
+
+
 def _pieces(like, sizes):
     """New int32 tensors of these sizes, one behind the other.  (Not views to autograd, which integers have no part in: 2.8 us for eight in place of 3.7.)"""
     return like.new_empty(sum(sizes)).unsafe_split_with_sizes(sizes)
@@ -263,6 +269,7 @@ def step_maps(ctx_lens, new_lens, held, block_tables, free_pages, cursor, rows, 
     if rows < 0 or not 0 <= words <= 8:
         raise _refused(f"{rows} rows, masks of {words} words")
     ld = _rows(at, block_tables, _I32, "block tables", rows=S)
+    _within(S, rows, ld, free_pages.numel())
     sizes = [S + 1, rows, rows, rows, S, 0 if inplace else S, 0 if inplace else 1, rows * words]
     starts, positions, slots, seqs, status, held_out, cursor_out, masks = _pieces(ctx_lens, sizes)
     if inplace:
@@ -287,6 +294,8 @@ def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_head
     S, T = ctx_lens.numel(), qkv.shape[0]
     _sized(starts, S + 1, "starts"), _sized(status, S, "status")
     words = _mask_words(masks, T)
+    ld = _rows(at, block_tables, _I32, "block tables", rows=S)
+    _within(S, T, ldq, ld, max_tree, max_ctx)
     fresh = out is None
     if fresh:
         out = qkv.new_empty((T, q_heads * 128))
@@ -295,7 +304,7 @@ def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_head
         ldo = _rows(at, out, _BF16, "out", columns=q_heads * 128)
         if out.shape[0] < T:
             raise _refused(f"out has {out.shape[0]} rows, not {T}")
-    ld = _rows(at, block_tables, _I32, "block tables", rows=S)
+        _within(ldo)
     a = TreeAttnArgs(S, T, q_heads, kv_heads, ldq, ldo, block_tables.shape[1], ld, words, max_tree, max_ctx, fresh, scale,
                      kv_layer.shape[0], qkv.data_ptr(), out.data_ptr(), kv_layer.data_ptr(), block_tables.data_ptr(), starts.data_ptr(), ctx_lens.data_ptr(), _ptr(masks))
     a.status = _ptr(status)
@@ -343,9 +352,11 @@ def constrain(logits, starts=None, history=None, hist_starts=None, prompt_lens=N
                 raise _refused(f"logits are kept as bf16 or fp32, not {out}")
             out = torch.empty(T, V, dtype=out, device=logits.device)
         out_ld = _rows(at, out, _LOGITS, "out", rows=T, columns=V)
+    said = history.numel() if history is not None else 0
+    _within(T, ld, out_ld, said, b_len, allow_ld, 0 if allow is None else len(allow))
     ids = torch.empty(T, dtype=torch.int32, device=logits.device) if pick else None
     a = ConstrainArgs(S, T, V, ld, logits.dtype is torch.float32, out_ld, out is not None and out.dtype is torch.float32, words,
-                      history.numel() if history is not None else 0, b_len, allow.shape[0] if allow is not None else 0, allow_ld, logits.data_ptr(), _ptr(out), _ptr(ids),
+                      said, b_len, allow.shape[0] if allow is not None else 0, allow_ld, logits.data_ptr(), _ptr(out), _ptr(ids),
                       _ptr(starts), _ptr(history), _ptr(hist_starts), _ptr(prompt_lens), _ptr(drafts), _ptr(masks), _ptr(penalties), _ptr(b_starts), _ptr(b_ids),
                       _ptr(b_values), _ptr(allow), _ptr(allow_rows), _ptr(status))
     check(lib().b200_op_constrain(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
@@ -377,6 +388,7 @@ def tree_accept(ids, drafts, parents, starts, ctx_lens, block_tables, kv, max_pa
     if not 1 <= max_path <= 256:
         raise _refused(f"paths of {max_path} rows")
     ld = _rows(at, block_tables, _I32, "block tables", rows=S)
+    _within(S, T, layers, heads, ld)
     sizes = [S, S, S * max_path, S * max_path]
     accepted, ctx, path, tokens = _pieces(ids, sizes)
     a = TreeAcceptArgs(S, T, block_tables.shape[1], ld, max_path, layers, heads, pages, apart, ids.data_ptr(), drafts.data_ptr(), _ptr(parents),

@@ -55,3 +55,31 @@ def test_rows_may_name_no_mask_where_there_are_none(ops, monkeypatch):
         with pytest.raises(B200Error, match="allow"):
             ops.constrain(x, **bad)
     assert len(calls) == 2
+
+
+@pytest.mark.parametrize("more", [1 << 31, (1 << 32) + 2])
+def test_sizes_that_pass_32_bits_are_refused_and_not_cut_off(ops, more):
+    """Of 2^32 + 2 the library would see 2.  (Tensors without memory: nothing follows their addresses.)"""
+    from kubeai_b200 import B200Error
+    far = lambda rows, n, dtype: torch.empty_strided((rows, n), (more + n, 1), dtype=dtype, device="meta")      # noqa: E731
+    q, kv, i, s = torch.zeros(2, 512).bfloat16(), torch.zeros(1, 2, 1, 16, 128).bfloat16(), ints(2), ints(3)
+    big = torch.empty(more, dtype=torch.int32, device="meta")
+    calls = [
+        lambda: ops.step_maps(i, i, i, ints(2, 4), i, ints(1), more),
+        lambda: ops.step_maps(i, i, i, far(2, 4, torch.int32), i, ints(1), 2),
+        lambda: ops.step_maps(i, i, i, ints(2, 4), big, ints(1), 2),
+        lambda: ops.paged_attn_tree(q, kv, ints(2, 4), s, i, None, 4, 1, more),
+        lambda: ops.paged_attn_tree(q, kv, ints(2, 4), s, i, None, 4, 1, 2, max_ctx=more),
+        lambda: ops.paged_attn_tree(far(2, 512, torch.bfloat16), kv, ints(2, 4), s, i, None, 4, 1, 2),
+        lambda: ops.paged_attn_tree(q, kv, ints(2, 4), s, i, None, 4, 1, 2, out=far(2, 512, torch.bfloat16)),
+        lambda: ops.constrain(far(2, 8, torch.float32), starts=s),
+        lambda: ops.constrain(torch.zeros(2, 8), starts=s, history=big, hist_starts=s),
+        lambda: ops.constrain(torch.zeros(2, 8), starts=s, allow=far(2, 1, torch.int32)),
+        lambda: ops.constrain(torch.zeros(2, 8), starts=s, out=far(2, 8, torch.float32)),
+        lambda: ops.tree_accept(i, i, None, s, i, far(2, 4, torch.int32), None, 2),
+        lambda: ops.tree_accept(big, big, None, s, i, ints(2, 4), None, 2),
+    ]
+    for k, call in enumerate(calls):
+        with pytest.raises(B200Error, match="32 bits"):
+            call()
+            pytest.fail(f"call {k} was taken")
