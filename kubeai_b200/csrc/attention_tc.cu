@@ -52,26 +52,6 @@ constexpr int kQTile = 2 * kQHalf;              // 32 KB per UMMA tile
 constexpr int kSmem = 1024 + kStages * kKvStage + 2 * kQTile + 256;   // 161 KB
 constexpr int kThreads = 288;                   // warp 0: driver (TMA + MMA); warps 1-4: rows of tile 0; warps 5-8: tile 1
 
-// Instruction descriptor: D=f32, A=B=bf16, A K-major, B K-major (b_mn = 0) or MN-major (b_mn = 1), M x N.
-__device__ __forceinline__ uint32_t idesc_bf16(uint32_t m, uint32_t n, uint32_t b_mn) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
-}
-// Shared-memory descriptor, 128B swizzle, explicit leading / stride byte offsets (units of 16 B in the descriptor).
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
-  uint64_t d = 0;
-  d |= static_cast<uint64_t>((addr & 0x3FFFFu) >> 4);
-  d |= static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFFu) << 16;
-  d |= static_cast<uint64_t>((sbo_bytes >> 4) & 0x3FFFu) << 32;
-  d |= static_cast<uint64_t>(1) << 46;
-  d |= static_cast<uint64_t>(2) << 61;
-  return d;
-}
-__device__ __forceinline__ void tma_load_3d(uint32_t dst_smem, const void* tmap, uint32_t bar, int32_t c0, int32_t c1, int32_t c2) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-               ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-               : "memory");
-}
-
 __global__ void __launch_bounds__(kThreads, 1)
 prefill_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ CUtensorMap tm_q,
                        __nv_bfloat16* __restrict__ out, int ldo, const int* __restrict__ block_tables, int max_blocks,
@@ -162,7 +142,7 @@ prefill_attn_tc_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_c
 
       const uint32_t idesc_s = idesc_bf16(128, kKvTile, 0);
       const uint32_t idesc_pv = idesc_bf16(128, kD, 1);
-      const uint64_t q_d = smem_desc_sw128(q_s, 16, 1024), k_d = smem_desc_sw128(kv_s, 16, 1024), v_d = smem_desc_sw128(kv_s + kKTile, kHalf, 1024);
+      const uint64_t q_d = desc_sw128(q_s, 16, 1024), k_d = desc_sw128(kv_s, 16, 1024), v_d = desc_sw128(kv_s + kKTile, kHalf, 1024);
       // S_i = Q_i K^T into the buffer of tile t's parity.  Its previous scores, of tile t - 2, have been read: group i's p_ready
       // arrival of that tile, waited for before PV_i(t - 2) was issued, came after its tcgen05.ld of S_i.
       auto scores = [&](int t) {

@@ -49,20 +49,7 @@ constexpr int kWaitLimit = 1 << 22;
 constexpr int kKeysAt = 2 * kQSlab, kValuesAt = kKeysAt + kDepth * kTile, kStageAt = kValuesAt + kDepth * kTile, kBars = kStageAt + 4 * 2048, kSmem = 1024 + kBars + 256;
 static_assert(kPlaces * (kSmem + 1024 + 128) <= 228 * 1024, "");
 
-__device__ __forceinline__ uint32_t idesc_bf16(uint32_t m, uint32_t n, uint32_t b_mn) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | (b_mn << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
-}
-// shared-memory descriptor, 128B swizzle, leading and stride byte offsets
-__device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | static_cast<uint64_t>((lbo >> 4) & 0x3FFFu) << 16 | static_cast<uint64_t>((sbo >> 4) & 0x3FFFu) << 32 |
-         static_cast<uint64_t>(1) << 46 | static_cast<uint64_t>(2) << 61;
-}
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, kWaitLimit)); }
-__device__ __forceinline__ void tma_load_3d(uint32_t dst_smem, const void* tmap, uint32_t bar, int32_t c0, int32_t c1, int32_t c2) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
-               ::"r"(dst_smem), "l"(reinterpret_cast<uint64_t>(tmap)), "r"(bar), "r"(c0), "r"(c1), "r"(c2)
-               : "memory");
-}
 // two bf16 without infinities and NaN
 __device__ __forceinline__ uint32_t without_odd(uint32_t u) { return ((u & 0x7f80u) == 0x7f80u ? 0u : u & 0xffffu) | ((u & 0x7f800000u) == 0x7f800000u ? 0u : u & 0xffff0000u); }
 
