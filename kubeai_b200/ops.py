@@ -228,12 +228,6 @@ def _mask_words(masks, T):
     return masks.shape[1]
 
 
-def _within(*sizes):
-    """Sizes go to the library as 32 bits, and one that does not fit would lose its upper ones."""
-    if max(sizes) >= 1 << 31:
-        raise _refused(f"{max(sizes)}: a size that passes 32 bits")
-
-
 def _pieces(like, sizes):
     """New int32 tensors of these sizes, one behind the other.  (Not views to autograd, which integers have no part in: 2.8 us for eight in place of 3.7.)"""
     return like.new_empty(sum(sizes)).unsafe_split_with_sizes(sizes)
@@ -243,6 +237,8 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+# sizes go to the library as 32 bits: one that does not fit would lose its upper ones
+_WIDE = "a size is negative or passes 32 bits"
 _I32, _BF16, _LOGITS = (torch.int32,), (torch.bfloat16,), (torch.bfloat16, torch.float32)
 
 
@@ -269,7 +265,8 @@ def step_maps(ctx_lens, new_lens, held, block_tables, free_pages, cursor, rows, 
     if rows < 0 or not 0 <= words <= 8:
         raise _refused(f"{rows} rows, masks of {words} words")
     ld = _rows(at, block_tables, _I32, "block tables", rows=S)
-    _within(S, rows, ld, free_pages.numel())
+    if (S | rows | ld | free_pages.numel()) >> 31:
+        raise _refused(_WIDE)
     sizes = [S + 1, rows, rows, rows, S, 0 if inplace else S, 0 if inplace else 1, rows * words]
     starts, positions, slots, seqs, status, held_out, cursor_out, masks = _pieces(ctx_lens, sizes)
     if inplace:
@@ -295,7 +292,8 @@ def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_head
     _sized(starts, S + 1, "starts"), _sized(status, S, "status")
     words = _mask_words(masks, T)
     ld = _rows(at, block_tables, _I32, "block tables", rows=S)
-    _within(S, T, ldq, ld, max_tree, max_ctx)
+    if (S | T | ldq | ld | max_tree | max_ctx) >> 31:
+        raise _refused(_WIDE)
     fresh = out is None
     if fresh:
         out = qkv.new_empty((T, q_heads * 128))
@@ -304,7 +302,8 @@ def paged_attn_tree(qkv, kv_layer, block_tables, starts, ctx_lens, masks, q_head
         ldo = _rows(at, out, _BF16, "out", columns=q_heads * 128)
         if out.shape[0] < T:
             raise _refused(f"out has {out.shape[0]} rows, not {T}")
-        _within(ldo)
+        if ldo >> 31:
+            raise _refused(_WIDE)
     a = TreeAttnArgs(S, T, q_heads, kv_heads, ldq, ldo, block_tables.shape[1], ld, words, max_tree, max_ctx, fresh, scale,
                      kv_layer.shape[0], qkv.data_ptr(), out.data_ptr(), kv_layer.data_ptr(), block_tables.data_ptr(), starts.data_ptr(), ctx_lens.data_ptr(), _ptr(masks))
     a.status = _ptr(status)
@@ -341,7 +340,7 @@ def constrain(logits, starts=None, history=None, hist_starts=None, prompt_lens=N
         if not (b_values.dtype is torch.float32 and b_values.get_device() == at and b_values.is_contiguous()):
             raise _refused(f"bias values: fp32 on cuda:{at}, got {b_values.dtype} on {b_values.device}")
     allow_ld = _rows(at, allow, _I32, "allow", columns=(V + 31) // 32) if allow is not None else 0
-    if allow is not None and not len(allow):      # no request has a grammar: every row's mask is one that is not there
+    if allow is not None and not allow.shape[0]:      # no request has a grammar: every row's mask is one that is not there
         if allow_rows is None and T:
             raise _refused(f"allow: no masks for {T} rows")
         allow = allow_rows = None
@@ -353,10 +352,12 @@ def constrain(logits, starts=None, history=None, hist_starts=None, prompt_lens=N
             out = torch.empty(T, V, dtype=out, device=logits.device)
         out_ld = _rows(at, out, _LOGITS, "out", rows=T, columns=V)
     said = history.numel() if history is not None else 0
-    _within(T, ld, out_ld, said, b_len, allow_ld, 0 if allow is None else len(allow))
+    masks_there = 0 if allow is None else allow.shape[0]
+    if (T | ld | out_ld | said | b_len | allow_ld | masks_there) >> 31:
+        raise _refused(_WIDE)
     ids = torch.empty(T, dtype=torch.int32, device=logits.device) if pick else None
     a = ConstrainArgs(S, T, V, ld, logits.dtype is torch.float32, out_ld, out is not None and out.dtype is torch.float32, words,
-                      said, b_len, allow.shape[0] if allow is not None else 0, allow_ld, logits.data_ptr(), _ptr(out), _ptr(ids),
+                      said, b_len, masks_there, allow_ld, logits.data_ptr(), _ptr(out), _ptr(ids),
                       _ptr(starts), _ptr(history), _ptr(hist_starts), _ptr(prompt_lens), _ptr(drafts), _ptr(masks), _ptr(penalties), _ptr(b_starts), _ptr(b_ids),
                       _ptr(b_values), _ptr(allow), _ptr(allow_rows), _ptr(status))
     check(lib().b200_op_constrain(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
@@ -388,7 +389,8 @@ def tree_accept(ids, drafts, parents, starts, ctx_lens, block_tables, kv, max_pa
     if not 1 <= max_path <= 256:
         raise _refused(f"paths of {max_path} rows")
     ld = _rows(at, block_tables, _I32, "block tables", rows=S)
-    _within(S, T, layers, heads, ld)
+    if (S | T | layers | heads | ld) >> 31:
+        raise _refused(_WIDE)
     sizes = [S, S, S * max_path, S * max_path]
     accepted, ctx, path, tokens = _pieces(ids, sizes)
     a = TreeAcceptArgs(S, T, block_tables.shape[1], ld, max_path, layers, heads, pages, apart, ids.data_ptr(), drafts.data_ptr(), _ptr(parents),
