@@ -11,8 +11,8 @@
 // every comparison prefers it.  Every wait for a copy has a limit, and a warp that gave up makes no other: its CTA has no more copied, sets an error mark and still meets the others.
 //
 // What bounds it: the lists' chain of look-ups, marks, slots and counts ahead of the rows, which is half of a CTA's time where it has one or two rows (128 rows of 128256
-// bf16 logits, 4000 tokens of history each: 25 us, of which the copies need 5; one row 8.2), and for trees the copies in and out behind it (288 rows of 99991 fp32
-// logits, kept: 82 us, 2.8 TB/s).  With the formula inside the pass over the vectors, where it ran in nearly every warp for a few of its lanes, and a row over 16 CTAs
+// bf16 logits, 4000 tokens of history each: 25 us, of which the copies need 5; one row 8.1), and for trees the copies in and out behind it (288 rows of 99991 fp32
+// logits, kept: 83 us, 2.8 TB/s).  With the formula inside the pass over the vectors, where it ran in nearly every warp for a few of its lanes, and a row over 16 CTAs
 // that all read the lists, the 128 rows took 99 us; a thread that takes the marked tokens of its own 32 of a chunk in place of a slot, 34 (and the trees 112); slots' tokens
 // found by walking the words in place of being written by who counts them, 28.
 #include <cuda_bf16.h>
@@ -552,7 +552,7 @@ int launch_with(const b200_constrain_args& a, int groups, int* error, cudaStream
 template <typename TIn, typename TOut>
 int launch(const b200_constrain_args& a, int* error, cudaStream_t st) {
   // A request has one row: as many CTAs as the SMs have places, a row over several of them where that leaves some free (128 rows of 128256 tokens: 28 us
-  // over two, 37 over one, 38 over four; one row 8.5 us over 16, 27 over one; with the tables as they were then; now 25 and 8.2).  Several rows: their numbers differ, and most groups of a row end at once, so four
+  // over two, 37 over one, 38 over four; one row 8.5 us over 16, 27 over one; with the tables as they were then; now 25 and 8.1).  Several rows: their numbers differ, and most groups of a row end at once, so four
   // times that (16 trees of up to 32 rows of 99991 fp32 logits: 82 us over four CTAs, 96 over one, 100 over two).  More rows than that: groups of several,
   // which read their request's lists once.
   const long long places = static_cast<long long>(kPlaces) * sm_count(), each = a.starts ? (a.T + a.S - 1) / a.S : 1;

@@ -11,10 +11,12 @@
 //   four warps (thread = row) do the softmax in fp32, base 2; a warp whose rows nobody owns only keeps step.
 // While one CTA of an SM ends an item, the other one keeps the memory busy.  (One CTA an SM with two softmax groups that took a row tile's keys in turn, or a row
 // tile each, stopped for 3 us at each item: 64 x 2048 74.8 us.)  More than 128 rows: items side by side, which find each other's pages in L2.
-// What bounds it: K and V's bytes to two thirds (64 requests of 2048 tokens, 32 heads on 8: 69 us, 320 MB, 4.7 TB/s; two of 32001: 57 us, 4.6 TB/s), the rest is
-// ranges' first loads, the softmax and the join; with 256 rows of a key head (48 x 1999 tokens, 64 rows, 93 us) the chain of a tile through its softmax warps.
+// What bounds it: the chain of a tile through its softmax warps, 1850 to 2000 cycles from scores to weights (load and maximum, exponentials, weights back to tensor memory; 600 of
+// them O's rescaling and the wait for the product ahead of it) and 400 more until the next scores are there, by two CTAs an SM; the exponentials' unit has work for 512 of a full
+// tile.  64 requests of 2048 tokens, 32 heads on 8: 69 us, 320 MB, 4.7 TB/s (the second kernel's 6 us left out 5.1); two of 32001: 58 us, 4.6 TB/s; 48 of 1999 with 64
+// rows, 256 rows of a key head: 93 us, exponentials' unit 27 % busy, tensor cores 32 %, issue slots 40 %.
 // Weights are relative to the row's largest score so far, so the largest weight is exactly 1 and its rounding to bf16 costs nothing.  Relative to up to 2^8 times an older
-// maximum, which saves most of the rescaling of O (62, 55 and 84 us), results were off by 1 to 13 % more (64 x 2048: 0.00232 of the output for 0.00222).
+// maximum, which saves most of the rescaling of O (63, 55 and 84 us), results were off by 1 to 13 % more (64 x 2048: 0.00232 of the output for 0.00222).
 // The masks' bits are looked at only in tiles that reach behind the context.  There the products' warp also clears what must not meet a weight of zero:
 // values behind the last key, and infinities and NaN among the drafts' values, which the rows that see them add at the end by themselves.
 // An item that a range's end cuts leaves unnormalised rows in the workspace, which a second kernel joins in a fixed order: the same bits every time.
@@ -629,8 +631,8 @@ __device__ __forceinline__ void join_row(int parts, Part part, int lane, uint2* 
 }
 
 // All such rows, a warp each: every block sums the cut items' rows for itself and takes its share.  What bounds it is the chain from the first kernel's end (the cuts,
-// a search, statistics, parts), some 5 us of a call.  A block for eight rows of each CTA's item, of which most had none, came in eleven waves and with the form of
-// twelve parts at once for every row: 64 x 2048 64.6 us a call in place of 62.4, 2 x 32001 59.9 in place of 55.4, 48 x 1999 with 64 rows 91.4 in place of 83.5.
+// a search, statistics, parts): 3 us of a call of 1 x 450, 6 of 64 x 2048, 5 of 2 x 32001, 11 of 48 x 1999 with 64 rows, whose parts are 19 MB.  A block for eight rows of each CTA's item,
+// of which most had none, came in eleven waves and with the form of twelve parts at once for every row: 2, 4.5 and 8 us more.
 __global__ void __launch_bounds__(kJoinThreads, kJoinPlaces)
 tree_attn_join_kernel(const __grid_constant__ b200_tree_attn_args a, int ctas, int blocks) {
   extern __shared__ int rows_before[];      // [ctas + 1] of each CTA's cut item
@@ -681,7 +683,7 @@ int64_t tree_attention_workspace(const b200_tree_attn_args&) { return static_cas
 int paged_attention_tree(const b200_tree_attn_args& a, int* error, cudaStream_t st) {
   const int group = a.q_heads / a.kv_heads;
   const int rows = static_cast<int>(std::min(static_cast<long long>(kRows), std::min(a.max_tree, a.T) * static_cast<long long>(group)));
-  // as many CTAs as there are places, or as the most work that the call may have feeds: 11.4 us for 1 x 450, over all places 12.0
+  // as many CTAs as there are places, or as the most work that the call may have feeds: 0.6 us less for 1 x 450 (11.0 now) than over all places
   const long long seen = std::min(a.max_ctx ? a.max_ctx : INT_MAX, a.max_blocks * tree::kPage) + static_cast<long long>(std::min(a.max_tree, a.T));
   const long long items = (static_cast<long long>(std::min(a.max_tree, a.T)) * group + kRows - 1) / kRows * a.kv_heads * a.S, cost = items * ((seen + kKeys - 1) / kKeys + tree::kItem);
   const int ctas = static_cast<int>(std::min<long long>(kPlaces * sm_count(), std::max<long long>(1, cost / tree::kLeast)));
