@@ -409,6 +409,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         t0 = 0;
         if ((more = rest > 0)) next_item();
       }
+      if (!ok && gt) warp_wait(s_full((gt - 1) & 1), ((gt - 1) >> 1) & 1);      // no product is under way when tensor memory is given back
     } else if (warp == kWarps - 1) {
       // ------------------------------------------------------------ outputs
       const bool one = elect_one();
@@ -458,6 +459,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant
         t0 = 0;
         if ((more = rest > 0)) next_item();
       }
+      if (!ok && gt) warp_wait(pv_full((gt - 1) & 1), ((gt - 1) >> 1) & 1);
     } else {
       // ------------------------------------------------------------ softmax: thread = row (token * group + head)
       const int q = warp & 3, row = q * 32 + lane;      // the quarter of the lanes that this warp may access
