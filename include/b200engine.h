@@ -587,6 +587,101 @@ typedef struct {
   const int32_t* status;
 } b200_tree_accept_args;
 int b200_op_tree_accept(const b200_tree_accept_args* a, void* stream);
+/* ---- a decode step whose requests share their beginnings, beams above all (csrc/beam_step.h).  No argument that the device holds makes a kernel read or write outside the buffers, calls
+ * may run side by side on several streams and be captured, and they keep nothing. */
+/* Norms and rotary positions of queries and keys, and keys and values into the paged cache, in one pass over qkv [T, (q_heads + 2 kv_heads) * 128] bf16, rows ldx apart.
+ * For each head of q and k, in fp32 and rounded once:  y = x w / sqrt(mean(x^2) + eps)  (q_norm, k_norm: 128 weights, or 128 for each head where q_norm_ld, k_norm_ld are 128; bf16 or
+ * fp32 (norm_f32); NULL: y = x), then the first dims values as pairs (d, d + dims / 2), or with interleaved (2 d, 2 d + 1), turned by positions[t] * freqs[d] (fp64 radians a
+ * position, d < dims / 2) and multiplied by gain; the others are y.  The angle is reduced to a part of a turn in integers, so far positions lose nothing.
+ * q goes to out [T, q_heads * 128], rows ldo apart (it may be qkv itself with ldo == ldx), k and v to the token's slot (page * 16 + offset) of kv_layer [num_pages][2][kv_heads][16][128];
+ * a slot that the cache does not have is written nowhere, and slots are distinct.  dims even, 0 to 128; ldx, ldo multiples of 8; qkv, out, kv_layer 16-byte aligned. */
+typedef struct {
+  int32_t T, q_heads, kv_heads, ldx, ldo, dims, interleaved, q_norm_ld, k_norm_ld, norm_f32;
+  float eps, gain;
+  int64_t num_pages;
+  const void* qkv;
+  void* out;
+  void* kv_layer;
+  const int32_t* positions;
+  const int32_t* slots;
+  const double* freqs;
+  const void* q_norm;
+  const void* k_norm;
+} b200_norm_rope_args;
+int b200_op_norm_rope_kvwrite(const b200_norm_rope_args* a, void* stream);
+/* Attention over the paged cache for groups of requests whose first pages are the same.  S requests as in b200_op_paged_attn_tree, without masks: row i of a request sees its ctx tokens in
+ * the cache and the request's rows 0 .. i, whose K and V are in the cache already.  Group g has the requests group_starts[g] .. group_starts[g + 1] - 1; the first
+ * shared[g] tokens of their tables, of which whole pages count and no more than the first request has in the cache, are the same in all of them and are read by the first one's table, once for the
+ * group's rows.  Requests of no group, of one that has a single request, with fewer tokens in the cache than are shared, or all where starts or group_starts do not ascend, are attended alone.
+ * max_rows: most rows of a request; max_ctx: most tokens in front of them, if known (0: what a row of the table holds), which only decides how the work is split.
+ * Everything else as for b200_op_paged_attn_tree: what is left out and zero_rest, pages that the cache does not have, odd values in what a row does not see, sizes and
+ * alignments, status.  S and G <= 65534. */
+typedef struct {
+  int32_t S, T, G, q_heads, kv_heads, ldq, ldo, max_blocks, ld_tables, max_rows, max_ctx, zero_rest;
+  float scale;
+  int64_t num_pages;
+  const void* q;
+  void* out;
+  const void* kv_layer;
+  const int32_t* block_tables;
+  const int32_t* starts;
+  const int32_t* ctx;
+  const int32_t* group_starts;
+  const int32_t* shared;
+  const int32_t* status;
+  void* workspace;
+  int64_t workspace_bytes;
+} b200_shared_attn_args;
+/* Bytes of a call's workspace, which it uses until its kernels have run and which needs no preparation: some tens of MB by the GPU, and 1 KB for each row and head where there are groups. */
+int64_t b200_op_paged_attn_shared_workspace(const b200_shared_attn_args* a);
+int b200_op_paged_attn_shared(const b200_shared_attn_args* a, void* stream);
+/* The k best candidates over a request's beams and the vocabulary, and the beams that go on.  logits [S * beams, V], rows ld apart, bf16 or fp32 (logits_f32), scores fp32 [S, beams]:
+ *   c(b, v) = scores[b] + x(b, v) - log(sum over w of exp(x(b, w)))   in 64 bits
+ * in descending order, equal ones by the lower beam; a beam's own by the larger logit, equal ones by the lower token.  NaN among logits or scores counts as -inf, and what is -inf is no candidate;
+ * +inf logits of a row share its probability.  Out: found_parents, found_tokens, found_scores [S, k] (-1, -1, -inf behind the last); parents, tokens, scores [S, beams]: the first beams of them whose
+ * token is none of ends [num_ends] (the same fillers).  beams <= 32, k <= 64, V <= 393216, num_ends <= 1024, rows of logits aligned as their type. */
+typedef struct {
+  int32_t S, beams, V, ld, logits_f32, k, num_ends;
+  const void* logits;
+  const float* scores;
+  const int32_t* ends;
+  int32_t* parents;
+  int32_t* tokens;
+  float* new_scores;
+  int32_t* found_parents;
+  int32_t* found_tokens;
+  float* found_scores;
+  void* workspace;
+  int64_t workspace_bytes;
+} b200_beam_select_args;
+/* Bytes of a call's workspace, which needs no preparation */
+int64_t b200_op_beam_select_workspace(const b200_beam_select_args* a);
+int b200_op_beam_select(const b200_beam_select_args* a, void* stream);
+/* Tables, texts and cache rows of the beams that go on.  Request s has rows s * beams .. of block_tables, texts, ctx and text_lens, its beams ctx tokens each in the cache, this step's among them (ctx[s * beams]; where
+ * its beams differ, the lengths do not fit its table or no parent is one of its beams, the request is left as it is).  parents [S, beams]: the beam that each new one continues; what is none follows the request's first one
+ * that is, without a token.  tables_out: row i has the pages of its parent; the last page, where ctx ends inside it, belongs to one beam alone: the first beam of a parent keeps the parent's,
+ * every other one takes that of a beam nobody continues, in order, into which the parent's rows are copied in every layer of kv [layers][num_pages][2][kv_heads][16][128]
+ * (layer_stride elements apart).  So every beam's last page has to be its own before the call, and is after it; pages behind it stay with their rows.
+ * shared [S]: tokens on leading whole pages that all new beams have; released [S * beams, max_blocks]: the number of a whole page of block_tables that no new beam has, where it first stands, else -1.
+ * texts [S * beams, room] (or NULL): texts_out row i is its parent's with tokens[i] behind its text_lens (where there is room), text_lens_out the length.
+ * beams <= 32; out buffers are others than the inputs. */
+typedef struct {
+  int32_t S, beams, max_blocks, ld_tables, ld_tables_out, layers, kv_heads, room, ld_texts, ld_texts_out;
+  int64_t num_pages, layer_stride;
+  const int32_t* parents;
+  const int32_t* tokens;
+  const int32_t* ctx;
+  const int32_t* block_tables;
+  int32_t* tables_out;
+  int32_t* released;
+  int32_t* shared;
+  void* kv;
+  const int32_t* texts;
+  int32_t* texts_out;
+  const int32_t* text_lens;
+  int32_t* text_lens_out;
+} b200_beam_reorder_args;
+int b200_op_beam_reorder(const b200_beam_reorder_args* a, void* stream);
 int b200_op_init_uniform(void* p, uint64_t n, uint32_t seed, float scale, float offset, void* stream);
 
 #ifdef __cplusplus

@@ -56,8 +56,13 @@ SOURCES = [
     "tree_attention.cu",
     "constrain.cu",
     "tree_accept.cu",
+    "norm_rope.cu",
+    "shared_attention.cu",
+    "beam_select.cu",
+    "beam_reorder.cu",
     "abi_ops.cu",
     "abi_tree.cu",
+    "abi_beam.cu",
     "engine.cu",
     "router.cc",
     "loader.cc",

@@ -65,6 +65,30 @@ class TreeAcceptArgs(C.Structure):
         [(n, C.c_void_p) for n in ("ids", "drafts", "parents", "starts", "ctx", "block_tables", "kv", "accepted", "path", "tokens", "new_ctx", "status")]
 
 
+class NormRopeArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("T", "q_heads", "kv_heads", "ldx", "ldo", "dims", "interleaved", "q_norm_ld", "k_norm_ld", "norm_f32")] + \
+        [(n, C.c_float) for n in ("eps", "gain")] + [("num_pages", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("qkv", "out", "kv_layer", "positions", "slots", "freqs", "q_norm", "k_norm")]
+
+
+class SharedAttnArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("S", "T", "G", "q_heads", "kv_heads", "ldq", "ldo", "max_blocks", "ld_tables", "max_rows", "max_ctx", "zero_rest")] + \
+        [("scale", C.c_float), ("num_pages", C.c_int64)] + \
+        [(n, C.c_void_p) for n in ("q", "out", "kv_layer", "block_tables", "starts", "ctx", "group_starts", "shared", "status", "workspace")] + [("workspace_bytes", C.c_int64)]
+
+
+class BeamSelectArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("S", "beams", "V", "ld", "logits_f32", "k", "num_ends")] + \
+        [(n, C.c_void_p) for n in ("logits", "scores", "ends", "parents", "tokens", "new_scores", "found_parents", "found_tokens", "found_scores", "workspace")] + \
+        [("workspace_bytes", C.c_int64)]
+
+
+class BeamReorderArgs(C.Structure):
+    _fields_ = [(n, C.c_int32) for n in ("S", "beams", "max_blocks", "ld_tables", "ld_tables_out", "layers", "kv_heads", "room", "ld_texts", "ld_texts_out")] + \
+        [(n, C.c_int64) for n in ("num_pages", "layer_stride")] + \
+        [(n, C.c_void_p) for n in ("parents", "tokens", "ctx", "block_tables", "tables_out", "released", "shared", "kv", "texts", "texts_out", "text_lens", "text_lens_out")]
+
+
 class FeedEntry(C.Structure):
     _fields_ = [("req_id", C.c_uint64), ("tokens", C.POINTER(C.c_int32)), ("n_tokens", C.c_int32),
                 ("want", C.POINTER(C.c_int32)), ("n_want", C.c_int32)]
@@ -240,6 +264,12 @@ SYMBOLS = {
     "b200_op_paged_attn_tree_workspace": (C.c_int64, [C.POINTER(TreeAttnArgs)]),
     "b200_op_constrain": (C.c_int, [C.POINTER(ConstrainArgs), _vp]),
     "b200_op_tree_accept": (C.c_int, [C.POINTER(TreeAcceptArgs), _vp]),
+    "b200_op_norm_rope_kvwrite": (C.c_int, [C.POINTER(NormRopeArgs), _vp]),
+    "b200_op_paged_attn_shared": (C.c_int, [C.POINTER(SharedAttnArgs), _vp]),
+    "b200_op_paged_attn_shared_workspace": (C.c_int64, [C.POINTER(SharedAttnArgs)]),
+    "b200_op_beam_select": (C.c_int, [C.POINTER(BeamSelectArgs), _vp]),
+    "b200_op_beam_select_workspace": (C.c_int64, [C.POINTER(BeamSelectArgs)]),
+    "b200_op_beam_reorder": (C.c_int, [C.POINTER(BeamReorderArgs), _vp]),
     "b200_op_init_uniform": (C.c_int, [_vp, _u64, C.c_uint32, _f, _f, _vp]),
 }
 

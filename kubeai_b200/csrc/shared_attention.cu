@@ -1,0 +1,497 @@
+// Attention over the paged cache for groups of requests whose first pages are the same.
+//
+//   out_t = sum_j softmax_j(scale q_t . k_j) v_j    over the shared keys j < P, once for all rows of a group, and the request's own j >= P up to the row itself
+//
+// Softmax over two sets of keys is a weighted sum of softmaxes over each, so the rows of a group meet the shared pages in an item of their own and every request's rows the pages behind
+// them in another, and the two are joined by their maxima and sums.
+// An item is a key head and up to 16 rows (row = token * group + head) with a range of pages.  All items' pages one behind the other are cut into as many equal ranges as there are places for
+// warps, and a warp walks its range without a gap: it loads pages ahead by TMA (128-byte swizzle) into a ring of its own, over an item's end, and multiplies with mma.sync: a row tile of
+// 16 leaves the tensor cores idle in any form, and memory is what bounds it.  No warp waits for another.
+// An item that a range's end cuts leaves unnormalised rows in the workspace, as every item does that shares its rows with another; a second kernel joins them in a fixed order.
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <limits.h>
+#include <math.h>
+
+#include <algorithm>
+
+#include "beam_step.h"
+#include "gemm.h"
+#include "kernels.h"
+#include "launch.h"
+#include "ptx.cuh"
+
+namespace b200 {
+namespace {
+
+typedef __nv_bfloat16 bf16;
+using beam::Lengths;
+using beam::Part;
+constexpr int kD = 128, kRows = 16, kPageBytes = 2 * 16 * kD * 2;      // bytes of a page's keys and values of a head
+constexpr int kThreads = 128, kWarps = kThreads / 32, kPlaces = 3, kDepth = 2, kItems = 4;      // kPlaces: CTAs of an SM; kDepth: pages of a warp on their way; kItems: items that those may lie in, and one
+constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
+constexpr int kJoinThreads = 256, kFew = 4;
+constexpr int kWaitLimit = 1 << 22;
+constexpr int kSmem = 1024 + kWarps * kDepth * kPageBytes;
+static_assert(kPlaces * (kSmem + 3072) <= 228 * 1024, "");
+static_assert(kItems > kDepth, "");
+
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, kWaitLimit)); }
+// two bf16 without infinities and NaN
+__device__ __forceinline__ uint32_t without_odd(uint32_t u) { return ((u & 0x7f80u) == 0x7f80u ? 0u : u & 0xffffu) | ((u & 0x7f800000u) == 0x7f800000u ? 0u : u & 0xffff0000u); }
+
+// Where the rows of a token and key head are: their own keys' part, and what their group shares.
+struct Place {
+  int slot, parts;      // parts 0: in the rows of all (or in the output), else in the slots of `parts` ranges, slot the first
+  int row;              // the token's first row there
+  int joined;           // own rows: the group's are to be added
+};
+struct Space {
+  Place* places;        // [2][T][kv_heads]: the groups', the requests' own
+  float* slots;         // [warps][2][16][kLd]: a range's first item, which another range began, and its last
+  float* rows;          // [2][T][q_heads][kLd]
+};
+__host__ __device__ inline Space space_of(const b200_shared_attn_args& a, long long warps) {
+  Space s;
+  s.places = static_cast<Place*>(a.workspace);
+  s.slots = reinterpret_cast<float*>(s.places + 2ll * a.T * a.kv_heads);
+  s.rows = s.slots + warps * 2 * kRows * kLd;
+  return s;
+}
+
+__device__ __forceinline__ Lengths lengths_of(const b200_shared_attn_args& a, bool ordered) {
+  return {a.starts, a.ctx, a.group_starts, a.shared, a.status, a.S, a.T, ordered ? a.G : 0, a.max_blocks, a.max_rows};
+}
+
+// ---- items
+struct Item {
+  int u, kvh, block;
+  Part p;
+  int first, nb, k1, pages;      // the block's tokens, the keys they may see
+};
+__device__ __forceinline__ int end_of(const Part& p, int bt, int block) { return p.all ? p.k1 : p.ctx + min(p.rows, (block + 1) * bt); }
+__device__ __forceinline__ int pages_of(const Part& p, int bt, int block) { return (end_of(p, bt, block) - p.k0 + 15) / 16; }
+__device__ __forceinline__ int blocks_of(const Part& p, int bt) { return (p.rows + bt - 1) / bt; }
+__device__ __forceinline__ int head_cost(const Part& p, int bt) {
+  const int blocks = blocks_of(p, bt);
+  if (p.all || blocks <= 1) return blocks ? blocks * (pages_of(p, bt, 0) + tree::kItem) : 0;
+  int n = 0;
+  for (int b = 0; b < blocks; ++b) n += pages_of(p, bt, b) + tree::kItem;
+  return n;
+}
+__device__ __forceinline__ void fill(int bt, Item* it) {
+  it->first = it->block * bt;
+  it->nb = min(bt, it->p.rows - it->first);
+  it->k1 = end_of(it->p, bt, it->block);
+  it->pages = pages_of(it->p, bt, it->block);
+}
+
+// An item's pages of a range, as the loads leave them for the products
+struct Piece {
+  int row0, rows, kvh;           // the first row of the step, rows (token * group + head)
+  int key, pages;                // first key, pages
+  int end, see;                  // keys behind the last, and behind the last that token 0 sees; token i sees i more
+  int table;
+  int whole, begins, own, joined;
+  int parts;
+};
+
+__global__ void __launch_bounds__(kThreads, kPlaces)
+shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ b200_shared_attn_args a, float scale_log2, int* error) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[kWarps * kDepth];
+  __shared__ int sums[kWarps], s_range[kWarps + 1], s_where[kWarps + 1][4];
+  __shared__ Piece pieces[kWarps][kItems];
+  const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem = smem_raw + (sbase - smem_u32(smem_raw));
+  const int warp = warp_number(), lane = threadIdx.x & 31, tid = threadIdx.x;
+  const int group = a.q_heads / a.kv_heads, bt = kRows / group, shift = __ffs(group) - 1;
+  const uint32_t ring = sbase + warp * kDepth * kPageBytes, full0 = smem_u32(bars + warp * kDepth);
+  if (lane == 0) {
+    for (int s = 0; s < kDepth; ++s) mbar_init(full0 + 8 * s, 1);
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_kv);
+  }
+  griddep_enter();
+  // ---- the warps' ranges: every thread sums some parts of the step, one behind the other, and the sums of the threads in front of it
+  bool ordered = a.G > 0;
+  if (ordered) ordered = __syncthreads_and(beam::ascends(a.group_starts, a.G, a.S, tid, kThreads) && beam::ascends(a.starts, a.S, a.T, tid, kThreads));
+  const Lengths n = lengths_of(a, ordered);
+  const int U = n.G + a.S, per = (U + kThreads - 1) / kThreads, u_begin = min(U, tid * per), u_end = min(U, u_begin + per);
+  int before = 0, N = 0;
+  for (int u = u_begin; u < u_end; ++u) before += head_cost(beam::part_of(n, u), bt) * a.kv_heads;
+  const int own = before;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += y;
+  }
+  if (lane == 31) sums[warp] = before;
+  __syncthreads();
+  before -= own;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const int x = sums[w];
+    if (w < warp) before += x;
+    N += x;
+  }
+  const int gw0 = blockIdx.x * kWarps, gw = gw0 + warp;
+  const tree::Ranges ranges = tree::ranges_of(N, gridDim.x * kWarps);
+  if (tid <= kWarps && gw0 + tid >= ranges.n) s_range[tid] = N;      // which lies in no item
+  if (N > 0 && gw0 < ranges.n) {
+    const int b_end = ranges.at(min(gw0 + kWarps, ranges.n - 1));
+    if (own && ranges.at(gw0) < before + own && b_end >= before)
+      for (int u = u_begin; u < u_end; ++u) {
+        const Part p = beam::part_of(n, u);
+        const int mine = head_cost(p, bt) * a.kv_heads;
+        for (int e = 0; e <= kWarps && gw0 + e < ranges.n; ++e) {
+          const int b = ranges.at(gw0 + e);
+          if (mine == 0 || b < before || b >= before + mine) continue;
+          int g0 = before, block = 0, pages = pages_of(p, bt, 0);
+          while (b >= g0 + (pages + tree::kItem) * a.kv_heads) g0 += (pages + tree::kItem) * a.kv_heads, pages = pages_of(p, bt, ++block);
+          const int kvh = (b - g0) / (pages + tree::kItem);
+          g0 += kvh * (pages + tree::kItem);
+          s_range[e] = tree::snapped(b, g0, pages, ranges.snap);
+          s_where[e][0] = u; s_where[e][1] = kvh; s_where[e][2] = block; s_where[e][3] = g0;
+        }
+        before += mine;
+      }
+  }
+  __syncthreads();
+  const int left = N > 0 && gw < ranges.n ? s_range[warp + 1] - s_range[warp] : 0;
+  if (left <= 0) return;
+  const Space space = space_of(a, static_cast<long long>(gridDim.x) * kWarps);
+
+  // ---- loads: item, its first page here, the range's cost to go
+  Item it;
+  it.u = s_where[warp][0]; it.kvh = s_where[warp][1]; it.block = s_where[warp][2];
+  it.p = beam::part_of(n, it.u);
+  fill(bt, &it);
+  int t0 = max(0, s_range[warp] - s_where[warp][3] - tree::kItem), rest = left;
+  auto next_item = [&] {
+    if (++it.kvh >= a.kv_heads) {
+      it.kvh = 0;
+      if (++it.block >= blocks_of(it.p, bt)) {
+        it.block = 0;
+        do it.p = beam::part_of(n, ++it.u);
+        while (it.p.rows == 0);      // (a range's pages are some part's: the walk ends in front of U)
+      }
+    }
+    fill(bt, &it);
+  };
+  if (t0 == it.pages) {              // the range begins where the item in front of it ends
+    t0 = 0;
+    next_item();
+  }
+  bool more = true, ok = true;
+  int take = 0, at = 0, items = 0, issued = 0, mine = 0, next = 0;      // the item's pages here, the page that is next; items so far; pages so far
+  const bool one = elect_one();
+  // the first row of a page's keys; a page that the cache does not have lies behind its last row, where a load finds zeros
+  auto look_up = [&](int p) {
+    const int page = p < t0 + take ? a.block_tables[static_cast<size_t>(it.p.table) * a.ld_tables + it.p.k0 / 16 + p] : -1;
+    return ((page >= 0 && page < a.num_pages ? page : static_cast<int>(a.num_pages)) * 2 * a.kv_heads + it.kvh) * 16;
+  };
+  auto begin = [&] {
+    take = tree::take_of(t0, it.pages, &rest);
+    at = 0;
+    mine = look_up(t0 + lane);
+    next = look_up(t0 + 32 + lane);
+    if (lane == 0) {
+      const bool whole = t0 == 0 && take == it.pages;
+      Piece x;
+      x.row0 = it.p.row0 + it.first;
+      x.rows = it.nb * group;
+      x.kvh = it.kvh;
+      x.key = it.p.k0 + 16 * t0;
+      x.pages = take;
+      x.end = it.k1;
+      x.see = it.p.all ? it.k1 : it.p.ctx + it.first + 1;
+      x.table = it.p.table;
+      x.whole = whole;
+      x.begins = t0 == 0;
+      x.own = !it.p.all;
+      x.joined = it.p.k0 > 0;
+      x.parts = whole ? 0 : t0 == 0 ? ranges.parts(gw, s_range[warp + 1] - take, it.pages) : 0;
+      pieces[warp][items % kItems] = x;
+    }
+    ++items;
+    __syncwarp();
+  };
+  // the next page of the range, into the place of the one that was used last
+  auto load = [&] {
+    if (!more) return;
+    if (at == take) {
+      if (rest <= 0) { more = false; return; }
+      t0 = 0;
+      next_item();
+      begin();
+    } else if (at && at % 32 == 0) {
+      mine = next;
+      next = look_up(t0 + at + 32 + lane);
+    }
+    const int row = __shfl_sync(0xffffffffu, mine, at & 31), st = issued % kDepth;
+    const uint32_t full = full0 + 8 * st, dst = ring + st * kPageBytes;
+    if (one) {
+      mbar_arrive_expect_tx(full, kPageBytes);
+      tma_load_2d(dst, &tm_kv, full, 0, row, kEvictNormal);
+      tma_load_2d(dst + 2048, &tm_kv, full, 64, row, kEvictNormal);
+      tma_load_2d(dst + 4096, &tm_kv, full, 0, row + 16 * a.kv_heads, kEvictNormal);
+      tma_load_2d(dst + 6144, &tm_kv, full, 64, row + 16 * a.kv_heads, kEvictNormal);
+    }
+    __syncwarp();
+    ++at;
+    ++issued;
+  };
+  begin();
+  for (int k = 0; k < kDepth; ++k) load();
+
+  // ---- products: this thread has rows g and g + 8
+  const int g = lane >> 2, q2 = (lane & 3) * 2, rr = lane & 7, tile = lane >> 3;
+  const uint32_t k_row = rr + (tile >> 1) * 8, k_chunk = tile & 1, v_row = rr + (tile & 1) * 8, v_chunk = tile >> 1;
+  int used = 0;
+  for (int item = 0; ok && used < issued; ++item) {
+    const Piece x = pieces[warp][item % kItems];
+    // queries: rows nobody owns are zeros
+    uint32_t qa[8][4];
+    const bf16* q = static_cast<const bf16*>(a.q) + x.kvh * group * kD + q2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = g + 8 * h;
+      const bf16* from = q + static_cast<size_t>(x.row0 + (r >> shift)) * a.ldq + (r & (group - 1)) * kD;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        qa[ks][h] = r < x.rows ? *reinterpret_cast<const uint32_t*>(from + ks * 16) : 0u;
+        qa[ks][2 + h] = r < x.rows ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 8) : 0u;
+      }
+    }
+    float o[16][4];
+#pragma unroll
+    for (int d = 0; d < 16; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[d][c] = 0.f;
+    float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // what the weights are relative to, in units of log 2; this thread's part of their sum
+    const int limit[2] = {min(x.see + (g >> shift), x.end), min(x.see + ((g + 8) >> shift), x.end)};
+    bool odd = false;
+    for (int j = 0; j < x.pages; ++j, ++used) {
+      const int st = used % kDepth, key0 = x.key + 16 * j;
+      if (!(ok = warp_wait(full0 + 8 * st, (used / kDepth) & 1))) break;
+      const uint32_t ks_ = ring + st * kPageBytes, vs_ = ks_ + 4096;
+      if (key0 + 16 > x.see) {
+        // what must not meet a weight of zero: values behind the last key, and infinities and NaN among values that some row does not see, which those that do add at the end
+        uint4* v = reinterpret_cast<uint4*>(smem + (vs_ - sbase));
+        bool found = false;
+        for (int e = lane; e < 256; e += 32) {
+          const int key = key0 + ((e & 127) >> 3);      // (a row's pieces in some order)
+          if (key < x.see) continue;
+          uint4 w = v[e];
+          if (key >= x.end) w = make_uint4(0, 0, 0, 0);
+          else {
+            const uint4 was = w;
+            w = make_uint4(without_odd(w.x), without_odd(w.y), without_odd(w.z), without_odd(w.w));
+            found = found || w.x != was.x || w.y != was.y || w.z != was.z || w.w != was.w;
+          }
+          v[e] = w;
+        }
+        odd = __any_sync(0xffffffffu, found) || odd;
+        fence_proxy_async();
+        __syncwarp();
+      }
+      float s[2][4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) s[0][c] = s[1][c] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        uint32_t b0, b1, b2, b3;
+        ldmatrix_x4(ks_ + (ks >> 2) * 2048 + k_row * 128 + ((((ks & 3) * 2 + k_chunk) ^ (k_row & 7)) << 4), b0, b1, b2, b3);
+        mma_bf16_16816(s[0], qa[ks], b0, b1);
+        mma_bf16_16816(s[1], qa[ks], b2, b3);
+      }
+      if (key0 + 16 > x.see) {
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            if (key0 + nb * 8 + q2 + (c & 1) >= limit[c >> 1]) s[nb][c] = -INFINITY;
+      }
+      float alpha[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float top = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2)) * scale_log2;
+        alpha[h] = 1.f;
+        if (top > ref[h]) {
+          alpha[h] = exp2_ftz(ref[h] - top);
+          ref[h] = top;
+        }
+      }
+      uint32_t pa[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float mu = ref[h] == -INFINITY ? 0.f : ref[h];
+        float ps = 0.f;
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+          const uint32_t w = pack_bf16x2(exp2_ftz(fmaf(s[nb][2 * h], scale_log2, -mu)), exp2_ftz(fmaf(s[nb][2 * h + 1], scale_log2, -mu)));
+          // the sum is that of the rounded weights: where one weight outweighs the others, its rounding cancels
+          ps += __uint_as_float(w << 16) + __uint_as_float(w & 0xffff0000u);
+          pa[2 * nb + h] = w;
+        }
+        l[h] = l[h] * alpha[h] + ps;
+      }
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+        for (int d = 0; d < 16; ++d)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[d][c] *= alpha[c >> 1];
+      }
+#pragma unroll
+      for (int dp = 0; dp < 8; ++dp) {
+        uint32_t b0, b1, b2, b3;
+        ldmatrix_x4_trans(vs_ + (dp >> 2) * 2048 + v_row * 128 + ((((dp & 3) * 2 + v_chunk) ^ (v_row & 7)) << 4), b0, b1, b2, b3);
+        mma_bf16_16816(o[2 * dp], pa, b0, b1);
+        mma_bf16_16816(o[2 * dp + 1], pa, b2, b3);
+      }
+      __syncwarp();      // all have read the page
+      load();
+    }
+    if (!ok) break;
+    // ---- the item's rows
+    if (odd) {
+      for (int p = max(x.see, x.key); p < min(x.end, x.key + 16 * x.pages); ++p) {
+        const long long row = tree::cache_row(a.block_tables + static_cast<size_t>(x.table) * a.ld_tables, p, a.num_pages);
+        if (row < 0) continue;
+        const bf16* value = static_cast<const bf16*>(a.kv_layer) + ((((row >> 4) * 2 + 1) * a.kv_heads + x.kvh) * 16 + (row & 15)) * kD + q2;
+#pragma unroll
+        for (int d = 0; d < 16; ++d)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const float y = __bfloat162float(value[d * 8 + (c & 1)]);
+            if (!isfinite(y) && p < limit[c >> 1]) o[d][c] += y;
+          }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+    if (x.begins) {
+      const int tokens = x.rows >> shift;
+      if (lane < tokens) space.places[(static_cast<size_t>(x.own) * a.T + x.row0 + lane) * a.kv_heads + x.kvh] = {2 * gw + 1, x.parts, lane << shift, x.joined};
+    }
+    const bool last = x.whole && x.own && !x.joined;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = g + 8 * h;
+      if (r >= x.rows) continue;
+      const size_t t = static_cast<size_t>(x.row0 + (r >> shift));
+      const int head = x.kvh * group + (r & (group - 1));
+      if (last) {
+        const float inv = l[h] == 0.f ? 0.f : 1.f / l[h];
+        bf16* out = static_cast<bf16*>(a.out) + t * a.ldo + head * kD + q2;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) *reinterpret_cast<uint32_t*>(out + d * 8) = pack_bf16x2(o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
+      } else {
+        float* out = x.whole ? space.rows + ((static_cast<size_t>(x.own) * a.T + t) * a.q_heads + head) * kLd : space.slots + (static_cast<size_t>(2 * gw + x.begins) * kRows + r) * kLd;
+#pragma unroll
+        for (int d = 0; d < 16; ++d) *reinterpret_cast<float2*>(out + d * 8 + q2) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
+        if ((lane & 3) == 0) *reinterpret_cast<float2*>(out + kD) = make_float2(ref[h], l[h]);
+      }
+    }
+  }
+  // the copies in flight land before the CTA ends, also where it gives up
+  for (int k = used; k < issued; ++k) warp_wait(full0 + 8 * (k % kDepth), (k / kDepth) & 1);
+  if (!ok) *reinterpret_cast<volatile int*>(error) = 1;
+}
+
+// sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts, in order, four dimensions a lane
+template <typename At>
+__device__ __forceinline__ uint2 join_row(int parts, At part, int lane) {
+  float m = -INFINITY, sum = 0.f;
+  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int p0 = 0; p0 < parts; p0 += kFew) {
+    float2 st[kFew];
+    float4 x[kFew];
+    float top = m;
+#pragma unroll
+    for (int k = 0; k < kFew; ++k) {
+      const bool there = p0 + k < parts;
+      st[k] = there ? *reinterpret_cast<const float2*>(part(p0 + k) + kD) : make_float2(-INFINITY, 0.f);
+      x[k] = there ? *reinterpret_cast<const float4*>(part(p0 + k) + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int k = 0; k < kFew; ++k) top = fmaxf(top, st[k].x);
+    const float base = top == -INFINITY ? 0.f : top, old = exp2f(m - base);
+    m = top;
+    sum *= old;
+    y = make_float4(y.x * old, y.y * old, y.z * old, y.w * old);
+#pragma unroll
+    for (int k = 0; k < kFew; ++k) {
+      const float w = exp2f(st[k].x - base);
+      sum += w == 0.f && st[k].y == st[k].y ? 0.f : st[k].y * w;
+      if (w != 0.f) y = make_float4(fmaf(x[k].x, w, y.x), fmaf(x[k].y, w, y.y), fmaf(x[k].z, w, y.z), fmaf(x[k].w, w, y.w));
+    }
+  }
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  return make_uint2(pack_bf16x2(y.x * inv, y.y * inv), pack_bf16x2(y.z * inv, y.w * inv));
+}
+
+// A CTA has a row and eight of its heads.
+__global__ void __launch_bounds__(kJoinThreads)
+shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, long long warps) {
+  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, head = blockIdx.y * (kJoinThreads / 32) + warp;
+  griddep_enter();
+  // whether some request has the row
+  bool mine = false;
+  for (int s = tid; s < a.S && !mine; s += kJoinThreads) {
+    const Lengths n = lengths_of(a, false);
+    const tree::Request r = n.request(s);
+    mine = t >= r.row0 && t < r.row0 + r.rows;
+  }
+  mine = __syncthreads_or(mine);
+  if (head >= a.q_heads) return;
+  uint2* out = reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + static_cast<size_t>(t) * a.ldo + head * kD) + lane;
+  if (!mine) {
+    if (a.zero_rest) *out = make_uint2(0, 0);
+    return;
+  }
+  const Space space = space_of(a, warps);
+  const int group = a.q_heads / a.kv_heads, kvh = head / group;
+  const Place own = space.places[(static_cast<size_t>(a.T) + t) * a.kv_heads + kvh];
+  if (!own.parts && !own.joined) return;      // written already
+  Place shared = {0, 0, 0, 0};
+  if (own.joined) shared = space.places[static_cast<size_t>(t) * a.kv_heads + kvh];
+  const int n_own = max(1, own.parts), n_all = n_own + (own.joined ? max(1, shared.parts) : 0);
+  // an item's beginning lies in its range's second slot, each other part in its range's first
+  auto part = [&](int p) -> const float* {
+    const bool first = p < n_own;
+    const Place& x = first ? own : shared;
+    const int k = first ? p : p - n_own;
+    if (!x.parts) return space.rows + ((static_cast<size_t>(first) * a.T + t) * a.q_heads + head) * kLd;
+    return space.slots + (static_cast<size_t>(k ? x.slot - 1 + 2 * k : x.slot) * kRows + x.row + head % group) * kLd;
+  };
+  *out = join_row(n_all, part, lane);
+}
+
+}  // namespace
+
+int64_t shared_attention_workspace(const b200_shared_attn_args& a) {
+  const int64_t T = a.T;
+  return 2 * T * a.kv_heads * static_cast<int64_t>(sizeof(Place)) + (static_cast<int64_t>(kPlaces) * sm_count() * kWarps * 2 * kRows + (a.G ? 2 * T * a.q_heads : 0)) * kLd * static_cast<int64_t>(sizeof(float));
+}
+
+int paged_attention_shared(const b200_shared_attn_args& a, int* error, cudaStream_t st) {
+  const int ctas = kPlaces * sm_count();
+  CUtensorMap tm_kv;
+  if (int rc = tmap_encode_bf16_2d(&tm_kv, a.kv_layer, static_cast<uint64_t>(a.num_pages) * 2 * a.kv_heads * 16, kD, kD, 16, 64, 1)) return rc;
+  static std::atomic<unsigned long long> attr_done{0};
+  if (!ensure_dynamic_smem(shared_attn_kernel, kSmem, &attr_done)) return -3;
+  launch_pdl(shared_attn_kernel, dim3(ctas), dim3(kThreads), kSmem, st, tm_kv, a, a.scale * 1.4426950408889634f, error);
+  if (cudaGetLastError() != cudaSuccess) return -2;
+  launch_pdl(shared_attn_join_kernel, dim3(a.T, (a.q_heads + 7) / 8), dim3(kJoinThreads), 0, st, a, static_cast<long long>(ctas) * kWarps);
+  return cudaGetLastError() == cudaSuccess ? 0 : -2;
+}
+
+}  // namespace b200

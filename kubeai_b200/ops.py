@@ -4,11 +4,13 @@ the library or a GPU these raise."""
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import NamedTuple
 
 import torch
 
-from ._lib import B200Error, ConstrainArgs, StepMapsArgs, TreeAcceptArgs, TreeAttnArgs, check, lib
+from ._lib import (B200Error, BeamReorderArgs, BeamSelectArgs, ConstrainArgs, NormRopeArgs, SharedAttnArgs, StepMapsArgs, TreeAcceptArgs, TreeAttnArgs, check,
+                   lib)
 
 
 def _p(t):
@@ -397,6 +399,212 @@ def tree_accept(ids, drafts, parents, starts, ctx_lens, block_tables, kv, max_pa
                        starts.data_ptr(), ctx_lens.data_ptr(), block_tables.data_ptr(), _ptr(kv), accepted.data_ptr(), path.data_ptr(), tokens.data_ptr(), ctx.data_ptr(), _ptr(status))
     check(lib().b200_op_tree_accept(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
     return TreeAccept(accepted, path.view(S, max_path), tokens.view(S, max_path), ctx)
+
+
+# ---- a decode step whose requests share their beginnings, beams above all (b200_op_norm_rope_kvwrite and the three behind it)
+def _cache(at, kv_layer, kv_heads):
+    if kv_layer.dtype is not torch.bfloat16 or kv_layer.get_device() != at or not kv_layer.is_contiguous() or kv_layer.shape[1:] != (2, kv_heads, 16, 128):
+        raise _refused(f"kv_layer: contiguous bf16 [pages, 2, {kv_heads}, 16, 128] on cuda:{at}, got {kv_layer.dtype} {tuple(kv_layer.shape)} on {kv_layer.device}")
+
+
+class Rotary(NamedTuple):
+    freqs: torch.Tensor
+    gain: float
+
+
+def rotary(dims=128, base=10000.0, scaling=None, device="cuda") -> Rotary:
+    """Radians a position (fp64) of each of dims / 2 pairs and the factor on what they turn, for norm_rope_kvwrite.  scaling: a configuration's `rope_scaling` as a dict, of type default, linear
+    (factor), llama3 (factor, low_freq_factor, high_freq_factor, original_max_position_embeddings) or yarn (factor, original_max_position_embeddings; beta_fast, beta_slow, attention_factor)."""
+    if dims < 0 or dims > 128 or dims % 2 or not base > 0:
+        raise _refused(f"an even number of up to 128 values of a head is turned, with a base above 0: got {dims}, {base}")
+    f = [base ** (-2 * i / dims) for i in range(dims // 2)]
+    scaling = scaling or {}
+    kind, gain = scaling.get("rope_type", scaling.get("type", "default")), 1.0
+    if kind not in ("default", "linear", "llama3", "yarn"):
+        raise _refused(f"rope scaling type {kind!r} is not supported (default, linear, llama3, yarn)")
+    try:
+        if kind != "default":
+            factor = float(scaling["factor"])
+            if not factor > 0:
+                raise _refused(f"a scaling factor above 0, got {factor}")
+        if kind == "linear":
+            f = [x / factor for x in f]
+        elif kind == "llama3":
+            low, high, length = (float(scaling[k]) for k in ("low_freq_factor", "high_freq_factor", "original_max_position_embeddings"))
+            # turns within the original length: below `low` the frequency is divided, above `high` it stays, between the two it goes over
+            part = [min(1.0, max(0.0, (length * x / (2 * math.pi) - low) / (high - low))) if high != low else float(length * x / (2 * math.pi) >= low) for x in f]
+            f = [x / factor * (1 - p) + x * p for x, p in zip(f, part)]
+        elif kind == "yarn":
+            length, fast, slow = float(scaling["original_max_position_embeddings"]), float(scaling.get("beta_fast", 32)), float(scaling.get("beta_slow", 1))
+            at = [dims * math.log(length / (2 * math.pi * turns)) / (2 * math.log(base)) for turns in (fast, slow)]
+            lo, hi = max(0, math.floor(at[0])), min(dims - 1, math.ceil(at[1]))
+            part = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(dims // 2)]
+            f = [x / factor * p + x * (1 - p) for x, p in zip(f, part)]
+            gain = scaling.get("attention_factor")
+            gain = float(gain) if gain is not None else 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+    except KeyError as e:
+        raise _refused(f"rope scaling {kind!r} lacks {e.args[0]!r}") from None
+    except ZeroDivisionError:
+        raise _refused(f"rope scaling {kind!r} of {scaling} with base {base} divides by zero") from None
+    return Rotary(torch.tensor(f, dtype=torch.float64, device=device), gain)
+
+
+def norm_rope_kvwrite(qkv, positions, slots, kv_layer, q_heads, kv_heads, freqs, gain=1.0, q_norm=None, k_norm=None, eps=1e-6, interleaved=False, out=None):
+    """Norms of queries and keys for each head, rotary positions in the same pass, and keys and values into the paged cache (b200_op_norm_rope_kvwrite).
+    qkv: bf16 [T, at least (q_heads + 2 kv_heads) * 128], rows may be a wider buffer's leading columns; positions, slots: int32 [T], a slot of -1 is written nowhere;
+    freqs: fp64 [pairs] radians a position, up to 64 (`rotary` makes them), the rest of a head is not turned; pairs are (d, d + pairs), or with interleaved (2 d, 2 d + 1).
+    q_norm, k_norm: bf16 or fp32 [128] or [heads, 128], None: no norm.  Returns the queries [T, q_heads * 128]: new, `out`, or in their place with out=qkv."""
+    at = _gpu(qkv)
+    width = (q_heads + 2 * kv_heads) * 128
+    ldx = _rows(at, qkv, _BF16, "qkv", columns=width)
+    T = qkv.shape[0]
+    _cache(at, kv_layer, kv_heads)
+    _ints(at, positions, slots), _sized(positions, T, "positions"), _sized(slots, T, "slots")
+    if freqs.dtype is not torch.float64 or freqs.get_device() != at or not freqs.is_contiguous() or freqs.dim() != 1 or freqs.numel() > 64:
+        raise _refused(f"freqs: contiguous fp64 [0 to 64] on cuda:{at}, got {freqs.dtype} {tuple(freqs.shape)} on {freqs.device}")
+    lds, kinds = [0, 0], set()
+    for k, (w, heads, what) in enumerate(((q_norm, q_heads, "q_norm"), (k_norm, kv_heads, "k_norm"))):
+        if w is None:
+            continue
+        if w.dtype not in _LOGITS or w.get_device() != at or not w.is_contiguous() or tuple(w.shape) not in ((128,), (heads, 128)):
+            raise _refused(f"{what}: contiguous bf16 or fp32 [128] or [{heads}, 128] on cuda:{at}, got {w.dtype} {tuple(w.shape)} on {w.device}")
+        lds[k] = 128 if w.dim() == 2 else 0
+        kinds.add(w.dtype)
+    if len(kinds) > 1:
+        raise _refused("q_norm and k_norm are of one type")
+    if out is None:
+        out = qkv.new_empty((T, q_heads * 128))
+        ldo = q_heads * 128
+    else:
+        ldo = _rows(at, out, _BF16, "out", columns=q_heads * 128)
+        if out.shape[0] < T:
+            raise _refused(f"out has {out.shape[0]} rows, not {T}")
+    if (T | ldx | ldo) >> 31:
+        raise _refused(_WIDE)
+    a = NormRopeArgs(T, q_heads, kv_heads, ldx, ldo, 2 * freqs.numel(), bool(interleaved), lds[0], lds[1], torch.float32 in kinds, eps, gain, kv_layer.shape[0],
+                     qkv.data_ptr(), out.data_ptr(), kv_layer.data_ptr(), positions.data_ptr(), slots.data_ptr(), freqs.data_ptr(), _ptr(q_norm), _ptr(k_norm))
+    check(lib().b200_op_norm_rope_kvwrite(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
+    return out
+
+
+def paged_attn_shared(qkv, kv_layer, block_tables, starts, ctx_lens, group_starts, shared_lens, q_heads, kv_heads, max_rows, max_ctx=0, scale=128 ** -0.5, out=None, status=None):
+    """Attention of a step's rows over the paged cache, where groups of requests have the same first pages (b200_op_paged_attn_shared).  Request s has rows starts[s] .. of qkv [T, at least
+    q_heads * 128], q first, ctx_lens[s] tokens in the cache in front of them, and their K and V in it too; row i sees the tokens in front and rows 0 .. i.
+    Group g: requests group_starts[g] .. group_starts[g + 1] - 1, whose first shared_lens[g] tokens (whole pages of them) lie on the same pages and pass once for all rows of the group; requests of no
+    group are attended alone.  max_rows: the most rows of a request; max_ctx: the most tokens in front of them, if known.  status [S]: step_maps' own, whose requests with 1 or 2 are left out.
+    Rows that no request owns, and those of one that is left out, are left as they were in `out` and are zeros in a new one."""
+    at = _gpu(qkv)
+    ldq = _rows(at, qkv, _BF16, "qkv", columns=q_heads * 128)
+    _cache(at, kv_layer, kv_heads)
+    _ints(at, starts, ctx_lens, group_starts, shared_lens, status)
+    S, T, G = ctx_lens.numel(), qkv.shape[0], shared_lens.numel()
+    _sized(starts, S + 1, "starts"), _sized(status, S, "status"), _sized(group_starts, G + 1, "group_starts")
+    ld = _rows(at, block_tables, _I32, "block tables", rows=S)
+    if (S | T | ldq | ld | max_rows | max_ctx) >> 31:
+        raise _refused(_WIDE)
+    fresh = out is None
+    if fresh:
+        out = qkv.new_empty((T, q_heads * 128))
+        ldo = q_heads * 128
+    else:
+        ldo = _rows(at, out, _BF16, "out", columns=q_heads * 128)
+        if out.shape[0] < T:
+            raise _refused(f"out has {out.shape[0]} rows, not {T}")
+        if ldo >> 31:
+            raise _refused(_WIDE)
+    a = SharedAttnArgs(S, T, G, q_heads, kv_heads, ldq, ldo, block_tables.shape[1], ld, max_rows, max_ctx, fresh, scale, kv_layer.shape[0], qkv.data_ptr(), out.data_ptr(),
+                       kv_layer.data_ptr(), block_tables.data_ptr(), starts.data_ptr(), ctx_lens.data_ptr(), group_starts.data_ptr(), shared_lens.data_ptr(), _ptr(status))
+    a.workspace_bytes = check(lib().b200_op_paged_attn_shared_workspace(C.byref(a)))
+    workspace = starts.new_empty((a.workspace_bytes + 3) // 4)
+    a.workspace = workspace.data_ptr()
+    check(lib().b200_op_paged_attn_shared(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
+    return out
+
+
+class BeamSelect(NamedTuple):
+    parents: torch.Tensor
+    tokens: torch.Tensor
+    scores: torch.Tensor
+    found_parents: torch.Tensor
+    found_tokens: torch.Tensor
+    found_scores: torch.Tensor
+
+
+def beam_select(logits, scores, k=None, ends=None) -> BeamSelect:
+    """The k best candidates over a request's beams and the vocabulary, best first, and the beams that go on: the first of them whose token is none of `ends` (b200_op_beam_select).
+    logits: [S * beams, V] bf16 or fp32, rows may be a wider buffer's leading columns; scores: fp32 [S, beams], the beams' log-probabilities so far, -inf for a beam that is none;
+    k: None stands for twice the beams; ends: int32 [any].  found_* [S, k]; parents, tokens, scores [S, beams]; behind the last -1, -1, -inf."""
+    at = _gpu(logits)
+    ld = _rows(at, logits, _LOGITS, "logits")
+    if scores.dtype is not torch.float32 or scores.get_device() != at or not scores.is_contiguous() or scores.dim() != 2:
+        raise _refused(f"scores: contiguous fp32 [requests, beams] on cuda:{at}, got {scores.dtype} {tuple(scores.shape)} on {scores.device}")
+    S, B = scores.shape
+    R, V = logits.shape
+    if R != S * B:
+        raise _refused(f"logits: {R} rows, not {S} times {B}")
+    _ints(at, ends)
+    k = 2 * B if k is None else k
+    if (S | B | V | ld | k) >> 31:
+        raise _refused(_WIDE)
+    a = BeamSelectArgs(S, B, V, ld, logits.dtype is torch.float32, k, 0 if ends is None else ends.numel(), logits.data_ptr(), scores.data_ptr(), _ptr(ends))
+    a.workspace_bytes = check(lib().b200_op_beam_select_workspace(C.byref(a)))
+    workspace, parents, tokens, found_parents, found_tokens = torch.empty((a.workspace_bytes + 3) // 4 + 2 * S * (B + k), dtype=torch.int32, device=logits.device).unsafe_split_with_sizes(
+        [(a.workspace_bytes + 3) // 4, S * B, S * B, S * k, S * k])
+    new_scores, found_scores = scores.new_empty(S * (B + k)).unsafe_split_with_sizes([S * B, S * k])
+    a.workspace, a.parents, a.tokens, a.new_scores = workspace.data_ptr(), parents.data_ptr(), tokens.data_ptr(), new_scores.data_ptr()
+    a.found_parents, a.found_tokens, a.found_scores = found_parents.data_ptr(), found_tokens.data_ptr(), found_scores.data_ptr()
+    check(lib().b200_op_beam_select(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
+    return BeamSelect(parents.view(S, B), tokens.view(S, B), new_scores.view(S, B), found_parents.view(S, k), found_tokens.view(S, k), found_scores.view(S, k))
+
+
+class BeamReorder(NamedTuple):
+    block_tables: torch.Tensor
+    shared: torch.Tensor
+    released: torch.Tensor
+    texts: torch.Tensor | None
+    text_lens: torch.Tensor | None
+
+
+def beam_reorder(parents, tokens, ctx_lens, block_tables, kv, texts=None, text_lens=None, out=None) -> BeamReorder:
+    """Block tables, texts and partly filled pages of the beams that go on (b200_op_beam_reorder).  parents, tokens: int32 [S, beams], as beam_select has them; ctx_lens [S * beams]: tokens in the
+    cache, this step's among them, the same for a request's beams; block_tables [S * beams, pages], in which a page that is not full has one owner; kv: bf16
+    [layers, pages, 2, kv_heads, 16, 128], None: nowhere; texts [S * beams, room] with text_lens tokens each, to which `tokens` are added.
+    Returns the new tables (or `out`), the tokens on pages that all beams of a request have, [S], the whole pages that nobody has any more, as a table with -1 elsewhere, and the new texts and lengths."""
+    at = _gpu(parents)
+    if parents.dim() != 2:
+        raise _refused(f"parents: int32 [requests, beams], got {tuple(parents.shape)}")
+    S, B = parents.shape
+    _ints(at, parents, tokens, ctx_lens, text_lens)
+    _sized(tokens, S * B, "tokens"), _sized(ctx_lens, S * B, "ctx_lens"), _sized(text_lens, S * B, "text_lens")
+    ld = _rows(at, block_tables, _I32, "block tables", rows=S * B)
+    layers, pages, heads, apart = 0, 0, 1, 0
+    if kv is not None:
+        shape = kv.shape
+        if not (kv.dtype is torch.bfloat16 and kv.get_device() == at and len(shape) == 6 and shape[2] == 2 and shape[4:] == (16, 128) and (kv.is_contiguous() or not len(kv) or kv[0].is_contiguous())):
+            raise _refused(f"kv: bf16 [layers, pages, 2, kv_heads, 16, 128] on cuda:{at}, got {kv.dtype} {tuple(shape)} on {kv.device}")
+        layers, pages, heads = shape[0], shape[1], shape[3]
+        apart = kv.stride(0) if layers > 1 else 0
+    width = block_tables.shape[1]
+    ldo = width
+    if out is not None:
+        ldo = _rows(at, out, _I32, "out", rows=S * B, columns=width)
+    room, ldt = 0, 0
+    if texts is not None:
+        if text_lens is None:
+            raise _refused("texts without their lengths")
+        ldt = _rows(at, texts, _I32, "texts", rows=S * B)
+        room = texts.shape[1]
+    if (S | B | layers | heads | ld | ldo | ldt) >> 31:
+        raise _refused(_WIDE)
+    sizes = [S, S * B * width, 0 if out is not None else S * B * width, 0 if texts is None else S * B, S * B * room]
+    shared, released, fresh, lens_out, texts_out = _pieces(parents, sizes)
+    if out is None:
+        out = fresh.view(S * B, width)
+    a = BeamReorderArgs(S, B, width, ld, ldo, layers, heads, room, ldt, room, pages, apart, parents.data_ptr(), tokens.data_ptr(), ctx_lens.data_ptr(), block_tables.data_ptr(), out.data_ptr(),
+                        released.data_ptr(), shared.data_ptr(), _ptr(kv), _ptr(texts), texts_out.data_ptr(), _ptr(text_lens), lens_out.data_ptr())
+    check(lib().b200_op_beam_reorder(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
+    there = texts is not None
+    return BeamReorder(out, shared, released.view(S * B, width), texts_out.view(S * B, room) if there else None, lens_out if there else None)
 
 
 def init_uniform(n, seed, scale, offset, device="cuda"):
