@@ -28,7 +28,7 @@ constexpr int kThreads = 512, kWarps = kThreads / 32, kVectors = 8, kList = 512;
 constexpr int kPart = kThreads * kVectors;                                            // pieces of a part at most
 constexpr int kMostParts = 32;                                                         // a lane each in the second kernel
 static_assert(kMostParts * 4 * (kPart - 1) > beam::kMaxVocab, "");
-constexpr int kLeastPart = 512;                                                        // pieces of a part at least, where the row has them
+constexpr int kLeastPart = 1024;                                                       // pieces of a part at least, where the row has them
 constexpr float kLog2eHi = 1.4426950216293335f, kLog2eLo = 1.9259629911e-8f;           // log2(e) as a sum
 
 struct PartHead {
@@ -43,7 +43,7 @@ struct Geometry {
 };
 Geometry geometry(const b200_beam_select_args& a) {
   const long long rows = static_cast<long long>(a.S) * a.beams;
-  const int per = a.logits_f32 ? 4 : 8, pieces = (a.V + per - 1) / per + 1;      // a row may begin inside a piece
+  const int per = a.logits_f32 ? 4 : 8, pieces = (a.V + per - 1) / per;
   // as many parts as fill the SMs twice, of no less than kLeastPart pieces, and as many as hold the row
   const long long wanted = std::min<long long>(2 * sm_count() / std::max<long long>(1, rows), pieces / kLeastPart);
   Geometry g;
@@ -71,23 +71,33 @@ __device__ __forceinline__ float value_in(const uint32_t* w, int i) {
   return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
 }
 
-// A row's piece: 16 bytes, of which some belong to somebody else at the row's ends: those, and NaN, are -inf.
+// A row's piece: the values of 16 bytes, by the widest loads that the row's beginning allows, so that which values meet in a sum goes by their tokens alone and equal rows have equal
+// sums wherever they lie.  What is behind the row's end is -inf.
 template <bool kF32>
-__device__ __forceinline__ void load_piece(uintptr_t base, int ahead, int V, int piece, bool there, uint32_t* w) {
-  constexpr int kPer = kF32 ? 4 : 8;
-  const int first = piece * kPer - ahead;
+__device__ __forceinline__ void load_piece(const uint8_t* row, int V, int piece, bool there, uint32_t* w) {
+  constexpr int kPer = kF32 ? 4 : 8, kSize = kF32 ? 4 : 2;
+  const uint8_t* at = row + static_cast<size_t>(piece) * 16;
+  const int align = static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15);
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = kF32 ? 0xff800000u : 0xff80ff80u;
   if (!there) return;
-  if (first >= 0 && first + kPer <= V) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4*>(base + static_cast<long long>(first) * (kF32 ? 4 : 2)));
-    w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+  if ((piece + 1) * kPer <= V && align % 4 == 0) {
+    if (align == 0) {
+      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(at));
+      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+    } else if (align == 8) {
+      const uint2 u = *reinterpret_cast<const uint2*>(at), v = *reinterpret_cast<const uint2*>(at + 8);
+      w[0] = u.x; w[1] = u.y; w[2] = v.x; w[3] = v.y;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(at)[i];
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      if (first + i < 0 || first + i >= V) continue;
-      if (kF32) w[i & 3] = reinterpret_cast<const uint32_t*>(base)[first + i];
-      else w[i / 2] = (w[i / 2] & (i & 1 ? 0x0000ffffu : 0xffff0000u)) | static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(base)[first + i]) << (i & 1 ? 16 : 0);
+      if (piece * kPer + i >= V) continue;
+      if (kF32) w[i & 3] = reinterpret_cast<const uint32_t*>(at)[i];
+      else w[i / 2] = __byte_perm(w[i / 2], *reinterpret_cast<const uint16_t*>(at + i * kSize), i & 1 ? 0x5410 : 0x3254);
     }
   }
 }
@@ -113,20 +123,19 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, int parts, si
   __shared__ float maxima[kWarps];
   __shared__ double sums[kWarps];
   __shared__ unsigned long long list[kList];
+  __shared__ double terms[kList];
   __shared__ int s_n, s_count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const long long row = blockIdx.x / parts;
   const int part = blockIdx.x % parts;
   griddep_enter();
-  const size_t size = kF32 ? 4 : 2;
-  const uintptr_t base = reinterpret_cast<uintptr_t>(a.logits) + static_cast<size_t>(row) * a.ld * size;
-  const int ahead = static_cast<int>(base % 16 / size);      // values of the row's first piece that belong to somebody else
-  const int pieces = (a.V + ahead + kPer - 1) / kPer;
+  const uint8_t* base = static_cast<const uint8_t*>(a.logits) + static_cast<size_t>(row) * a.ld * (kF32 ? 4 : 2);
+  const int pieces = (a.V + kPer - 1) / kPer;
   const int v0 = static_cast<int>(static_cast<long long>(pieces) * part / parts), v1 = static_cast<int>(static_cast<long long>(pieces) * (part + 1) / parts);
 
   uint32_t x[kVectors][4];
 #pragma unroll
-  for (int v = 0; v < kVectors; ++v) load_piece<kF32>(base, ahead, a.V, v0 + v * kThreads + tid, v0 + v * kThreads + tid < v1, x[v]);
+  for (int v = 0; v < kVectors; ++v) load_piece<kF32>(base, a.V, v0 + v * kThreads + tid, v0 + v * kThreads + tid < v1, x[v]);
   float mine = -INFINITY;
 #pragma unroll
   for (int v = 0; v < kVectors; ++v) {
@@ -163,7 +172,7 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, int parts, si
       const float f = value_in<kF32>(x[v], i), d = f - top;
       if (f >= least) {
         const int at = atomicAdd(&s_n, 1);
-        if (at < kList) list[at] = key_of(f, (v0 + v * kThreads + tid) * kPer + i - ahead);
+        if (at < kList) list[at] = key_of(f, (v0 + v * kThreads + tid) * kPer + i);
       } else rest += exp2_ftz(fmaf(d, kLog2eHi, d * kLog2eLo));
     }
   __syncthreads();
@@ -174,10 +183,10 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, int parts, si
 #pragma unroll 1
       for (int piece = v0 + tid; piece < v1; piece += kThreads) {
         uint32_t w[4];
-        load_piece<kF32>(base, ahead, a.V, piece, true, w);
+        load_piece<kF32>(base, a.V, piece, true, w);
         without_nan<kF32>(w);
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) what(value_in<kF32>(w, i), piece * kPer + i - ahead);
+        for (int i = 0; i < kPer; ++i) what(value_in<kF32>(w, i), piece * kPer + i);
       }
     };
     auto count_all = [&](auto is) {
@@ -215,6 +224,7 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, int parts, si
     n = min(s_n, kList);
   }
   // ---- places in the list, and the sum
+  static_assert(kList <= kThreads, "");
   double sum = rest;
   uint2* out = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.workspace) + entries) + (row * parts + part) * a.k;
   for (int i = tid; i < n; i += kThreads) {
@@ -223,8 +233,10 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, int parts, si
     for (int j = 0; j < n; ++j) place += list[j] > key;
     if (place < a.k) out[place] = make_uint2(static_cast<uint32_t>(key), static_cast<uint32_t>(key >> 32));
     const float f = key_value(key);
-    sum += f == top ? 1.0 : exp(static_cast<double>(f) - top);
+    terms[place] = f == top ? 1.0 : exp(static_cast<double>(f) - top);
   }
+  __syncthreads();
+  if (tid < n) sum += terms[tid];      // in the values' order, not in the list's
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) sums[warp] = sum;
@@ -236,7 +248,7 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, int parts, si
   }
 }
 
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kStaged = kMostParts * beam::kMaxFound;
 
 __global__ void __launch_bounds__(kJoinThreads)
 beam_join_kernel(const __grid_constant__ b200_beam_select_args a, int parts, size_t entries) {
@@ -245,16 +257,15 @@ beam_join_kernel(const __grid_constant__ b200_beam_select_args a, int parts, siz
   __shared__ float tops[beam::kMaxBeams];
   __shared__ int count[beam::kMaxBeams], found_token[beam::kMaxFound], found_parent[beam::kMaxFound], ends_text[beam::kMaxFound];
   __shared__ float found_score[beam::kMaxFound];
+  __shared__ unsigned long long staged[kStaged];
+  __shared__ uint8_t counts[beam::kMaxBeams * kMostParts];
   const int s = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, B = a.beams, k = a.k;
   griddep_enter();
   const PartHead* heads = static_cast<const PartHead*>(a.workspace) + static_cast<size_t>(s) * B * parts;
   const uint2* lists = reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.workspace) + entries) + static_cast<size_t>(s) * B * parts * k;
-  auto entry = [&](int list, int i) -> unsigned long long {
-    const uint2 e = lists[static_cast<size_t>(list) * k + i];
-    return static_cast<unsigned long long>(e.y) << 32 | e.x;
-  };
   for (int b = warp; b < B; b += kJoinThreads / 32) {      // a lane has a part
     const PartHead h = lane < parts ? heads[b * parts + lane] : PartHead{-INFINITY, 0, 0.0};
+    if (lane < parts) counts[b * parts + lane] = h.n;
     const float score = a.scores[static_cast<size_t>(s) * B + b];
     float top = h.top;
     double sum = 0.0;
@@ -277,25 +288,34 @@ beam_join_kernel(const __grid_constant__ b200_beam_select_args a, int parts, siz
     ends_text[i] = 0;
   }
   __syncthreads();
-  // ---- a row's candidates in order
-  for (int e = tid; e < B * parts * k; e += kJoinThreads) {
-    const int list = e / k, i = e % k, b = list / parts;
-    if (!count[b] || i >= heads[list].n) continue;
-    const unsigned long long key = entry(list, i);
-    int place = i;
-    for (int p = b * parts; p < (b + 1) * parts && place < k; ++p) {
-      if (p == list) continue;
-      int lo = 0, hi = heads[p].n;      // how many of its are larger
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (entry(p, mid) > key) lo = mid + 1;
-        else hi = mid;
-      }
-      place += lo;
+  // ---- a row's candidates in order, of as many beams at a time as there is room for
+  const int at_once = max(1, kStaged / (parts * k));
+  for (int b0 = 0; b0 < B; b0 += at_once) {
+    const int some = min(at_once, B - b0) * parts;
+    for (int e = tid; e < some * k; e += kJoinThreads) {
+      const uint2 x = lists[static_cast<size_t>(b0) * parts * k + e];
+      staged[e] = e % k < counts[b0 * parts + e / k] ? static_cast<unsigned long long>(x.y) << 32 | x.x : 0ull;      // (0 is below every value)
     }
-    if (place < k) best[b][place] = key;
+    __syncthreads();
+    for (int e = tid; e < some * k; e += kJoinThreads) {
+      const unsigned long long key = staged[e];
+      const int list = e / k, b = list / parts;
+      if (!key || !count[b0 + b]) continue;
+      int place = e % k;
+      for (int p = b * parts; p < (b + 1) * parts && place < k; ++p) {
+        if (p == list) continue;
+        int lo = 0, hi = k;      // how many of its are larger
+        while (lo < hi) {
+          const int mid = (lo + hi) / 2;
+          if (staged[p * k + mid] > key) lo = mid + 1;
+          else hi = mid;
+        }
+        place += lo;
+      }
+      if (place < k) best[b0 + b][place] = key;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   // ---- and a request's
   auto c_of = [&](int b, int i) {
     const float x = key_value(best[b][i]);

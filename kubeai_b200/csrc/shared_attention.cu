@@ -16,76 +16,23 @@
 
 #include <algorithm>
 
-#include "beam_step.h"
 #include "gemm.h"
 #include "kernels.h"
 #include "launch.h"
 #include "ptx.cuh"
+#include "shared_attention.cuh"
 
 namespace b200 {
 namespace {
 
 typedef __nv_bfloat16 bf16;
-using beam::Lengths;
-using beam::Part;
-constexpr int kD = 128, kRows = 16, kPageBytes = 2 * 16 * kD * 2;      // bytes of a page's keys and values of a head
+using namespace shared_attn;
+constexpr int kPageBytes = 2 * 16 * kD * 2;      // bytes of a page's keys and values of a head
 constexpr int kThreads = 128, kWarps = kThreads / 32, kPlaces = 3, kDepth = 2, kItems = 4;      // kPlaces: CTAs of an SM; kDepth: pages of a warp on their way; kItems: items that those may lie in, and one
-constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
 constexpr int kJoinThreads = 256, kFew = 4;
-constexpr int kWaitLimit = 1 << 22;
 constexpr int kSmem = 1024 + kWarps * kDepth * kPageBytes;
 static_assert(kPlaces * (kSmem + 3072) <= 228 * 1024, "");
 static_assert(kItems > kDepth, "");
-
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, kWaitLimit)); }
-// two bf16 without infinities and NaN
-__device__ __forceinline__ uint32_t without_odd(uint32_t u) { return ((u & 0x7f80u) == 0x7f80u ? 0u : u & 0xffffu) | ((u & 0x7f800000u) == 0x7f800000u ? 0u : u & 0xffff0000u); }
-
-// Where the rows of a token and key head are: their own keys' part, and what their group shares.
-struct Place {
-  int slot, parts;      // parts 0: in the rows of all (or in the output), else in the slots of `parts` ranges, slot the first
-  int row;              // the token's first row there
-  int joined;           // own rows: the group's are to be added
-};
-struct Space {
-  Place* places;        // [2][T][kv_heads]: the groups', the requests' own
-  float* slots;         // [warps][2][16][kLd]: a range's first item, which another range began, and its last
-  float* rows;          // [2][T][q_heads][kLd]
-};
-__host__ __device__ inline Space space_of(const b200_shared_attn_args& a, long long warps) {
-  Space s;
-  s.places = static_cast<Place*>(a.workspace);
-  s.slots = reinterpret_cast<float*>(s.places + 2ll * a.T * a.kv_heads);
-  s.rows = s.slots + warps * 2 * kRows * kLd;
-  return s;
-}
-
-__device__ __forceinline__ Lengths lengths_of(const b200_shared_attn_args& a, bool ordered) {
-  return {a.starts, a.ctx, a.group_starts, a.shared, a.status, a.S, a.T, ordered ? a.G : 0, a.max_blocks, a.max_rows};
-}
-
-// ---- items
-struct Item {
-  int u, kvh, block;
-  Part p;
-  int first, nb, k1, pages;      // the block's tokens, the keys they may see
-};
-__device__ __forceinline__ int end_of(const Part& p, int bt, int block) { return p.all ? p.k1 : p.ctx + min(p.rows, (block + 1) * bt); }
-__device__ __forceinline__ int pages_of(const Part& p, int bt, int block) { return (end_of(p, bt, block) - p.k0 + 15) / 16; }
-__device__ __forceinline__ int blocks_of(const Part& p, int bt) { return (p.rows + bt - 1) / bt; }
-__device__ __forceinline__ int head_cost(const Part& p, int bt) {
-  const int blocks = blocks_of(p, bt);
-  if (p.all || blocks <= 1) return blocks ? blocks * (pages_of(p, bt, 0) + tree::kItem) : 0;
-  int n = 0;
-  for (int b = 0; b < blocks; ++b) n += pages_of(p, bt, b) + tree::kItem;
-  return n;
-}
-__device__ __forceinline__ void fill(int bt, Item* it) {
-  it->first = it->block * bt;
-  it->nb = min(bt, it->p.rows - it->first);
-  it->k1 = end_of(it->p, bt, it->block);
-  it->pages = pages_of(it->p, bt, it->block);
-}
 
 // An item's pages of a range, as the loads leave them for the products
 struct Piece {
@@ -98,7 +45,8 @@ struct Piece {
 };
 
 __global__ void __launch_bounds__(kThreads, kPlaces)
-shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ b200_shared_attn_args a, float scale_log2, int* error) {
+shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ b200_shared_attn_args a, const Sizes sizes, float scale_log2, int* error) {
+  typedef Items<false> I;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[kWarps * kDepth];
   __shared__ int sums[kWarps], s_range[kWarps + 1], s_where[kWarps + 1][4];
@@ -106,83 +54,40 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (sbase - smem_u32(smem_raw));
   const int warp = warp_number(), lane = threadIdx.x & 31, tid = threadIdx.x;
-  const int group = a.q_heads / a.kv_heads, bt = kRows / group, shift = __ffs(group) - 1;
+  const int group = a.q_heads / a.kv_heads, bt = kNarrow / group, shift = __ffs(group) - 1;
   const uint32_t ring = sbase + warp * kDepth * kPageBytes, full0 = smem_u32(bars + warp * kDepth);
   if (lane == 0) {
     for (int s = 0; s < kDepth; ++s) mbar_init(full0 + 8 * s, 1);
     fence_mbar_init();
     tma_prefetch_desc(&tm_kv);
   }
-  griddep_enter();
-  // ---- the warps' ranges: every thread sums some parts of the step, one behind the other, and the sums of the threads in front of it
+  // Behind the wide kernel, which this one needs nothing of, it begins as soon as there is room: that kernel let it in behind its own wait for what both read.  The wait that makes this
+  // one's end the end of both stands at its end.
+  const bool behind = sizes.ctas > 0;
+  if (!behind) griddep_wait();
+  griddep_launch();
   bool ordered = a.G > 0;
   if (ordered) ordered = __syncthreads_and(beam::ascends(a.group_starts, a.G, a.S, tid, kThreads) && beam::ascends(a.starts, a.S, a.T, tid, kThreads));
   const Lengths n = lengths_of(a, ordered);
-  const int U = n.G + a.S, per = (U + kThreads - 1) / kThreads, u_begin = min(U, tid * per), u_end = min(U, u_begin + per);
-  int before = 0, N = 0;
-  for (int u = u_begin; u < u_end; ++u) before += head_cost(beam::part_of(n, u), bt) * a.kv_heads;
-  const int own = before;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += y;
-  }
-  if (lane == 31) sums[warp] = before;
+  const int gw = blockIdx.x * kWarps + warp;
+  const tree::Ranges ranges = find_ranges<false, kThreads>(n, a.kv_heads, group, blockIdx.x * kWarps, kWarps, sizes.warps, sums, s_range, s_where);
   __syncthreads();
-  before -= own;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    const int x = sums[w];
-    if (w < warp) before += x;
-    N += x;
+  const int left = gw < ranges.n ? s_range[warp + 1] - s_range[warp] : 0;
+  if (left <= 0) {
+    if (behind) griddep_wait();
+    return;
   }
-  const int gw0 = blockIdx.x * kWarps, gw = gw0 + warp;
-  const tree::Ranges ranges = tree::ranges_of(N, gridDim.x * kWarps);
-  if (tid <= kWarps && gw0 + tid >= ranges.n) s_range[tid] = N;      // which lies in no item
-  if (N > 0 && gw0 < ranges.n) {
-    const int b_end = ranges.at(min(gw0 + kWarps, ranges.n - 1));
-    if (own && ranges.at(gw0) < before + own && b_end >= before)
-      for (int u = u_begin; u < u_end; ++u) {
-        const Part p = beam::part_of(n, u);
-        const int mine = head_cost(p, bt) * a.kv_heads;
-        for (int e = 0; e <= kWarps && gw0 + e < ranges.n; ++e) {
-          const int b = ranges.at(gw0 + e);
-          if (mine == 0 || b < before || b >= before + mine) continue;
-          int g0 = before, block = 0, pages = pages_of(p, bt, 0);
-          while (b >= g0 + (pages + tree::kItem) * a.kv_heads) g0 += (pages + tree::kItem) * a.kv_heads, pages = pages_of(p, bt, ++block);
-          const int kvh = (b - g0) / (pages + tree::kItem);
-          g0 += kvh * (pages + tree::kItem);
-          s_range[e] = tree::snapped(b, g0, pages, ranges.snap);
-          s_where[e][0] = u; s_where[e][1] = kvh; s_where[e][2] = block; s_where[e][3] = g0;
-        }
-        before += mine;
-      }
-  }
-  __syncthreads();
-  const int left = N > 0 && gw < ranges.n ? s_range[warp + 1] - s_range[warp] : 0;
-  if (left <= 0) return;
-  const Space space = space_of(a, static_cast<long long>(gridDim.x) * kWarps);
+  const Space space = space_of(a, sizes);
 
   // ---- loads: item, its first page here, the range's cost to go
-  Item it;
+  Item<false> it;
   it.u = s_where[warp][0]; it.kvh = s_where[warp][1]; it.block = s_where[warp][2];
-  it.p = beam::part_of(n, it.u);
-  fill(bt, &it);
+  it.p = I::part(n, it.u, group);
+  it.fill(bt);
   int t0 = max(0, s_range[warp] - s_where[warp][3] - tree::kItem), rest = left;
-  auto next_item = [&] {
-    if (++it.kvh >= a.kv_heads) {
-      it.kvh = 0;
-      if (++it.block >= blocks_of(it.p, bt)) {
-        it.block = 0;
-        do it.p = beam::part_of(n, ++it.u);
-        while (it.p.rows == 0);      // (a range's pages are some part's: the walk ends in front of U)
-      }
-    }
-    fill(bt, &it);
-  };
-  if (t0 == it.pages) {              // the range begins where the item in front of it ends
+  if (t0 == it.units) {              // the range begins where the item in front of it ends
     t0 = 0;
-    next_item();
+    it.next(n, a.kv_heads, group, bt);
   }
   bool more = true, ok = true;
   int take = 0, at = 0, items = 0, issued = 0, mine = 0, next = 0;      // the item's pages here, the page that is next; items so far; pages so far
@@ -193,12 +98,12 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
     return ((page >= 0 && page < a.num_pages ? page : static_cast<int>(a.num_pages)) * 2 * a.kv_heads + it.kvh) * 16;
   };
   auto begin = [&] {
-    take = tree::take_of(t0, it.pages, &rest);
+    take = tree::take_of(t0, it.units, &rest);
     at = 0;
     mine = look_up(t0 + lane);
     next = look_up(t0 + 32 + lane);
     if (lane == 0) {
-      const bool whole = t0 == 0 && take == it.pages;
+      const bool whole = t0 == 0 && take == it.units;
       Piece x;
       x.row0 = it.p.row0 + it.first;
       x.rows = it.nb * group;
@@ -212,7 +117,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
       x.begins = t0 == 0;
       x.own = !it.p.all;
       x.joined = it.p.k0 > 0;
-      x.parts = whole ? 0 : t0 == 0 ? ranges.parts(gw, s_range[warp + 1] - take, it.pages) : 0;
+      x.parts = whole ? 0 : t0 == 0 ? ranges.parts(gw, s_range[warp + 1] - take, it.units) : 0;
       pieces[warp][items % kItems] = x;
     }
     ++items;
@@ -224,7 +129,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
     if (at == take) {
       if (rest <= 0) { more = false; return; }
       t0 = 0;
-      next_item();
+      it.next(n, a.kv_heads, group, bt);
       begin();
     } else if (at && at % 32 == 0) {
       mine = next;
@@ -379,7 +284,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
     }
     if (x.begins) {
       const int tokens = x.rows >> shift;
-      if (lane < tokens) space.places[(static_cast<size_t>(x.own) * a.T + x.row0 + lane) * a.kv_heads + x.kvh] = {2 * gw + 1, x.parts, lane << shift, x.joined};
+      if (lane < tokens) space.places[(static_cast<size_t>(x.own) * a.T + x.row0 + lane) * a.kv_heads + x.kvh] = {2 * gw + 1, x.parts, lane << shift, x.joined ? kJoined : 0};
     }
     const bool last = x.whole && x.own && !x.joined;
 #pragma unroll
@@ -394,7 +299,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
 #pragma unroll
         for (int d = 0; d < 16; ++d) *reinterpret_cast<uint32_t*>(out + d * 8) = pack_bf16x2(o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
       } else {
-        float* out = x.whole ? space.rows + ((static_cast<size_t>(x.own) * a.T + t) * a.q_heads + head) * kLd : space.slots + (static_cast<size_t>(2 * gw + x.begins) * kRows + r) * kLd;
+        float* out = x.whole ? space.rows + ((static_cast<size_t>(x.own) * a.T + t) * a.q_heads + head) * kLd : space.narrow + (static_cast<size_t>(2 * gw + x.begins) * kNarrow + r) * kLd;
 #pragma unroll
         for (int d = 0; d < 16; ++d) *reinterpret_cast<float2*>(out + d * 8 + q2) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
         if ((lane & 3) == 0) *reinterpret_cast<float2*>(out + kD) = make_float2(ref[h], l[h]);
@@ -404,6 +309,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
   // the copies in flight land before the CTA ends, also where it gives up
   for (int k = used; k < issued; ++k) warp_wait(full0 + 8 * (k % kDepth), (k / kDepth) & 1);
   if (!ok) *reinterpret_cast<volatile int*>(error) = 1;
+  if (behind) griddep_wait();
 }
 
 // sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts, in order, four dimensions a lane
@@ -440,7 +346,7 @@ __device__ __forceinline__ uint2 join_row(int parts, At part, int lane) {
 
 // A CTA has a row and eight of its heads.
 __global__ void __launch_bounds__(kJoinThreads)
-shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, long long warps) {
+shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const Sizes sizes) {
   const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, head = blockIdx.y * (kJoinThreads / 32) + warp;
   griddep_enter();
   // whether some request has the row
@@ -457,40 +363,47 @@ shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, long lo
     if (a.zero_rest) *out = make_uint2(0, 0);
     return;
   }
-  const Space space = space_of(a, warps);
+  const Space space = space_of(a, sizes);
   const int group = a.q_heads / a.kv_heads, kvh = head / group;
   const Place own = space.places[(static_cast<size_t>(a.T) + t) * a.kv_heads + kvh];
-  if (!own.parts && !own.joined) return;      // written already
+  if (!own.parts && !(own.flags & kJoined)) return;      // written already
   Place shared = {0, 0, 0, 0};
-  if (own.joined) shared = space.places[static_cast<size_t>(t) * a.kv_heads + kvh];
-  const int n_own = max(1, own.parts), n_all = n_own + (own.joined ? max(1, shared.parts) : 0);
+  if (own.flags & kJoined) shared = space.places[static_cast<size_t>(t) * a.kv_heads + kvh];
+  const int n_own = max(1, own.parts), n_all = n_own + (own.flags & kJoined ? max(1, shared.parts) : 0);
   // an item's beginning lies in its range's second slot, each other part in its range's first
   auto part = [&](int p) -> const float* {
     const bool first = p < n_own;
     const Place& x = first ? own : shared;
     const int k = first ? p : p - n_own;
     if (!x.parts) return space.rows + ((static_cast<size_t>(first) * a.T + t) * a.q_heads + head) * kLd;
-    return space.slots + (static_cast<size_t>(k ? x.slot - 1 + 2 * k : x.slot) * kRows + x.row + head % group) * kLd;
+    const bool wide = x.flags & kWide;
+    return (wide ? space.wide : space.narrow) + (static_cast<size_t>(k ? x.slot - 1 + 2 * k : x.slot) * (wide ? kWideRows : kNarrow) + x.row + head % group) * kLd;
   };
   *out = join_row(n_all, part, lane);
 }
 
 }  // namespace
 
+static Sizes sizes_of(const b200_shared_attn_args& a) { return {kPlaces * sm_count() * kWarps, shared_attention_wide_ctas(a)}; }
+
 int64_t shared_attention_workspace(const b200_shared_attn_args& a) {
+  const Sizes n = sizes_of(a);
   const int64_t T = a.T;
-  return 2 * T * a.kv_heads * static_cast<int64_t>(sizeof(Place)) + (static_cast<int64_t>(kPlaces) * sm_count() * kWarps * 2 * kRows + (a.G ? 2 * T * a.q_heads : 0)) * kLd * static_cast<int64_t>(sizeof(float));
+  return 2 * T * a.kv_heads * static_cast<int64_t>(sizeof(Place)) +
+         (2ll * n.warps * kNarrow + 2ll * n.ctas * kWideRows + (a.G ? 2 * T * a.q_heads : 0)) * kLd * static_cast<int64_t>(sizeof(float));
 }
 
 int paged_attention_shared(const b200_shared_attn_args& a, int* error, cudaStream_t st) {
-  const int ctas = kPlaces * sm_count();
+  const Sizes sizes = sizes_of(a);
+  if (sizes.ctas)
+    if (int rc = shared_attention_wide(a, sizes, error, st)) return rc;
   CUtensorMap tm_kv;
   if (int rc = tmap_encode_bf16_2d(&tm_kv, a.kv_layer, static_cast<uint64_t>(a.num_pages) * 2 * a.kv_heads * 16, kD, kD, 16, 64, 1)) return rc;
   static std::atomic<unsigned long long> attr_done{0};
   if (!ensure_dynamic_smem(shared_attn_kernel, kSmem, &attr_done)) return -3;
-  launch_pdl(shared_attn_kernel, dim3(ctas), dim3(kThreads), kSmem, st, tm_kv, a, a.scale * 1.4426950408889634f, error);
+  launch_pdl(shared_attn_kernel, dim3(sizes.warps / kWarps), dim3(kThreads), kSmem, st, tm_kv, a, sizes, a.scale * 1.4426950408889634f, error);
   if (cudaGetLastError() != cudaSuccess) return -2;
-  launch_pdl(shared_attn_join_kernel, dim3(a.T, (a.q_heads + 7) / 8), dim3(kJoinThreads), 0, st, a, static_cast<long long>(ctas) * kWarps);
+  launch_pdl(shared_attn_join_kernel, dim3(a.T, (a.q_heads + 7) / 8), dim3(kJoinThreads), 0, st, a, sizes);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 

@@ -1,0 +1,153 @@
+// What the kernels of shared_attention.cu and shared_attention_wide.cu have in common: which rows and keys an item has, and where its rows go.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "beam_step.h"
+#include "ptx.cuh"
+
+namespace b200 {
+namespace shared_attn {
+
+using beam::Lengths;
+using beam::Part;
+constexpr int kD = 128, kNarrow = 16;      // kNarrow: rows (token * group + head) of a part that go to the narrow kernel, whose row tile that is
+constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
+constexpr int kWaitLimit = 1 << 22;
+
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_limited(bar, parity, kWaitLimit)); }
+// two bf16 without infinities and NaN
+__device__ __forceinline__ uint32_t without_odd(uint32_t u) { return ((u & 0x7f80u) == 0x7f80u ? 0u : u & 0xffffu) | ((u & 0x7f800000u) == 0x7f800000u ? 0u : u & 0xffff0000u); }
+
+// Where the rows of a token and key head are: their own keys' part, and what their group shares.
+struct Place {
+  int slot, parts;      // parts 0: in the rows of all (or in the output), else in the slots of `parts` ranges, slot the first
+  int row;              // the token's first row there
+  int flags;
+};
+constexpr int kJoined = 1, kWide = 2;      // own rows: the group's are to be added; the slots are the wide kernel's
+struct Space {
+  Place* places;        // [2][T][kv_heads]: the groups', the requests' own
+  float* narrow;        // [warps][2][16][kLd]: a range's first item, which another range began, and its last
+  float* wide;          // [CTAs][2][128][kLd], the same
+  float* rows;          // [2][T][q_heads][kLd]
+};
+struct Sizes {
+  int warps, ctas;      // of the narrow and the wide kernel
+};
+constexpr int kWideRows = 128;
+__host__ __device__ inline Space space_of(const b200_shared_attn_args& a, const Sizes& n) {
+  Space s;
+  s.places = static_cast<Place*>(a.workspace);
+  s.narrow = reinterpret_cast<float*>(s.places + 2ll * a.T * a.kv_heads);
+  s.wide = s.narrow + static_cast<long long>(n.warps) * 2 * kNarrow * kLd;
+  s.rows = s.wide + static_cast<long long>(n.ctas) * 2 * kWideRows * kLd;
+  return s;
+}
+
+__device__ __forceinline__ Lengths lengths_of(const b200_shared_attn_args& a, bool ordered) {
+  return {a.starts, a.ctx, a.group_starts, a.shared, a.status, a.S, a.T, ordered ? a.G : 0, a.max_blocks, a.max_rows};
+}
+
+// ---- items: a part's key head and a block of its rows; what a unit of kUnit keys is to a range
+template <bool kIsWide>
+struct Items {
+  static constexpr int kUnit = kIsWide ? 64 : 16, kRows = kIsWide ? kWideRows : kNarrow;
+  // part u, without rows where it is the other kernel's
+  static __device__ __forceinline__ Part part(const Lengths& n, int u, int group) {
+    Part p = beam::part_of(n, u);
+    if ((p.rows * group > kNarrow) != kIsWide) p.rows = 0;
+    return p;
+  }
+  static __device__ __forceinline__ int end_of(const Part& p, int bt, int block) { return p.all ? p.k1 : p.ctx + min(p.rows, (block + 1) * bt); }
+  static __device__ __forceinline__ int units_of(const Part& p, int bt, int block) { return (end_of(p, bt, block) - p.k0 + kUnit - 1) / kUnit; }
+  static __device__ __forceinline__ int blocks_of(const Part& p, int bt) { return (p.rows + bt - 1) / bt; }
+  static __device__ __forceinline__ int head_cost(const Part& p, int bt) {
+    const int blocks = blocks_of(p, bt);
+    if (p.all || blocks <= 1) return blocks ? blocks * (units_of(p, bt, 0) + tree::kItem) : 0;
+    int n = 0;
+    for (int b = 0; b < blocks; ++b) n += units_of(p, bt, b) + tree::kItem;
+    return n;
+  }
+};
+template <bool kIsWide>
+struct Item {
+  typedef Items<kIsWide> I;
+  int u, kvh, block;
+  Part p;
+  int first, nb, k1, units;      // the block's tokens, the keys they may see
+  __device__ __forceinline__ void fill(int bt) {
+    first = block * bt;
+    nb = min(bt, p.rows - first);
+    k1 = I::end_of(p, bt, block);
+    units = I::units_of(p, bt, block);
+  }
+  __device__ __forceinline__ void next(const Lengths& n, int kv_heads, int group, int bt) {
+    if (++kvh >= kv_heads) {
+      kvh = 0;
+      if (++block >= I::blocks_of(p, bt)) {
+        block = 0;
+        do p = I::part(n, ++u, group);
+        while (p.rows == 0);      // (a range's units are some part's: the walk ends in front of the last)
+      }
+    }
+    fill(bt);
+  }
+};
+
+// Where `count` ranges from range `first` on begin and end: every thread sums some parts of the step, one behind the other, and the sums of the threads in front of it.  range
+// [count + 1], where [count + 1][4]: part, key head, block, and the first unit of the item that a range begins in.  Returns all ranges; to be followed by a barrier.
+template <bool kIsWide, int kThreads>
+__device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, int kv_heads, int group, int first, int count, int most, int* sums, int* range, int (*where)[4]) {
+  typedef Items<kIsWide> I;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bt = I::kRows / group;
+  const int U = n.G + n.S, per = (U + kThreads - 1) / kThreads, u_begin = min(U, tid * per), u_end = min(U, u_begin + per);
+  int before = 0, N = 0;
+  for (int u = u_begin; u < u_end; ++u) before += I::head_cost(I::part(n, u, group), bt) * kv_heads;
+  const int own = before;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += y;
+  }
+  if (lane == 31) sums[warp] = before;
+  __syncthreads();
+  before -= own;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    const int x = sums[w];
+    if (w < warp) before += x;
+    N += x;
+  }
+  tree::Ranges ranges = tree::ranges_of(N, most);
+  if (N == 0) ranges.n = 0;
+  if (tid <= count && first + tid >= ranges.n) range[tid] = N;      // which lies in no item
+  if (first < ranges.n) {
+    const int b_end = ranges.at(min(first + count, ranges.n - 1));
+    if (own && ranges.at(first) < before + own && b_end >= before)
+      for (int u = u_begin; u < u_end; ++u) {
+        const Part p = I::part(n, u, group);
+        const int mine = I::head_cost(p, bt) * kv_heads;
+        for (int e = 0; e <= count && first + e < ranges.n; ++e) {
+          const int b = ranges.at(first + e);
+          if (mine == 0 || b < before || b >= before + mine) continue;
+          int g0 = before, block = 0, units = I::units_of(p, bt, 0);
+          while (b >= g0 + (units + tree::kItem) * kv_heads) g0 += (units + tree::kItem) * kv_heads, units = I::units_of(p, bt, ++block);
+          const int kvh = (b - g0) / (units + tree::kItem);
+          g0 += kvh * (units + tree::kItem);
+          range[e] = tree::snapped(b, g0, units, ranges.snap);
+          where[e][0] = u; where[e][1] = kvh; where[e][2] = block; where[e][3] = g0;
+        }
+        before += mine;
+      }
+  }
+  return ranges;
+}
+
+}  // namespace shared_attn
+
+// The kernel of parts with more rows than kNarrow
+int shared_attention_wide(const b200_shared_attn_args& a, const shared_attn::Sizes& sizes, int* error, cudaStream_t st);
+int shared_attention_wide_ctas(const b200_shared_attn_args& a);
+
+}  // namespace b200
