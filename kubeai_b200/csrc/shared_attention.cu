@@ -28,10 +28,10 @@ namespace {
 typedef __nv_bfloat16 bf16;
 using namespace shared_attn;
 constexpr int kPageBytes = 2 * 16 * kD * 2;      // bytes of a page's keys and values of a head
-constexpr int kThreads = 128, kWarps = kThreads / 32, kPlaces = 3, kDepth = 2, kItems = 4;      // kPlaces: CTAs of an SM; kDepth: pages of a warp on their way; kItems: items that those may lie in, and one
-constexpr int kJoinThreads = 256, kFew = 4;
+constexpr int kThreads = 128, kWarps = kThreads / 32, kPlaces = 3, kDepth = 2, kItems = 4, kLeast = 4;      // kPlaces: CTAs of an SM; kDepth: pages of a warp on their way; kItems: items that those may lie in, and one; kLeast: pages of a range
+constexpr int kJoinThreads = 256, kAtOnce = 4;      // kAtOnce: parts of a row on their way
 constexpr int kSmem = 1024 + kWarps * kDepth * kPageBytes;
-static_assert(kPlaces * (kSmem + 3072) <= 228 * 1024, "");
+static_assert(kPlaces * (kSmem + 3072 + static_cast<int>(sizeof(Staged))) <= 228 * 1024, "");
 static_assert(kItems > kDepth, "");
 
 // An item's pages of a range, as the loads leave them for the products
@@ -51,6 +51,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
   __shared__ __align__(8) uint64_t bars[kWarps * kDepth];
   __shared__ int sums[kWarps], s_range[kWarps + 1], s_where[kWarps + 1][4];
   __shared__ Piece pieces[kWarps][kItems];
+  __shared__ Staged staged;
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (sbase - smem_u32(smem_raw));
   const int warp = warp_number(), lane = threadIdx.x & 31, tid = threadIdx.x;
@@ -66,11 +67,9 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
   const bool behind = sizes.ctas > 0;
   if (!behind) griddep_wait();
   griddep_launch();
-  bool ordered = a.G > 0;
-  if (ordered) ordered = __syncthreads_and(beam::ascends(a.group_starts, a.G, a.S, tid, kThreads) && beam::ascends(a.starts, a.S, a.T, tid, kThreads));
-  const Lengths n = lengths_of(a, ordered);
+  const Lengths n = lengths_of(a, &staged, tid, kThreads);
   const int gw = blockIdx.x * kWarps + warp;
-  const tree::Ranges ranges = find_ranges<false, kThreads>(n, a.kv_heads, group, blockIdx.x * kWarps, kWarps, sizes.warps, sums, s_range, s_where);
+  const tree::Ranges ranges = find_ranges<false, kThreads>(n, a.kv_heads, group, blockIdx.x * kWarps, kWarps, sizes.warps, kLeast, sums, s_range, s_where);
   __syncthreads();
   const int left = gw < ranges.n ? s_range[warp + 1] - s_range[warp] : 0;
   if (left <= 0) {
@@ -312,32 +311,41 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
   if (behind) griddep_wait();
 }
 
-// sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts, in order, four dimensions a lane
+// A row: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts, in order, four dimensions a lane; a lane has the maximum, sum and weight of one part in 32.
 template <typename At>
 __device__ __forceinline__ uint2 join_row(int parts, At part, int lane) {
   float m = -INFINITY, sum = 0.f;
   float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int p0 = 0; p0 < parts; p0 += kFew) {
-    float2 st[kFew];
-    float4 x[kFew];
-    float top = m;
+  for (int p0 = 0; p0 < parts; p0 += 32) {
+    const int count = min(32, parts - p0);
+    const float* mine = part(p0 + min(lane, count - 1));
+    float4 x[kAtOnce];
+    auto load = [&](int k0) {
 #pragma unroll
-    for (int k = 0; k < kFew; ++k) {
-      const bool there = p0 + k < parts;
-      st[k] = there ? *reinterpret_cast<const float2*>(part(p0 + k) + kD) : make_float2(-INFINITY, 0.f);
-      x[k] = there ? *reinterpret_cast<const float4*>(part(p0 + k) + lane * 4) : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float* from = reinterpret_cast<const float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mine), (k0 + k) & 31));
+        if (k0 + k < count) x[k] = *reinterpret_cast<const float4*>(from + lane * 4);
+      }
+    };
+    const float2 st = lane < count ? *reinterpret_cast<const float2*>(mine + kD) : make_float2(-INFINITY, 0.f);
+    load(0);
+    float top = fmaxf(m, st.x);
 #pragma unroll
-    for (int k = 0; k < kFew; ++k) top = fmaxf(top, st[k].x);
-    const float base = top == -INFINITY ? 0.f : top, old = exp2f(m - base);
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    const float base = top == -INFINITY ? 0.f : top, old = exp2f(m - base), w = exp2f(st.x - base);
     m = top;
-    sum *= old;
-    y = make_float4(y.x * old, y.y * old, y.z * old, y.w * old);
+    float l = w == 0.f && st.y == st.y ? 0.f : st.y * w;
 #pragma unroll
-    for (int k = 0; k < kFew; ++k) {
-      const float w = exp2f(st[k].x - base);
-      sum += w == 0.f && st[k].y == st[k].y ? 0.f : st[k].y * w;
-      if (w != 0.f) y = make_float4(fmaf(x[k].x, w, y.x), fmaf(x[k].y, w, y.y), fmaf(x[k].z, w, y.z), fmaf(x[k].w, w, y.w));
+    for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    sum = sum * old + l;
+    y = make_float4(y.x * old, y.y * old, y.z * old, y.w * old);
+    for (int k0 = 0; k0 < count; k0 += kAtOnce) {
+      if (k0) load(k0);
+#pragma unroll
+      for (int k = 0; k < kAtOnce; ++k) {
+        const float wk = __shfl_sync(0xffffffffu, w, (k0 + k) & 31);
+        if (k0 + k < count && wk != 0.f) y = make_float4(fmaf(x[k].x, wk, y.x), fmaf(x[k].y, wk, y.y), fmaf(x[k].z, wk, y.z), fmaf(x[k].w, wk, y.w));
+      }
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
@@ -349,11 +357,13 @@ __global__ void __launch_bounds__(kJoinThreads)
 shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const Sizes sizes) {
   const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, head = blockIdx.y * (kJoinThreads / 32) + warp;
   griddep_enter();
-  // whether some request has the row
+  const Space space = space_of(a, sizes);
+  const int group = a.q_heads / a.kv_heads, kvh = min(head, a.q_heads - 1) / group;
+  // (what lies there counts where some request has the row)
+  const Place shared = space.places[static_cast<size_t>(t) * a.kv_heads + kvh], own = space.places[(static_cast<size_t>(a.T) + t) * a.kv_heads + kvh];
   bool mine = false;
   for (int s = tid; s < a.S && !mine; s += kJoinThreads) {
-    const Lengths n = lengths_of(a, false);
-    const tree::Request r = n.request(s);
+    const tree::Request r = tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, a.max_rows, a.status);
     mine = t >= r.row0 && t < r.row0 + r.rows;
   }
   mine = __syncthreads_or(mine);
@@ -363,21 +373,15 @@ shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const S
     if (a.zero_rest) *out = make_uint2(0, 0);
     return;
   }
-  const Space space = space_of(a, sizes);
-  const int group = a.q_heads / a.kv_heads, kvh = head / group;
-  const Place own = space.places[(static_cast<size_t>(a.T) + t) * a.kv_heads + kvh];
   if (!own.parts && !(own.flags & kJoined)) return;      // written already
-  Place shared = {0, 0, 0, 0};
-  if (own.flags & kJoined) shared = space.places[static_cast<size_t>(t) * a.kv_heads + kvh];
   const int n_own = max(1, own.parts), n_all = n_own + (own.flags & kJoined ? max(1, shared.parts) : 0);
   // an item's beginning lies in its range's second slot, each other part in its range's first
   auto part = [&](int p) -> const float* {
     const bool first = p < n_own;
-    const Place& x = first ? own : shared;
-    const int k = first ? p : p - n_own;
-    if (!x.parts) return space.rows + ((static_cast<size_t>(first) * a.T + t) * a.q_heads + head) * kLd;
-    const bool wide = x.flags & kWide;
-    return (wide ? space.wide : space.narrow) + (static_cast<size_t>(k ? x.slot - 1 + 2 * k : x.slot) * (wide ? kWideRows : kNarrow) + x.row + head % group) * kLd;
+    const int k = first ? p : p - n_own, parts = first ? own.parts : shared.parts, slot = first ? own.slot : shared.slot, row = first ? own.row : shared.row;
+    if (!parts) return space.rows + ((static_cast<size_t>(first) * a.T + t) * a.q_heads + head) * kLd;
+    const bool wide = (first ? own.flags : shared.flags) & kWide;
+    return (wide ? space.wide : space.narrow) + (static_cast<size_t>(k ? slot - 1 + 2 * k : slot) * (wide ? kWideRows : kNarrow) + row + head % group) * kLd;
   };
   *out = join_row(n_all, part, lane);
 }

@@ -29,13 +29,13 @@ constexpr int kJoined = 1, kWide = 2;      // own rows: the group's are to be ad
 struct Space {
   Place* places;        // [2][T][kv_heads]: the groups', the requests' own
   float* narrow;        // [warps][2][16][kLd]: a range's first item, which another range began, and its last
-  float* wide;          // [CTAs][2][128][kLd], the same
+  float* wide;          // [CTAs][2][kWideRows][kLd], the same
   float* rows;          // [2][T][q_heads][kLd]
 };
 struct Sizes {
   int warps, ctas;      // of the narrow and the wide kernel
 };
-constexpr int kWideRows = 128;
+constexpr int kWideRows = 256;      // rows of an item of the wide kernel
 __host__ __device__ inline Space space_of(const b200_shared_attn_args& a, const Sizes& n) {
   Space s;
   s.places = static_cast<Place*>(a.workspace);
@@ -45,28 +45,58 @@ __host__ __device__ inline Space space_of(const b200_shared_attn_args& a, const 
   return s;
 }
 
-__device__ __forceinline__ Lengths lengths_of(const b200_shared_attn_args& a, bool ordered) {
-  return {a.starts, a.ctx, a.group_starts, a.shared, a.status, a.S, a.T, ordered ? a.G : 0, a.max_blocks, a.max_rows};
+// The lengths, in shared memory where they fit: parts are looked up by chains of dependent loads, at the head of a kernel and at every item's beginning.  With a barrier behind it; `groups`
+// where they are wanted.
+constexpr int kStaged = 256;
+struct Staged {
+  int starts[kStaged + 1], ctx[kStaged], status[kStaged], group_starts[kStaged + 1], shared[kStaged];
+};
+__device__ __forceinline__ Lengths lengths_of(const b200_shared_attn_args& a, Staged* to, int tid, int threads) {
+  Lengths n = {a.starts, a.ctx, a.group_starts, a.shared, a.status, a.S, a.T, a.G, a.max_blocks, a.max_rows};
+  if (a.S <= kStaged && a.G <= kStaged) {
+    for (int s = tid; s <= a.S; s += threads) {
+      to->starts[s] = a.starts[s];
+      if (s < a.S) to->ctx[s] = a.ctx[s];
+      if (s < a.S && a.status) to->status[s] = a.status[s];
+    }
+    if (a.G)
+      for (int g = tid; g <= a.G; g += threads) {
+        to->group_starts[g] = a.group_starts[g];
+        if (g < a.G) to->shared[g] = a.shared[g];
+      }
+    n.starts = to->starts; n.ctx = to->ctx; n.group_starts = to->group_starts; n.shared = to->shared;
+    if (a.status) n.status = to->status;
+  }
+  __syncthreads();
+  if (a.G && !__syncthreads_and(beam::ascends(n.group_starts, a.G, a.S, tid, threads) && beam::ascends(n.starts, a.S, a.T, tid, threads))) n.G = 0;
+  return n;
 }
 
-// ---- items: a part's key head and a block of its rows; what a unit of kUnit keys is to a range
+// ---- items: a part's key head and a block of its rows.  Its keys come in units: pages, or steps of the wide kernel, which has two tiles of 128 scores at once: those of two row tiles and 128 keys
+// where there are more than 128 rows, else of one row tile and 256 keys.
 template <bool kIsWide>
 struct Items {
-  static constexpr int kUnit = kIsWide ? 64 : 16, kRows = kIsWide ? kWideRows : kNarrow;
+  static constexpr int kRows = kIsWide ? kWideRows : kNarrow;
   // part u, without rows where it is the other kernel's
   static __device__ __forceinline__ Part part(const Lengths& n, int u, int group) {
     Part p = beam::part_of(n, u);
     if ((p.rows * group > kNarrow) != kIsWide) p.rows = 0;
     return p;
   }
+  static __device__ __forceinline__ int tokens_of(const Part& p, int bt, int block) { return min(bt, p.rows - block * bt); }
+  static __device__ __forceinline__ int unit_of(int tokens, int bt) { return !kIsWide ? 16 : 2 * tokens > bt ? 128 : 256; }
   static __device__ __forceinline__ int end_of(const Part& p, int bt, int block) { return p.all ? p.k1 : p.ctx + min(p.rows, (block + 1) * bt); }
-  static __device__ __forceinline__ int units_of(const Part& p, int bt, int block) { return (end_of(p, bt, block) - p.k0 + kUnit - 1) / kUnit; }
+  static __device__ __forceinline__ int units_of(const Part& p, int bt, int block) {
+    const int unit = unit_of(tokens_of(p, bt, block), bt);
+    return (end_of(p, bt, block) - p.k0 + unit - 1) / unit;
+  }
   static __device__ __forceinline__ int blocks_of(const Part& p, int bt) { return (p.rows + bt - 1) / bt; }
   static __device__ __forceinline__ int head_cost(const Part& p, int bt) {
     const int blocks = blocks_of(p, bt);
-    if (p.all || blocks <= 1) return blocks ? blocks * (units_of(p, bt, 0) + tree::kItem) : 0;
-    int n = 0;
-    for (int b = 0; b < blocks; ++b) n += units_of(p, bt, b) + tree::kItem;
+    if (blocks <= 1) return blocks ? units_of(p, bt, 0) + tree::kItem : 0;
+    int n = units_of(p, bt, blocks - 1) + tree::kItem;      // (the last block may be of the other unit)
+    if (p.all) return n + (blocks - 1) * (units_of(p, bt, 0) + tree::kItem);
+    for (int b = 0; b < blocks - 1; ++b) n += units_of(p, bt, b) + tree::kItem;
     return n;
   }
 };
@@ -83,10 +113,10 @@ struct Item {
     units = I::units_of(p, bt, block);
   }
   __device__ __forceinline__ void next(const Lengths& n, int kv_heads, int group, int bt) {
-    if (++kvh >= kv_heads) {
-      kvh = 0;
-      if (++block >= I::blocks_of(p, bt)) {
-        block = 0;
+    if (++block >= I::blocks_of(p, bt)) {      // a head's blocks come one behind the other: CTAs side by side read the same pages
+      block = 0;
+      if (++kvh >= kv_heads) {
+        kvh = 0;
         do p = I::part(n, ++u, group);
         while (p.rows == 0);      // (a range's units are some part's: the walk ends in front of the last)
       }
@@ -96,9 +126,9 @@ struct Item {
 };
 
 // Where `count` ranges from range `first` on begin and end: every thread sums some parts of the step, one behind the other, and the sums of the threads in front of it.  range
-// [count + 1], where [count + 1][4]: part, key head, block, and the first unit of the item that a range begins in.  Returns all ranges; to be followed by a barrier.
+// [count + 1], where [count + 1][4]: part, key head, block, and the first unit of the item that a range begins in.  No range has less than `least` units.  Returns all ranges; to be followed by a barrier.
 template <bool kIsWide, int kThreads>
-__device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, int kv_heads, int group, int first, int count, int most, int* sums, int* range, int (*where)[4]) {
+__device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, int kv_heads, int group, int first, int count, int most, int least, int* sums, int* range, int (*where)[4]) {
   typedef Items<kIsWide> I;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bt = I::kRows / group;
   const int U = n.G + n.S, per = (U + kThreads - 1) / kThreads, u_begin = min(U, tid * per), u_end = min(U, u_begin + per);
@@ -119,7 +149,7 @@ __device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, int kv_hea
     if (w < warp) before += x;
     N += x;
   }
-  tree::Ranges ranges = tree::ranges_of(N, most);
+  tree::Ranges ranges = tree::ranges_of(N, max(1, min(most, N / least)));
   if (N == 0) ranges.n = 0;
   if (tid <= count && first + tid >= ranges.n) range[tid] = N;      // which lies in no item
   if (first < ranges.n) {
@@ -127,14 +157,13 @@ __device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, int kv_hea
     if (own && ranges.at(first) < before + own && b_end >= before)
       for (int u = u_begin; u < u_end; ++u) {
         const Part p = I::part(n, u, group);
-        const int mine = I::head_cost(p, bt) * kv_heads;
+        const int head = I::head_cost(p, bt), mine = head * kv_heads;
         for (int e = 0; e <= count && first + e < ranges.n; ++e) {
           const int b = ranges.at(first + e);
           if (mine == 0 || b < before || b >= before + mine) continue;
-          int g0 = before, block = 0, units = I::units_of(p, bt, 0);
-          while (b >= g0 + (units + tree::kItem) * kv_heads) g0 += (units + tree::kItem) * kv_heads, units = I::units_of(p, bt, ++block);
-          const int kvh = (b - g0) / (units + tree::kItem);
-          g0 += kvh * (units + tree::kItem);
+          const int kvh = (b - before) / head;
+          int g0 = before + kvh * head, block = 0, units = I::units_of(p, bt, 0);
+          while (b >= g0 + units + tree::kItem) g0 += units + tree::kItem, units = I::units_of(p, bt, ++block);
           range[e] = tree::snapped(b, g0, units, ranges.snap);
           where[e][0] = u; where[e][1] = kvh; where[e][2] = block; where[e][3] = g0;
         }
