@@ -43,29 +43,6 @@ constexpr float kSlack = 1.f;                                       // by how mu
 constexpr int kRingAt = 2 * kTile, kStageAt = kRingAt + kRing * kTile, kBars = kStageAt + 8 * 2048, kSmem = 1024 + kBars + 256;
 static_assert(kSmem + static_cast<int>(sizeof(Staged)) + 4096 <= 227 * 1024, "");
 
-// Two floats in a 64-bit register pair: one instruction for both
-__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
-  uint64_t p;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "r"(lo), "r"(hi));
-  return p;
-}
-__device__ __forceinline__ float2 floats_of(uint64_t p) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
-  return f;
-}
-__device__ __forceinline__ uint64_t pair_of(float lo, float hi) { return pair_of(__float_as_uint(lo), __float_as_uint(hi)); }
-__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -341,11 +318,15 @@ shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
             if (one) mbar_arrive_expect_tx(full(seq), count * 4096);
             __syncwarp();
             const uint32_t dst = ring + (seq % kRing) * kTile;
-            for (int p = 0; p < count; ++p) {
-              const int row = __shfl_sync(0xffffffffu, mine, (p0 + p) & 31) + (values ? 16 * a.kv_heads : 0);
-              if (one) {
-                tma_load_2d(dst + p * 2048, &tm_kv, full(seq), 0, row, hint);
-                tma_load_2d(dst + kSlab + p * 2048, &tm_kv, full(seq), 64, row, hint);
+            int row[8];
+#pragma unroll
+            for (int p = 0; p < 8; ++p) row[p] = __shfl_sync(0xffffffffu, mine, (p0 + p) & 31) + (values ? 16 * a.kv_heads : 0);
+            if (one) {
+#pragma unroll
+              for (int p = 0; p < 8; ++p) {
+                if (p >= count) break;
+                tma_load_2d(dst + p * 2048, &tm_kv, full(seq), 0, row[p], hint);
+                tma_load_2d(dst + kSlab + p * 2048, &tm_kv, full(seq), 64, row[p], hint);
               }
             }
             __syncwarp();
