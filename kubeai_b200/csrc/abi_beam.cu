@@ -83,7 +83,7 @@ static int select_sizes(const b200_beam_select_args* a, const char* op) {
   if (a->k < 1 || a->k > beam::kMaxFound) return refuse(op, "1 to 64 candidates");
   if (a->V > beam::kMaxVocab) return refuse(op, "more than 393216 tokens");
   if (a->num_ends > beam::kMaxEnds) return refuse(op, "more than 1024 tokens that end a text");
-  if (a->S > INT_MAX / (32 * a->beams)) return refuse(op, "too many requests for a launch");
+  if (a->S > INT_MAX / (64 * a->beams)) return refuse(op, "too many requests for a launch");
   return 0;
 }
 
@@ -102,7 +102,9 @@ int b200_op_beam_select(const b200_beam_select_args* a, void* stream) {
   if (a->new_scores == a->scores) return refuse(op, "new scores have a buffer of their own");
   if (!a->workspace || !aligned(a->workspace, 16) || a->workspace_bytes < beam_select_workspace(*a)) return refuse(op, "the workspace is missing, too small or not 16-byte aligned");
   if (int rc = require_device()) return rc;
-  return launched(op, beam_select(*a, static_cast<cudaStream_t>(stream)));
+  int* mark = nullptr;
+  if (int rc = op_mark(&mark)) return rc;
+  return launched(op, beam_select(*a, mark, static_cast<cudaStream_t>(stream)));
 }
 
 int b200_op_beam_reorder(const b200_beam_reorder_args* a, void* stream) {

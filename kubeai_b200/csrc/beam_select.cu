@@ -4,14 +4,15 @@
 //
 // A row's best candidates by c are its best by x, which needs no rounding, so one pass over the logits takes them by x, together with the sum; c, which decides between beams, is
 // made in 64 bits for a few hundred candidates.
-// First kernel: a row is cut into parts of at most 16384 bf16 (8192 fp32) logits, a CTA each, whose values stay in registers.  A lower bound of the k-th largest value that few values besides the
+// First kernel: a row is cut into parts of at most 26624 bf16 (13312 fp32) logits, a CTA each, that come into shared memory by a bulk copy, four CTAs an SM.  A lower bound of the k-th largest value that few values besides the
 // k best reach: of every warp the r-th largest of its lanes' maxima (r = k / 4), and of those the fourth largest, as four warps have r lanes each that reach it.  What does goes to a list,
 // where each one's place is the number of better ones.  Where more reach it than the list holds (rows of equal values), the k-th value and the last token that still belongs are found bit by bit over all values.
-// The sum's large terms, those of the list, are taken in 64 bits, the others as 2^t in 32, t in two products: what an fp32 sum loses would decide between beams whose candidates lie close
-// together.
+// The sum's large terms, those of the list, are taken in 64 bits, the others in 32: what an fp32 sum loses of the large ones would decide between beams whose
+// candidates lie close together.
 // Second kernel, a CTA a request: a candidate's place among those of all parts, then of all beams, is its place in its own list and, by bisection, in every other.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
+#include <float.h>
 #include <math.h>
 
 #include <algorithm>
@@ -25,12 +26,12 @@
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kVectors = 8, kList = 256, kPlaces = 4, kAtOnce = 4;      // kVectors: pieces of 16 bytes of a thread; kPlaces: CTAs of an SM; kAtOnce: threads' values on their way to the list
+constexpr int kThreads = 256, kWarps = kThreads / 32, kVectors = 13, kList = 256, kPlaces = 4, kWaitLimit = 1 << 22;      // kVectors: pieces of 16 bytes of a thread; kPlaces: CTAs of an SM
 constexpr int kPart = kThreads * kVectors;                                            // pieces of a part at most
 constexpr int kMostParts = 64;                                                         // two of a lane in the second kernel
 static_assert(kMostParts * 4 * (kPart - 1) > beam::kMaxVocab && kWarps >= 4 && 4 * 32 >= beam::kMaxFound, "");
 constexpr int kLeastPart = 1024;                                                       // pieces of a part at least, where the row has them
-constexpr float kLog2eHi = 1.4426950216293335f, kLog2eLo = 1.9259629911e-8f;           // log2(e) as a sum
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct PartHead {
   float top;      // the part's largest logit
@@ -75,17 +76,13 @@ __device__ __forceinline__ float value_in(const uint32_t* w, int i) {
 // A row's piece, the values of 16 bytes, by the widest loads that the row's beginning allows (which values meet in a sum goes by their tokens alone: equal rows have equal sums wherever they lie).
 // What is behind the row's end is -inf.
 template <bool kF32, int kAlign>
-__device__ __forceinline__ void load_piece(const uint8_t* row, int V, int piece, bool there, uint32_t* w) {
+__device__ __forceinline__ void load_piece(const uint8_t* row, int V, int piece, uint32_t* w) {
   constexpr int kPer = kF32 ? 4 : 8, kSize = kF32 ? 4 : 2;
   const uint8_t* at = row + static_cast<size_t>(piece) * 16;
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = kF32 ? 0xff800000u : 0xff80ff80u;
-  if (!there) return;
   if ((piece + 1) * kPer <= V) {
-    if constexpr (kAlign == 16) {
-      const uint4 u = __ldcs(reinterpret_cast<const uint4*>(at));
-      w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-    } else if constexpr (kAlign == 8) {
+    if constexpr (kAlign == 8) {
       const uint2 u = *reinterpret_cast<const uint2*>(at), v = *reinterpret_cast<const uint2*>(at + 8);
       w[0] = u.x; w[1] = u.y; w[2] = v.x; w[3] = v.y;
     } else if constexpr (kAlign == 4) {
@@ -97,21 +94,30 @@ __device__ __forceinline__ void load_piece(const uint8_t* row, int V, int piece,
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) {
+    for (int i = 0; i < kPer - 1; ++i) {      // (not all of them)
       if (piece * kPer + i >= V) continue;
       if constexpr (kF32) w[i] = reinterpret_cast<const uint32_t*>(at)[i];
       else w[i / 2] = __byte_perm(w[i / 2], *reinterpret_cast<const uint16_t*>(at + i * kSize), i & 1 ? 0x5410 : 0x3254);
     }
   }
 }
+__device__ __forceinline__ __nv_bfloat162 bf16x2_of(uint32_t w) {
+  __nv_bfloat162 p;
+  *reinterpret_cast<uint32_t*>(&p) = w;
+  return p;
+}
 template <bool kF32>
-__device__ __forceinline__ float largest_in(const uint32_t* w) {
-  if (kF32) return fmaxf(fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1])), fmaxf(__uint_as_float(w[2]), __uint_as_float(w[3])));
-  __nv_bfloat162 p[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(&p[i]) = w[i];
+__device__ __forceinline__ uint32_t largest_in(const uint4& u) {      // as a word: of bf16 one for each half
+  if (kF32) return __float_as_uint(fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w))));
+  const __nv_bfloat162 p[4] = {bf16x2_of(u.x), bf16x2_of(u.y), bf16x2_of(u.z), bf16x2_of(u.w)};
   const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
-  return fmaxf(__low2float(m), __high2float(m));
+  return *reinterpret_cast<const uint32_t*>(&m);
+}
+// the bits of those values of a word that are at least this one, which is a value of the type
+template <bool kF32>
+__device__ __forceinline__ uint32_t those_at_least(uint32_t w, float least) {
+  if (kF32) return __uint_as_float(w) >= least ? ~0u : 0u;
+  return __hge2_mask(bf16x2_of(w), __float2bfloat162_rn(least));
 }
 // NaN becomes -inf
 template <bool kF32>
@@ -128,36 +134,68 @@ __device__ __forceinline__ void without_nan(uint32_t* w) {
   }
 }
 
+// A row's pieces in parts: `more` of them have one more than `each`
+struct Cut {
+  int parts, each, more;
+};
+
 template <bool kF32>
 __global__ void __launch_bounds__(kThreads, kPlaces)
-beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, int parts, size_t entries) {
+beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, const Cut cut, size_t entries, int* error) {
   constexpr int kPer = kF32 ? 4 : 8;
+  constexpr uint32_t kNone = kF32 ? 0xff800000u : 0xff80ff80u;
+  extern __shared__ uint4 here[];      // the part
+  __shared__ __align__(8) uint64_t bar_word;
   __shared__ uint32_t mosts[kWarps], bounds[kWarps];
   __shared__ double sums[kWarps];
-  __shared__ unsigned long long list[kList];
-  __shared__ double terms[kList];
+  __shared__ unsigned long long list[kList], sorted[kList];
   __shared__ int s_n, s_count;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const long long row = blockIdx.x / parts;
-  const int part = blockIdx.x % parts;
-  griddep_enter();
+  const unsigned number = blockIdx.x, row = number / static_cast<unsigned>(cut.parts), part = number - row * cut.parts;      // (64-bit quotients were a third of the kernel's instructions)
   const uint8_t* base = static_cast<const uint8_t*>(a.logits) + static_cast<size_t>(row) * a.ld * (kF32 ? 4 : 2);
-  const int pieces = (a.V + kPer - 1) / kPer;
-  const int v0 = static_cast<int>(static_cast<long long>(pieces) * part / parts), v1 = static_cast<int>(static_cast<long long>(pieces) * (part + 1) / parts);
-
-  uint32_t x[kVectors][4];
-  auto load = [&](auto align) {
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v) load_piece<kF32, decltype(align)::value>(base, a.V, v0 + v * kThreads + tid, v0 + v * kThreads + tid < v1, x[v]);
-  };
+  const int v0 = part * cut.each + min(static_cast<int>(part), cut.more), count = cut.each + (static_cast<int>(part) < cut.more);
   const int align = static_cast<int>(reinterpret_cast<uintptr_t>(base) & 15);
-  if (align == 0) load(std::integral_constant<int, 16>());
-  else if (align == 8) load(std::integral_constant<int, 8>());
-  else if (align % 4 == 0) load(std::integral_constant<int, 4>());
-  else load(std::integral_constant<int, 2>());
+  const int whole = align ? 0 : min(count, a.V / kPer - v0);      // pieces that a bulk copy brings: those of a row on 16 bytes that its end does not cut
+  const uint32_t bar = smem_u32(&bar_word);
+  if (tid == 0) {
+    mbar_init(bar, 1);
+    fence_mbar_init();
+    s_n = 0;
+  }
+  griddep_enter();
+  bool ok = true;
+  if (tid == 0 && whole > 0) {
+    mbar_arrive_expect_tx(bar, static_cast<uint32_t>(whole) * 16);
+    bulk_load_1d(smem_u32(here), base + static_cast<size_t>(v0) * 16, static_cast<uint32_t>(whole) * 16, bar);
+  }
+  // the others go the same way, and behind the last are pieces of nothing: a thread's own, which it alone reads
+  const int slots = (count + kThreads - 1) / kThreads;
+  for (int i = max(0, whole) / kThreads * kThreads + tid; i < slots * kThreads; i += kThreads) {
+    if (i < whole) continue;
+    uint32_t w[4] = {kNone, kNone, kNone, kNone};
+    if (i < count) {
+      if (align % 8 == 0) load_piece<kF32, 8>(base, a.V, v0 + i, w);
+      else if (align % 4 == 0) load_piece<kF32, 4>(base, a.V, v0 + i, w);
+      else load_piece<kF32, kF32 ? 4 : 2>(base, a.V, v0 + i, w);
+    }
+    here[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  __syncthreads();      // (the barrier's first phase is known to all)
+  if (whole > 0) ok = mbar_wait_limited(bar, 0, kWaitLimit);
+  // ---- the largest of every piece, two of bf16, and of all
+  uint32_t tops[kVectors];
+#pragma unroll
+  for (int v = 0; v < kVectors; ++v) {
+    tops[v] = kNone;
+    if (v < slots) tops[v] = largest_in<kF32>(here[v * kThreads + tid]);
+  }
   float mine = -INFINITY;
 #pragma unroll
-  for (int v = 0; v < kVectors; ++v) mine = fmaxf(mine, largest_in<kF32>(x[v]));
+  for (int v = 0; v < kVectors; v += 4) {
+    auto at = [&](int i) { return tops[min(i, kVectors - 1)]; };
+    const uint32_t m = largest_in<kF32>(make_uint4(at(v), at(v + 1), at(v + 2), at(v + 3)));
+    mine = fmaxf(mine, kF32 ? __uint_as_float(m) : fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u)));
+  }
   // ---- the warp's largest, and the r-th largest of its lanes' maxima (equal ones, which a lane each has, are counted once a round)
   const int r = (a.k + 3) / 4;
   const uint32_t order = order_of(mine), most = __reduce_max_sync(0xffffffffu, order);
@@ -173,86 +211,101 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, int parts, si
     mosts[warp] = most;
     bounds[warp] = rth;
   }
-  if (tid == 0) s_n = 0;
-  __syncthreads();
-  uint32_t all = 0, bound = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) all = max(all, mosts[w]);
-  const float top = value_of(all);
-  PartHead* head = static_cast<PartHead*>(a.workspace) + row * parts + part;
+  if (!__syncthreads_and(ok)) {      // (a thread that saw the copy come goes on past it: it has come)
+    if (tid == 0) *reinterpret_cast<volatile int*>(error) = 1;
+    if (whole > 0) mbar_wait_limited(bar, 0, kWaitLimit);
+    return;
+  }
+  static_assert(kWarps == 8, "");
+  const float top = value_of(__reduce_max_sync(0xffffffffu, mosts[lane & 7]));
+  PartHead* head = static_cast<PartHead*>(a.workspace) + number;
   if (top == -INFINITY) {      // nothing here is a candidate
     if (tid == 0) *head = {-INFINITY, 0, 0.0};
     return;
   }
-  {      // the fourth largest of the warps' bounds
-    const uint32_t mine4 = bounds[lane % kWarps];
+  // the fourth largest of the warps' bounds: four warps have r lanes each that reach it
+  uint32_t bound = bounds[lane & 7];
+  {
     int place = 0;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) place += bounds[w] > mine4 || (bounds[w] == mine4 && w < lane % kWarps);
-    bound = __reduce_max_sync(0xffffffffu, place == 3 ? mine4 : 0u);
+    for (int o = 1; o < 8; ++o) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, bound, o);
+      place += other > bound || (other == bound && ((lane ^ o) & 7) < (lane & 7));
+    }
+    bound = __reduce_max_sync(0xffffffffu, place == 3 ? bound : 0u);
   }
-  if (bound <= order_of(-INFINITY)) bound = order_of(-INFINITY) + 1;      // the smallest value that is one
-  float least = value_of(bound);
-  // ---- the sum of those below it, by every thread that has no others
-  const uint64_t less = pair_of(-top, -top), hi = pair_of(kLog2eHi, kLog2eHi), lo = pair_of(kLog2eLo, kLog2eLo);
-  float rest = 0.f;
-  const unsigned some = __ballot_sync(0xffffffffu, mine >= least);
-  if (mine < least) {
-#pragma unroll 1
-    for (int again = 0; again < 2; ++again) {
-      uint64_t sum2[2] = {0, 0};
+  bound = max(bound, order_of(kF32 ? -FLT_MAX : __uint_as_float(0xff7f0000u)));      // the type's lowest value is one, -inf is none
+  const float least = value_of(bound);
+  // ---- the list, and the sum of the others
+  // exp(x - top) = 2^(x L + c) 2^-(top L + c) for any c: the product inside the sum is exact, so with c near -top L each term has one rounding, and what c's own took from all of them comes
+  // back in 64 bits at the end.  (Where top is so large that this does not fit, the difference is taken first.)
+  const float from = -top * kLog2e;
+  const bool far = !(fabsf(top) < 1048576.f);
+  // the list: every lane goes through its own pieces that reach the bound, one or two in all, and takes what does out of them
+  uint32_t pieces_left = 0;
 #pragma unroll
-      for (int v = 0; v < kVectors; ++v)
+  for (int v = 0; v < kVectors; ++v)
+    if (those_at_least<kF32>(tops[v], least)) pieces_left |= 1u << v;
+  for (; pieces_left; pieces_left &= pieces_left - 1) {
+    const int at = (__ffs(pieces_left) - 1) * kThreads + tid;
+    const uint4 u = here[at];
+    uint32_t w[4] = {u.x, u.y, u.z, u.w}, found = 0;      // bit j: the value, or the lower one, of word j; bit 16 + j: the upper one
 #pragma unroll
-        for (int i = 0; i < kPer; i += 2) {
-          const uint64_t d = add_pair(pair_of(value_in<kF32>(x[v], i), value_in<kF32>(x[v], i + 1)), less);
-          const float2 t = floats_of(fma_pair(d, hi, mul_pair(d, lo)));
-          sum2[v & 1] = add_pair(sum2[v & 1], pair_of(exp2_ftz(t.x), exp2_ftz(t.y)));
-        }
-      const float2 p = floats_of(sum2[0]), q = floats_of(sum2[1]);
-      rest = (p.x + p.y) + (q.x + q.y);
-      if (rest == rest) break;
-#pragma unroll
-      for (int v = 0; v < kVectors; ++v) without_nan<kF32>(x[v]);      // NaN among the logits: once more without them
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t is = those_at_least<kF32>(w[j], least);
+      found |= is & ((kF32 ? 0x00000001u : 0x00010001u) << j);
+      w[j] = (w[j] & ~is) | (kNone & is);
+    }
+    here[at] = make_uint4(w[0], w[1], w[2], w[3]);
+    for (; found; found &= found - 1) {
+      const int bit = __ffs(found) - 1, k = kF32 ? bit : 2 * (bit & 15) + (bit >> 4), word = kF32 ? bit : bit & 15, to = atomicAdd(&s_n, 1);
+      const uint32_t x = word & 2 ? (word & 1 ? u.w : u.z) : (word & 1 ? u.y : u.x);
+      if (to < kList) list[to] = key_of(kF32 ? __uint_as_float(x) : __uint_as_float(bit & 16 ? x & 0xffff0000u : x << 16), (v0 + at) * kPer + k);
     }
   }
-  // ---- the few threads that have something for the list, one behind the other by their warp: a lane has a word of theirs, from where it lies in L2
-  float apart = 0.f;
-  for (unsigned left = some; left;) {
-    uint32_t word[kAtOnce];
-    int token[kAtOnce];
+  __syncwarp();      // else the lanes of each way go through the sum by themselves: 3.6 times the exponentials
+  float rest;
+  for (;;) {
+    float part_of[4] = {0.f, 0.f, 0.f, 0.f};
+    if (!far) {
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k) {
-      const int piece = v0 + (lane >> 2) * kThreads + warp * 32 + (left ? __ffs(left) - 1 : 0);
-      token[k] = left && piece < v1 ? piece * kPer + (lane & 3) * (kF32 ? 1 : 2) : a.V;
-      left &= left - 1;
-      word[k] = 0;
-      if (token[k] >= a.V) continue;
-      if constexpr (kF32) word[k] = reinterpret_cast<const uint32_t*>(base)[token[k]];
-      else word[k] = reinterpret_cast<const uint16_t*>(base)[token[k]] | static_cast<uint32_t>(reinterpret_cast<const uint16_t*>(base)[min(token[k] + 1, a.V - 1)]) << 16;
-    }
+      for (int v = 0; v < kVectors; ++v) {
+        if (v >= slots) break;
+        const uint4 u = here[v * kThreads + tid];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-    for (int k = 0; k < kAtOnce; ++k)
-#pragma unroll
-      for (int i = 0; i < (kF32 ? 1 : 2); ++i) {
-        const float f = kF32 ? __uint_as_float(word[k]) : __uint_as_float(i ? word[k] & 0xffff0000u : word[k] << 16), d = f - top;
-        if (token[k] + i >= a.V) continue;
-        if (f >= least) {
-          const int at = atomicAdd(&s_n, 1);
-          if (at < kList) list[at] = key_of(f, token[k] + i);
-        } else if (f == f) apart += exp2_ftz(fmaf(d, kLog2eHi, d * kLog2eLo));
+        for (int k = 0; k < kPer; ++k) part_of[k & 3] += exp2_ftz(fmaf(value_in<kF32>(w, k), kLog2e, from));
       }
+    } else {
+#pragma unroll 1
+      for (int v = 0; v < slots; ++v) {
+        const uint4 u = here[v * kThreads + tid];
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int k = 0; k < kPer; ++k) part_of[k & 3] += exp2_ftz((value_in<kF32>(w, k) - top) * kLog2e);
+      }
+    }
+    rest = (part_of[0] + part_of[1]) + (part_of[2] + part_of[3]);
+    if (__all_sync(0xffffffffu, rest == rest)) break;
+    // NaN among the logits: once more without them
+#pragma unroll 1
+    for (int v = 0; v < slots; ++v) {
+      const uint4 u = here[v * kThreads + tid];
+      uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      without_nan<kF32>(w);
+      here[v * kThreads + tid] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
-  rest += apart;
   __syncthreads();
   int n = s_n;
-  if (n > kList) {
+  const bool slow = n > kList;
+  if (slow) {
     // ---- more than the list holds: the k-th value, bit by bit, over the logits as they lie in L2
     auto each = [&](auto what) {
 #pragma unroll 1
-      for (int piece = v0 + tid; piece < v1; piece += kThreads) {
+      for (int piece = v0 + tid; piece < v0 + count; piece += kThreads) {
         uint32_t w[4];
-        load_piece<kF32, kF32 ? 4 : 2>(base, a.V, piece, true, w);
+        load_piece<kF32, kF32 ? 4 : 2>(base, a.V, piece, w);
         without_nan<kF32>(w);
 #pragma unroll
         for (int i = 0; i < kPer; ++i) what(value_in<kF32>(w, i), piece * kPer + i);
@@ -287,33 +340,38 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, int parts, si
         const int at = atomicAdd(&s_n, 1);
         if (at < kList) list[at] = key_of(f, token);
       } else if (f == top) rest += 1.f;
-      else rest += exp2_ftz(fmaf(f - top, kLog2eHi, (f - top) * kLog2eLo));
+      else rest += exp2_ftz((f - top) * kLog2e);
     });
     __syncthreads();
     n = min(s_n, kList);
   }
-  // ---- places in the list, and the sum
-  static_assert(kList <= kThreads, "");
-  double sum = rest;
-  uint2* out = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.workspace) + entries) + (row * parts + part) * a.k;
-  for (int i = tid; i < n; i += kThreads) {
-    const unsigned long long key = list[i];
-    int place = 0;
-    for (int j = 0; j < n; ++j) place += list[j] > key;
-    if (place < a.k) out[place] = make_uint2(static_cast<uint32_t>(key), static_cast<uint32_t>(key >> 32));
-    const float f = key_value(key);
-    terms[place] = f == top ? 1.0 : exp(static_cast<double>(f) - top);
-  }
-  __syncthreads();
-  if (tid < n) sum += terms[tid];      // in the values' order, not in the list's
+  // ---- places in the list, eight threads a value, and the sum
+  double sum = rest;      // (of the slow way: relative to top itself)
 #pragma unroll
   for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) sums[warp] = sum;
+  uint2* out = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.workspace) + entries) + static_cast<size_t>(number) * a.k;
+  for (int i0 = 0; i0 < n; i0 += kThreads / 8) {
+    const int i = i0 + (tid >> 3);
+    const unsigned long long key = list[min(i, n - 1)];
+    int place = 0;
+    for (int j = tid & 7; j < n; j += 8) place += list[j] > key;
+#pragma unroll
+    for (int o = 4; o; o >>= 1) place += __shfl_xor_sync(0xffffffffu, place, o);
+    if (i < n && (tid & 7) == 0) sorted[place] = key;
+  }
   __syncthreads();
-  if (tid == 0) {
-    double all = 0.0;
-    for (int w = 0; w < kWarps; ++w) all += sums[w];
-    *head = {top, min(n, a.k), all};
+  if (warp == 0) {      // in the values' order, not in the list's
+    double all = lane < kWarps ? sums[lane] * (far || slow ? 1.0 : exp2(-(static_cast<double>(top) * kLog2e + from))) : 0.0;
+    for (int i = lane; i < n; i += 32) {
+      const unsigned long long key = sorted[i];
+      const float f = key_value(key);
+      all += f == top ? 1.0 : exp(static_cast<double>(f) - top);
+      if (i < a.k) out[i] = make_uint2(static_cast<uint32_t>(key), static_cast<uint32_t>(key >> 32));
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+    if (lane == 0) *head = {top, min(n, a.k), all};
   }
 }
 
@@ -450,10 +508,15 @@ beam_join_kernel(const __grid_constant__ b200_beam_select_args a, int parts, siz
 
 int64_t beam_select_workspace(const b200_beam_select_args& a) { return static_cast<int64_t>(geometry(a).bytes); }
 
-int beam_select(const b200_beam_select_args& a, cudaStream_t st) {
+int beam_select(const b200_beam_select_args& a, int* error, cudaStream_t st) {
   const Geometry g = geometry(a);
-  const dim3 grid(static_cast<unsigned>(a.S) * a.beams * g.parts);
-  launch_pdl(a.logits_f32 ? beam_parts_kernel<true> : beam_parts_kernel<false>, grid, dim3(kThreads), 0, st, a, g.parts, g.entries);
+  const int per = a.logits_f32 ? 4 : 8, pieces = (a.V + per - 1) / per;
+  const Cut cut = {g.parts, pieces / g.parts, pieces % g.parts};
+  const int slots = (cut.each + (cut.more > 0) + kThreads - 1) / kThreads;
+  auto kernel = a.logits_f32 ? beam_parts_kernel<true> : beam_parts_kernel<false>;
+  static std::atomic<unsigned long long> parts_done[2]{};
+  if (!ensure_dynamic_smem(kernel, kPart * 16, &parts_done[!!a.logits_f32])) return -3;
+  launch_pdl(kernel, dim3(static_cast<unsigned>(a.S) * a.beams * g.parts), dim3(kThreads), static_cast<size_t>(slots) * kThreads * 16, st, a, cut, g.entries, error);
   if (cudaGetLastError() != cudaSuccess) return -2;
   static std::atomic<unsigned long long> attr_done{0};
   if (!ensure_dynamic_smem(beam_join_kernel, kStaged * 8, &attr_done)) return -3;

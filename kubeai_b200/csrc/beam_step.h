@@ -111,7 +111,7 @@ int norm_rope_kv_write(const b200_norm_rope_args& a, cudaStream_t st);
 int64_t shared_attention_workspace(const b200_shared_attn_args& a);
 int paged_attention_shared(const b200_shared_attn_args& a, int* error, cudaStream_t st);      // error: pinned, set where a wait ran out
 int64_t beam_select_workspace(const b200_beam_select_args& a);
-int beam_select(const b200_beam_select_args& a, cudaStream_t st);
+int beam_select(const b200_beam_select_args& a, int* error, cudaStream_t st);
 int beam_reorder(const b200_beam_reorder_args& a, cudaStream_t st);
 #endif
 
