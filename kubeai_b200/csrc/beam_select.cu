@@ -4,7 +4,7 @@
 //
 // A row's best candidates by c are its best by x, which needs no rounding, so one pass over the logits takes them by x, together with the sum; c, which decides between beams, is
 // made in 64 bits for a few hundred candidates.
-// First kernel: a row is cut into parts of at most 26624 bf16 (13312 fp32) logits, a CTA each, that come into shared memory by a bulk copy, four CTAs an SM.  A lower bound of the k-th largest value that few values besides the
+// First kernel: a row is cut into parts of at most 16384 bf16 (8192 fp32) logits, a CTA each, that come into shared memory by a bulk copy, six CTAs an SM.  A lower bound of the k-th largest value that few values besides the
 // k best reach: of every warp the r-th largest of its lanes' maxima (r = k / 4), and of those the fourth largest, as four warps have r lanes each that reach it.  What does goes to a list,
 // where each one's place is the number of better ones.  Where more reach it than the list holds (rows of equal values), the k-th value and the last token that still belongs are found bit by bit over all values.
 // The sum's large terms, those of the list, are taken in 64 bits, the others in 32: what an fp32 sum loses of the large ones would decide between beams whose
@@ -26,7 +26,7 @@
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kVectors = 13, kList = 256, kPlaces = 4, kWaitLimit = 1 << 22;      // kVectors: pieces of 16 bytes of a thread; kPlaces: CTAs of an SM
+constexpr int kThreads = 256, kWarps = kThreads / 32, kVectors = 8, kList = 256, kPlaces = 6, kWaitLimit = 1 << 22;      // kVectors: pieces of 16 bytes of a thread; kPlaces: CTAs of an SM
 constexpr int kPart = kThreads * kVectors;                                            // pieces of a part at most
 constexpr int kMostParts = 64;                                                         // two of a lane in the second kernel
 static_assert(kMostParts * 4 * (kPart - 1) > beam::kMaxVocab && kWarps >= 4 && 4 * 32 >= beam::kMaxFound, "");
@@ -265,7 +265,7 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, const Cut cut
   }
   __syncwarp();      // else the lanes of each way go through the sum by themselves: 3.6 times the exponentials
   float rest;
-  for (;;) {
+  for (int again = 0;; ++again) {
     float part_of[4] = {0.f, 0.f, 0.f, 0.f};
     if (!far) {
 #pragma unroll
@@ -286,7 +286,7 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, const Cut cut
       }
     }
     rest = (part_of[0] + part_of[1]) + (part_of[2] + part_of[3]);
-    if (__all_sync(0xffffffffu, rest == rest)) break;
+    if (__all_sync(0xffffffffu, rest == rest) || again) break;
     // NaN among the logits: once more without them
 #pragma unroll 1
     for (int v = 0; v < slots; ++v) {
@@ -384,39 +384,44 @@ beam_join_kernel(const __grid_constant__ b200_beam_select_args a, int parts, siz
   __shared__ float tops[beam::kMaxBeams];
   __shared__ int count[beam::kMaxBeams], found_token[beam::kMaxFound], found_parent[beam::kMaxFound], ends_text[beam::kMaxFound];
   __shared__ float found_score[beam::kMaxFound];
+  __shared__ int places[beam::kMaxBeams][beam::kMaxFound], s_ends[beam::kMaxEnds];
   extern __shared__ unsigned long long staged[];
   __shared__ uint8_t counts[beam::kMaxBeams * kMostParts];
   const int s = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, B = a.beams, k = a.k;
   griddep_enter();
   const PartHead* heads = static_cast<const PartHead*>(a.workspace) + static_cast<size_t>(s) * B * parts;
   const uint2* lists = reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.workspace) + entries) + static_cast<size_t>(s) * B * parts * k;
-  for (int b = warp; b < B; b += kJoinThreads / 32) {      // a lane has a part
-    PartHead h[2];
-    float top = -INFINITY;
+  for (int i = tid; i < a.num_ends; i += kJoinThreads) s_ends[i] = a.ends[i];
+  for (int i = tid; i < B * k; i += kJoinThreads) places[i / k][i % k] = 0;
+  auto sums_of_rows = [&] {
+    for (int b = warp; b < B; b += kJoinThreads / 32) {      // a lane has a part
+      PartHead h[2];
+      float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int p = lane + 32 * i;
-      h[i] = p < parts ? heads[b * parts + p] : PartHead{-INFINITY, 0, 0.0};
-      if (p < parts) counts[b * parts + p] = h[i].n;
-      top = fmaxf(top, h[i].top);
+      for (int i = 0; i < 2; ++i) {
+        const int p = lane + 32 * i;
+        h[i] = p < parts ? heads[b * parts + p] : PartHead{-INFINITY, 0, 0.0};
+        if (p < parts) counts[b * parts + p] = h[i].n;
+        top = fmaxf(top, h[i].top);
+      }
+      const float score = a.scores[static_cast<size_t>(s) * B + b];
+      double sum = 0.0;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        if (h[i].top != -INFINITY) sum += h[i].top == top ? h[i].sum : h[i].sum * exp(static_cast<double>(h[i].top) - top);
+#pragma unroll
+      for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      const int n = __reduce_add_sync(0xffffffffu, h[0].n + h[1].n);
+      const bool real = score > -INFINITY;      // NaN is none
+      if (lane == 0) {
+        offset[b] = real && n ? score - log(sum) : 0.0;
+        tops[b] = top;
+        count[b] = real ? min(n, k) : 0;
+      }
     }
-    const float score = a.scores[static_cast<size_t>(s) * B + b];
-    double sum = 0.0;
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (h[i].top != -INFINITY) sum += h[i].top == top ? h[i].sum : h[i].sum * exp(static_cast<double>(h[i].top) - top);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    const int n = __reduce_add_sync(0xffffffffu, h[0].n + h[1].n);
-    const bool real = score > -INFINITY;      // NaN is none
-    if (lane == 0) {
-      offset[b] = real && n ? score - log(sum) : 0.0;
-      tops[b] = top;
-      count[b] = real ? min(n, k) : 0;
-    }
-  }
+  };
   for (int i = tid; i < beam::kMaxFound; i += kJoinThreads) {
     found_token[i] = found_parent[i] = -1;
     found_score[i] = -INFINITY;
@@ -430,6 +435,7 @@ beam_join_kernel(const __grid_constant__ b200_beam_select_args a, int parts, siz
       const uint2 x = lists[static_cast<size_t>(b0) * parts * k + e];
       staged[e] = static_cast<unsigned long long>(x.y) << 32 | x.x;      // (what lies behind a part's last is not looked at)
     }
+    if (!b0) sums_of_rows();      // under the lists' loads
     __syncthreads();
     for (int b = b0 + warp; b < b0 + some; b += kJoinThreads / 32) {
       const unsigned long long* mine = staged + static_cast<size_t>(b - b0) * parts * k;
@@ -444,8 +450,12 @@ beam_join_kernel(const __grid_constant__ b200_beam_select_args a, int parts, siz
         const bool second = first[1] > first[0];
         const unsigned long long key = second ? first[1] : first[0];
         const uint32_t hi = static_cast<uint32_t>(key >> 32), most = __reduce_max_sync(0xffffffffu, hi);
-        const uint32_t low = __reduce_max_sync(0xffffffffu, hi == most ? static_cast<uint32_t>(key) : 0u);      // (tokens are all different)
-        if (hi == most && static_cast<uint32_t>(key) == low) {
+        bool wins = hi == most;
+        if (__popc(__ballot_sync(0xffffffffu, wins)) > 1) {      // equal values: the lowest token (they are all different)
+          const uint32_t low = __reduce_max_sync(0xffffffffu, wins ? static_cast<uint32_t>(key) : 0u);
+          wins = wins && static_cast<uint32_t>(key) == low;
+        }
+        if (wins) {
           best[b][i] = key;
           const float x = value_of(most);
           c_of[b][i] = off + (x == top ? 0.0 : static_cast<double>(x) - top);
@@ -458,33 +468,31 @@ beam_join_kernel(const __grid_constant__ b200_beam_select_args a, int parts, siz
     }
   }
   __syncthreads();
-  // ---- and a request's
+  // ---- and a request's: a candidate's place is its own among its beam's, and how many of every other beam's are ahead of it
+  for (int e = tid; e < B * k * B; e += kJoinThreads) {
+    const int o = e % B, i = e / B % k, b = e / B / k;
+    if (i >= count[b] || !(c_of[b][i] > -INFINITY)) continue;
+    const double c = c_of[b][i];
+    int lo = o == b ? i : 0, hi = o == b ? i : count[o];
+    while (lo < hi) {
+      const int mid = (lo + hi) / 2;
+      const double other = c_of[o][mid];
+      if (other > c || (other == c && o < b)) lo = mid + 1;
+      else hi = mid;
+    }
+    if (lo) atomicAdd(&places[b][i], lo);
+  }
+  __syncthreads();
   for (int e = tid; e < B * k; e += kJoinThreads) {
     const int b = e / k, i = e % k;
-    if (i >= count[b]) continue;
-    const double c = c_of[b][i];
-    if (!(c > -INFINITY)) continue;
-    int place = i;
-    for (int o = 0; o < B && place < k; ++o) {
-      if (o == b) continue;
-      int lo = 0, hi = count[o];
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        const double other = c_of[o][mid];
-        if (other > c || (other == c && o < b)) lo = mid + 1;
-        else hi = mid;
-      }
-      place += lo;
-    }
-    if (place < k) {
-      const int token = key_token(best[b][i]);
-      found_token[place] = token;
-      found_parent[place] = b;
-      found_score[place] = static_cast<float>(c);
-      bool ends = false;
-      for (int x = 0; x < a.num_ends; ++x) ends = ends || a.ends[x] == token;
-      ends_text[place] = ends;
-    }
+    if (i >= count[b] || !(c_of[b][i] > -INFINITY) || places[b][i] >= k) continue;
+    const int token = key_token(best[b][i]), place = places[b][i];
+    found_token[place] = token;
+    found_parent[place] = b;
+    found_score[place] = static_cast<float>(c_of[b][i]);
+    bool ends = false;
+    for (int x = 0; x < a.num_ends; ++x) ends = ends || s_ends[x] == token;
+    ends_text[place] = ends;
   }
   __syncthreads();
   for (int i = tid; i < k; i += kJoinThreads) {
@@ -493,14 +501,24 @@ beam_join_kernel(const __grid_constant__ b200_beam_select_args a, int parts, siz
     a.found_tokens[at] = found_token[i];
     a.found_scores[at] = found_score[i];
   }
-  for (int i = tid; i < B; i += kJoinThreads) {
-    int at = 0;
-    for (int left = i; at < k; ++at)
-      if (found_parent[at] >= 0 && !ends_text[at] && left-- == 0) break;
-    const size_t to = static_cast<size_t>(s) * B + i;
-    a.parents[to] = at < k ? found_parent[at] : -1;
-    a.tokens[to] = at < k ? found_token[at] : -1;
-    a.new_scores[to] = at < k ? found_score[at] : -INFINITY;
+  if (warp == 1) {      // those that do not end go on, in order
+    const bool goes[2] = {found_parent[lane] >= 0 && !ends_text[lane], found_parent[lane + 32] >= 0 && !ends_text[lane + 32]};
+    const unsigned first = __ballot_sync(0xffffffffu, goes[0]), rest = __ballot_sync(0xffffffffu, goes[1]);
+    const int all = __popc(first) + __popc(rest);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int to = h ? __popc(first) + __popc(rest & ((1u << lane) - 1)) : __popc(first & ((1u << lane) - 1)), i = lane + 32 * h;
+      if (!goes[h] || to >= B) continue;
+      const size_t at = static_cast<size_t>(s) * B + to;
+      a.parents[at] = found_parent[i];
+      a.tokens[at] = found_token[i];
+      a.new_scores[at] = found_score[i];
+    }
+    if (lane >= all && lane < B) {
+      const size_t at = static_cast<size_t>(s) * B + lane;
+      a.parents[at] = a.tokens[at] = -1;
+      a.new_scores[at] = -INFINITY;
+    }
   }
 }
 
