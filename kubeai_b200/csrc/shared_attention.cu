@@ -4,9 +4,9 @@
 //
 // Softmax over two sets of keys is a weighted sum of softmaxes over each, so the rows of a group meet the shared pages in an item of their own and every request's rows the pages behind
 // them in another, and the two are joined by their maxima and sums.
-// An item is a key head and up to 16 rows (row = token * group + head) with a range of pages.  All items' pages one behind the other are cut into as many equal ranges as there are places for
-// warps, and a warp walks its range without a gap: it loads pages ahead by TMA (128-byte swizzle) into a ring of its own, over an item's end, and multiplies with mma.sync: a row tile of
-// 16 leaves the tensor cores idle in any form, and memory is what bounds it.  No warp waits for another.
+// An item is a key head and up to 64 rows (row = token * group + head) with a range of pages.  A team of 1, 2 or 4 warps has it, 16 rows a warp.  The CTAs are shared out to the three kinds of teams
+// by their work; all items' pages of a kind one behind the other are cut into as many equal ranges as it has teams, and a team walks its range without a gap: its first warp loads pages ahead
+// by TMA (128-byte swizzle) into the team's ring, over an item's end, and all multiply with mma.sync: row tiles of 16 leave the tensor cores idle in any form, and memory is what bounds this.
 // An item that a range's end cuts leaves unnormalised rows in the workspace, as every item does that shares its rows with another; a second kernel joins them in a fixed order.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -28,10 +28,10 @@ namespace {
 typedef __nv_bfloat16 bf16;
 using namespace shared_attn;
 constexpr int kPageBytes = 2 * 16 * kD * 2;      // bytes of a page's keys and values of a head
-constexpr int kThreads = 128, kWarps = kThreads / 32, kPlaces = 3, kDepth = 2, kItems = 4, kLeast = 4;      // kPlaces: CTAs of an SM; kDepth: pages of a warp on their way; kItems: items that those may lie in, and one; kLeast: pages of a range
+constexpr int kThreads = 128, kWarps = kThreads / 32, kPlaces = 3, kDepth = 2, kItems = 4, kLeast = 4;      // kPlaces: CTAs of an SM; kDepth: pages a warp on their way; kItems: items a warp that those may lie in, and one; kLeast: pages of a range
 constexpr int kJoinThreads = 256, kAtOnce = 4;      // kAtOnce: parts of a row on their way
 constexpr int kSmem = 1024 + kWarps * kDepth * kPageBytes;
-static_assert(kPlaces * (kSmem + 3072 + static_cast<int>(sizeof(Staged))) <= 228 * 1024, "");
+static_assert(kPlaces * (kSmem + 3584 + static_cast<int>(sizeof(Staged))) <= 228 * 1024, "");
 static_assert(kItems > kDepth, "");
 
 // An item's pages of a range, as the loads leave them for the products
@@ -40,53 +40,78 @@ struct Piece {
   int key, pages;                // first key, pages
   int end, see;                  // keys behind the last, and behind the last that token 0 sees; token i sees i more
   int table;
-  int whole, begins, own, joined;
+  int whole, begins, own, joined, last;
   int parts;
 };
 
 __global__ void __launch_bounds__(kThreads, kPlaces)
 shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ b200_shared_attn_args a, const Sizes sizes, float scale_log2, int* error) {
-  typedef Items<false> I;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[kWarps * kDepth];
-  __shared__ int sums[kWarps], s_range[kWarps + 1], s_where[kWarps + 1][4];
-  __shared__ Piece pieces[kWarps][kItems];
+  __shared__ __align__(8) uint64_t bars[2][kWarps * kDepth];
+  __shared__ int sums[kWarps], costs_sums[kWarps][3], s_range[kWarps + 1], s_where[kWarps + 1][4];
+  __shared__ Piece all_pieces[kWarps * kItems];
+  __shared__ int all_odd[kWarps * kItems];      // the last item of each piece's place with infinities or NaN among values that some row does not see
   __shared__ Staged staged;
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (sbase - smem_u32(smem_raw));
   const int warp = warp_number(), lane = threadIdx.x & 31, tid = threadIdx.x;
-  const int group = a.q_heads / a.kv_heads, bt = kNarrow / group, shift = __ffs(group) - 1;
-  const uint32_t ring = sbase + warp * kDepth * kPageBytes, full0 = smem_u32(bars + warp * kDepth);
-  if (lane == 0) {
-    for (int s = 0; s < kDepth; ++s) mbar_init(full0 + 8 * s, 1);
-    fence_mbar_init();
-    tma_prefetch_desc(&tm_kv);
-  }
+  const int group = a.q_heads / a.kv_heads, shift = __ffs(group) - 1;
+  if (tid < kWarps * kItems) all_odd[tid] = -1;
   // Behind the wide kernel, which this one needs nothing of, it begins as soon as there is room: that kernel let it in behind its own wait for what both read.  The wait that makes this
   // one's end the end of both stands at its end.
   const bool behind = sizes.ctas > 0;
   if (!behind) griddep_wait();
   griddep_launch();
   const Lengths n = lengths_of(a, &staged, tid, kThreads);
-  const int gw = blockIdx.x * kWarps + warp;
-  const tree::Ranges ranges = find_ranges<false, kThreads>(n, a.kv_heads, group, blockIdx.x * kWarps, kWarps, sizes.warps, kLeast, sums, s_range, s_where);
+  // ---- which team: CTAs by the warps' pages of each kind, one at least
+  long long costs[3];
+  costs_of<kThreads>(n, a.kv_heads, group, costs_sums, costs);
+  const int ctas = sizes.warps / kWarps;
+  int team = 1, first_cta = 0, its = ctas;
+  {
+    const long long all = costs[0] + 2 * costs[1] + 4 * costs[2];
+    int left = ctas, begin = 0;
+    for (int i = 2; i >= 0; --i) {
+      const int others = (i > 0 && costs[0] > 0) + (i > 1 && costs[1] > 0);      // kinds behind it
+      const int count = !costs[i] ? 0 : !others ? left : min(left - others, max(1, static_cast<int>((costs[i] << i) * ctas / all)));
+      if (static_cast<int>(blockIdx.x) >= begin && static_cast<int>(blockIdx.x) < begin + count) team = 1 << i, first_cta = begin, its = count;
+      begin += count;
+      left -= count;
+    }
+  }
+  const Items I(team, group);
+  const int stream = warp / team, member = warp % team, streams = kWarps / team, gs = (blockIdx.x - first_cta) * streams + stream;      // gs: the team's number among its kind
+  const int depth = kDepth * team, cap = kItems * team;
+  const uint32_t ring = sbase + stream * depth * kPageBytes, full0 = smem_u32(bars[0] + stream * depth), empty0 = smem_u32(bars[1] + stream * depth);
+  Piece* pieces = all_pieces + stream * cap;
+  volatile int* odd_item = all_odd + stream * cap;
+  if (lane == 0 && member == 0) {
+    for (int s = 0; s < depth; ++s) {
+      mbar_init(full0 + 8 * s, 1);
+      mbar_init(empty0 + 8 * s, team);
+    }
+    fence_mbar_init();
+    tma_prefetch_desc(&tm_kv);
+  }
+  const tree::Ranges ranges = find_ranges<kThreads>(n, I, a.kv_heads, (blockIdx.x - first_cta) * streams, streams, its * streams, kLeast, sums, s_range, s_where);
   __syncthreads();
-  const int left = gw < ranges.n ? s_range[warp + 1] - s_range[warp] : 0;
+  const int left = gs < ranges.n ? s_range[stream + 1] - s_range[stream] : 0;
   if (left <= 0) {
     if (behind) griddep_wait();
     return;
   }
   const Space space = space_of(a, sizes);
+  const int slot = (first_cta * kWarps + gs * team) * 2;      // of 16 rows: the range's first item, a team's tiles behind it the last
 
-  // ---- loads: item, its first page here, the range's cost to go
-  Item<false> it;
-  it.u = s_where[warp][0]; it.kvh = s_where[warp][1]; it.block = s_where[warp][2];
-  it.p = I::part(n, it.u, group);
-  it.fill(bt);
-  int t0 = max(0, s_range[warp] - s_where[warp][3] - tree::kItem), rest = left;
+  // ---- loads (the team's first warp): item, its first page here, the range's cost to go
+  Item it;
+  it.u = s_where[stream][0]; it.kvh = s_where[stream][1]; it.block = s_where[stream][2];
+  it.p = I.part(n, it.u);
+  it.fill(I);
+  int t0 = max(0, s_range[stream] - s_where[stream][3] - tree::kItem), rest = left;
   if (t0 == it.units) {              // the range begins where the item in front of it ends
     t0 = 0;
-    it.next(n, a.kv_heads, group, bt);
+    it.next(n, I, a.kv_heads);
   }
   bool more = true, ok = true;
   int take = 0, at = 0, items = 0, issued = 0, mine = 0, next = 0;      // the item's pages here, the page that is next; items so far; pages so far
@@ -116,8 +141,9 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
       x.begins = t0 == 0;
       x.own = !it.p.all;
       x.joined = it.p.k0 > 0;
-      x.parts = whole ? 0 : t0 == 0 ? ranges.parts(gw, s_range[warp + 1] - take, it.units) : 0;
-      pieces[warp][items % kItems] = x;
+      x.parts = whole ? 0 : t0 == 0 ? ranges.parts(gs, s_range[stream + 1] - take, it.units) : 0;
+      x.last = rest <= 0;
+      pieces[items % cap] = x;
     }
     ++items;
     __syncwarp();
@@ -128,13 +154,14 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
     if (at == take) {
       if (rest <= 0) { more = false; return; }
       t0 = 0;
-      it.next(n, a.kv_heads, group, bt);
+      it.next(n, I, a.kv_heads);
       begin();
     } else if (at && at % 32 == 0) {
       mine = next;
       next = look_up(t0 + at + 32 + lane);
     }
-    const int row = __shfl_sync(0xffffffffu, mine, at & 31), st = issued % kDepth;
+    const int row = __shfl_sync(0xffffffffu, mine, at & 31), st = issued & (depth - 1);
+    if (team > 1 && !(ok = warp_wait(empty0 + 8 * st, ((issued / depth) & 1) ^ 1u))) return;      // all warps of the team have read what lay there
     const uint32_t full = full0 + 8 * st, dst = ring + st * kPageBytes;
     if (one) {
       mbar_arrive_expect_tx(full, kPageBytes);
@@ -147,21 +174,26 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
     ++at;
     ++issued;
   };
-  begin();
-  for (int k = 0; k < kDepth; ++k) load();
+  if (member == 0) {
+    begin();
+    for (int k = 0; k < depth; ++k) load();
+  }
 
   // ---- products: this thread has rows g and g + 8
   const int g = lane >> 2, q2 = (lane & 3) * 2, rr = lane & 7, tile = lane >> 3;
   const uint32_t k_row = rr + (tile >> 1) * 8, k_chunk = tile & 1, v_row = rr + (tile & 1) * 8, v_chunk = tile >> 1;
   int used = 0;
-  for (int item = 0; ok && used < issued; ++item) {
-    const Piece x = pieces[warp][item % kItems];
+  for (int item = 0; ok; ++item) {
+    if (!(ok = warp_wait(full0 + 8 * (used & (depth - 1)), (used / depth) & 1))) break;      // the item's first page, and the piece in front of it
+    const Piece x = pieces[item % cap];
+    const int r0 = 16 * member;
+    const bool some = r0 < x.rows;      // this warp has rows
     // queries: rows nobody owns are zeros
     uint32_t qa[8][4];
     const bf16* q = static_cast<const bf16*>(a.q) + x.kvh * group * kD + q2;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = g + 8 * h;
+      const int r = r0 + g + 8 * h;
       const bf16* from = q + static_cast<size_t>(x.row0 + (r >> shift)) * a.ldq + (r & (group - 1)) * kD;
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
@@ -175,17 +207,17 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
 #pragma unroll
       for (int c = 0; c < 4; ++c) o[d][c] = 0.f;
     float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // what the weights are relative to, in units of log 2; this thread's part of their sum
-    const int limit[2] = {min(x.see + (g >> shift), x.end), min(x.see + ((g + 8) >> shift), x.end)};
-    bool odd = false;
+    const int limit[2] = {min(x.see + ((r0 + g) >> shift), x.end), min(x.see + ((r0 + g + 8) >> shift), x.end)};
     for (int j = 0; j < x.pages; ++j, ++used) {
-      const int st = used % kDepth, key0 = x.key + 16 * j;
-      if (!(ok = warp_wait(full0 + 8 * st, (used / kDepth) & 1))) break;
+      const int st = used & (depth - 1), key0 = x.key + 16 * j;
+      if (!(ok = warp_wait(full0 + 8 * st, (used / depth) & 1))) break;
       const uint32_t ks_ = ring + st * kPageBytes, vs_ = ks_ + 4096;
+      if (some) {
       if (key0 + 16 > x.see) {
         // what must not meet a weight of zero: values behind the last key, and infinities and NaN among values that some row does not see, which those that do add at the end
         uint4* v = reinterpret_cast<uint4*>(smem + (vs_ - sbase));
-        bool found = false;
         for (int e = lane; e < 256; e += 32) {
+          bool found;
           const int key = key0 + ((e & 127) >> 3);      // (a row's pieces in some order)
           if (key < x.see) continue;
           uint4 w = v[e];
@@ -193,11 +225,14 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
           else {
             const uint4 was = w;
             w = make_uint4(without_odd(w.x), without_odd(w.y), without_odd(w.z), without_odd(w.w));
-            found = found || w.x != was.x || w.y != was.y || w.z != was.z || w.w != was.w;
+            found = w.x != was.x || w.y != was.y || w.z != was.z || w.w != was.w;
+            if (found) {      // ahead of what another warp of the team may find without them
+              odd_item[item % cap] = item;
+              __threadfence_block();
+            }
           }
           v[e] = w;
         }
-        odd = __any_sync(0xffffffffu, found) || odd;
         fence_proxy_async();
         __syncwarp();
       }
@@ -257,12 +292,16 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
         mma_bf16_16816(o[2 * dp], pa, b0, b1);
         mma_bf16_16816(o[2 * dp + 1], pa, b2, b3);
       }
+      }
       __syncwarp();      // all have read the page
-      load();
+      if (team > 1 && lane == 0) mbar_arrive(empty0 + 8 * st);
+      if (member == 0) load();
+      if (!ok) break;
     }
     if (!ok) break;
     // ---- the item's rows
-    if (odd) {
+    __threadfence_block();
+    if (some && odd_item[item % cap] == item) {
       for (int p = max(x.see, x.key); p < min(x.end, x.key + 16 * x.pages); ++p) {
         const long long row = tree::cache_row(a.block_tables + static_cast<size_t>(x.table) * a.ld_tables, p, a.num_pages);
         if (row < 0) continue;
@@ -281,14 +320,13 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     }
-    if (x.begins) {
-      const int tokens = x.rows >> shift;
-      if (lane < tokens) space.places[(static_cast<size_t>(x.own) * a.T + x.row0 + lane) * a.kv_heads + x.kvh] = {2 * gw + 1, x.parts, lane << shift, x.joined ? kJoined : 0};
-    }
+    if (x.begins && member == 0)
+      for (int i = lane; i < x.rows >> shift; i += 32)
+        space.places[(static_cast<size_t>(x.own) * a.T + x.row0 + i) * a.kv_heads + x.kvh] = {slot + team, x.parts, i << shift, kTeam * team + (x.joined ? kJoined : 0)};
     const bool last = x.whole && x.own && !x.joined;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int r = g + 8 * h;
+      const int r = r0 + g + 8 * h;
       if (r >= x.rows) continue;
       const size_t t = static_cast<size_t>(x.row0 + (r >> shift));
       const int head = x.kvh * group + (r & (group - 1));
@@ -298,15 +336,16 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
 #pragma unroll
         for (int d = 0; d < 16; ++d) *reinterpret_cast<uint32_t*>(out + d * 8) = pack_bf16x2(o[d][2 * h] * inv, o[d][2 * h + 1] * inv);
       } else {
-        float* out = x.whole ? space.rows + ((static_cast<size_t>(x.own) * a.T + t) * a.q_heads + head) * kLd : space.narrow + (static_cast<size_t>(2 * gw + x.begins) * kNarrow + r) * kLd;
+        float* out = x.whole ? space.rows + ((static_cast<size_t>(x.own) * a.T + t) * a.q_heads + head) * kLd : space.narrow + (static_cast<size_t>(slot + (x.begins ? team : 0)) * kTile16 + r) * kLd;
 #pragma unroll
         for (int d = 0; d < 16; ++d) *reinterpret_cast<float2*>(out + d * 8 + q2) = make_float2(o[d][2 * h], o[d][2 * h + 1]);
         if ((lane & 3) == 0) *reinterpret_cast<float2*>(out + kD) = make_float2(ref[h], l[h]);
       }
     }
+    if (x.last) break;
   }
   // the copies in flight land before the CTA ends, also where it gives up
-  for (int k = used; k < issued; ++k) warp_wait(full0 + 8 * (k % kDepth), (k / kDepth) & 1);
+  for (int k = used; k < issued; ++k) warp_wait(full0 + 8 * (k & (depth - 1)), (k / depth) & 1);
   if (!ok) *reinterpret_cast<volatile int*>(error) = 1;
   if (behind) griddep_wait();
 }
@@ -380,8 +419,8 @@ shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const S
     const bool first = p < n_own;
     const int k = first ? p : p - n_own, parts = first ? own.parts : shared.parts, slot = first ? own.slot : shared.slot, row = first ? own.row : shared.row;
     if (!parts) return space.rows + ((static_cast<size_t>(first) * a.T + t) * a.q_heads + head) * kLd;
-    const bool wide = (first ? own.flags : shared.flags) & kWide;
-    return (wide ? space.wide : space.narrow) + (static_cast<size_t>(k ? slot - 1 + 2 * k : slot) * (wide ? kWideRows : kNarrow) + row + head % group) * kLd;
+    const int team = (first ? own.flags : shared.flags) / kTeam, behind = max(1, team);      // from a range's second slot to its first, and half of what lies between two ranges
+    return (team ? space.narrow : space.wide) + (static_cast<size_t>(k ? slot - behind + 2 * behind * k : slot) * (team ? kTile16 : kWideRows) + row + head % group) * kLd;
   };
   *out = join_row(n_all, part, lane);
 }
@@ -394,7 +433,7 @@ int64_t shared_attention_workspace(const b200_shared_attn_args& a) {
   const Sizes n = sizes_of(a);
   const int64_t T = a.T;
   return 2 * T * a.kv_heads * static_cast<int64_t>(sizeof(Place)) +
-         (2ll * n.warps * kNarrow + 2ll * n.ctas * kWideRows + (a.G ? 2 * T * a.q_heads : 0)) * kLd * static_cast<int64_t>(sizeof(float));
+         (2ll * n.warps * kTile16 + 2ll * n.ctas * kWideRows + (a.G ? 2 * T * a.q_heads : 0)) * kLd * static_cast<int64_t>(sizeof(float));
 }
 
 int paged_attention_shared(const b200_shared_attn_args& a, int* error, cudaStream_t st) {

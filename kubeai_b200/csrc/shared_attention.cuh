@@ -11,7 +11,7 @@ namespace shared_attn {
 
 using beam::Lengths;
 using beam::Part;
-constexpr int kD = 128, kNarrow = 16;      // kNarrow: rows (token * group + head) of a part that go to the narrow kernel, whose row tile that is
+constexpr int kD = 128, kTile16 = 16, kNarrow = 64;      // kNarrow: rows (token * group + head) of a part that go to the narrow kernel, whose warps have tiles of 16
 constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
 constexpr int kWaitLimit = 1 << 22;
 
@@ -21,14 +21,14 @@ __device__ __forceinline__ uint32_t without_odd(uint32_t u) { return ((u & 0x7f8
 
 // Where the rows of a token and key head are: their own keys' part, and what their group shares.
 struct Place {
-  int slot, parts;      // parts 0: in the rows of all (or in the output), else in the slots of `parts` ranges, slot the first
+  int slot, parts;      // parts 0: in the rows of all (or in the output), else in the slots of `parts` ranges, slot the first: of kWideRows rows, or of 16 and a team's tiles
   int row;              // the token's first row there
   int flags;
 };
-constexpr int kJoined = 1, kWide = 2;      // own rows: the group's are to be added; the slots are the wide kernel's
+constexpr int kJoined = 1, kTeam = 4;      // own rows: the group's are to be added; times the team of the narrow kernel, 0 for the wide one
 struct Space {
   Place* places;        // [2][T][kv_heads]: the groups', the requests' own
-  float* narrow;        // [warps][2][16][kLd]: a range's first item, which another range began, and its last
+  float* narrow;        // [warps][2][16][kLd], a team's warps together: a range's first item, which another range began, and its last
   float* wide;          // [CTAs][2][kWideRows][kLd], the same
   float* rows;          // [2][T][q_heads][kLd]
 };
@@ -40,7 +40,7 @@ __host__ __device__ inline Space space_of(const b200_shared_attn_args& a, const 
   Space s;
   s.places = static_cast<Place*>(a.workspace);
   s.narrow = reinterpret_cast<float*>(s.places + 2ll * a.T * a.kv_heads);
-  s.wide = s.narrow + static_cast<long long>(n.warps) * 2 * kNarrow * kLd;
+  s.wide = s.narrow + static_cast<long long>(n.warps) * 2 * kTile16 * kLd;
   s.rows = s.wide + static_cast<long long>(n.ctas) * 2 * kWideRows * kLd;
   return s;
 }
@@ -72,68 +72,93 @@ __device__ __forceinline__ Lengths lengths_of(const b200_shared_attn_args& a, St
   return n;
 }
 
-// ---- items: a part's key head and a block of its rows.  Its keys come in units: pages, or steps of the wide kernel, which has two tiles of 128 scores at once: those of two row tiles and 128 keys
-// where there are more than 128 rows, else of one row tile and 256 keys.
-template <bool kIsWide>
+// ---- items: a part's key head and a block of its rows.  Parts of up to 64 rows go to the narrow kernel, to teams of 1, 2 or 4 warps with 16 rows each; the others (team 0) to the wide one, 256 rows
+// a block.  An item's keys come in units: pages, or steps of the wide kernel, which has two tiles of 128 scores at once: those of two row tiles and 128 keys where there are more than 128 rows, else of
+// one row tile and 256 keys.
+__device__ __forceinline__ int team_of(int rows) { return rows <= kTile16 ? 1 : rows <= 2 * kTile16 ? 2 : rows <= kNarrow ? 4 : 0; }
 struct Items {
-  static constexpr int kRows = kIsWide ? kWideRows : kNarrow;
-  // part u, without rows where it is the other kernel's
-  static __device__ __forceinline__ Part part(const Lengths& n, int u, int group) {
+  int team, group, bt;      // bt: tokens of a block
+  __device__ __forceinline__ Items(int team, int group) : team(team), group(group), bt((team ? kTile16 * team : kWideRows) / group) {}
+  // part u, without rows where it is another team's
+  __device__ __forceinline__ Part part(const Lengths& n, int u) const {
     Part p = beam::part_of(n, u);
-    if ((p.rows * group > kNarrow) != kIsWide) p.rows = 0;
+    if (team_of(p.rows * group) != team) p.rows = 0;
     return p;
   }
-  static __device__ __forceinline__ int tokens_of(const Part& p, int bt, int block) { return min(bt, p.rows - block * bt); }
-  static __device__ __forceinline__ int unit_of(int tokens, int bt) { return !kIsWide ? 16 : 2 * tokens > bt ? 128 : 256; }
-  static __device__ __forceinline__ int end_of(const Part& p, int bt, int block) { return p.all ? p.k1 : p.ctx + min(p.rows, (block + 1) * bt); }
-  static __device__ __forceinline__ int units_of(const Part& p, int bt, int block) {
-    const int unit = unit_of(tokens_of(p, bt, block), bt);
-    return (end_of(p, bt, block) - p.k0 + unit - 1) / unit;
+  __device__ __forceinline__ int unit_of(int tokens) const { return team ? 16 : 2 * tokens > bt ? 128 : 256; }
+  __device__ __forceinline__ int end_of(const Part& p, int block) const { return p.all ? p.k1 : p.ctx + min(p.rows, (block + 1) * bt); }
+  __device__ __forceinline__ int units_of(const Part& p, int block) const {
+    const int unit = unit_of(min(bt, p.rows - block * bt));
+    return (end_of(p, block) - p.k0 + unit - 1) / unit;
   }
-  static __device__ __forceinline__ int blocks_of(const Part& p, int bt) { return (p.rows + bt - 1) / bt; }
-  static __device__ __forceinline__ int head_cost(const Part& p, int bt) {
-    const int blocks = blocks_of(p, bt);
-    if (blocks <= 1) return blocks ? units_of(p, bt, 0) + tree::kItem : 0;
-    int n = units_of(p, bt, blocks - 1) + tree::kItem;      // (the last block may be of the other unit)
-    if (p.all) return n + (blocks - 1) * (units_of(p, bt, 0) + tree::kItem);
-    for (int b = 0; b < blocks - 1; ++b) n += units_of(p, bt, b) + tree::kItem;
+  __device__ __forceinline__ int blocks_of(const Part& p) const { return (p.rows + bt - 1) / bt; }
+  __device__ __forceinline__ int head_cost(const Part& p) const {
+    const int blocks = blocks_of(p);
+    if (blocks <= 1) return blocks ? units_of(p, 0) + tree::kItem : 0;
+    int n = units_of(p, blocks - 1) + tree::kItem;      // (the last block may be of the other unit)
+    if (p.all) return n + (blocks - 1) * (units_of(p, 0) + tree::kItem);
+    for (int b = 0; b < blocks - 1; ++b) n += units_of(p, b) + tree::kItem;
     return n;
   }
 };
-template <bool kIsWide>
 struct Item {
-  typedef Items<kIsWide> I;
   int u, kvh, block;
   Part p;
   int first, nb, k1, units;      // the block's tokens, the keys they may see
-  __device__ __forceinline__ void fill(int bt) {
-    first = block * bt;
-    nb = min(bt, p.rows - first);
-    k1 = I::end_of(p, bt, block);
-    units = I::units_of(p, bt, block);
+  __device__ __forceinline__ void fill(const Items& I) {
+    first = block * I.bt;
+    nb = min(I.bt, p.rows - first);
+    k1 = I.end_of(p, block);
+    units = I.units_of(p, block);
   }
-  __device__ __forceinline__ void next(const Lengths& n, int kv_heads, int group, int bt) {
-    if (++block >= I::blocks_of(p, bt)) {      // a head's blocks come one behind the other: CTAs side by side read the same pages
+  __device__ __forceinline__ void next(const Lengths& n, const Items& I, int kv_heads) {
+    if (++block >= I.blocks_of(p)) {      // a head's blocks come one behind the other: CTAs side by side read the same pages
       block = 0;
       if (++kvh >= kv_heads) {
         kvh = 0;
-        do p = I::part(n, ++u, group);
+        do p = I.part(n, ++u);
         while (p.rows == 0);      // (a range's units are some part's: the walk ends in front of the last)
       }
     }
-    fill(bt);
+    fill(I);
   }
 };
 
+// The cost of all items of each of three teams (1, 2, 4), to every thread; with barriers
+template <int kThreads>
+__device__ __forceinline__ void costs_of(const Lengths& n, int kv_heads, int group, int (*sums)[3], long long* costs) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  int mine[3] = {0, 0, 0};
+  for (int u = tid; u < n.G + n.S; u += kThreads) {
+    const Part p = beam::part_of(n, u);
+    const int team = team_of(p.rows * group);
+    if (!p.rows || !team) continue;
+    const int cost = Items(team, group).head_cost(p) * kv_heads;
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+      if (team == 1 << i) mine[i] += cost;
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    mine[i] = __reduce_add_sync(0xffffffffu, mine[i]);
+    if (lane == 0) sums[warp][i] = mine[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {
+    costs[i] = 0;
+    for (int w = 0; w < kThreads / 32; ++w) costs[i] += sums[w][i];
+  }
+}
+
 // Where `count` ranges from range `first` on begin and end: every thread sums some parts of the step, one behind the other, and the sums of the threads in front of it.  range
 // [count + 1], where [count + 1][4]: part, key head, block, and the first unit of the item that a range begins in.  No range has less than `least` units.  Returns all ranges; to be followed by a barrier.
-template <bool kIsWide, int kThreads>
-__device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, int kv_heads, int group, int first, int count, int most, int least, int* sums, int* range, int (*where)[4]) {
-  typedef Items<kIsWide> I;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, bt = I::kRows / group;
+template <int kThreads>
+__device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, const Items& I, int kv_heads, int first, int count, int most, int least, int* sums, int* range, int (*where)[4]) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int U = n.G + n.S, per = (U + kThreads - 1) / kThreads, u_begin = min(U, tid * per), u_end = min(U, u_begin + per);
   int before = 0, N = 0;
-  for (int u = u_begin; u < u_end; ++u) before += I::head_cost(I::part(n, u, group), bt) * kv_heads;
+  for (int u = u_begin; u < u_end; ++u) before += I.head_cost(I.part(n, u)) * kv_heads;
   const int own = before;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -156,14 +181,14 @@ __device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, int kv_hea
     const int b_end = ranges.at(min(first + count, ranges.n - 1));
     if (own && ranges.at(first) < before + own && b_end >= before)
       for (int u = u_begin; u < u_end; ++u) {
-        const Part p = I::part(n, u, group);
-        const int head = I::head_cost(p, bt), mine = head * kv_heads;
+        const Part p = I.part(n, u);
+        const int head = I.head_cost(p), mine = head * kv_heads;
         for (int e = 0; e <= count && first + e < ranges.n; ++e) {
           const int b = ranges.at(first + e);
           if (mine == 0 || b < before || b >= before + mine) continue;
           const int kvh = (b - before) / head;
-          int g0 = before + kvh * head, block = 0, units = I::units_of(p, bt, 0);
-          while (b >= g0 + units + tree::kItem) g0 += units + tree::kItem, units = I::units_of(p, bt, ++block);
+          int g0 = before + kvh * head, block = 0, units = I.units_of(p, 0);
+          while (b >= g0 + units + tree::kItem) g0 += units + tree::kItem, units = I.units_of(p, ++block);
           range[e] = tree::snapped(b, g0, units, ranges.snap);
           where[e][0] = u; where[e][1] = kvh; where[e][2] = block; where[e][3] = g0;
         }

@@ -32,7 +32,6 @@ namespace {
 
 typedef __nv_bfloat16 bf16;
 using namespace shared_attn;
-typedef Items<true> I;
 constexpr int kTileRows = 128, kKeys = 128;                         // of a tile of scores
 constexpr int kSlab = 128 * 128, kTile = 2 * kSlab;                 // bytes: 64 columns of 128 rows, a tile
 constexpr int kThreads = 384, kWarps = kThreads / 32, kRing = 4;    // warps 0 to 3 and 4 to 7: softmax, 8: loads, 9: products; kRing: tiles of keys and values
@@ -235,7 +234,8 @@ shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   griddep_enter();
   const int cta = blockIdx.x, group = a.q_heads / a.kv_heads, shift = __ffs(group) - 1;
   const Lengths n = lengths_of(a, &staged, tid, kThreads);
-  const tree::Ranges ranges = find_ranges<true, kThreads>(n, a.kv_heads, group, cta, 1, sizes.ctas, kLeast, sums, s_range, s_where);
+  const Items I(0, group);
+  const tree::Ranges ranges = find_ranges<kThreads>(n, I, a.kv_heads, cta, 1, sizes.ctas, kLeast, sums, s_range, s_where);
   bool ok = true;
   tc_fence_before();
   __syncthreads();
@@ -250,15 +250,15 @@ shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     if (some_work && warp == 8) {
       // ------------------------------------------------------------ loads
       const bool one = elect_one();
-      const int bt = kWideRows / group;
-      Item<true> it;
+      const int bt = I.bt;
+      Item it;
       it.u = s_where[0][0]; it.kvh = s_where[0][1]; it.block = s_where[0][2];
-      it.p = I::part(n, it.u, group);
-      it.fill(bt);
+      it.p = I.part(n, it.u);
+      it.fill(I);
       int t0 = max(0, s_range[0] - s_where[0][3] - tree::kItem), rest = s_range[1] - s_range[0];
       if (t0 == it.units) {      // the range begins where the item in front of it ends
         t0 = 0;
-        it.next(n, a.kv_heads, group, bt);
+        it.next(n, I, a.kv_heads);
       }
       Space space = space_of(a, sizes);
       int seq = 0, item = 0, queries = 0;      // tiles issued, items, items whose queries are on their way
@@ -334,13 +334,13 @@ shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
         }
         if (!ok) break;
         if (t0 == 0) {      // where the item's rows are: their tokens', 32 at a time
-          const int parts = whole ? 0 : ranges.parts(cta, s_range[1] - take, it.units), flags = kWide | (it.p.k0 > 0 ? kJoined : 0);
+          const int parts = whole ? 0 : ranges.parts(cta, s_range[1] - take, it.units), flags = it.p.k0 > 0 ? kJoined : 0;
           for (int i = lane; i < it.nb; i += 32)
             space.places[(static_cast<size_t>(!it.p.all) * a.T + row0 + i) * a.kv_heads + it.kvh] = {2 * cta + 1, parts, i << shift, flags};
         }
         if (rest <= 0) break;
         t0 = 0;
-        it.next(n, a.kv_heads, group, bt);
+        it.next(n, I, a.kv_heads);
       }
       // the copies in flight land before the CTA ends, also where it gives up
       if (queries) warp_wait(q_full, (queries - 1) & 1);
