@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(kThreads, kPlaces)
 shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ b200_shared_attn_args a, const Sizes sizes, float scale_log2, int* error) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[2][kWarps * kDepth];
-  __shared__ int sums[kWarps], costs_sums[kWarps][3], s_range[kWarps + 1], s_where[kWarps + 1][4];
+  __shared__ int sums[kWarps][3], s_range[kWarps + 1], s_where[kWarps + 1][4];
   __shared__ Piece all_pieces[kWarps * kItems];
   __shared__ int all_odd[kWarps * kItems];      // the last item of each piece's place with infinities or NaN among values that some row does not see
   __shared__ Staged staged;
@@ -64,24 +64,27 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
   griddep_launch();
   const Lengths n = lengths_of(a, &staged, tid, kThreads);
   // ---- which team: CTAs by the warps' pages of each kind, one at least
-  long long costs[3];
-  costs_of<kThreads>(n, a.kv_heads, group, costs_sums, costs);
+  Costs<3> costs;
+  find_costs<3, kThreads>(n, a.kv_heads, group, sums, &costs);
   const int ctas = sizes.warps / kWarps;
-  int team = 1, first_cta = 0, its = ctas;
+  int kind = 0, first_cta = 0, its = ctas;
   {
-    const long long all = costs[0] + 2 * costs[1] + 4 * costs[2];
+    const long long all = costs.all[0] + 2ll * costs.all[1] + 4ll * costs.all[2];
     int left = ctas, begin = 0;
+#pragma unroll
     for (int i = 2; i >= 0; --i) {
-      const int others = (i > 0 && costs[0] > 0) + (i > 1 && costs[1] > 0);      // kinds behind it
-      const int count = !costs[i] ? 0 : !others ? left : min(left - others, max(1, static_cast<int>((costs[i] << i) * ctas / all)));
-      if (static_cast<int>(blockIdx.x) >= begin && static_cast<int>(blockIdx.x) < begin + count) team = 1 << i, first_cta = begin, its = count;
+      const int others = (i > 0 && costs.all[0] > 0) + (i > 1 && costs.all[1] > 0);      // kinds behind it
+      const int count = !costs.all[i] ? 0 : !others ? left : min(left - others, max(1, static_cast<int>(static_cast<float>(costs.all[i]) * (1 << i) * ctas / static_cast<float>(all))));
+      if (static_cast<int>(blockIdx.x) >= begin && static_cast<int>(blockIdx.x) < begin + count) kind = i, first_cta = begin, its = count;
       begin += count;
       left -= count;
     }
   }
+  const int team = 1 << kind;
   const Items I(team, group);
-  const int stream = warp / team, member = warp % team, streams = kWarps / team, gs = (blockIdx.x - first_cta) * streams + stream;      // gs: the team's number among its kind
-  const int depth = kDepth * team, cap = kItems * team;
+  const int stream = warp >> kind, member = warp & (team - 1), streams = kWarps >> kind, gs = (blockIdx.x - first_cta) * streams + stream;      // gs: the team's number among its kind
+  static_assert(kDepth == 2, "");
+  const int depth = kDepth * team, depth_log = kind + 1, cap = kItems * team;
   const uint32_t ring = sbase + stream * depth * kPageBytes, full0 = smem_u32(bars[0] + stream * depth), empty0 = smem_u32(bars[1] + stream * depth);
   Piece* pieces = all_pieces + stream * cap;
   volatile int* odd_item = all_odd + stream * cap;
@@ -93,7 +96,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
     fence_mbar_init();
     tma_prefetch_desc(&tm_kv);
   }
-  const tree::Ranges ranges = find_ranges<kThreads>(n, I, a.kv_heads, (blockIdx.x - first_cta) * streams, streams, its * streams, kLeast, sums, s_range, s_where);
+  const tree::Ranges ranges = find_ranges<3>(n, I, costs, kind, a.kv_heads, (blockIdx.x - first_cta) * streams, streams, its * streams, kLeast, s_range, s_where);
   __syncthreads();
   const int left = gs < ranges.n ? s_range[stream + 1] - s_range[stream] : 0;
   if (left <= 0) {
@@ -143,7 +146,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
       x.joined = it.p.k0 > 0;
       x.parts = whole ? 0 : t0 == 0 ? ranges.parts(gs, s_range[stream + 1] - take, it.units) : 0;
       x.last = rest <= 0;
-      pieces[items % cap] = x;
+      pieces[items & (cap - 1)] = x;
     }
     ++items;
     __syncwarp();
@@ -161,7 +164,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
       next = look_up(t0 + at + 32 + lane);
     }
     const int row = __shfl_sync(0xffffffffu, mine, at & 31), st = issued & (depth - 1);
-    if (team > 1 && !(ok = warp_wait(empty0 + 8 * st, ((issued / depth) & 1) ^ 1u))) return;      // all warps of the team have read what lay there
+    if (team > 1 && !(ok = warp_wait(empty0 + 8 * st, ((issued >> depth_log) & 1) ^ 1u))) return;      // all warps of the team have read what lay there
     const uint32_t full = full0 + 8 * st, dst = ring + st * kPageBytes;
     if (one) {
       mbar_arrive_expect_tx(full, kPageBytes);
@@ -184,8 +187,8 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
   const uint32_t k_row = rr + (tile >> 1) * 8, k_chunk = tile & 1, v_row = rr + (tile & 1) * 8, v_chunk = tile >> 1;
   int used = 0;
   for (int item = 0; ok; ++item) {
-    if (!(ok = warp_wait(full0 + 8 * (used & (depth - 1)), (used / depth) & 1))) break;      // the item's first page, and the piece in front of it
-    const Piece x = pieces[item % cap];
+    if (!(ok = warp_wait(full0 + 8 * (used & (depth - 1)), (used >> depth_log) & 1))) break;      // the item's first page, and the piece in front of it
+    const Piece x = pieces[item & (cap - 1)];
     const int r0 = 16 * member;
     const bool some = r0 < x.rows;      // this warp has rows
     // queries: rows nobody owns are zeros
@@ -210,7 +213,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
     const int limit[2] = {min(x.see + ((r0 + g) >> shift), x.end), min(x.see + ((r0 + g + 8) >> shift), x.end)};
     for (int j = 0; j < x.pages; ++j, ++used) {
       const int st = used & (depth - 1), key0 = x.key + 16 * j;
-      if (!(ok = warp_wait(full0 + 8 * st, (used / depth) & 1))) break;
+      if (!(ok = warp_wait(full0 + 8 * st, (used >> depth_log) & 1))) break;
       const uint32_t ks_ = ring + st * kPageBytes, vs_ = ks_ + 4096;
       if (some) {
       if (key0 + 16 > x.see) {
@@ -227,7 +230,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
             w = make_uint4(without_odd(w.x), without_odd(w.y), without_odd(w.z), without_odd(w.w));
             found = w.x != was.x || w.y != was.y || w.z != was.z || w.w != was.w;
             if (found) {      // ahead of what another warp of the team may find without them
-              odd_item[item % cap] = item;
+              odd_item[item & (cap - 1)] = item;
               __threadfence_block();
             }
           }
@@ -301,7 +304,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
     if (!ok) break;
     // ---- the item's rows
     __threadfence_block();
-    if (some && odd_item[item % cap] == item) {
+    if (some && odd_item[item & (cap - 1)] == item) {
       for (int p = max(x.see, x.key); p < min(x.end, x.key + 16 * x.pages); ++p) {
         const long long row = tree::cache_row(a.block_tables + static_cast<size_t>(x.table) * a.ld_tables, p, a.num_pages);
         if (row < 0) continue;
@@ -345,7 +348,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
     if (x.last) break;
   }
   // the copies in flight land before the CTA ends, also where it gives up
-  for (int k = used; k < issued; ++k) warp_wait(full0 + 8 * (k & (depth - 1)), (k / depth) & 1);
+  for (int k = used; k < issued; ++k) warp_wait(full0 + 8 * (k & (depth - 1)), (k >> depth_log) & 1);
   if (!ok) *reinterpret_cast<volatile int*>(error) = 1;
   if (behind) griddep_wait();
 }

@@ -77,21 +77,23 @@ __device__ __forceinline__ Lengths lengths_of(const b200_shared_attn_args& a, St
 // one row tile and 256 keys.
 __device__ __forceinline__ int team_of(int rows) { return rows <= kTile16 ? 1 : rows <= 2 * kTile16 ? 2 : rows <= kNarrow ? 4 : 0; }
 struct Items {
-  int team, group, bt;      // bt: tokens of a block
-  __device__ __forceinline__ Items(int team, int group) : team(team), group(group), bt((team ? kTile16 * team : kWideRows) / group) {}
+  int team, group, bt, bt_log;      // bt: tokens of a block, a power of two
+  __device__ __forceinline__ Items(int team, int group) : team(team), group(group), bt_log((team ? 4 + (team > 1) + (team > 2) : 8) - (group > 1) - (group > 2) - (group > 4)) { bt = 1 << bt_log; }
+  // whether a part of so many rows is this team's
+  __device__ __forceinline__ bool has(const Part& p) const { return p.rows && team_of(p.rows * group) == team; }
   // part u, without rows where it is another team's
   __device__ __forceinline__ Part part(const Lengths& n, int u) const {
     Part p = beam::part_of(n, u);
-    if (team_of(p.rows * group) != team) p.rows = 0;
+    if (!has(p)) p.rows = 0;
     return p;
   }
-  __device__ __forceinline__ int unit_of(int tokens) const { return team ? 16 : 2 * tokens > bt ? 128 : 256; }
-  __device__ __forceinline__ int end_of(const Part& p, int block) const { return p.all ? p.k1 : p.ctx + min(p.rows, (block + 1) * bt); }
+  __device__ __forceinline__ int unit_log(int tokens) const { return team ? 4 : 2 * tokens > bt ? 7 : 8; }
+  __device__ __forceinline__ int end_of(const Part& p, int block) const { return p.all ? p.k1 : p.ctx + min(p.rows, (block + 1) << bt_log); }
   __device__ __forceinline__ int units_of(const Part& p, int block) const {
-    const int unit = unit_of(min(bt, p.rows - block * bt));
-    return (end_of(p, block) - p.k0 + unit - 1) / unit;
+    const int log = unit_log(min(bt, p.rows - (block << bt_log)));
+    return (end_of(p, block) - p.k0 + (1 << log) - 1) >> log;
   }
-  __device__ __forceinline__ int blocks_of(const Part& p) const { return (p.rows + bt - 1) / bt; }
+  __device__ __forceinline__ int blocks_of(const Part& p) const { return (p.rows + bt - 1) >> bt_log; }
   __device__ __forceinline__ int head_cost(const Part& p) const {
     const int blocks = blocks_of(p);
     if (blocks <= 1) return blocks ? units_of(p, 0) + tree::kItem : 0;
@@ -106,7 +108,7 @@ struct Item {
   Part p;
   int first, nb, k1, units;      // the block's tokens, the keys they may see
   __device__ __forceinline__ void fill(const Items& I) {
-    first = block * I.bt;
+    first = block << I.bt_log;
     nb = min(I.bt, p.rows - first);
     k1 = I.end_of(p, block);
     units = I.units_of(p, block);
@@ -124,76 +126,84 @@ struct Item {
   }
 };
 
-// The cost of all items of each of three teams (1, 2, 4), to every thread; with barriers
-template <int kThreads>
-__device__ __forceinline__ void costs_of(const Lengths& n, int kv_heads, int group, int (*sums)[3], long long* costs) {
+// Every thread's share of the step's parts, one behind the other, and what the items of each kind cost: its own, in front of it, and in all.  Kinds: the teams of 1, 2 and 4 warps, or the wide kernel's.
+template <int kKinds>
+struct Costs {
+  int u_begin, u_end;
+  Part first;      // the first part of the share
+  int own[kKinds], before[kKinds], all[kKinds];
+};
+template <int kKinds>
+__device__ __forceinline__ int kind_team(int kind) { return kKinds == 1 ? 0 : 1 << kind; }
+// ... with one barrier
+template <int kKinds, int kThreads>
+__device__ __forceinline__ void find_costs(const Lengths& n, int kv_heads, int group, int (*sums)[kKinds], Costs<kKinds>* c) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  int mine[3] = {0, 0, 0};
-  for (int u = tid; u < n.G + n.S; u += kThreads) {
-    const Part p = beam::part_of(n, u);
-    const int team = team_of(p.rows * group);
-    if (!p.rows || !team) continue;
-    const int cost = Items(team, group).head_cost(p) * kv_heads;
+  const int U = n.G + n.S, per = (U + kThreads - 1) / kThreads;
+  c->u_begin = min(U, tid * per);
+  c->u_end = min(U, c->u_begin + per);
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
-      if (team == 1 << i) mine[i] += cost;
+  for (int i = 0; i < kKinds; ++i) c->own[i] = 0;
+  for (int u = c->u_end - 1; u >= c->u_begin; --u) {
+    c->first = beam::part_of(n, u);
+#pragma unroll
+    for (int i = 0; i < kKinds; ++i) {
+      const Items I(kind_team<kKinds>(i), group);
+      if (I.has(c->first)) c->own[i] += I.head_cost(c->first) * kv_heads;
+    }
   }
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    mine[i] = __reduce_add_sync(0xffffffffu, mine[i]);
-    if (lane == 0) sums[warp][i] = mine[i];
+  for (int i = 0; i < kKinds; ++i) {
+    int x = c->own[i];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) sums[warp][i] = x;
+    c->before[i] = x - c->own[i];
+    c->all[i] = 0;
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 3; ++i) {
-    costs[i] = 0;
-    for (int w = 0; w < kThreads / 32; ++w) costs[i] += sums[w][i];
-  }
+  for (int w = 0; w < kThreads / 32; ++w)
+#pragma unroll
+    for (int i = 0; i < kKinds; ++i) {
+      const int x = sums[w][i];
+      if (w < warp) c->before[i] += x;
+      c->all[i] += x;
+    }
 }
 
-// Where `count` ranges from range `first` on begin and end: every thread sums some parts of the step, one behind the other, and the sums of the threads in front of it.  range
-// [count + 1], where [count + 1][4]: part, key head, block, and the first unit of the item that a range begins in.  No range has less than `least` units.  Returns all ranges; to be followed by a barrier.
-template <int kThreads>
-__device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, const Items& I, int kv_heads, int first, int count, int most, int least, int* sums, int* range, int (*where)[4]) {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int U = n.G + n.S, per = (U + kThreads - 1) / kThreads, u_begin = min(U, tid * per), u_end = min(U, u_begin + per);
-  int before = 0, N = 0;
-  for (int u = u_begin; u < u_end; ++u) before += I.head_cost(I.part(n, u)) * kv_heads;
-  const int own = before;
+// Where `count` ranges from range `first` on begin and end, of at most `most` that the items of a kind are cut into, none with less than `least` units.  range [count + 1], where
+// [count + 1][4]: part, key head, block, and the first unit of the item that a range begins in.  Returns all ranges; to be followed by a barrier.
+template <int kKinds>
+__device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, const Items& I, const Costs<kKinds>& c, int kind, int kv_heads, int first, int count, int most, int least, int* range, int (*where)[4]) {
+  const int tid = threadIdx.x;
+  int N = c.all[0], before = c.before[0], own = c.own[0];
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, before, o);
-    if (lane >= o) before += y;
-  }
-  if (lane == 31) sums[warp] = before;
-  __syncthreads();
-  before -= own;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    const int x = sums[w];
-    if (w < warp) before += x;
-    N += x;
-  }
+  for (int i = 1; i < kKinds; ++i)
+    if (i == kind) N = c.all[i], before = c.before[i], own = c.own[i];
   tree::Ranges ranges = tree::ranges_of(N, max(1, min(most, N / least)));
   if (N == 0) ranges.n = 0;
   if (tid <= count && first + tid >= ranges.n) range[tid] = N;      // which lies in no item
-  if (first < ranges.n) {
-    const int b_end = ranges.at(min(first + count, ranges.n - 1));
-    if (own && ranges.at(first) < before + own && b_end >= before)
-      for (int u = u_begin; u < u_end; ++u) {
-        const Part p = I.part(n, u);
-        const int head = I.head_cost(p), mine = head * kv_heads;
-        for (int e = 0; e <= count && first + e < ranges.n; ++e) {
-          const int b = ranges.at(first + e);
-          if (mine == 0 || b < before || b >= before + mine) continue;
-          const int kvh = (b - before) / head;
-          int g0 = before + kvh * head, block = 0, units = I.units_of(p, 0);
-          while (b >= g0 + units + tree::kItem) g0 += units + tree::kItem, units = I.units_of(p, ++block);
-          range[e] = tree::snapped(b, g0, units, ranges.snap);
-          where[e][0] = u; where[e][1] = kvh; where[e][2] = block; where[e][3] = g0;
-        }
-        before += mine;
+  if (first < ranges.n && own && ranges.at(first) < before + own && ranges.at(min(first + count, ranges.n - 1)) >= before) {
+    for (int u = c.u_begin; u < c.u_end; ++u) {
+      Part p = c.first;
+      if (u > c.u_begin) p = beam::part_of(n, u);
+      if (!I.has(p)) continue;
+      const int head = I.head_cost(p), mine = head * kv_heads;
+      for (int e = 0; e <= count && first + e < ranges.n; ++e) {
+        const int b = ranges.at(first + e);
+        if (b < before || b >= before + mine) continue;
+        const int kvh = (b - before) / head;
+        int g0 = before + kvh * head, block = 0, units = I.units_of(p, 0);
+        while (b >= g0 + units + tree::kItem) g0 += units + tree::kItem, units = I.units_of(p, ++block);
+        range[e] = tree::snapped(b, g0, units, ranges.snap);
+        where[e][0] = u; where[e][1] = kvh; where[e][2] = block; where[e][3] = g0;
       }
+      before += mine;
+    }
   }
   return ranges;
 }

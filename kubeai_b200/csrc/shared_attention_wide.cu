@@ -189,7 +189,7 @@ shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   extern __shared__ uint8_t smem_raw[];
   __shared__ Staged staged;
   __shared__ float2 states[2][kTileRows];      // maximum and sum of each group's rows, where two groups have the same ones
-  __shared__ int sums[kWarps], s_range[2], s_where[2][4];
+  __shared__ int sums[kWarps][1], s_range[2], s_where[2][4];
   __shared__ Piece pieces[kPieces];
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (sbase - smem_u32(smem_raw));
@@ -207,6 +207,12 @@ shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   volatile int* odd_item = reinterpret_cast<volatile int*>(tmem_slot + 2);      // [2]: the last item of each parity with infinities or NaN among values that some row does not see
   const int warp = warp_number(), lane = threadIdx.x & 31, tid = threadIdx.x;
 
+  griddep_enter();
+  const int cta = blockIdx.x, group = a.q_heads / a.kv_heads, shift = __ffs(group) - 1;
+  const Lengths n = lengths_of(a, &staged, tid, kThreads);
+  Costs<1> costs;
+  find_costs<1, kThreads>(n, a.kv_heads, group, sums, &costs);
+  if (costs.all[0] == 0) return;      // nobody has so many rows
   if (warp == 0) {
     if (lane == 0) {
       for (int s = 0; s < kRing; ++s) {
@@ -231,11 +237,8 @@ shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     tmem_alloc(slot, 512);
     tmem_relinquish();
   }
-  griddep_enter();
-  const int cta = blockIdx.x, group = a.q_heads / a.kv_heads, shift = __ffs(group) - 1;
-  const Lengths n = lengths_of(a, &staged, tid, kThreads);
   const Items I(0, group);
-  const tree::Ranges ranges = find_ranges<kThreads>(n, I, a.kv_heads, cta, 1, sizes.ctas, kLeast, sums, s_range, s_where);
+  const tree::Ranges ranges = find_ranges<1>(n, I, costs, 0, a.kv_heads, cta, 1, sizes.ctas, kLeast, s_range, s_where);
   bool ok = true;
   tc_fence_before();
   __syncthreads();
