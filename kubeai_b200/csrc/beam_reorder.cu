@@ -16,7 +16,7 @@
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 256, kColumns = 64, kBatch = 4;
+constexpr int kThreads = 256, kColumns = 64, kBatch = 8;
 
 __global__ void __launch_bounds__(kThreads)
 beam_reorder_kernel(const b200_beam_reorder_args a) {
@@ -113,24 +113,26 @@ beam_reorder_kernel(const b200_beam_reorder_args a) {
     }
   }
   // ---- copies
-  const int moves = s_moves, heads = 2 * a.kv_heads, pieces = heads * part * 16;      // of 16 bytes: a head's rows lie one behind the other
+  const int moves = s_moves, heads = 2 * a.kv_heads, rows = heads * part, piece = tid & 15;      // a head's rows lie one behind the other, 16 pieces of 16 bytes each
+  const unsigned inverse = part > 1 ? 0xffffffffu / part + 1 : 0u;      // row / part = the upper half of row * inverse (parts below 16)
   for (int l = worker; l < a.layers && moves; l += workers) {
     uint4* kv = static_cast<uint4*>(a.kv) + static_cast<size_t>(l) * (a.layer_stride / 8);
-    for (int e = tid; e < pieces * moves; e += kThreads * kBatch) {
-      uint4 v[kBatch];
-      size_t at[kBatch];
+    for (int m = 0; m < moves; ++m) {
+      const uint4* from = kv + static_cast<size_t>(source[m]) * heads * 256 + piece;
+      uint4* to = kv + static_cast<size_t>(target[m]) * heads * 256 + piece;
+      for (int r0 = tid >> 4; r0 < rows; r0 += kBatch * (kThreads / 16)) {
+        uint4 v[kBatch];
+        auto at = [&](int k) {
+          const int r = r0 + k * (kThreads / 16), head = part > 1 ? __umulhi(r, inverse) : r;
+          return static_cast<size_t>(head) * 256 + (r - head * part) * 16;
+        };
 #pragma unroll
-      for (int k = 0; k < kBatch; ++k) {
-        const int x = e + k * kThreads, m = min(x / pieces, moves - 1), in = x % pieces, head = in / (part * 16), piece = in % (part * 16);
-        at[k] = static_cast<size_t>(head) * 256 + piece;
-        if (x < pieces * moves) {
-          v[k] = kv[static_cast<size_t>(source[m]) * heads * 256 + at[k]];
-          at[k] += static_cast<size_t>(target[m]) * heads * 256;
-        }
+        for (int k = 0; k < kBatch; ++k)
+          if (r0 + k * (kThreads / 16) < rows) v[k] = from[at(k)];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k)
+          if (r0 + k * (kThreads / 16) < rows) to[at(k)] = v[k];
       }
-#pragma unroll
-      for (int k = 0; k < kBatch; ++k)
-        if (e + k * kThreads < pieces * moves) kv[at[k]] = v[k];
     }
   }
 }
@@ -138,7 +140,7 @@ beam_reorder_kernel(const b200_beam_reorder_args a) {
 }  // namespace
 
 int beam_reorder(const b200_beam_reorder_args& a, cudaStream_t st) {
-  const int workers = std::min(std::max(a.layers, a.texts ? a.beams : 1), std::max(1, 8 * sm_count() / a.S));
+  const int workers = std::min(std::max(a.layers, a.texts ? a.beams : 1), std::max(1, 16 * sm_count() / a.S));
   launch_pdl(beam_reorder_kernel, dim3(a.S, 1 + workers), dim3(kThreads), 0, st, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
