@@ -19,7 +19,8 @@
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kAhead = 3, kD = 128;      // kAhead: heads of a thread on their way
+constexpr int kAhead = 3, kD = 128;      // kAhead: heads of a thread on their way
+constexpr int kManyRows = 2048;          // rows from which on a CTA has 128 threads for its row, not 256: 8191 rows 47.2 us -> 42.8, four rows 3.1 -> 4.1
 
 struct Piece {
   float v[4];
@@ -29,9 +30,10 @@ __device__ __forceinline__ Piece widen(uint2 u) {
 }
 
 // kStaged: halves of a number of pairs that four does not divide
-template <bool kStaged>
+template <bool kStaged, int kThreads>
 __global__ void __launch_bounds__(kThreads)
 norm_rope_kernel(const b200_norm_rope_args a) {
+  constexpr int kWarps = kThreads / 32;
   __shared__ float2 turn[kD / 2];
   __shared__ float stage[kStaged ? kWarps * 2 : 1][kD];
   const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, j = lane & 15, n = a.dims / 2;
@@ -157,7 +159,8 @@ norm_rope_kernel(const b200_norm_rope_args a) {
 
 int norm_rope_kv_write(const b200_norm_rope_args& a, cudaStream_t st) {
   const bool staged = !a.interleaved && a.dims % 8 != 0;
-  launch_pdl(staged ? norm_rope_kernel<true> : norm_rope_kernel<false>, dim3(a.T), dim3(kThreads), 0, st, a);
+  if (a.T >= kManyRows) launch_pdl(staged ? norm_rope_kernel<true, 128> : norm_rope_kernel<false, 128>, dim3(a.T), dim3(128), 0, st, a);
+  else launch_pdl(staged ? norm_rope_kernel<true, 256> : norm_rope_kernel<false, 256>, dim3(a.T), dim3(256), 0, st, a);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 
