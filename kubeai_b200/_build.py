@@ -58,7 +58,6 @@ SOURCES = [
     "tree_accept.cu",
     "norm_rope.cu",
     "shared_attention.cu",
-    "shared_attention_wide.cu",
     "beam_select.cu",
     "beam_reorder.cu",
     "abi_ops.cu",

@@ -4,9 +4,11 @@
 //
 // Softmax over two sets of keys is a weighted sum of softmaxes over each, so the rows of a group meet the shared pages in an item of their own and every request's rows the pages behind
 // them in another, and the two are joined by their maxima and sums.
-// An item is a key head and up to 64 rows (row = token * group + head) with a range of pages.  A team of 1, 2 or 4 warps has it, 16 rows a warp.  The CTAs are shared out to the three kinds of teams
-// by their work; all items' pages of a kind one behind the other are cut into as many equal ranges as it has teams, and a team walks its range without a gap: its first warp loads pages ahead
-// by TMA (128-byte swizzle) into the team's ring, over an item's end, and all multiply with mma.sync: row tiles of 16 leave the tensor cores idle in any form, and memory is what bounds this.
+// An item is a key head and rows (row = token * group + head) with a range of keys.  Parts of up to 64 rows go to narrow CTAs, whose teams of 1, 2 or 4 warps have 16 rows a warp; the others to wide
+// ones (shared_attention_wide.cuh).  One launch has both: its CTAs are shared out to the kinds by their work, and all items' keys of a kind, one behind the other, are cut into as many equal ranges as
+// it has teams or CTAs.  (In two launches, either waits for the other's SMs: 16 x 8 beams 79 us and 72.5 in one, 128 rows behind 2048 tokens 62 and 50.)
+// A team walks its range without a gap: its first warp loads pages ahead by TMA (128-byte swizzle) into the team's ring, over an item's end, and all multiply with mma.sync: row tiles of 16 leave the
+// tensor cores idle in any form, and memory is what bounds this.
 // An item that a range's end cuts leaves unnormalised rows in the workspace, as every item does that shares its rows with another; a second kernel joins them in a fixed order.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -21,18 +23,24 @@
 #include "launch.h"
 #include "ptx.cuh"
 #include "shared_attention.cuh"
+#include "shared_attention_wide.cuh"
 
 namespace b200 {
 namespace {
 
-typedef __nv_bfloat16 bf16;
 using namespace shared_attn;
 constexpr int kPageBytes = 2 * 16 * kD * 2;      // bytes of a page's keys and values of a head
-constexpr int kThreads = 128, kWarps = kThreads / 32, kPlaces = 3, kDepth = 2, kItems = 4, kLeast = 4;      // kPlaces: CTAs of an SM; kDepth: pages a warp on their way; kItems: items a warp that those may lie in, and one; kLeast: pages of a range
+constexpr int kDepth = 2, kItems = 4, kLeast = 4;      // kDepth: pages a warp on their way; kItems: items a warp that those may lie in, and one; kLeast: pages of a range
 constexpr int kJoinThreads = 256, kAtOnce = 4;      // kAtOnce: parts of a row on their way
-constexpr int kSmem = 1024 + kWarps * kDepth * kPageBytes;
-static_assert(kPlaces * (kSmem + 3584 + static_cast<int>(sizeof(Staged))) <= 228 * 1024, "");
-static_assert(kItems > kDepth, "");
+// The two forms of the kernel: with CTAs that may be wide, one an SM; and without, three an SM, which begin sooner: 1 x 4 beams behind 450 tokens 16.3 us, and 18.1 us in the other form.
+template <bool kWide>
+struct Form {
+  static constexpr int kThreads = kWide ? wide::kThreads : 128, kWarps = kThreads / 32, kPlaces = wide::kThreads / kThreads, kKinds = kWide ? 4 : 3;
+  static constexpr int kRings = 1024 + kWarps * kDepth * kPageBytes, kSmem = kWide ? std::max(kRings, wide::kSmem) : kRings;
+};
+// What a page of each team, and a step of a wide CTA, take of an SM's time: by these the CTAs are shared out.  128 rows behind 2048 tokens, teams of one next to wide CTAs: 26 50 us, 12 62, 6 82.  16 x 8
+// beams, teams of one and two: 1.6 72.5 us, 2 77, 3 93, 1.3 74.  2 x 24 questions, a few teams of four next to wide CTAs: 8 256 us, 6 258, 3 426 (too few CTAs, which all others wait for).
+__device__ constexpr float kShare[4] = {1.f, 1.6f, 8.f, 26.f};
 
 // An item's pages of a range, as the loads leave them for the products
 struct Piece {
@@ -44,50 +52,84 @@ struct Piece {
   int parts;
 };
 
-__global__ void __launch_bounds__(kThreads, kPlaces)
-shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ b200_shared_attn_args a, const Sizes sizes, float scale_log2, int* error) {
+template <int kWarps>
+struct Narrow {
+  uint64_t bars[2][kWarps * kDepth];
+  Piece pieces[kWarps * kItems];
+  int odd[kWarps * kItems];      // the last item of each piece's place with infinities or NaN among values that some row does not see
+};
+template <bool kWide> union Halves;
+template <> union Halves<true> {
+  Narrow<Form<true>::kWarps> narrow;
+  wide::Shared wide;
+  __device__ Halves() {}
+};
+template <> union Halves<false> {
+  Narrow<Form<false>::kWarps> narrow;
+  __device__ Halves() {}
+};
+static_assert(Form<true>::kSmem + sizeof(Halves<true>) + sizeof(Staged) + 3072 <= 227 * 1024, "");
+static_assert(3 * (Form<false>::kSmem + sizeof(Halves<false>) + sizeof(Staged) + 2048) <= 228 * 1024, "");
+
+template <bool kWide>
+__global__ void __launch_bounds__(Form<kWide>::kThreads, Form<kWide>::kPlaces)
+shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ b200_shared_attn_args a, const Sizes sizes, float scale_log2, int* error) {
+  constexpr int kThreads = Form<kWide>::kThreads, kWarps = Form<kWide>::kWarps, kKinds = Form<kWide>::kKinds;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2][kWarps * kDepth];
-  __shared__ int sums[kWarps][3], s_range[kWarps + 1], s_where[kWarps + 1][4];
-  __shared__ Piece all_pieces[kWarps * kItems];
-  __shared__ int all_odd[kWarps * kItems];      // the last item of each piece's place with infinities or NaN among values that some row does not see
+  __shared__ __align__(16) Halves<kWide> both;
+  __shared__ __align__(16) int sums[kWarps][4];
+  __shared__ int shares[kThreads], s_range[kWarps][2], s_where[kWarps][4];
   __shared__ Staged staged;
   const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem = smem_raw + (sbase - smem_u32(smem_raw));
   const int warp = warp_number(), lane = threadIdx.x & 31, tid = threadIdx.x;
   const int group = a.q_heads / a.kv_heads, shift = __ffs(group) - 1;
-  if (tid < kWarps * kItems) all_odd[tid] = -1;
-  // Behind the wide kernel, which this one needs nothing of, it begins as soon as there is room: that kernel let it in behind its own wait for what both read.  The wait that makes this
-  // one's end the end of both stands at its end.
-  const bool behind = sizes.ctas > 0;
-  if (!behind) griddep_wait();
+  griddep_wait();
   griddep_launch();
   const Lengths n = lengths_of(a, &staged, tid, kThreads);
-  // ---- which team: CTAs by the warps' pages of each kind, one at least
-  Costs<3> costs;
-  find_costs<3, kThreads>(n, a.kv_heads, group, sums, &costs);
-  const int ctas = sizes.warps / kWarps;
-  int kind = 0, first_cta = 0, its = ctas;
+  // ---- which kind: CTAs by the work of each, one at least
+  Costs<kKinds> costs;
+  find_costs<kThreads>(n, a.kv_heads, group, sums, &costs);
+  int kind = 0, first_cta = 0, its = gridDim.x, first, count;
   {
-    const long long all = costs.all[0] + 2ll * costs.all[1] + 4ll * costs.all[2];
-    int left = ctas, begin = 0;
+    float part[kKinds], all = 0.f;
 #pragma unroll
-    for (int i = 2; i >= 0; --i) {
-      const int others = (i > 0 && costs.all[0] > 0) + (i > 1 && costs.all[1] > 0);      // kinds behind it
-      const int count = !costs.all[i] ? 0 : !others ? left : min(left - others, max(1, static_cast<int>(static_cast<float>(costs.all[i]) * (1 << i) * ctas / static_cast<float>(all))));
+    for (int i = 0; i < kKinds; ++i) part[i] = static_cast<float>(costs.all[i]) * kShare[i], all += part[i];
+    const float each = gridDim.x / all;
+    // rounded up, so that none is left far behind; what is left of the last kind, the wide CTAs where there are any: most of the work is theirs then, or they are as many as may be
+    int left = gridDim.x, begin = 0;
+#pragma unroll
+    for (int k = 0; k < kKinds; ++k) {
+      constexpr int kOrder[4] = {2, 1, 0, 3};
+      const int i = kOrder[k];
+      int behind = 0;      // kinds behind it
+#pragma unroll
+      for (int j = k + 1; j < kKinds; ++j) behind += costs.all[kOrder[j]] > 0;
+      int count = costs.all[i] == 0 ? 0 : behind == 0 ? left : max(1, min(left - behind, static_cast<int>(ceilf(part[i] * each))));
+      if (i == 3) count = min(count, sizes.ctas);
       if (static_cast<int>(blockIdx.x) >= begin && static_cast<int>(blockIdx.x) < begin + count) kind = i, first_cta = begin, its = count;
       begin += count;
       left -= count;
     }
+    if (static_cast<int>(blockIdx.x) >= begin) return;      // nothing that it might have
   }
+  const int cta = blockIdx.x - first_cta;
+  if constexpr (kWide) {
+    if (kind == 3) {
+      const tree::Ranges ranges = find_ranges<kThreads>(n, Items(0, group), costs, 3, a.kv_heads, cta, its, 1, wide::kLeast, shares, &first, &count, s_range, s_where);
+      if (count) wide::walk(tm_q, tm_kv, a, sizes, scale_log2, error, smem, both.wide, n, ranges, cta, s_range[0], s_where);
+      return;
+    }
+  }
+  if (tid < kWarps * kItems) both.narrow.odd[tid] = -1;
   const int team = 1 << kind;
   const Items I(team, group);
-  const int stream = warp >> kind, member = warp & (team - 1), streams = kWarps >> kind, gs = (blockIdx.x - first_cta) * streams + stream;      // gs: the team's number among its kind
+  const int stream = warp >> kind, member = warp & (team - 1), streams = kWarps >> kind;
   static_assert(kDepth == 2, "");
   const int depth = kDepth * team, depth_log = kind + 1, cap = kItems * team;
-  const uint32_t ring = sbase + stream * depth * kPageBytes, full0 = smem_u32(bars[0] + stream * depth), empty0 = smem_u32(bars[1] + stream * depth);
-  Piece* pieces = all_pieces + stream * cap;
-  volatile int* odd_item = all_odd + stream * cap;
+  const uint32_t ring = sbase + stream * depth * kPageBytes, full0 = smem_u32(both.narrow.bars[0] + stream * depth), empty0 = smem_u32(both.narrow.bars[1] + stream * depth);
+  Piece* pieces = both.narrow.pieces + stream * cap;
+  volatile int* odd_item = both.narrow.odd + stream * cap;
   if (lane == 0 && member == 0) {
     for (int s = 0; s < depth; ++s) {
       mbar_init(full0 + 8 * s, 1);
@@ -96,13 +138,11 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
     fence_mbar_init();
     tma_prefetch_desc(&tm_kv);
   }
-  const tree::Ranges ranges = find_ranges<3>(n, I, costs, kind, a.kv_heads, (blockIdx.x - first_cta) * streams, streams, its * streams, kLeast, s_range, s_where);
+  const tree::Ranges ranges = find_ranges<kThreads>(n, I, costs, kind, a.kv_heads, cta, its, streams, kLeast, shares, &first, &count, s_range, s_where);
   __syncthreads();
-  const int left = gs < ranges.n ? s_range[stream + 1] - s_range[stream] : 0;
-  if (left <= 0) {
-    if (behind) griddep_wait();
-    return;
-  }
+  const int gs = first + stream;      // the team's range
+  const int left = stream < count ? s_range[stream][1] - s_range[stream][0] : 0;
+  if (left <= 0) return;
   const Space space = space_of(a, sizes);
   const int slot = (first_cta * kWarps + gs * team) * 2;      // of 16 rows: the range's first item, a team's tiles behind it the last
 
@@ -111,7 +151,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
   it.u = s_where[stream][0]; it.kvh = s_where[stream][1]; it.block = s_where[stream][2];
   it.p = I.part(n, it.u);
   it.fill(I);
-  int t0 = max(0, s_range[stream] - s_where[stream][3] - tree::kItem), rest = left;
+  int t0 = max(0, s_range[stream][0] - s_where[stream][3] - tree::kItem), rest = left;
   if (t0 == it.units) {              // the range begins where the item in front of it ends
     t0 = 0;
     it.next(n, I, a.kv_heads);
@@ -144,7 +184,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
       x.begins = t0 == 0;
       x.own = !it.p.all;
       x.joined = it.p.k0 > 0;
-      x.parts = whole ? 0 : t0 == 0 ? ranges.parts(gs, s_range[stream + 1] - take, it.units) : 0;
+      x.parts = whole ? 0 : t0 == 0 ? ranges.parts(gs, s_range[stream][1] - take, it.units) : 0;
       x.last = rest <= 0;
       pieces[items & (cap - 1)] = x;
     }
@@ -350,7 +390,6 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_kv, const __grid_const
   // the copies in flight land before the CTA ends, also where it gives up
   for (int k = used; k < issued; ++k) warp_wait(full0 + 8 * (k & (depth - 1)), (k >> depth_log) & 1);
   if (!ok) *reinterpret_cast<volatile int*>(error) = 1;
-  if (behind) griddep_wait();
 }
 
 // A row: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts, in order, four dimensions a lane; a lane has the maximum, sum and weight of one part in 32.
@@ -394,20 +433,30 @@ __device__ __forceinline__ uint2 join_row(int parts, At part, int lane) {
   return make_uint2(pack_bf16x2(y.x * inv, y.y * inv), pack_bf16x2(y.z * inv, y.w * inv));
 }
 
+// Whether all parts of a place lie in the workspace: not so where a wait ran out in front of it and it was not written
+__device__ __forceinline__ bool in_bounds(const Place& p, const Sizes& sizes, int group) {
+  if (p.parts == 0) return true;
+  const int team = p.flags / kTeam, behind = max(1, team);
+  const long long first = p.slot, last = first - behind + 2ll * behind * (p.parts - 1), slots = 2ll * (team ? sizes.warps : sizes.ctas) - behind;
+  return p.parts > 0 && p.flags >= 0 && team <= 4 && first >= behind && first <= slots && last <= slots && p.row >= 0 && p.row <= (team ? team * kTile16 : kWideRows) - group;
+}
+
 // A CTA has a row and eight of its heads.
 __global__ void __launch_bounds__(kJoinThreads)
 shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const Sizes sizes) {
   const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, head = blockIdx.y * (kJoinThreads / 32) + warp;
-  griddep_enter();
-  const Space space = space_of(a, sizes);
-  const int group = a.q_heads / a.kv_heads, kvh = min(head, a.q_heads - 1) / group;
-  // (what lies there counts where some request has the row)
-  const Place shared = space.places[static_cast<size_t>(t) * a.kv_heads + kvh], own = space.places[(static_cast<size_t>(a.T) + t) * a.kv_heads + kvh];
+  // the lengths were there before the kernel in front of this one let it in
+  griddep_launch();
   bool mine = false;
   for (int s = tid; s < a.S && !mine; s += kJoinThreads) {
     const tree::Request r = tree::request_of(a.starts, a.ctx, s, a.T, a.max_blocks, a.max_rows, a.status);
     mine = t >= r.row0 && t < r.row0 + r.rows;
   }
+  griddep_wait();
+  const Space space = space_of(a, sizes);
+  const int group = a.q_heads / a.kv_heads, kvh = min(head, a.q_heads - 1) / group;
+  // (what lies there counts where some request has the row)
+  const Place shared = space.places[static_cast<size_t>(t) * a.kv_heads + kvh], own = space.places[(static_cast<size_t>(a.T) + t) * a.kv_heads + kvh];
   mine = __syncthreads_or(mine);
   if (head >= a.q_heads) return;
   uint2* out = reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + static_cast<size_t>(t) * a.ldo + head * kD) + lane;
@@ -416,6 +465,7 @@ shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const S
     return;
   }
   if (!own.parts && !(own.flags & kJoined)) return;      // written already
+  if (!in_bounds(own, sizes, group) || (own.flags & kJoined && !in_bounds(shared, sizes, group))) return;
   const int n_own = max(1, own.parts), n_all = n_own + (own.flags & kJoined ? max(1, shared.parts) : 0);
   // an item's beginning lies in its range's second slot, each other part in its range's first
   auto part = [&](int p) -> const float* {
@@ -430,7 +480,17 @@ shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const S
 
 }  // namespace
 
-static Sizes sizes_of(const b200_shared_attn_args& a) { return {kPlaces * sm_count() * kWarps, shared_attention_wide_ctas(a)}; }
+// How many CTAs may be wide: none where no part can have so many rows, else as many as there are SMs, or as the most work that the call may have feeds
+static int wide_ctas(const b200_shared_attn_args& a) {
+  const long long group = a.q_heads / a.kv_heads, T = a.T, most = std::min<long long>(a.max_rows, T);
+  const bool shared = a.G && T * group > kNarrow, own = most * group > kNarrow;
+  if (!shared && !own) return 0;
+  const long long seen = std::min<long long>(a.max_ctx ? a.max_ctx : INT_MAX, a.max_blocks * static_cast<long long>(tree::kPage)) + most;
+  const long long items = ((shared ? (T * group + kWideRows - 1) / kWideRows + a.G : 0) + (own ? (most * group + kWideRows - 1) / kWideRows * a.S : 0)) * a.kv_heads;
+  return static_cast<int>(std::min<long long>(sm_count(), std::max<long long>(1, items * ((seen + wide::kKeys - 1) / wide::kKeys + tree::kItem) / wide::kLeast)));
+}
+
+static Sizes sizes_of(const b200_shared_attn_args& a) { return {sm_count() * Form<true>::kWarps, wide_ctas(a)}; }
 
 int64_t shared_attention_workspace(const b200_shared_attn_args& a) {
   const Sizes n = sizes_of(a);
@@ -441,14 +501,20 @@ int64_t shared_attention_workspace(const b200_shared_attn_args& a) {
 
 int paged_attention_shared(const b200_shared_attn_args& a, int* error, cudaStream_t st) {
   const Sizes sizes = sizes_of(a);
-  if (sizes.ctas)
-    if (int rc = shared_attention_wide(a, sizes, error, st)) return rc;
-  CUtensorMap tm_kv;
+  const int group = a.q_heads / a.kv_heads;
+  CUtensorMap tm_kv, tm_q;
   if (int rc = tmap_encode_bf16_2d(&tm_kv, a.kv_layer, static_cast<uint64_t>(a.num_pages) * 2 * a.kv_heads * 16, kD, kD, 16, 64, 1)) return rc;
-  static std::atomic<unsigned long long> attr_done{0};
-  if (!ensure_dynamic_smem(shared_attn_kernel, kSmem, &attr_done)) return -3;
-  launch_pdl(shared_attn_kernel, dim3(sizes.warps / kWarps), dim3(kThreads), kSmem, st, tm_kv, a, sizes, a.scale * 1.4426950408889634f, error);
-  if (cudaGetLastError() != cudaSuccess) return -2;
+  tm_q = tm_kv;
+  if (sizes.ctas)
+    if (int rc = tmap_encode_bf16_3d(&tm_q, a.q, kD, a.q_heads, a.T, kD, a.ldq, 64, group, wide::kTileRows / group)) return rc;
+  auto launch = [&](auto kernel, auto form, std::atomic<unsigned long long>* attr_done) {
+    using F = decltype(form);
+    if (!ensure_dynamic_smem(kernel, F::kSmem, attr_done)) return -3;
+    launch_pdl(kernel, dim3(sizes.warps / F::kWarps), dim3(F::kThreads), F::kSmem, st, tm_q, tm_kv, a, sizes, a.scale * 1.4426950408889634f, error);
+    return cudaGetLastError() == cudaSuccess ? 0 : -2;
+  };
+  static std::atomic<unsigned long long> wide_done{0}, narrow_done{0};
+  if (int rc = sizes.ctas ? launch(shared_attn_kernel<true>, Form<true>{}, &wide_done) : launch(shared_attn_kernel<false>, Form<false>{}, &narrow_done)) return rc;
   launch_pdl(shared_attn_join_kernel, dim3(a.T, (a.q_heads + 7) / 8), dim3(kJoinThreads), 0, st, a, sizes);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }

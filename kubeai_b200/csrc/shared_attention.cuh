@@ -1,4 +1,4 @@
-// What the kernels of shared_attention.cu and shared_attention_wide.cu have in common: which rows and keys an item has, and where its rows go.
+// What the two halves of the kernel of shared_attention.cu have in common: which rows and keys an item has, and where its rows go.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -11,7 +11,8 @@ namespace shared_attn {
 
 using beam::Lengths;
 using beam::Part;
-constexpr int kD = 128, kTile16 = 16, kNarrow = 64;      // kNarrow: rows (token * group + head) of a part that go to the narrow kernel, whose warps have tiles of 16
+typedef __nv_bfloat16 bf16;
+constexpr int kD = 128, kTile16 = 16, kNarrow = 64;      // kNarrow: rows (token * group + head) of a part that go to narrow CTAs, whose warps have tiles of 16
 constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
 constexpr int kWaitLimit = 1 << 22;
 
@@ -25,7 +26,7 @@ struct Place {
   int row;              // the token's first row there
   int flags;
 };
-constexpr int kJoined = 1, kTeam = 4;      // own rows: the group's are to be added; times the team of the narrow kernel, 0 for the wide one
+constexpr int kJoined = 1, kTeam = 4;      // own rows: the group's are to be added; times the team, 0 for a wide CTA
 struct Space {
   Place* places;        // [2][T][kv_heads]: the groups', the requests' own
   float* narrow;        // [warps][2][16][kLd], a team's warps together: a range's first item, which another range began, and its last
@@ -33,9 +34,9 @@ struct Space {
   float* rows;          // [2][T][q_heads][kLd]
 };
 struct Sizes {
-  int warps, ctas;      // of the narrow and the wide kernel
+  int warps, ctas;      // of all CTAs, which may all be narrow, and how many may be wide
 };
-constexpr int kWideRows = 256;      // rows of an item of the wide kernel
+constexpr int kWideRows = 256;      // rows of an item of a wide CTA
 __host__ __device__ inline Space space_of(const b200_shared_attn_args& a, const Sizes& n) {
   Space s;
   s.places = static_cast<Place*>(a.workspace);
@@ -72,8 +73,8 @@ __device__ __forceinline__ Lengths lengths_of(const b200_shared_attn_args& a, St
   return n;
 }
 
-// ---- items: a part's key head and a block of its rows.  Parts of up to 64 rows go to the narrow kernel, to teams of 1, 2 or 4 warps with 16 rows each; the others (team 0) to the wide one, 256 rows
-// a block.  An item's keys come in units: pages, or steps of the wide kernel, which has two tiles of 128 scores at once: those of two row tiles and 128 keys where there are more than 128 rows, else of
+// ---- items: a part's key head and a block of its rows.  Parts of up to 64 rows go to narrow CTAs, to teams of 1, 2 or 4 warps with 16 rows each; the others (team 0) to wide ones, 256 rows
+// a block.  An item's keys come in units: pages, or steps of a wide CTA, which has two tiles of 128 scores at once: those of two row tiles and 128 keys where there are more than 128 rows, else of
 // one row tile and 256 keys.
 __device__ __forceinline__ int team_of(int rows) { return rows <= kTile16 ? 1 : rows <= 2 * kTile16 ? 2 : rows <= kNarrow ? 4 : 0; }
 struct Items {
@@ -126,42 +127,40 @@ struct Item {
   }
 };
 
-// Every thread's share of the step's parts, one behind the other, and what the items of each kind cost: its own, in front of it, and in all.  Kinds: the teams of 1, 2 and 4 warps, or the wide kernel's.
+// What the items of each kind cost, in front of a thread's share of the step's parts and in all.  Kinds: teams of 1, 2 and 4 warps, and wide CTAs.
 template <int kKinds>
 struct Costs {
-  int u_begin, u_end;
-  Part first;      // the first part of the share
-  int own[kKinds], before[kKinds], all[kKinds];
+  int per;      // parts of a share
+  int before[kKinds], all[kKinds];
 };
-template <int kKinds>
-__device__ __forceinline__ int kind_team(int kind) { return kKinds == 1 ? 0 : 1 << kind; }
+__device__ __forceinline__ int kind_team(int kind) { return kind == 3 ? 0 : 1 << kind; }
 // ... with one barrier
-template <int kKinds, int kThreads>
-__device__ __forceinline__ void find_costs(const Lengths& n, int kv_heads, int group, int (*sums)[kKinds], Costs<kKinds>* c) {
+template <int kThreads, int kKinds>
+__device__ __forceinline__ void find_costs(const Lengths& n, int kv_heads, int group, int (*sums)[4], Costs<kKinds>* c) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int U = n.G + n.S, per = (U + kThreads - 1) / kThreads;
-  c->u_begin = min(U, tid * per);
-  c->u_end = min(U, c->u_begin + per);
+  const int U = n.G + n.S, per = (U + kThreads - 1) / kThreads, end = min(U, (tid + 1) * per);
+  c->per = per;
+  int own[kKinds];
 #pragma unroll
-  for (int i = 0; i < kKinds; ++i) c->own[i] = 0;
-  for (int u = c->u_end - 1; u >= c->u_begin; --u) {
-    c->first = beam::part_of(n, u);
+  for (int i = 0; i < kKinds; ++i) own[i] = 0;
+  for (int u = tid * per; u < end; ++u) {
+    const Part p = beam::part_of(n, u);
 #pragma unroll
     for (int i = 0; i < kKinds; ++i) {
-      const Items I(kind_team<kKinds>(i), group);
-      if (I.has(c->first)) c->own[i] += I.head_cost(c->first) * kv_heads;
+      const Items I(kind_team(i), group);
+      if (I.has(p)) own[i] += I.head_cost(p) * kv_heads;
     }
   }
 #pragma unroll
   for (int i = 0; i < kKinds; ++i) {
-    int x = c->own[i];
+    int x = own[i];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int y = __shfl_up_sync(0xffffffffu, x, o);
       if (lane >= o) x += y;
     }
     if (lane == 31) sums[warp][i] = x;
-    c->before[i] = x - c->own[i];
+    c->before[i] = x - own[i];
     c->all[i] = 0;
   }
   __syncthreads();
@@ -175,43 +174,49 @@ __device__ __forceinline__ void find_costs(const Lengths& n, int kv_heads, int g
     }
 }
 
-// Where `count` ranges from range `first` on begin and end, of at most `most` that the items of a kind are cut into, none with less than `least` units.  range [count + 1], where
-// [count + 1][4]: part, key head, block, and the first unit of the item that a range begins in.  Returns all ranges; to be followed by a barrier.
-template <int kKinds>
-__device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, const Items& I, const Costs<kKinds>& c, int kind, int kv_heads, int first, int count, int most, int least, int* range, int (*where)[4]) {
+// The ranges of CTA `cta` of the `ctas` that a kind has, of `streams` at most each: all items' units are cut into as many as there are, none with less than `least` units, and every CTA has as many
+// of them, side by side, where there are fewer: the memory of all SMs is wanted.  A thread each looks for the share of parts that an end lies in.  first: the CTA's first range; range [count][2],
+// where [count][4]: part, key head, block, and the first unit of the item that a range begins in.  Returns all ranges; to be followed by a barrier.
+template <int kThreads, int kKinds>
+__device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, const Items& I, const Costs<kKinds>& c, int kind, int kv_heads, int cta, int ctas, int streams, int least, int* shares, int* first,
+                                                    int* count, int (*range)[2], int (*where)[4]) {
   const int tid = threadIdx.x;
-  int N = c.all[0], before = c.before[0], own = c.own[0];
+  int N = c.all[0], before = c.before[0];
 #pragma unroll
   for (int i = 1; i < kKinds; ++i)
-    if (i == kind) N = c.all[i], before = c.before[i], own = c.own[i];
-  tree::Ranges ranges = tree::ranges_of(N, max(1, min(most, N / least)));
+    if (i == kind) N = c.all[i], before = c.before[i];
+  shares[tid] = before;
+  tree::Ranges ranges = tree::ranges_of(N, max(1, min(ctas * streams, N / least)));
   if (N == 0) ranges.n = 0;
-  if (tid <= count && first + tid >= ranges.n) range[tid] = N;      // which lies in no item
-  if (first < ranges.n && own && ranges.at(first) < before + own && ranges.at(min(first + count, ranges.n - 1)) >= before) {
-    for (int u = c.u_begin; u < c.u_end; ++u) {
-      Part p = c.first;
-      if (u > c.u_begin) p = beam::part_of(n, u);
-      if (!I.has(p)) continue;
-      const int head = I.head_cost(p), mine = head * kv_heads;
-      for (int e = 0; e <= count && first + e < ranges.n; ++e) {
-        const int b = ranges.at(first + e);
-        if (b < before || b >= before + mine) continue;
-        const int kvh = (b - before) / head;
-        int g0 = before + kvh * head, block = 0, units = I.units_of(p, 0);
-        while (b >= g0 + units + tree::kItem) g0 += units + tree::kItem, units = I.units_of(p, ++block);
-        range[e] = tree::snapped(b, g0, units, ranges.snap);
-        where[e][0] = u; where[e][1] = kvh; where[e][2] = block; where[e][3] = g0;
+  const int per = (ranges.n + ctas - 1) / ctas;
+  *first = cta * per;
+  *count = max(0, min(per, ranges.n - *first));
+  __syncthreads();
+  const int e = tid >> 1, end = tid & 1, r = *first + e + end;
+  if (e < *count) {
+    int at = N;      // behind the last item
+    if (r < ranges.n) {
+      const int b = ranges.at(r), share = tree::last_at_most(shares, kThreads - 1, b);      // the last share that begins there or in front of it: one with items
+      int u = share * c.per, g0 = shares[share], head;
+      Part p;
+      for (;; ++u) {
+        p = I.part(n, u);
+        head = I.head_cost(p);
+        if (b < g0 + head * kv_heads) break;
+        g0 += head * kv_heads;
       }
-      before += mine;
+      const int kvh = (b - g0) / head;
+      g0 += kvh * head;
+      int block = 0, units = I.units_of(p, 0);
+      while (b >= g0 + units + tree::kItem) g0 += units + tree::kItem, units = I.units_of(p, ++block);
+      at = tree::snapped(b, g0, units, ranges.snap);
+      if (!end) where[e][0] = u, where[e][1] = kvh, where[e][2] = block, where[e][3] = g0;
     }
+    range[e][end] = at;
   }
   return ranges;
 }
 
 }  // namespace shared_attn
-
-// The kernel of parts with more rows than kNarrow
-int shared_attention_wide(const b200_shared_attn_args& a, const shared_attn::Sizes& sizes, int* error, cudaStream_t st);
-int shared_attention_wide_ctas(const b200_shared_attn_args& a);
 
 }  // namespace b200

@@ -13,34 +13,21 @@
 // Only steps that reach behind what every row sees are masked.  There the products' warp also clears what must not meet a weight of zero: values behind the last key, and infinities and NaN
 // among values that some row does not see, which the rows that see them add at the end by themselves.
 // Every wait has a limit; a CTA that gives up sets an error mark and still meets at the end.
-#include <cuda.h>
-#include <cuda_bf16.h>
-#include <cuda_runtime.h>
-#include <limits.h>
-#include <math.h>
-
-#include <algorithm>
-
-#include "gemm.h"
-#include "kernels.h"
-#include "launch.h"
-#include "ptx.cuh"
+#pragma once
 #include "shared_attention.cuh"
 
 namespace b200 {
-namespace {
+namespace shared_attn {
+namespace wide {
 
-typedef __nv_bfloat16 bf16;
-using namespace shared_attn;
 constexpr int kTileRows = 128, kKeys = 128;                         // of a tile of scores
 constexpr int kSlab = 128 * 128, kTile = 2 * kSlab;                 // bytes: 64 columns of 128 rows, a tile
-constexpr int kThreads = 384, kWarps = kThreads / 32, kRing = 4;    // warps 0 to 3 and 4 to 7: softmax, 8: loads, 9: products; kRing: tiles of keys and values
+constexpr int kThreads = 384, kRing = 4;                                            // tiles of keys and values.  Warps 0 to 3 and 4 to 7: softmax, 8: loads, 9: products
 constexpr int kLeast = 4;                                           // steps of a range: its rows leave as 132 KB, as much as eight tiles
 constexpr float kSlack = 1.f;                                       // by how much, in units of log 2, a row's maximum may grow before its weights are made relative to it
 
 // shared memory: queries, ring, 2 KB a softmax warp for its way out, barriers
 constexpr int kRingAt = 2 * kTile, kStageAt = kRingAt + kRing * kTile, kBars = kStageAt + 8 * 2048, kSmem = 1024 + kBars + 256;
-static_assert(kSmem + static_cast<int>(sizeof(Staged)) + 4096 <= 227 * 1024, "");
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
@@ -183,16 +170,17 @@ struct Rows {
   }
 };
 
-__global__ void __launch_bounds__(kThreads, 1)
-shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_kv, const __grid_constant__ b200_shared_attn_args a, const Sizes sizes, float scale_log2,
-                        int* error) {
-  extern __shared__ uint8_t smem_raw[];
-  __shared__ Staged staged;
-  __shared__ float2 states[2][kTileRows];      // maximum and sum of each group's rows, where two groups have the same ones
-  __shared__ int sums[kWarps][1], s_range[2], s_where[2][4];
-  __shared__ Piece pieces[kPieces];
-  const uint32_t sbase = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  uint8_t* smem = smem_raw + (sbase - smem_u32(smem_raw));
+struct Shared {
+  float2 states[2][kTileRows];      // maximum and sum of each group's rows, where two groups have the same ones
+  Piece pieces[kPieces];
+};
+
+// The range of CTA `cta` of this half, which begins and ends as `range` and `where` have it
+__device__ __forceinline__ void walk(const CUtensorMap& tm_q, const CUtensorMap& tm_kv, const b200_shared_attn_args& a, const Sizes& sizes, float scale_log2, int* error, uint8_t* smem, Shared& shared,
+                                     const Lengths& n, const tree::Ranges& ranges, int cta, const int* s_range, const int (*s_where)[4]) {
+  Piece* pieces = shared.pieces;
+  auto& states = shared.states;
+  const uint32_t sbase = smem_u32(smem);
   const uint32_t q_s = sbase, ring = sbase + kRingAt, bars = sbase + kBars;
   auto full = [&](int n) { return bars + 8u * (n % kRing); };
   auto empty = [&](int n) { return bars + 8u * (kRing + n % kRing); };
@@ -207,12 +195,7 @@ shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   volatile int* odd_item = reinterpret_cast<volatile int*>(tmem_slot + 2);      // [2]: the last item of each parity with infinities or NaN among values that some row does not see
   const int warp = warp_number(), lane = threadIdx.x & 31, tid = threadIdx.x;
 
-  griddep_enter();
-  const int cta = blockIdx.x, group = a.q_heads / a.kv_heads, shift = __ffs(group) - 1;
-  const Lengths n = lengths_of(a, &staged, tid, kThreads);
-  Costs<1> costs;
-  find_costs<1, kThreads>(n, a.kv_heads, group, sums, &costs);
-  if (costs.all[0] == 0) return;      // nobody has so many rows
+  const int group = a.q_heads / a.kv_heads, shift = __ffs(group) - 1;
   if (warp == 0) {
     if (lane == 0) {
       for (int s = 0; s < kRing; ++s) {
@@ -238,7 +221,6 @@ shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
     tmem_relinquish();
   }
   const Items I(0, group);
-  const tree::Ranges ranges = find_ranges<1>(n, I, costs, 0, a.kv_heads, cta, 1, sizes.ctas, kLeast, s_range, s_where);
   bool ok = true;
   tc_fence_before();
   __syncthreads();
@@ -247,7 +229,7 @@ shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   auto tm_s = [&](int g) { return tmem + 128u * g; };
   auto tm_o = [&](int g) { return tmem + 256u + 128u * g; };
 
-  const bool some_work = cta < ranges.n && s_range[1] > s_range[0];
+  const bool some_work = s_range[1] > s_range[0];
   if (warp >= 8) {
     fewer_registers<72>();
     if (some_work && warp == 8) {
@@ -570,27 +552,6 @@ shared_attn_wide_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_c
   }
 }
 
-}  // namespace
-
-int shared_attention_wide_ctas(const b200_shared_attn_args& a) {
-  const long long group = a.q_heads / a.kv_heads, T = a.T, most = std::min<long long>(a.max_rows, T);
-  const bool shared = a.G && T * group > kNarrow, own = most * group > kNarrow;
-  if (!shared && !own) return 0;
-  // as many CTAs as there are SMs, or as the most work that the call may have feeds
-  const long long seen = std::min<long long>(a.max_ctx ? a.max_ctx : INT_MAX, a.max_blocks * static_cast<long long>(tree::kPage)) + most;
-  const long long items = ((shared ? (T * group + kWideRows - 1) / kWideRows + a.G : 0) + (own ? (most * group + kWideRows - 1) / kWideRows * a.S : 0)) * a.kv_heads;
-  return static_cast<int>(std::min<long long>(sm_count(), std::max<long long>(1, items * ((seen + kKeys - 1) / kKeys + tree::kItem) / kLeast)));
-}
-
-int shared_attention_wide(const b200_shared_attn_args& a, const Sizes& sizes, int* error, cudaStream_t st) {
-  const int group = a.q_heads / a.kv_heads;
-  CUtensorMap tm_q, tm_kv;
-  if (int rc = tmap_encode_bf16_3d(&tm_q, a.q, kD, a.q_heads, a.T, kD, a.ldq, 64, group, kTileRows / group)) return rc;
-  if (int rc = tmap_encode_bf16_2d(&tm_kv, a.kv_layer, static_cast<uint64_t>(a.num_pages) * 2 * a.kv_heads * 16, kD, kD, 16, 64, 1)) return rc;
-  static std::atomic<unsigned long long> attr_done{0};
-  if (!ensure_dynamic_smem(shared_attn_wide_kernel, kSmem, &attr_done)) return -3;
-  launch_pdl(shared_attn_wide_kernel, dim3(sizes.ctas), dim3(kThreads), kSmem, st, tm_q, tm_kv, a, sizes, a.scale * 1.4426950408889634f, error);
-  return cudaGetLastError() == cudaSuccess ? 0 : -2;
-}
-
+}  // namespace wide
+}  // namespace shared_attn
 }  // namespace b200
