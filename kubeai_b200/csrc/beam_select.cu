@@ -26,11 +26,11 @@
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 256, kWarps = kThreads / 32, kVectors = 8, kList = 256, kPlaces = 6, kWaitLimit = 1 << 22;      // kVectors: pieces of 16 bytes of a thread; kPlaces: CTAs of an SM
+constexpr int kThreads = 128, kWarps = kThreads / 32, kVectors = 16, kList = 256, kPlaces = 6, kWaitLimit = 1 << 22;      // kVectors: pieces of 16 bytes of a thread; kPlaces: CTAs of an SM
 constexpr int kPart = kThreads * kVectors;                                            // pieces of a part at most
 constexpr int kMostParts = 64;                                                         // two of a lane in the second kernel
 static_assert(kMostParts * 4 * (kPart - 1) > beam::kMaxVocab && kWarps >= 4 && 4 * 32 >= beam::kMaxFound, "");
-constexpr int kLeastPart = 1024;                                                       // pieces of a part at least, where the row has them
+constexpr int kLeastPart = 512;                                                       // pieces of a part at least, where the row has them
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct PartHead {
@@ -216,21 +216,20 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, const Cut cut
     if (whole > 0) mbar_wait_limited(bar, 0, kWaitLimit);
     return;
   }
-  static_assert(kWarps == 8, "");
-  const float top = value_of(__reduce_max_sync(0xffffffffu, mosts[lane & 7]));
+  const float top = value_of(__reduce_max_sync(0xffffffffu, mosts[lane & (kWarps - 1)]));
   PartHead* head = static_cast<PartHead*>(a.workspace) + number;
   if (top == -INFINITY) {      // nothing here is a candidate
     if (tid == 0) *head = {-INFINITY, 0, 0.0};
     return;
   }
   // the fourth largest of the warps' bounds: four warps have r lanes each that reach it
-  uint32_t bound = bounds[lane & 7];
+  uint32_t bound = bounds[lane & (kWarps - 1)];
   {
     int place = 0;
 #pragma unroll
-    for (int o = 1; o < 8; ++o) {
+    for (int o = 1; o < kWarps; ++o) {
       const uint32_t other = __shfl_xor_sync(0xffffffffu, bound, o);
-      place += other > bound || (other == bound && ((lane ^ o) & 7) < (lane & 7));
+      place += other > bound || (other == bound && ((lane ^ o) & (kWarps - 1)) < (lane & (kWarps - 1)));
     }
     bound = __reduce_max_sync(0xffffffffu, place == 3 ? bound : 0u);
   }
@@ -268,14 +267,21 @@ beam_parts_kernel(const __grid_constant__ b200_beam_select_args a, const Cut cut
   for (int again = 0;; ++again) {
     float part_of[4] = {0.f, 0.f, 0.f, 0.f};
     if (!far) {
+      const uint64_t scale2 = pair_of(kLog2e, kLog2e), from2 = pair_of(from, from);
+      uint64_t two[2] = {0, 0};
 #pragma unroll
       for (int v = 0; v < kVectors; ++v) {
         if (v >= slots) break;
         const uint4 u = here[v * kThreads + tid];
         const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-        for (int k = 0; k < kPer; ++k) part_of[k & 3] += exp2_ftz(fmaf(value_in<kF32>(w, k), kLog2e, from));
+        for (int k = 0; k < kPer; k += 2) {
+          const float2 x = floats_of(fma_pair(pair_of(value_in<kF32>(w, k), value_in<kF32>(w, k + 1)), scale2, from2));
+          two[k / 2 & 1] = add_pair(two[k / 2 & 1], pair_of(exp2_ftz(x.x), exp2_ftz(x.y)));
+        }
       }
+      const float2 t0 = floats_of(two[0]), t1 = floats_of(two[1]);
+      part_of[0] = t0.x; part_of[1] = t0.y; part_of[2] = t1.x; part_of[3] = t1.y;
     } else {
 #pragma unroll 1
       for (int v = 0; v < slots; ++v) {
