@@ -407,6 +407,7 @@ beam_join_kernel(const __grid_constant__ b200_beam_select_args a, int parts, siz
       for (int i = 0; i < 2; ++i) {
         const int p = lane + 32 * i;
         h[i] = p < parts ? heads[b * parts + p] : PartHead{-INFINITY, 0, 0.0};
+        h[i].n = min(max(h[i].n, 0), k);      // whatever a part left whose wait ran out
         if (p < parts) counts[b * parts + p] = h[i].n;
         top = fmaxf(top, h[i].top);
       }
