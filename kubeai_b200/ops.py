@@ -548,13 +548,16 @@ def beam_select(logits, scores, k=None, ends=None) -> BeamSelect:
         raise _refused(_WIDE)
     a = BeamSelectArgs(S, B, V, ld, logits.dtype is torch.float32, k, 0 if ends is None else ends.numel(), logits.data_ptr(), scores.data_ptr(), _ptr(ends))
     a.workspace_bytes = check(lib().b200_op_beam_select_workspace(C.byref(a)))
-    workspace, parents, tokens, found_parents, found_tokens = torch.empty((a.workspace_bytes + 3) // 4 + 2 * S * (B + k), dtype=torch.int32, device=logits.device).unsafe_split_with_sizes(
-        [(a.workspace_bytes + 3) // 4, S * B, S * B, S * k, S * k])
-    new_scores, found_scores = scores.new_empty(S * (B + k)).unsafe_split_with_sizes([S * B, S * k])
-    a.workspace, a.parents, a.tokens, a.new_scores = workspace.data_ptr(), parents.data_ptr(), tokens.data_ptr(), new_scores.data_ptr()
-    a.found_parents, a.found_tokens, a.found_scores = found_parents.data_ptr(), found_tokens.data_ptr(), found_scores.data_ptr()
+    # two buffers, of which everything is a part (as_strided: 9.4 us for all six, where splits and views took 12.1)
+    ints, floats = torch.empty(2 * S * (B + k) + (a.workspace_bytes + 3) // 4, dtype=torch.int32, device=logits.device), scores.new_empty(S * (B + k))
+    at_ints, at_floats, n, m = ints.data_ptr(), floats.data_ptr(), S * B, S * k
+    front = (a.workspace_bytes + 3) // 4
+    a.workspace, a.parents, a.tokens, a.found_parents, a.found_tokens = at_ints, at_ints + 4 * front, at_ints + 4 * (front + n), at_ints + 4 * (front + 2 * n), at_ints + 4 * (front + 2 * n + m)
+    a.new_scores, a.found_scores = at_floats, at_floats + 4 * n
     check(lib().b200_op_beam_select(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
-    return BeamSelect(parents.view(S, B), tokens.view(S, B), new_scores.view(S, B), found_parents.view(S, k), found_tokens.view(S, k), found_scores.view(S, k))
+    on, found, by_beam, by_place = (S, B), (S, k), (B, 1), (k, 1)
+    return BeamSelect(ints.as_strided(on, by_beam, front), ints.as_strided(on, by_beam, front + n), floats.as_strided(on, by_beam, 0), ints.as_strided(found, by_place, front + 2 * n),
+                      ints.as_strided(found, by_place, front + 2 * n + m), floats.as_strided(found, by_place, n))
 
 
 class BeamReorder(NamedTuple):
