@@ -227,7 +227,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const uint32_t k_row = rr + (tile >> 1) * 8, k_chunk = tile & 1, v_row = rr + (tile & 1) * 8, v_chunk = tile >> 1;
   int used = 0;
   for (int item = 0; ok; ++item) {
-    if (!(ok = warp_wait(full0 + 8 * (used & (depth - 1)), (used >> depth_log) & 1))) break;      // the item's first page, and the piece in front of it
+    if (team > 1 && !(ok = warp_wait(full0 + 8 * (used & (depth - 1)), (used >> depth_log) & 1))) break;      // the item's first page, and in front of it the piece, which a warp alone has written itself
     const Piece x = pieces[item & (cap - 1)];
     const int r0 = 16 * member;
     const bool some = r0 < x.rows;      // this warp has rows
