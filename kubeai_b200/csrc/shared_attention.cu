@@ -4,12 +4,14 @@
 //
 // Softmax over two sets of keys is a weighted sum of softmaxes over each, so the rows of a group meet the shared pages in an item of their own and every request's rows the pages behind
 // them in another, and the two are joined by their maxima and sums.
-// An item is a key head and rows (row = token * group + head) with a range of keys.  Parts of up to 64 rows go to narrow CTAs, whose teams of 1, 2 or 4 warps have 16 rows a warp; the others to wide
+// An item is a key head and rows (row = token * group + head) with a range of keys.  Parts of up to 32 rows go to narrow CTAs, whose teams of 1 or 2 warps have 16 rows a warp; the others to wide
 // ones (shared_attention_wide.cuh).  One launch has both: its CTAs are shared out to the kinds by their work, and all items' keys of a kind, one behind the other, are cut into as many equal ranges as
-// it has teams or CTAs.  (In two launches, either waits for the other's SMs: 16 x 8 beams 79 us and 72.5 in one, 128 rows behind 2048 tokens 62 and 50.)
+// it has teams or CTAs.  (In two launches, either waits for the other's SMs: 16 x 8 beams 79 us and 72.5 in one, 128 rows behind 2048 tokens 62 and 51.)
 // A team walks its range without a gap: its first warp loads pages ahead by TMA (128-byte swizzle) into the team's ring, over an item's end, and all multiply with mma.sync: row tiles of 16 leave the
 // tensor cores idle in any form, and memory is what bounds this.
 // An item that a range's end cuts leaves unnormalised rows in the workspace, as every item does that shares its rows with another; a second kernel joins them in a fixed order.
+// 16 x 8 beams behind up to 4001 tokens, 273 MB: 72.5 us, of which the join has 6 and the first kernel 66, 4.1 TB/s (pages of random places by TMA reach 5.8 with nothing else to
+// do): the last team ends 15 % behind the mean one, as what each gets of the memory differs.  128 rows behind 2048 tokens, 144 MB: 50 to 51.  1 x 4 beams behind 450: 14.5, a chain of lengths, costs, ranges, page table, four pages, the rows' way out and the join.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -30,17 +32,17 @@ namespace {
 
 using namespace shared_attn;
 constexpr int kPageBytes = 2 * 16 * kD * 2;      // bytes of a page's keys and values of a head
-constexpr int kDepth = 2, kItems = 4, kLeast = 4;      // kDepth: pages a warp on their way; kItems: items a warp that those may lie in, and one; kLeast: pages of a range
-constexpr int kJoinThreads = 256, kAtOnce = 4;      // kAtOnce: parts of a row on their way
-// The two forms of the kernel: with CTAs that may be wide, one an SM; and without, three an SM, which begin sooner: 1 x 4 beams behind 450 tokens 16.3 us, and 18.1 us in the other form.
+constexpr int kDepth = 2, kItems = 4, kLeast = 4;      // kDepth: pages a warp on their way, 16 KB, 192 of an SM; kItems: items a warp that those may lie in, and one; kLeast: pages of a range
+constexpr int kJoinThreads = 256, kJoinWarps = kJoinThreads / 32, kAtOnce = 4, kJoinPlaces = 4;      // kAtOnce: parts of a row on their way; kJoinPlaces: CTAs an SM, one wave, up to which more warps have a row's head
+// The two forms of the kernel: with CTAs that may be wide, one an SM; and without, three an SM, which begin sooner: 1 x 4 beams behind 450 tokens took 16.3 us so, and 18.1 in the other form.
 template <bool kWide>
 struct Form {
-  static constexpr int kThreads = kWide ? wide::kThreads : 128, kWarps = kThreads / 32, kPlaces = wide::kThreads / kThreads, kKinds = kWide ? 4 : 3;
+  static constexpr int kThreads = kWide ? wide::kThreads : 128, kWarps = kThreads / 32, kPlaces = wide::kThreads / kThreads, kKinds = kWide ? 3 : 2;
   static constexpr int kRings = 1024 + kWarps * kDepth * kPageBytes, kSmem = kWide ? std::max(kRings, wide::kSmem) : kRings;
 };
-// What a page of each team, and a step of a wide CTA, take of an SM's time: by these the CTAs are shared out.  128 rows behind 2048 tokens, teams of one next to wide CTAs: 26 50 us, 12 62, 6 82.  16 x 8
-// beams, teams of one and two: 1.6 72.5 us, 2 77, 3 93, 1.3 74.  2 x 24 questions, a few teams of four next to wide CTAs: 8 256 us, 6 258, 3 426 (too few CTAs, which all others wait for).
-__device__ constexpr float kShare[4] = {1.f, 1.6f, 8.f, 26.f};
+// What a page of each team, and a step of a wide CTA, take of an SM's time: by these the CTAs are shared out.  Teams of one next to wide CTAs: 128 rows behind 2048 tokens 20 51.3 us, 23 50.6, 26 50, 30 50.7,
+// 12 62; 64 groups of 48 rows behind 450 106, 111, 114, 119; 4 of 160 rows behind 8000 59.5, 60.5, 64, 70.  Teams of one and two, 16 x 8 beams: 1.6 72.4 us, 1.5 73.5, 1.4 74, 2 77, 3 93.
+__device__ constexpr float kShare[3] = {1.f, 1.6f, 22.f};
 
 // An item's pages of a range, as the loads leave them for the products
 struct Piece {
@@ -100,13 +102,13 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     int left = gridDim.x, begin = 0;
 #pragma unroll
     for (int k = 0; k < kKinds; ++k) {
-      constexpr int kOrder[4] = {2, 1, 0, 3};
+      constexpr int kOrder[3] = {1, 0, 2};
       const int i = kOrder[k];
       int behind = 0;      // kinds behind it
 #pragma unroll
       for (int j = k + 1; j < kKinds; ++j) behind += costs.all[kOrder[j]] > 0;
       int count = costs.all[i] == 0 ? 0 : behind == 0 ? left : max(1, min(left - behind, static_cast<int>(ceilf(part[i] * each))));
-      if (i == 3) count = min(count, sizes.ctas);
+      if (i == 2) count = min(count, sizes.ctas);
       if (static_cast<int>(blockIdx.x) >= begin && static_cast<int>(blockIdx.x) < begin + count) kind = i, first_cta = begin, its = count;
       begin += count;
       left -= count;
@@ -115,8 +117,8 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   }
   const int cta = blockIdx.x - first_cta;
   if constexpr (kWide) {
-    if (kind == 3) {
-      const tree::Ranges ranges = find_ranges<kThreads>(n, Items(0, group), costs, 3, a.kv_heads, cta, its, 1, wide::kLeast, shares, &first, &count, s_range, s_where);
+    if (kind == 2) {
+      const tree::Ranges ranges = find_ranges<kThreads>(n, Items(0, group), costs, 2, a.kv_heads, cta, its, 1, wide::kLeast, shares, &first, &count, s_range, s_where);
       if (count) wide::walk(tm_q, tm_kv, a, sizes, scale_log2, error, smem, both.wide, n, ranges, cta, s_range[0], s_where);
       return;
     }
@@ -392,11 +394,15 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   if (!ok) *reinterpret_cast<volatile int*>(error) = 1;
 }
 
+// Bound by its dependent trips: places, maxima with four parts' outputs, further ones; six or eight parts at a time cost more registers and instructions than they save trips (16 x 8 beams 74 and 74.7 us).
 // A row: sum_p 2^(m_p - m) o_p / sum_p 2^(m_p - m) l_p over the parts, in order, four dimensions a lane; a lane has the maximum, sum and weight of one part in 32.
+struct Joined {
+  float m, sum;
+  float4 y;
+};
 template <typename At>
-__device__ __forceinline__ uint2 join_row(int parts, At part, int lane) {
-  float m = -INFINITY, sum = 0.f;
-  float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+__device__ __forceinline__ Joined join_parts(int parts, At part, int lane) {
+  Joined j = {-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
   for (int p0 = 0; p0 < parts; p0 += 32) {
     const int count = min(32, parts - p0);
     const float* mine = part(p0 + min(lane, count - 1));
@@ -410,27 +416,26 @@ __device__ __forceinline__ uint2 join_row(int parts, At part, int lane) {
     };
     const float2 st = lane < count ? *reinterpret_cast<const float2*>(mine + kD) : make_float2(-INFINITY, 0.f);
     load(0);
-    float top = fmaxf(m, st.x);
+    float top = fmaxf(j.m, st.x);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    const float base = top == -INFINITY ? 0.f : top, old = exp2f(m - base), w = exp2f(st.x - base);
-    m = top;
+    const float base = top == -INFINITY ? 0.f : top, old = exp2f(j.m - base), w = exp2f(st.x - base);
+    j.m = top;
     float l = w == 0.f && st.y == st.y ? 0.f : st.y * w;
 #pragma unroll
     for (int o = 16; o; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    sum = sum * old + l;
-    y = make_float4(y.x * old, y.y * old, y.z * old, y.w * old);
+    j.sum = j.sum * old + l;
+    j.y = make_float4(j.y.x * old, j.y.y * old, j.y.z * old, j.y.w * old);
     for (int k0 = 0; k0 < count; k0 += kAtOnce) {
       if (k0) load(k0);
 #pragma unroll
       for (int k = 0; k < kAtOnce; ++k) {
         const float wk = __shfl_sync(0xffffffffu, w, (k0 + k) & 31);
-        if (k0 + k < count && wk != 0.f) y = make_float4(fmaf(x[k].x, wk, y.x), fmaf(x[k].y, wk, y.y), fmaf(x[k].z, wk, y.z), fmaf(x[k].w, wk, y.w));
+        if (k0 + k < count && wk != 0.f) j.y = make_float4(fmaf(x[k].x, wk, j.y.x), fmaf(x[k].y, wk, j.y.y), fmaf(x[k].z, wk, j.y.z), fmaf(x[k].w, wk, j.y.w));
       }
     }
   }
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  return make_uint2(pack_bf16x2(y.x * inv, y.y * inv), pack_bf16x2(y.z * inv, y.w * inv));
+  return j;
 }
 
 // Whether all parts of a place lie in the workspace: not so where a wait ran out in front of it and it was not written
@@ -438,13 +443,16 @@ __device__ __forceinline__ bool in_bounds(const Place& p, const Sizes& sizes, in
   if (p.parts == 0) return true;
   const int team = p.flags / kTeam, behind = max(1, team);
   const long long first = p.slot, last = first - behind + 2ll * behind * (p.parts - 1), slots = 2ll * (team ? sizes.warps : sizes.ctas) - behind;
-  return p.parts > 0 && p.flags >= 0 && team <= 4 && first >= behind && first <= slots && last <= slots && p.row >= 0 && p.row <= (team ? team * kTile16 : kWideRows) - group;
+  return p.parts > 0 && p.flags >= 0 && team <= 2 && first >= behind && first <= slots && last <= slots && p.row >= 0 && p.row <= (team ? team * kTile16 : kWideRows) - group;
 }
 
-// A CTA has a row and eight of its heads.
+// kWarps have a head of a row, and every kWarps-th of its parts each: as many as leave one wave of CTAs.  1 x 4 beams behind 1500 tokens 20 us -> 15.3, behind 4000 31 -> 17.7; in two waves 128 rows behind
+// 2048 tokens 52.9, and 50.
+template <int kWarps>
 __global__ void __launch_bounds__(kJoinThreads)
 shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const Sizes sizes) {
-  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, head = blockIdx.y * (kJoinThreads / 32) + warp;
+  const int t = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, head = (blockIdx.y * kJoinWarps + warp) / kWarps, member = warp % kWarps;
+  __shared__ Joined joined[kWarps > 1 ? kJoinWarps : 1][32];
   // the lengths were there before the kernel in front of this one let it in
   griddep_launch();
   bool mine = false;
@@ -461,7 +469,7 @@ shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const S
   if (head >= a.q_heads) return;
   uint2* out = reinterpret_cast<uint2*>(static_cast<bf16*>(a.out) + static_cast<size_t>(t) * a.ldo + head * kD) + lane;
   if (!mine) {
-    if (a.zero_rest) *out = make_uint2(0, 0);
+    if (a.zero_rest && !member) *out = make_uint2(0, 0);
     return;
   }
   if (!own.parts && !(own.flags & kJoined)) return;      // written already
@@ -475,7 +483,28 @@ shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const S
     const int team = (first ? own.flags : shared.flags) / kTeam, behind = max(1, team);      // from a range's second slot to its first, and half of what lies between two ranges
     return (team ? space.narrow : space.wide) + (static_cast<size_t>(k ? slot - behind + 2 * behind * k : slot) * (team ? kTile16 : kWideRows) + row + head % group) * kLd;
   };
-  *out = join_row(n_all, part, lane);
+  Joined j;
+  if constexpr (kWarps > 1) {
+    joined[warp][lane] = join_parts((n_all + kWarps - 1 - member) / kWarps, [&](int p) { return part(p * kWarps + member); }, lane);
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / kWarps), "n"(kWarps * 32) : "memory");      // (a head's warps take every way together)
+    if (member) return;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) m = fmaxf(m, joined[warp + w][lane].m);
+    j = {m, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const Joined x = joined[warp + w][lane];
+      const float f = exp2f(x.m - base);
+      if (f == 0.f && x.sum == x.sum) continue;
+      j.sum += x.sum * f;
+      j.y = make_float4(fmaf(x.y.x, f, j.y.x), fmaf(x.y.y, f, j.y.y), fmaf(x.y.z, f, j.y.z), fmaf(x.y.w, f, j.y.w));
+    }
+  } else
+    j = join_parts(n_all, part, lane);
+  const float inv = j.sum == 0.f ? 0.f : 1.f / j.sum;
+  *out = make_uint2(pack_bf16x2(j.y.x * inv, j.y.y * inv), pack_bf16x2(j.y.z * inv, j.y.w * inv));
 }
 
 }  // namespace
@@ -515,7 +544,12 @@ int paged_attention_shared(const b200_shared_attn_args& a, int* error, cudaStrea
   };
   static std::atomic<unsigned long long> wide_done{0}, narrow_done{0};
   if (int rc = sizes.ctas ? launch(shared_attn_kernel<true>, Form<true>{}, &wide_done) : launch(shared_attn_kernel<false>, Form<false>{}, &narrow_done)) return rc;
-  launch_pdl(shared_attn_join_kernel, dim3(a.T, (a.q_heads + 7) / 8), dim3(kJoinThreads), 0, st, a, sizes);
+  auto join = [&](auto kernel, int warps) { launch_pdl(kernel, dim3(a.T, (a.q_heads * warps + kJoinWarps - 1) / kJoinWarps), dim3(kJoinThreads), 0, st, a, sizes); };
+  const long long most = static_cast<long long>(kJoinPlaces) * sm_count() * kJoinWarps, heads = static_cast<long long>(a.T) * a.q_heads;
+  if (heads * 8 <= most) join(shared_attn_join_kernel<8>, 8);
+  else if (heads * 4 <= most) join(shared_attn_join_kernel<4>, 4);
+  else if (heads * 2 <= most) join(shared_attn_join_kernel<2>, 2);
+  else join(shared_attn_join_kernel<1>, 1);
   return cudaGetLastError() == cudaSuccess ? 0 : -2;
 }
 

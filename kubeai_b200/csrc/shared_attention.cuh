@@ -12,7 +12,9 @@ namespace shared_attn {
 using beam::Lengths;
 using beam::Part;
 typedef __nv_bfloat16 bf16;
-constexpr int kD = 128, kTile16 = 16, kNarrow = 64;      // kNarrow: rows (token * group + head) of a part that go to narrow CTAs, whose warps have tiles of 16
+constexpr int kD = 128, kTile16 = 16, kNarrow = 2 * kTile16;
+// kNarrow: rows (token * group + head) of a part that go to narrow CTAs, whose warps have tiles of 16.  8 groups of 32 rows behind up to 4000 tokens take 46 us there and 41 in wide CTAs, behind up to 450, 64 of
+// them, 72 and 94; of 48 rows in teams of four warps 114 us, and 42 in wide CTAs, behind up to 450 137 and 113.
 constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
 constexpr int kWaitLimit = 1 << 22;
 
@@ -73,13 +75,13 @@ __device__ __forceinline__ Lengths lengths_of(const b200_shared_attn_args& a, St
   return n;
 }
 
-// ---- items: a part's key head and a block of its rows.  Parts of up to 64 rows go to narrow CTAs, to teams of 1, 2 or 4 warps with 16 rows each; the others (team 0) to wide ones, 256 rows
+// ---- items: a part's key head and a block of its rows.  Parts of up to 32 rows go to narrow CTAs, to teams of 1 or 2 warps with 16 rows each; the others (team 0) to wide ones, 256 rows
 // a block.  An item's keys come in units: pages, or steps of a wide CTA, which has two tiles of 128 scores at once: those of two row tiles and 128 keys where there are more than 128 rows, else of
 // one row tile and 256 keys.
-__device__ __forceinline__ int team_of(int rows) { return rows <= kTile16 ? 1 : rows <= 2 * kTile16 ? 2 : rows <= kNarrow ? 4 : 0; }
+__device__ __forceinline__ int team_of(int rows) { return rows <= kTile16 ? 1 : rows <= kNarrow ? 2 : 0; }
 struct Items {
   int team, group, bt, bt_log;      // bt: tokens of a block, a power of two
-  __device__ __forceinline__ Items(int team, int group) : team(team), group(group), bt_log((team ? 4 + (team > 1) + (team > 2) : 8) - (group > 1) - (group > 2) - (group > 4)) { bt = 1 << bt_log; }
+  __device__ __forceinline__ Items(int team, int group) : team(team), group(group), bt_log((team ? 4 + (team > 1) : 8) - (group > 1) - (group > 2) - (group > 4)) { bt = 1 << bt_log; }
   // whether a part of so many rows is this team's
   __device__ __forceinline__ bool has(const Part& p) const { return p.rows && team_of(p.rows * group) == team; }
   // part u, without rows where it is another team's
@@ -127,13 +129,13 @@ struct Item {
   }
 };
 
-// What the items of each kind cost, in front of a thread's share of the step's parts and in all.  Kinds: teams of 1, 2 and 4 warps, and wide CTAs.
+// What the items of each kind cost, in front of a thread's share of the step's parts and in all.  Kinds: teams of 1 and 2 warps, and wide CTAs.
 template <int kKinds>
 struct Costs {
   int per;      // parts of a share
   int before[kKinds], all[kKinds];
 };
-__device__ __forceinline__ int kind_team(int kind) { return kind == 3 ? 0 : 1 << kind; }
+__device__ __forceinline__ int kind_team(int kind) { return kind == 2 ? 0 : 1 << kind; }
 // ... with one barrier
 template <int kThreads, int kKinds>
 __device__ __forceinline__ void find_costs(const Lengths& n, int kv_heads, int group, int (*sums)[4], Costs<kKinds>* c) {
