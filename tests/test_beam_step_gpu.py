@@ -190,6 +190,21 @@ def test_long_and_short_parts(shared, own):
     Batch([(4, shared)], [own, own // 2 + 1, 1, own], [1] * 4, 1, 4, seed=shared).check()
 
 
+@pytest.mark.parametrize("S,rows", [(257, [1]), (700, [0, 1, 3, 1]), (1500, [1, 0, 0])])
+def test_more_requests_than_lie_in_shared_memory(S, rows):
+    groups = [(7, 32)] * (S // 7) + ([(S % 7, 16)] if S % 7 else [])
+    b = Batch(groups, [4 + s % 5 for s in range(S)], [rows[s % len(rows)] for s in range(S)], 2, 2, seed=S)
+    out = torch.full((b.T, b.heads * D), 3.0, device="cuda").bfloat16()
+    status = [2 if s % 11 == 5 else 0 for s in range(S)]      # some have no place in the cache
+    got = b.call(status=dev(status), out=out)
+    want, size = b.want()
+    for s, no in enumerate(status):
+        if no:
+            want[b.starts[s]:b.starts[s + 1]], size[b.starts[s]:b.starts[s + 1]] = 3.0, 0.0
+    assert got.data_ptr() == out.data_ptr()
+    near_attention(got, want, size)
+
+
 def test_long_chains_behind_a_document():
     Batch([(3, 3000), (2, 1000)], [40, 64, 70, 33, 90], [33, 64, 1, 7, 50], 2, 4, seed=3).check()
 
