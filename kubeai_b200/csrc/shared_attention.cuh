@@ -122,7 +122,7 @@ struct Item {
       if (++kvh >= kv_heads) {
         kvh = 0;
         do p = I.part(n, ++u);
-        while (p.rows == 0);      // (a range's units are some part's: the walk ends in front of the last)
+        while (p.rows == 0 && u + 1 < n.G + n.S);      // (a range's units are some part's, unless lengths change under the kernel)
       }
     }
     fill(I);
@@ -204,13 +204,13 @@ __device__ __forceinline__ tree::Ranges find_ranges(const Lengths& n, const Item
       for (;; ++u) {
         p = I.part(n, u);
         head = I.head_cost(p);
-        if (b < g0 + head * kv_heads) break;
+        if (b < g0 + head * kv_heads || u + 1 >= n.G + n.S) break;
         g0 += head * kv_heads;
       }
-      const int kvh = (b - g0) / head;
+      const int kvh = head ? min((b - g0) / head, kv_heads - 1) : 0;
       g0 += kvh * head;
       int block = 0, units = I.units_of(p, 0);
-      while (b >= g0 + units + tree::kItem) g0 += units + tree::kItem, units = I.units_of(p, ++block);
+      while (b >= g0 + units + tree::kItem && block + 1 < I.blocks_of(p)) g0 += units + tree::kItem, units = I.units_of(p, ++block);
       at = tree::snapped(b, g0, units, ranges.snap);
       if (!end) where[e][0] = u, where[e][1] = kvh, where[e][2] = block, where[e][3] = g0;
     }
