@@ -8,8 +8,9 @@
 // A CTA has a token; its first threads make the token's cosines and sines while the heads are on their way.  Sixteen lanes have a head, eight values each in two
 // pieces of four that hold both values of their pairs: (j, j + n / 4) where halves pair up, (2 j, 2 j + 1) where neighbours do.  Halves of a number of pairs that four does not
 // divide go through shared memory.
-// Memory bounds it: 8191 rows of 32 + 8 + 8 heads are 201 MB in and out, 42.8 us, 4.7 TB/s of 6.55 that a copy reaches.  Four rows are a launch and three dependent trips (slot and position, heads,
-// stores), 3.1 us; 999 rows 4.4.
+// Memory bounds it: 8191 rows of 32 + 8 + 8 heads are 201 MB in and out, 41.1 us, 4.9 TB/s of 6.55 that a copy reaches (42.8 when values went
+// through the norm's sums as well; two values an instruction took 63 registers, not 45, and 46 us).  Four rows are a launch and three dependent trips (slot and position, heads,
+// stores), 3.1 us; 999 rows 4.6.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
@@ -73,85 +74,90 @@ norm_rope_kernel(const b200_norm_rope_args a) {
     for (int k = 0; k < kAhead; ++k) {
       const int h = h0 + 2 * kWarps * k;
       if (h - (lane >> 4) >= heads) break;      // for both halves of the warp
-      Piece y0 = widen(u0[k]), y1 = widen(u1[k]);
-      const void* w = h < a.q_heads ? a.q_norm : a.k_norm;
-      float sum = 0.f;
+      uint2 r0 = u0[k], r1 = u1[k];      // values pass as they are, odd ones too
+      if (h - (lane >> 4) < turned) {
+        Piece y0 = widen(u0[k]), y1 = widen(u1[k]);
+        const void* w = h < a.q_heads ? a.q_norm : a.k_norm;
+        float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += y0.v[i] * y0.v[i] + y1.v[i] * y1.v[i];
+        for (int i = 0; i < 4; ++i) sum += y0.v[i] * y0.v[i] + y1.v[i] * y1.v[i];
 #pragma unroll
-      for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-      if (h < turned && w) {
-        const float inv = rsqrtf(sum * (1.f / kD) + a.eps);
-        const size_t at = static_cast<size_t>(h < a.q_heads ? h * a.q_norm_ld : (h - a.q_heads) * a.k_norm_ld);
-        Piece w0, w1;
-        if (a.norm_f32) {
-          const float4 f0 = reinterpret_cast<const float4*>(static_cast<const float*>(w) + at)[p0], f1 = reinterpret_cast<const float4*>(static_cast<const float*>(w) + at)[p1];
-          w0 = {f0.x, f0.y, f0.z, f0.w};
-          w1 = {f1.x, f1.y, f1.z, f1.w};
-        } else {
-          w0 = widen(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(w) + at)[p0]);
-          w1 = widen(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(w) + at)[p1]);
+        for (int o = 8; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (h < turned && w) {
+          const float inv = rsqrtf(sum * (1.f / kD) + a.eps);
+          const size_t at = static_cast<size_t>(h < a.q_heads ? h * a.q_norm_ld : (h - a.q_heads) * a.k_norm_ld);
+          Piece w0, w1;
+          if (a.norm_f32) {
+            const float4 f0 = reinterpret_cast<const float4*>(static_cast<const float*>(w) + at)[p0], f1 = reinterpret_cast<const float4*>(static_cast<const float*>(w) + at)[p1];
+            w0 = {f0.x, f0.y, f0.z, f0.w};
+            w1 = {f1.x, f1.y, f1.z, f1.w};
+          } else {
+            w0 = widen(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(w) + at)[p0]);
+            w1 = widen(reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(w) + at)[p1]);
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            y0.v[i] *= inv * w0.v[i];
+            y1.v[i] *= inv * w1.v[i];
+          }
         }
+        if (kStaged) {
+          float* row = stage[warp * 2 + (lane >> 4)];
+          __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          y0.v[i] *= inv * w0.v[i];
-          y1.v[i] *= inv * w1.v[i];
-        }
-      }
-      if (kStaged) {
-        float* row = stage[warp * 2 + (lane >> 4)];
-        __syncwarp();
+          for (int i = 0; i < 4; ++i) {
+            row[4 * p0 + i] = y0.v[i];
+            row[4 * p1 + i] = y1.v[i];
+          }
+          __syncwarp();
+          if (h < turned) {
+            auto turn_one = [&](int d, float& y) {
+              if (d >= 2 * n) return;
+              const float2 cs = turn[d < n ? d : d - n];
+              y = d < n ? y * cs.x - row[d + n] * cs.y : y * cs.x + row[d - n] * cs.y;
+            };
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          row[4 * p0 + i] = y0.v[i];
-          row[4 * p1 + i] = y1.v[i];
+            for (int i = 0; i < 4; ++i) {
+              turn_one(4 * p0 + i, y0.v[i]);
+              turn_one(4 * p1 + i, y1.v[i]);
+            }
+          }
+        } else if (h < turned) {
+          if (a.interleaved) {
+            auto turn_pair = [&](int pair, float& y, float& z) {
+              if (pair >= n) return;
+              const float2 cs = turn[pair];
+              const float was = y;
+              y = was * cs.x - z * cs.y;
+              z = z * cs.x + was * cs.y;
+            };
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              turn_pair(2 * p0 + i, y0.v[2 * i], y0.v[2 * i + 1]);
+              turn_pair(2 * p1 + i, y1.v[2 * i], y1.v[2 * i + 1]);
+            }
+          } else if (j < n / 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 cs = turn[4 * j + i];
+              const float was = y0.v[i];
+              y0.v[i] = was * cs.x - y1.v[i] * cs.y;
+              y1.v[i] = y1.v[i] * cs.x + was * cs.y;
+            }
+          }
         }
-        __syncwarp();
         if (h < turned) {
-          auto turn_one = [&](int d, float& y) {
-            if (d >= 2 * n) return;
-            const float2 cs = turn[d < n ? d : d - n];
-            y = d < n ? y * cs.x - row[d + n] * cs.y : y * cs.x + row[d - n] * cs.y;
-          };
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            turn_one(4 * p0 + i, y0.v[i]);
-            turn_one(4 * p1 + i, y1.v[i]);
-          }
-        }
-      } else if (h < turned) {
-        if (a.interleaved) {
-          auto turn_pair = [&](int pair, float& y, float& z) {
-            if (pair >= n) return;
-            const float2 cs = turn[pair];
-            const float was = y;
-            y = was * cs.x - z * cs.y;
-            z = z * cs.x + was * cs.y;
-          };
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            turn_pair(2 * p0 + i, y0.v[2 * i], y0.v[2 * i + 1]);
-            turn_pair(2 * p1 + i, y1.v[2 * i], y1.v[2 * i + 1]);
-          }
-        } else if (j < n / 4) {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 cs = turn[4 * j + i];
-            const float was = y0.v[i];
-            y0.v[i] = was * cs.x - y1.v[i] * cs.y;
-            y1.v[i] = y1.v[i] * cs.x + was * cs.y;
-          }
+          r0 = make_uint2(pack_bf16x2(y0.v[0], y0.v[1]), pack_bf16x2(y0.v[2], y0.v[3]));
+          r1 = make_uint2(pack_bf16x2(y1.v[0], y1.v[1]), pack_bf16x2(y1.v[2], y1.v[3]));
         }
       }
-      const uint2 r0 = make_uint2(pack_bf16x2(y0.v[0], y0.v[1]), pack_bf16x2(y0.v[2], y0.v[3])), r1 = make_uint2(pack_bf16x2(y1.v[0], y1.v[1]), pack_bf16x2(y1.v[2], y1.v[3]));
       uint2* to = nullptr;
       if (h < a.q_heads) to = reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + static_cast<size_t>(t) * a.ldo + h * kD);
       else if (h < heads && kept)      // a page has the heads' keys one behind the other, then the values
         to = reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.kv_layer) + ((static_cast<size_t>(slot >> 4) * 2 * a.kv_heads + (h - a.q_heads)) * 16 + (slot & 15)) * kD);
       if (to) {
-        const bool copied = h >= turned;      // values pass as they are, odd ones too
-        to[p0] = copied ? u0[k] : r0;
-        to[p1] = copied ? u1[k] : r1;
+        to[p0] = r0;
+        to[p1] = r1;
       }
     }
   }
