@@ -518,3 +518,55 @@ def test_layers_may_lie_apart():
     assert torch.equal(kv[::2, 2, :, :, :5], was[::2, 4, :, :, :5]) and torch.equal(kv[::2, 2, :, :, 5:], was[::2, 2, :, :, 5:])
     kv[::2, 2] = was[::2, 2]
     assert torch.equal(kv, was)
+
+
+# ------------------------------------------------------------------ calls of no size, and hints
+def test_calls_of_no_size():
+    from kubeai_b200 import ops
+    kv = torch.zeros(2, 2, 1, PAGE, D, device="cuda").bfloat16()
+    q = torch.ones(3, D, device="cuda").bfloat16()
+    none, table = dev([]), torch.zeros(0, 4, dtype=torch.int32, device="cuda")
+    y = ops.paged_attn_shared(q, kv, table, dev([0]), none, dev([0]), none, 1, 1, 1)
+    assert y.shape == (3, D) and not y.any()
+    kept = torch.ones(3, D, device="cuda").bfloat16()
+    ops.paged_attn_shared(q, kv, table, dev([0]), none, dev([0]), none, 1, 1, 1, out=kept)
+    assert bool((kept == 1).all())
+    assert ops.paged_attn_shared(q[:0], kv, table, dev([0]), none, dev([0]), none, 1, 1, 1).shape == (0, D)
+    turn = ops.rotary()
+    assert ops.norm_rope_kvwrite(torch.zeros(0, 3 * D, device="cuda").bfloat16(), none, none, kv, 1, 1, turn.freqs).shape == (0, D)
+    best = ops.beam_select(torch.zeros(0, 9, device="cuda"), torch.zeros(0, 4, device="cuda"))
+    assert best.parents.shape == (0, 4) and best.found_scores.shape == (0, 8)
+    moved = ops.beam_reorder(torch.zeros(0, 4, dtype=torch.int32, device="cuda"), none, none, table, None)
+    assert moved.block_tables.shape == (0, 4) and moved.shared.shape == (0,)
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("max_ctx", [0, 1, 600, 1 << 30])
+@pytest.mark.parametrize("max_rows", [3, 1000])
+def test_hints_do_not_change_what_is_attended(max_ctx, max_rows):
+    b = Batch([(40, 500), (3, 333)], [3 + 7 * s % 60 for s in range(43)], [1 + s % 3 for s in range(43)], 2, 4, seed=21)
+    b.check(max_ctx=max_ctx, max_rows=max_rows)
+
+
+def test_pages_behind_the_first_four_gigabytes():
+    from kubeai_b200 import ops
+    kvh, n = 8, 72000      # 2.36 * 10^9 values
+    kv = torch.zeros(1, n, 2, kvh, PAGE, D, dtype=torch.bfloat16, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    ends = [n - 1 - i for i in range(24)]
+    kv[0, dev(ends, torch.long)] = torch.randn(24, 2, kvh, PAGE, D, generator=gen, device="cuda").bfloat16()
+    # four beams behind three shared pages, each with its own fourth
+    tables = [[ends[0], ends[1], ends[2], ends[3 + s]] for s in range(4)]
+    q = torch.randn(4, kvh * 4 * D, generator=gen, device="cuda").bfloat16()
+    small = kv[0, dev(ends, torch.long)]
+    near = [[0, 1, 2, 3 + s] for s in range(4)]
+    args = (dev([0, 1, 2, 3, 4]), dev([52, 53, 51, 55]), dev([0, 4]), dev([48]), 32, 8, 1)
+    assert torch.equal(ops.paged_attn_shared(q, kv[0], dev(tables), *args), ops.paged_attn_shared(q, small, dev(near), *args))
+    # rows into them
+    qkv = torch.randn(2, (32 + 16) * D, generator=gen, device="cuda").bfloat16()
+    ops.norm_rope_kvwrite(qkv, dev([3, 4]), dev([ends[10] * PAGE + 5, ends[11] * PAGE + 15]), kv[0], 32, 8, ops.rotary().freqs)
+    assert torch.equal(kv[0, ends[10], 1, :, 5], qkv[0, 40 * D:].view(8, D)) and torch.equal(kv[0, ends[11], 1, :, 15], qkv[1, 40 * D:].view(8, D))
+    # and from one to another
+    moved = ops.beam_reorder(dev([[0, 0, 2, 3]]), dev([[1, 2, 3, 4]]), dev([53] * 4), dev(tables), kv)
+    assert moved.block_tables.tolist() == tables
+    assert torch.equal(kv[0, ends[4], :, :, :5], small[3, :, :, :5]) and torch.equal(kv[0, ends[4], :, :, 5:], small[4, :, :, 5:])
