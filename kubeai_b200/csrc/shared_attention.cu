@@ -115,18 +115,19 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     }
     if (static_cast<int>(blockIdx.x) >= begin) return;      // nothing that it might have
   }
-  const int cta = blockIdx.x - first_cta;
+  // (one look for the ranges of either half: what comes once costs its instructions' way from memory)
+  const int cta = blockIdx.x - first_cta, team = kind_team(kind), streams = team ? kWarps >> kind : 1;
+  static_assert(kLeast == wide::kLeast, "");
+  const Items I(team, group);
+  const tree::Ranges ranges = find_ranges<kThreads>(n, I, costs, kind, a.kv_heads, cta, its, streams, kLeast, shares, &first, &count, s_range, s_where);
   if constexpr (kWide) {
-    if (kind == 2) {
-      const tree::Ranges ranges = find_ranges<kThreads>(n, Items(0, group), costs, 2, a.kv_heads, cta, its, 1, wide::kLeast, shares, &first, &count, s_range, s_where);
+    if (!team) {
       if (count) wide::walk(tm_q, tm_kv, a, sizes, scale_log2, error, smem, both.wide, n, ranges, cta, s_range[0], s_where);
       return;
     }
   }
   if (tid < kWarps * kItems) both.narrow.odd[tid] = -1;
-  const int team = 1 << kind;
-  const Items I(team, group);
-  const int stream = warp >> kind, member = warp & (team - 1), streams = kWarps >> kind;
+  const int stream = warp >> kind, member = warp & (team - 1);
   static_assert(kDepth == 2, "");
   const int depth = kDepth * team, depth_log = kind + 1, cap = kItems * team;
   const uint32_t ring = sbase + stream * depth * kPageBytes, full0 = smem_u32(both.narrow.bars[0] + stream * depth), empty0 = smem_u32(both.narrow.bars[1] + stream * depth);
@@ -140,7 +141,6 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     fence_mbar_init();
     tma_prefetch_desc(&tm_kv);
   }
-  const tree::Ranges ranges = find_ranges<kThreads>(n, I, costs, kind, a.kv_heads, cta, its, streams, kLeast, shares, &first, &count, s_range, s_where);
   __syncthreads();
   const int gs = first + stream;      // the team's range
   const int left = stream < count ? s_range[stream][1] - s_range[stream][0] : 0;

@@ -147,11 +147,9 @@ __device__ __forceinline__ void find_costs(const Lengths& n, int kv_heads, int g
   for (int i = 0; i < kKinds; ++i) own[i] = 0;
   for (int u = tid * per; u < end; ++u) {
     const Part p = beam::part_of(n, u);
+    const int team = team_of(p.rows * group), cost = p.rows ? Items(team, group).head_cost(p) * kv_heads : 0;
 #pragma unroll
-    for (int i = 0; i < kKinds; ++i) {
-      const Items I(kind_team(i), group);
-      if (I.has(p)) own[i] += I.head_cost(p) * kv_heads;
-    }
+    for (int i = 0; i < kKinds; ++i) own[i] += team == kind_team(i) ? cost : 0;
   }
 #pragma unroll
   for (int i = 0; i < kKinds; ++i) {
