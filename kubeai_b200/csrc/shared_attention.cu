@@ -58,6 +58,7 @@ template <int kWarps>
 struct Narrow {
   uint64_t bars[2][kWarps * kDepth];
   Piece pieces[kWarps * kItems];
+  Item items[kWarps];            // where the loads of each team are: kept here, as registers are wanted for the products
   int odd[kWarps * kItems];      // the last item of each piece's place with infinities or NaN among values that some row does not see
 };
 template <bool kWide> union Halves;
@@ -149,14 +150,22 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   const int slot = (first_cta * kWarps + gs * team) * 2;      // of 16 rows: the range's first item, a team's tiles behind it the last
 
   // ---- loads (the team's first warp): item, its first page here, the range's cost to go
-  Item it;
-  it.u = s_where[stream][0]; it.kvh = s_where[stream][1]; it.block = s_where[stream][2];
-  it.p = I.part(n, it.u);
-  it.fill(I);
+  Item& it = both.narrow.items[stream];
+  if (member == 0 && lane == 0) {
+    it.u = s_where[stream][0]; it.kvh = s_where[stream][1]; it.block = s_where[stream][2];
+    it.p = I.part(n, it.u);
+    it.fill(I);
+  }
+  auto go_on = [&] {
+    __syncwarp();
+    if (lane == 0) it.next(n, I, a.kv_heads);
+    __syncwarp();
+  };
+  __syncwarp();
   int t0 = max(0, s_range[stream][0] - s_where[stream][3] - tree::kItem), rest = left;
-  if (t0 == it.units) {              // the range begins where the item in front of it ends
+  if (member == 0 && t0 == it.units) {              // the range begins where the item in front of it ends
     t0 = 0;
-    it.next(n, I, a.kv_heads);
+    go_on();
   }
   bool more = true, ok = true;
   int take = 0, at = 0, items = 0, issued = 0, mine = 0, next = 0;      // the item's pages here, the page that is next; items so far; pages so far
@@ -199,7 +208,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     if (at == take) {
       if (rest <= 0) { more = false; return; }
       t0 = 0;
-      it.next(n, I, a.kv_heads);
+      go_on();
       begin();
     } else if (at && at % 32 == 0) {
       mine = next;
