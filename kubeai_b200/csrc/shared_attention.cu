@@ -239,9 +239,10 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   int used = 0;
   for (int item = 0; ok; ++item) {
     if (team > 1 && !(ok = warp_wait(full0 + 8 * (used & (depth - 1)), (used >> depth_log) & 1))) break;      // the item's first page, and in front of it the piece, which a warp alone has written itself
-    const Piece x = pieces[item & (cap - 1)];
+    const Piece& x = pieces[item & (cap - 1)];      // (its place is used again some items on)
+    const int rows = x.rows, first_key = x.key, pages_here = x.pages, see = x.see, end = x.end;
     const int r0 = 16 * member;
-    const bool some = r0 < x.rows;      // this warp has rows
+    const bool some = r0 < rows;      // this warp has rows
     // queries: rows nobody owns are zeros
     uint32_t qa[8][4];
     const bf16* q = static_cast<const bf16*>(a.q) + x.kvh * group * kD + q2;
@@ -251,8 +252,8 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       const bf16* from = q + static_cast<size_t>(x.row0 + (r >> shift)) * a.ldq + (r & (group - 1)) * kD;
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
-        qa[ks][h] = r < x.rows ? *reinterpret_cast<const uint32_t*>(from + ks * 16) : 0u;
-        qa[ks][2 + h] = r < x.rows ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 8) : 0u;
+        qa[ks][h] = r < rows ? *reinterpret_cast<const uint32_t*>(from + ks * 16) : 0u;
+        qa[ks][2 + h] = r < rows ? *reinterpret_cast<const uint32_t*>(from + ks * 16 + 8) : 0u;
       }
     }
     float o[16][4];
@@ -261,21 +262,21 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
 #pragma unroll
       for (int c = 0; c < 4; ++c) o[d][c] = 0.f;
     float ref[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};      // what the weights are relative to, in units of log 2; this thread's part of their sum
-    const int limit[2] = {min(x.see + ((r0 + g) >> shift), x.end), min(x.see + ((r0 + g + 8) >> shift), x.end)};
-    for (int j = 0; j < x.pages; ++j, ++used) {
-      const int st = used & (depth - 1), key0 = x.key + 16 * j;
+    const int limit[2] = {min(see + ((r0 + g) >> shift), end), min(see + ((r0 + g + 8) >> shift), end)};
+    for (int j = 0; j < pages_here; ++j, ++used) {
+      const int st = used & (depth - 1), key0 = first_key + 16 * j;
       if (!(ok = warp_wait(full0 + 8 * st, (used >> depth_log) & 1))) break;
       const uint32_t ks_ = ring + st * kPageBytes, vs_ = ks_ + 4096;
       if (some) {
-      if (key0 + 16 > x.see) {
+      if (key0 + 16 > see) {
         // what must not meet a weight of zero: values behind the last key, and infinities and NaN among values that some row does not see, which those that do add at the end
         uint4* v = reinterpret_cast<uint4*>(smem + (vs_ - sbase));
         for (int e = lane; e < 256; e += 32) {
           bool found;
           const int key = key0 + ((e & 127) >> 3);      // (a row's pieces in some order)
-          if (key < x.see) continue;
+          if (key < see) continue;
           uint4 w = v[e];
-          if (key >= x.end) w = make_uint4(0, 0, 0, 0);
+          if (key >= end) w = make_uint4(0, 0, 0, 0);
           else {
             const uint4 was = w;
             w = make_uint4(without_odd(w.x), without_odd(w.y), without_odd(w.z), without_odd(w.w));
@@ -300,7 +301,7 @@ shared_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
         mma_bf16_16816(s[0], qa[ks], b0, b1);
         mma_bf16_16816(s[1], qa[ks], b2, b3);
       }
-      if (key0 + 16 > x.see) {
+      if (key0 + 16 > see) {
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
