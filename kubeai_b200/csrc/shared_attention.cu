@@ -42,7 +42,7 @@ struct Form {
 };
 // What a page of each team, and a step of a wide CTA, take of an SM's time: by these the CTAs are shared out.  Teams of one next to wide CTAs: 128 rows behind 2048 tokens 20 51.3 us, 23 50.6, 26 50, 30 50.7,
 // 12 62; 64 groups of 48 rows behind 450 106, 111, 114, 119; 4 of 160 rows behind 8000 59.5, 60.5, 64, 70.  Teams of one and two, 16 x 8 beams: 1.6 72.4 us, 1.5 73.5, 1.4 74, 2 77, 3 93.
-__device__ constexpr float kShare[3] = {1.f, 1.6f, 22.f};
+__device__ constexpr float kShare[3] = {1.f, 1.6f, 26.f};
 
 // An item's pages of a range, as the loads leave them for the products
 struct Piece {
