@@ -6,12 +6,14 @@
 // them in another, and the two are joined by their maxima and sums.
 // An item is a key head and rows (row = token * group + head) with a range of keys.  Parts of up to 32 rows go to narrow CTAs, whose teams of 1 or 2 warps have 16 rows a warp; the others to wide
 // ones (shared_attention_wide.cuh).  One launch has both: its CTAs are shared out to the kinds by their work, and all items' keys of a kind, one behind the other, are cut into as many equal ranges as
-// it has teams or CTAs.  (In two launches, either waits for the other's SMs: 16 x 8 beams 79 us and 72.5 in one, 128 rows behind 2048 tokens 62 and 51.)
+// it has teams or CTAs.  (In two launches, either waits for the other's SMs: 16 x 8 beams took 79 us so and 72.5 in one, 128 rows behind 2048 tokens 62 and 50.)
 // A team walks its range without a gap: its first warp loads pages ahead by TMA (128-byte swizzle) into the team's ring, over an item's end, and all multiply with mma.sync: row tiles of 16 leave the
 // tensor cores idle in any form, and memory is what bounds this.
 // An item that a range's end cuts leaves unnormalised rows in the workspace, as every item does that shares its rows with another; a second kernel joins them in a fixed order.
-// 16 x 8 beams behind up to 4001 tokens, 273 MB: 72.5 us, of which the join has 6 and the first kernel 66, 4.1 TB/s (pages of random places by TMA reach 5.8 with nothing else to
-// do): the last team ends 15 % behind the mean one, as what each gets of the memory differs.  128 rows behind 2048 tokens, 144 MB: 50 to 51.  1 x 4 beams behind 450: 14.5, a chain of lengths, costs, ranges, page table, four pages, the rows' way out and the join.
+// 16 x 8 beams behind up to 4001 tokens, 273 MB: 67.4 us, of which the join has 6 and the first kernel 61, 4.5 TB/s (pages of random places by TMA reach 5.8 with nothing else to do): the last team ends 15 %
+// behind the mean one, as what each gets of the memory differs.  128 rows behind 2048 tokens, 144 MB: 48.5.  64 x 8 beams behind up to 450, 173 MB: 62.7; three warps a scheduler wait on their own chains
+// (products, maxima, exponentials, products), at two of three a page's time, and 168 registers leave no more.  What the loads know of their place lies in shared memory: in registers it spilled others (72).
+// 1 x 4 beams behind 450: 13.8, a chain of lengths, costs, ranges (4 us of them, most of it instructions' first way from memory), page table, four pages, the rows' way out and the join.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -40,8 +42,9 @@ struct Form {
   static constexpr int kThreads = kWide ? wide::kThreads : 128, kWarps = kThreads / 32, kPlaces = wide::kThreads / kThreads, kKinds = kWide ? 3 : 2;
   static constexpr int kRings = 1024 + kWarps * kDepth * kPageBytes, kSmem = kWide ? std::max(kRings, wide::kSmem) : kRings;
 };
-// What a page of each team, and a step of a wide CTA, take of an SM's time: by these the CTAs are shared out.  Teams of one next to wide CTAs: 128 rows behind 2048 tokens 20 51.3 us, 23 50.6, 26 50, 30 50.7,
-// 12 62; 64 groups of 48 rows behind 450 106, 111, 114, 119; 4 of 160 rows behind 8000 59.5, 60.5, 64, 70.  Teams of one and two, 16 x 8 beams: 1.6 72.4 us, 1.5 73.5, 1.4 74, 2 77, 3 93.
+// What a page of each team, and a step of a wide CTA, take of an SM's time: by these the CTAs are shared out.  Teams of one next to wide CTAs: 128 rows behind 2048 tokens 22 52 us, 24 51.2, 26 48.5, 28 48.7;
+// 64 groups of 48 rows behind 450 96.1, 96.8, 97.5, 100.9; 4 of 160 rows behind 8000 56.5, 56.2, 56.5, 58.6.  Teams of one and two: 16 x 8 beams 1.4 66.9, 1.6 67.3, 1.8 70.9, 64 x 8 behind 450 63.6, 62.7,
+// 62.5.
 __device__ constexpr float kShare[3] = {1.f, 1.6f, 26.f};
 
 // An item's pages of a range, as the loads leave them for the products
@@ -456,8 +459,8 @@ __device__ __forceinline__ bool in_bounds(const Place& p, const Sizes& sizes, in
   return p.parts > 0 && p.flags >= 0 && team <= 2 && first >= behind && first <= slots && last <= slots && p.row >= 0 && p.row <= (team ? team * kTile16 : kWideRows) - group;
 }
 
-// kWarps have a head of a row, and every kWarps-th of its parts each: as many as leave one wave of CTAs.  1 x 4 beams behind 1500 tokens 20 us -> 15.3, behind 4000 31 -> 17.7; in two waves 128 rows behind
-// 2048 tokens 52.9, and 50.
+// kWarps have a head of a row, and every kWarps-th of its parts each: as many as leave one wave of CTAs.  1 x 4 beams behind 1500 tokens 20 us -> 15.3, behind 4000 31 -> 17.7 (14.3 and
+// 16.8 since); in two waves 128 rows behind 2048 tokens took 52.9, and 50 in one.
 template <int kWarps>
 __global__ void __launch_bounds__(kJoinThreads)
 shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const Sizes sizes) {
