@@ -2,8 +2,8 @@
 // (shared_attention.cu has the parts, the joining and what parts of few rows take).
 //
 // An item is a part's key head and up to 256 of its rows (row = token * group + head).  Every step forms two tiles of scores, 128 rows by 128 keys: of two row tiles that share 128 keys, or
-// where there are no more than 128 rows of one row tile and 256 keys.  All items' steps one behind the other are cut into as many equal ranges as there are SMs, and a CTA walks its range without
-// a gap:
+// where there are no more than 128 rows of one row tile and 256 keys.  All items' steps one behind the other are cut into as many equal ranges as there are CTAs of this kind, one an SM, and
+// a CTA walks its range without a gap:
 //   a warp looks pages up and loads by TMA, 128-byte swizzle: queries, and tiles of 128 keys or values into a ring of four;
 //   a warp issues tcgen05.mma: S_g = Q K^T and O_g += P_g V (M = N = 128), P_g in TMEM over its scores: the next scores of one tile are formed under the other's softmax;
 //   two groups of four warps (thread = row) do the softmax in fp32, base 2; a warp whose rows nobody owns only keeps step.
