@@ -449,6 +449,15 @@ def rotary(dims=128, base=10000.0, scaling=None, device="cuda") -> Rotary:
     return Rotary(torch.tensor(f, dtype=torch.float64, device=device), gain)
 
 
+def _norm(at, w, heads, what):
+    """How far apart the heads' weights are; -1 without any."""
+    if w is None:
+        return -1
+    if w.dtype not in _LOGITS or w.get_device() != at or not w.is_contiguous() or w.shape not in ((128,), (heads, 128)):
+        raise _refused(f"{what}: contiguous bf16 or fp32 [128] or [{heads}, 128] on cuda:{at}, got {w.dtype} {tuple(w.shape)} on {w.device}")
+    return 128 if w.dim() == 2 else 0
+
+
 def norm_rope_kvwrite(qkv, positions, slots, kv_layer, q_heads, kv_heads, freqs, gain=1.0, q_norm=None, k_norm=None, eps=1e-6, interleaved=False, out=None):
     """Norms of queries and keys for each head, rotary positions in the same pass, and keys and values into the paged cache (b200_op_norm_rope_kvwrite).
     qkv: bf16 [T, at least (q_heads + 2 kv_heads) * 128], rows may be a wider buffer's leading columns; positions, slots: int32 [T], a slot of -1 is written nowhere;
@@ -462,16 +471,10 @@ def norm_rope_kvwrite(qkv, positions, slots, kv_layer, q_heads, kv_heads, freqs,
     _ints(at, positions, slots), _sized(positions, T, "positions"), _sized(slots, T, "slots")
     if freqs.dtype is not torch.float64 or freqs.get_device() != at or not freqs.is_contiguous() or freqs.dim() != 1 or freqs.numel() > 64:
         raise _refused(f"freqs: contiguous fp64 [0 to 64] on cuda:{at}, got {freqs.dtype} {tuple(freqs.shape)} on {freqs.device}")
-    lds, kinds = [0, 0], set()
-    for k, (w, heads, what) in enumerate(((q_norm, q_heads, "q_norm"), (k_norm, kv_heads, "k_norm"))):
-        if w is None:
-            continue
-        if w.dtype not in _LOGITS or w.get_device() != at or not w.is_contiguous() or tuple(w.shape) not in ((128,), (heads, 128)):
-            raise _refused(f"{what}: contiguous bf16 or fp32 [128] or [{heads}, 128] on cuda:{at}, got {w.dtype} {tuple(w.shape)} on {w.device}")
-        lds[k] = 128 if w.dim() == 2 else 0
-        kinds.add(w.dtype)
-    if len(kinds) > 1:
+    ldq, ldk = _norm(at, q_norm, q_heads, "q_norm"), _norm(at, k_norm, kv_heads, "k_norm")
+    if q_norm is not None and k_norm is not None and q_norm.dtype is not k_norm.dtype:
         raise _refused("q_norm and k_norm are of one type")
+    f32 = (k_norm if q_norm is None else q_norm).dtype is torch.float32 if ldq >= 0 or ldk >= 0 else False
     if out is None:
         out = qkv.new_empty((T, q_heads * 128))
         ldo = q_heads * 128
@@ -481,7 +484,7 @@ def norm_rope_kvwrite(qkv, positions, slots, kv_layer, q_heads, kv_heads, freqs,
             raise _refused(f"out has {out.shape[0]} rows, not {T}")
     if (T | ldx | ldo) >> 31:
         raise _refused(_WIDE)
-    a = NormRopeArgs(T, q_heads, kv_heads, ldx, ldo, 2 * freqs.numel(), bool(interleaved), lds[0], lds[1], torch.float32 in kinds, eps, gain, kv_layer.shape[0],
+    a = NormRopeArgs(T, q_heads, kv_heads, ldx, ldo, 2 * freqs.numel(), bool(interleaved), max(ldq, 0), max(ldk, 0), f32, eps, gain, kv_layer.shape[0],
                      qkv.data_ptr(), out.data_ptr(), kv_layer.data_ptr(), positions.data_ptr(), slots.data_ptr(), freqs.data_ptr(), _ptr(q_norm), _ptr(k_norm))
     check(lib().b200_op_norm_rope_kvwrite(C.byref(a), torch._C._cuda_getCurrentRawStream(at)))
     return out
