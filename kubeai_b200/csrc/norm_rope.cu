@@ -48,7 +48,8 @@ norm_rope_kernel(const b200_norm_rope_args a) {
   const bool beside = a.interleaved || kStaged;
   const int p0 = beside ? 2 * j : j < n / 4 ? j : 2 * j, p1 = beside ? 2 * j + 1 : j < n / 4 ? j + n / 4 : 2 * j + 1;
   bool first = true;
-  for (int h0 = warp * 2 + (lane >> 4); h0 - (lane >> 4) < heads; h0 += 2 * kWarps * kAhead) {
+  int h0 = warp * 2 + (lane >> 4);
+  do {      // once for every warp: one that has no heads has pairs of the table
     uint2 u0[kAhead], u1[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
@@ -160,7 +161,8 @@ norm_rope_kernel(const b200_norm_rope_args a) {
         to[p1] = r1;
       }
     }
-  }
+    h0 += 2 * kWarps * kAhead;
+  } while (h0 - (lane >> 4) < heads);
 }
 
 }  // namespace

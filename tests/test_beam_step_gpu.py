@@ -570,3 +570,12 @@ def test_pages_behind_the_first_four_gigabytes():
     moved = ops.beam_reorder(dev([[0, 0, 2, 3]]), dev([[1, 2, 3, 4]]), dev([53] * 4), dev(tables), kv)
     assert moved.block_tables.tolist() == tables
     assert torch.equal(kv[0, ends[4], :, :, :5], small[3, :, :, :5]) and torch.equal(kv[0, ends[4], :, :, 5:], small[4, :, :, 5:])
+
+
+# ------------------------------------------------------------------ rotation of few heads, and far positions
+@pytest.mark.parametrize("heads,kvh", [(0, 1), (1, 0), (2, 0), (0, 2), (1, 1)])
+@pytest.mark.parametrize("dims,interleaved", [(128, False), (128, True), (72, False), (66, False), (96, True)])
+@pytest.mark.parametrize("T", [3, 2050])
+def test_rotation_of_one_or_two_heads(T, heads, kvh, dims, interleaved):
+    """The first warps alone have heads, and all pairs' angles are wanted."""
+    turned(T, heads, kvh, dims, interleaved, "one", 4000, seed=heads + dims)
