@@ -412,16 +412,28 @@ class Rotary(NamedTuple):
     gain: float
 
 
+# What a configuration's rope_scaling may say: keys of every type, and of each
+_SCALING_KEYS = {"rope_type", "type", "rope_theta", "partial_rotary_factor", "original_max_position_embeddings"}
+_SCALING_KEYS_OF = {"default": set(), "linear": {"factor"}, "llama3": {"factor", "low_freq_factor", "high_freq_factor"},
+                    "yarn": {"factor", "beta_fast", "beta_slow", "attention_factor", "mscale", "mscale_all_dim", "truncate"}}
+
+
 def rotary(dims=128, base=10000.0, scaling=None, device="cuda") -> Rotary:
     """Radians a position (fp64) of each of dims / 2 pairs and the factor on what they turn, for norm_rope_kvwrite.  scaling: a configuration's `rope_scaling` as a dict, of type default, linear
-    (factor), llama3 (factor, low_freq_factor, high_freq_factor, original_max_position_embeddings) or yarn (factor, original_max_position_embeddings; beta_fast, beta_slow, attention_factor)."""
+    (factor), llama3 (factor, low_freq_factor, high_freq_factor, original_max_position_embeddings) or yarn (factor, original_max_position_embeddings; beta_fast, beta_slow, truncate, and
+    attention_factor or mscale with mscale_all_dim).  A value of None counts as not there; other keys are refused, and a rope_theta or partial_rotary_factor that says otherwise than base and dims."""
     if dims < 0 or dims > 128 or dims % 2 or not base > 0:
         raise _refused(f"an even number of up to 128 values of a head is turned, with a base above 0: got {dims}, {base}")
     f = [base ** (-2 * i / dims) for i in range(dims // 2)]
-    scaling = scaling or {}
+    scaling = {k: v for k, v in (scaling or {}).items() if v is not None}
     kind, gain = scaling.get("rope_type", scaling.get("type", "default")), 1.0
-    if kind not in ("default", "linear", "llama3", "yarn"):
+    if kind not in _SCALING_KEYS_OF:
         raise _refused(f"rope scaling type {kind!r} is not supported (default, linear, llama3, yarn)")
+    unknown = sorted(set(scaling) - _SCALING_KEYS - _SCALING_KEYS_OF[kind])
+    if unknown:
+        raise _refused(f"rope scaling {kind!r} with {', '.join(map(repr, unknown))} is not supported")
+    if scaling.get("rope_theta", base) != base or int(128 * scaling.get("partial_rotary_factor", dims / 128)) != dims:
+        raise _refused(f"rope scaling {scaling} says otherwise than a base of {base} and {dims} of 128 values")
     try:
         if kind != "default":
             factor = float(scaling["factor"])
@@ -436,16 +448,22 @@ def rotary(dims=128, base=10000.0, scaling=None, device="cuda") -> Rotary:
             f = [x / factor * (1 - p) + x * p for x, p in zip(f, part)]
         elif kind == "yarn":
             length, fast, slow = float(scaling["original_max_position_embeddings"]), float(scaling.get("beta_fast", 32)), float(scaling.get("beta_slow", 1))
-            at = [dims * math.log(length / (2 * math.pi * turns)) / (2 * math.log(base)) for turns in (fast, slow)]
-            lo, hi = max(0, math.floor(at[0])), min(dims - 1, math.ceil(at[1]))
-            part = [min(1.0, max(0.0, (i - lo) / max(hi - lo, 0.001))) for i in range(dims // 2)]
+            lo, hi = (dims * math.log(length / (2 * math.pi * turns)) / (2 * math.log(base)) for turns in (fast, slow))
+            if scaling.get("truncate", True):
+                lo, hi = math.floor(lo), math.ceil(hi)
+            lo, hi = max(0, lo), min(dims - 1, hi)
+            hi = hi if hi != lo else hi + 0.001
+            part = [min(1.0, max(0.0, (i - lo) / (hi - lo))) for i in range(dims // 2)]
             f = [x / factor * p + x * (1 - p) for x, p in zip(f, part)]
-            gain = scaling.get("attention_factor")
-            gain = float(gain) if gain is not None else 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+            grown = lambda m: 0.1 * m * math.log(factor) + 1 if factor > 1 else 1.0      # noqa: E731
+            both = float(scaling.get("mscale", 0)), float(scaling.get("mscale_all_dim", 0))
+            gain = float(scaling["attention_factor"]) if "attention_factor" in scaling else grown(both[0]) / grown(both[1]) if all(both) else grown(1.0)
     except KeyError as e:
         raise _refused(f"rope scaling {kind!r} lacks {e.args[0]!r}") from None
     except ZeroDivisionError:
         raise _refused(f"rope scaling {kind!r} of {scaling} with base {base} divides by zero") from None
+    except (TypeError, ValueError, OverflowError):
+        raise _refused(f"rope scaling {kind!r} of {scaling} with base {base} has values that it cannot be made of") from None
     return Rotary(torch.tensor(f, dtype=torch.float64, device=device), gain)
 
 

@@ -189,3 +189,48 @@ def test_gain_of_yarn():
     y = dict(type="yarn", factor=32.0, original_max_position_embeddings=4096)
     assert math.isclose(ops.rotary(128, 1e4, y, device="cpu").gain, 0.1 * math.log(32) + 1)
     assert ops.rotary(128, 1e4, y | dict(attention_factor=1.5), device="cpu").gain == 1.5
+
+
+def configured(dims, base, scaling):
+    """Frequencies and gain as transformers makes them of a configuration, in 32 bits."""
+    from transformers import LlamaConfig
+    from transformers.modeling_rope_utils import ROPE_INIT_FUNCTIONS
+    cfg = LlamaConfig(hidden_size=dims, num_attention_heads=1, head_dim=dims, max_position_embeddings=131072, rope_theta=base, rope_scaling=scaling | dict(rope_theta=base))
+    f, gain = ROPE_INIT_FUNCTIONS[scaling["rope_type"]](cfg, "cpu")
+    return f.double().numpy(), gain
+
+
+YARN = dict(rope_type="yarn", factor=32.0, original_max_position_embeddings=4096)
+
+
+@pytest.mark.parametrize("dims,base,more", [
+    (64, 150000.0, dict(truncate=False)), (64, 150000.0, dict(truncate=True)), (128, 10000.0, dict(truncate=False, beta_fast=20.0, beta_slow=2.0)), (128, 1e6, dict(truncate=False, factor=4.0)),
+    (64, 10000.0, dict(mscale=1.0, mscale_all_dim=1.0, factor=40.0)), (64, 10000.0, dict(mscale=0.707, mscale_all_dim=1.0, factor=40.0)), (64, 10000.0, dict(mscale=0.707, factor=40.0)),
+    (64, 10000.0, dict(mscale_all_dim=0.5)), (64, 10000.0, dict(mscale=0, mscale_all_dim=0)), (128, 10000.0, dict(mscale=1.0, mscale_all_dim=0.707, attention_factor=1.5)),
+    (128, 10000.0, dict(attention_factor=None, beta_fast=None, mscale=None, truncate=False)), (128, 10000.0, dict(factor=1.0, mscale=2.0, mscale_all_dim=1.0))])
+def test_further_forms_of_yarn(dims, base, more):
+    """2^-20 for the 32 bits of the other side (a power, its quotient, two products and a sum), and what its ramp p loses: an end of up to 2^6 is rounded by 2^-19 where the ramp is longer than 2^3, p
+    and 1 - p by 2^-24 each, so 1 - p is off by less than 2^-21; a frequency is f (p / factor + 1 - p) and no less than f / factor, so that is 2^-21 of it times the factor."""
+    from kubeai_b200 import ops
+    want, gain = configured(dims, base, YARN | {k: v for k, v in more.items() if v is not None})
+    r = ops.rotary(dims, base, YARN | more, device="cpu")
+    assert abs(r.gain - gain) < 1e-6, (r.gain, gain)
+    assert np.allclose(r.freqs.numpy(), want, rtol=2.0 ** -20 + 2.0 ** -21 * more.get("factor", 32.0), atol=0)
+
+
+@pytest.mark.parametrize("dims,base,scaling,why", [
+    (64, 1e4, YARN | dict(finetuned=True), "'finetuned'"), (64, 1e4, dict(rope_type="linear", factor=2.0, beta_fast=32), "'beta_fast'"), (64, 1e4, dict(rope_type="linear", factor=2.0, attention_factor=2.0), "'attention_factor'"),
+    (128, 1e4, dict(rope_type="default", mrope_section=[16, 24, 24]), "'mrope_section'"), (128, 1e4, dict(short_factor=[1.0], long_factor=[1.0]), "'long_factor', 'short_factor'"),
+    (128, 1e4, dict(factor=2.0), "'factor'"), (128, 1e4, dict(rope_theta=5e5), "says otherwise"), (128, 1e4, dict(partial_rotary_factor=0.5), "says otherwise"),
+    (64, 1e4, YARN | dict(factor=None), "lacks 'factor'"), (64, 1e4, YARN | dict(factor="many"), "cannot be made of"), (64, 1e4, YARN | dict(beta_fast=-1.0), "cannot be made of"), (64, 1e4, YARN | dict(mscale=[1]), "cannot be made of")])
+def test_scalings_that_are_not_handled_are_refused(dims, base, scaling, why):
+    from kubeai_b200 import B200Error, ops
+    with pytest.raises(B200Error, match=why):
+        ops.rotary(dims, base, scaling, device="cpu")
+
+
+def test_a_scaling_may_say_what_the_call_says():
+    from kubeai_b200 import ops
+    plain = ops.rotary(64, 1e6, device="cpu")
+    same = ops.rotary(64, 1e6, dict(rope_type="default", rope_theta=1e6, partial_rotary_factor=0.5, original_max_position_embeddings=4096, factor=None), device="cpu")
+    assert torch.equal(plain.freqs, same.freqs) and plain.gain == same.gain
