@@ -11,7 +11,7 @@
 // tensor cores idle in any form, and memory is what bounds this.
 // An item that a range's end cuts leaves unnormalised rows in the workspace, as every item does that shares its rows with another; a second kernel joins them in a fixed order.
 // 16 x 8 beams behind up to 4001 tokens, 273 MB: 67.4 us, of which the join has 6 and the first kernel 61, 4.5 TB/s (pages of random places by TMA reach 5.8 with nothing else to do): the last team ends 15 %
-// behind the mean one, as what each gets of the memory differs.  128 rows behind 2048 tokens, 144 MB: 48.5.  64 x 8 beams behind up to 450, 173 MB: 62.7; three warps a scheduler wait on their own chains
+// behind the mean one, as what each gets of the memory differs.  128 rows behind 2048 tokens, 144 MB: 50.5.  64 x 8 beams behind up to 450, 173 MB: 62.7; three warps a scheduler wait on their own chains
 // (products, maxima, exponentials, products), at two of three a page's time, and 168 registers leave no more.  What the loads know of their place lies in shared memory: in registers it spilled others (72).
 // 1 x 4 beams behind 450: 13.8, a chain of lengths, costs, ranges (4 us of them, most of it instructions' first way from memory), page table, four pages, the rows' way out and the join.
 #include <cuda.h>
@@ -42,8 +42,8 @@ struct Form {
   static constexpr int kThreads = kWide ? wide::kThreads : 128, kWarps = kThreads / 32, kPlaces = wide::kThreads / kThreads, kKinds = kWide ? 3 : 2;
   static constexpr int kRings = 1024 + kWarps * kDepth * kPageBytes, kSmem = kWide ? std::max(kRings, wide::kSmem) : kRings;
 };
-// What a page of each team, and a step of a wide CTA, take of an SM's time: by these the CTAs are shared out.  Teams of one next to wide CTAs: 128 rows behind 2048 tokens 22 52 us, 24 51.2, 26 48.5, 28 48.7;
-// 64 groups of 48 rows behind 450 96.1, 96.8, 97.5, 100.9; 4 of 160 rows behind 8000 56.5, 56.2, 56.5, 58.6.  Teams of one and two: 16 x 8 beams 1.4 66.9, 1.6 67.3, 1.8 70.9, 64 x 8 behind 450 63.6, 62.7,
+// What a page of each team, and a step of a wide CTA, take of an SM's time: by these the CTAs are shared out.  Teams of one next to wide CTAs: 128 rows behind 2048 tokens 24 52.8 us, 26 50.9, 28 51.2, 30 50.4;
+// 64 groups of 48 rows behind 450 101.1, 101.1, 102.9, 104.2; 4 of 160 rows behind 8000 62.1, 61.7, 62.1, 63.5.  Teams of one and two: 16 x 8 beams 1.4 66.9, 1.6 67.3, 1.8 70.9, 64 x 8 behind 450 63.6, 62.7,
 // 62.5.
 __device__ constexpr float kShare[3] = {1.f, 1.6f, 26.f};
 

@@ -8,12 +8,13 @@
 //   a warp issues tcgen05.mma: S_g = Q K^T and O_g += P_g V (M = N = 128), P_g in TMEM over its scores: the next scores of one tile are formed under the other's softmax;
 //   two groups of four warps (thread = row) do the softmax in fp32, base 2; a warp whose rows nobody owns only keeps step.
 // The scores of a step come behind the products with the last step's values in the order of their issue, so a tile whose scores are there has its O at rest: no other wait stands in front of its rescaling.
-// Weights are relative to the row's largest score as it was when it last grew by a factor of two: O is rescaled a few times a row and not at two thirds of the tiles; a weight is then
-// up to 2, and what its rounding to bf16 costs relative to it is the same.
+// Weights are relative to the row's largest score so far, rounded to bf16 (by up to 2^-8 of each) and divided by the sum of the rounded ones, as in narrow CTAs: what all values have in common has no
+// part of the rounding.  The sum of the unrounded weights left up to 2^-8 of the output there and was cheaper: 128 rows behind 2048 tokens 49.3 us, not 50.9, 4 groups of 160 rows behind 8000 57.3, not 61.8,
+// the questions below 256, not 265.  (An older maximum, kept until it grew by a factor of two, spares rescalings of O: 263 for the questions; nothing elsewhere.)
 // Only steps that reach behind what every row sees are masked.  There the products' warp also clears what must not meet a weight of zero: values behind the last key, and infinities and NaN
 // among values that some row does not see, which the rows that see them add at the end by themselves.
 // Every wait has a limit; a CTA that gives up sets an error mark and still meets at the end.
-// 2 x 24 questions of up to 32 tokens about 16001, 211 GFLOP: 255 us, 0.83 PFLOP/s, 52 % of what a large product reaches.  A step of two tiles takes 4700 cycles: the exponentials' unit is busy for 42 %,
+// 2 x 24 questions of up to 32 tokens about 16001, 211 GFLOP: 265 us, 0.80 PFLOP/s, 50 % of what a large product reaches.  A step of two tiles takes 4900 cycles: the exponentials' unit is busy for 42 %,
 // issue slots for 37 %.  What bounds it is a tile's chain (scores, load, maximum, 128 exponentials a thread, weights out, products): without loads it takes 221 us, without the softmax 219.  Half tiles of
 // 64 keys with scores ahead of them 300, sixteen softmax warps 287, another order of the exponentials' instructions the same.
 #pragma once
@@ -27,7 +28,6 @@ constexpr int kTileRows = 128, kKeys = 128;                         // of a tile
 constexpr int kSlab = 128 * 128, kTile = 2 * kSlab;                 // bytes: 64 columns of 128 rows, a tile
 constexpr int kThreads = 384, kRing = 4;                                            // tiles of keys and values.  Warps 0 to 3 and 4 to 7: softmax, 8: loads, 9: products
 constexpr int kLeast = 4;                                           // steps of a range at least: its rows leave as 132 KB, as much as four tiles
-constexpr float kSlack = 1.f;                                       // by how much, in units of log 2, a row's maximum may grow before its weights are made relative to it
 
 // shared memory: queries, ring, 2 KB a softmax warp for its way out, barriers
 constexpr int kRingAt = 2 * kTile, kStageAt = kRingAt + kRing * kTile, kBars = kStageAt + 8 * 2048, kSmem = 1024 + kBars + 256;
@@ -460,7 +460,7 @@ __device__ __forceinline__ void walk(const CUtensorMap& tm_q, const CUtensorMap&
               for (int c = 0; c < 4; ++c) mx[c] = max3(mx[c], __uint_as_float(s[c][i]), __uint_as_float(s[c][i + 1]));
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * scale_log2;
             float alpha = 1.f;
-            if (top > ref + kSlack) {
+            if (top > ref) {
               alpha = exp2_ftz(ref - top);
               ref = top;
             }
@@ -485,9 +485,9 @@ __device__ __forceinline__ void walk(const CUtensorMap& tm_q, const CUtensorMap&
               for (int i = 0; i < 32; ++i) {
                 const int c = 2 * h + (i >> 4), e = 2 * (i & 15);
                 const float2 t = floats_of(fma_pair(pair_of(s[c][e], s[c][e + 1]), scale2, less2));
-                const float x = exp2_ftz(t.x), y = exp2_ftz(t.y);
-                ps[i & 1] = add_pair(ps[i & 1], pair_of(x, y));
-                pk[i] = pack_bf16x2(x, y);
+                // the sum is that of the rounded weights
+                pk[i] = pack_bf16x2(exp2_ftz(t.x), exp2_ftz(t.y));
+                ps[i & 1] = add_pair(ps[i & 1], pair_of(pk[i] << 16, pk[i] & 0xffff0000u));
               }
               tmem_st_32x32(tm + 32 * h, pk);      // P in place of the scores
               if (h == 0) {      // the products with the first half's values may begin
