@@ -193,9 +193,11 @@ __device__ __forceinline__ void walk(const CUtensorMap& tm_q, const CUtensorMap&
   auto pv_full = [&](int g) { return bars + 8u * (14 + g); };
   auto meet = [&](int q) { return bars + 8u * (16 + q); };      // of the two warps of a quarter of the lanes
   const uint32_t q_full = bars + 8u * 20, q_empty = bars + 8u * 21, piece_full = bars + 8u * 22, slot = bars + 8u * 26;
-  static_assert(kRing == 4 && kPieces == 4, "");
+  static_assert(kRing == 4 && kPieces == 4 && 8 * 26 + 8 + 4 * kPieces <= 256, "");
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + (slot - sbase));
-  volatile int* odd_item = reinterpret_cast<volatile int*>(tmem_slot + 2);      // [2]: the last item of each parity with infinities or NaN among values that some row does not see
+  volatile int* odd_item = reinterpret_cast<volatile int*>(tmem_slot + 2);      // [kPieces]: the last item of each piece's place with infinities or NaN among values that some row does not see.
+  // (The products may be two items ahead of a group without scores in the one between: item i + 2's marks may be made before that group has looked at item i's.  Its end is where both groups meet,
+  // in front of any product of item i + 3.)
   const int warp = warp_number(), lane = threadIdx.x & 31, tid = threadIdx.x;
 
   const int group = a.q_heads / a.kv_heads, shift = __ffs(group) - 1;
@@ -215,7 +217,7 @@ __device__ __forceinline__ void walk(const CUtensorMap& tm_q, const CUtensorMap&
       mbar_init(q_full, 1);
       mbar_init(q_empty, 1);
       fence_mbar_init();
-      odd_item[0] = odd_item[1] = -1;
+      for (int i = 0; i < kPieces; ++i) odd_item[i] = -1;
       tma_prefetch_desc(&tm_q);
       tma_prefetch_desc(&tm_kv);
     }
@@ -375,7 +377,7 @@ __device__ __forceinline__ void walk(const CUtensorMap& tm_q, const CUtensorMap&
             }
             for (int e = end * 8 + lane; e < kKeys * 8; e += 32) x[e] = make_uint4(0, 0, 0, 0);
           }
-          if (odd) odd_item[v.item & 1] = v.item;
+          if (odd) odd_item[v.item % kPieces] = v.item;
           __threadfence_block();
           fence_proxy_async();
           __syncwarp();
@@ -520,7 +522,7 @@ __device__ __forceinline__ void walk(const CUtensorMap& tm_q, const CUtensorMap&
                  w.x.whole && w.x.own && !w.x.joined, 0, 0};
         if (!(ok = warp_wait(pv_full(g), (steps[g] - 1) & 1))) break;
         auto odd = [&] {
-          if (odd_item[w.item & 1] != w.item) return;
+          if (odd_item[w.item % kPieces] != w.item) return;
           out.odd_from = max(see, begin);
           out.odd_to = min(limit, end);
         };

@@ -124,6 +124,18 @@ def test_odd_values_that_some_rows_see(kind, at):
     check(b)
 
 
+def test_odd_values_in_items_one_behind_the_other():
+    """A CTA's items of one and of two row tiles in turn, short and with odd values in each: behind one of two tiles comes one without scores for the second group, and another with odd values."""
+    rows = [64, 9, 40, 17, 12, 64, 20, 33] * 10
+    b = Batch([(8, 16)] * 10, [n + 2 + 11 * s % 60 for s, n in enumerate(rows)], rows, 4, 4, seed=7)
+    for s in range(0, b.S, 3):
+        first = b.lens[s] - b.rows[s]
+        for k, dim in ((1, 3), (b.rows[s] // 2, 40), (b.rows[s] - 1, 100)):
+            page, i = token_of(b, s, first + k)
+            b.kv[page, 1, :, i, dim] = float("inf") if s % 2 else float("nan")
+    check(b)
+
+
 @kinds
 def test_pages_that_the_cache_does_not_have_read_as_zeros(kind):
     b = KINDS[kind](8)
