@@ -613,6 +613,7 @@ int b200_op_norm_rope_kvwrite(const b200_norm_rope_args* a, void* stream);
  * the cache and the request's rows 0 .. i, whose K and V are in the cache already.  Group g has the requests group_starts[g] .. group_starts[g + 1] - 1; the first
  * shared[g] tokens of their tables, of which whole pages count and no more than the first request has in the cache, are the same in all of them and are read by the first one's table, once for the
  * group's rows.  Requests of no group, of one that has a single request, with fewer tokens in the cache than are shared, or all where starts or group_starts do not ascend, are attended alone.
+ * Where max_rows (at most T) times S is so large that the pages of all requests pass 32 bits, but T rows stay within them, nobody is attended if starts do not ascend.
  * max_rows: most rows of a request; max_ctx: most tokens in front of them, if known (0: what a row of the table holds), which only decides how the work is split.
  * Everything else as for b200_op_paged_attn_tree: what is left out and zero_rest, pages that the cache does not have, odd values in what a row does not see, sizes and
  * alignments, status.  S and G <= 65534. */

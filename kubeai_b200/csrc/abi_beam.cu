@@ -47,9 +47,7 @@ static int shared_sizes(const b200_shared_attn_args* a, const char* op) {
   if (static_cast<int64_t>(a->q_heads) * 128 > a->ldq || static_cast<int64_t>(a->q_heads) * 128 > a->ldo || a->ldq % 8 || a->ldo % 8) return refuse(op, "rows of q and out are whole heads, a multiple of 8 apart");
   if (!(a->scale > 0.f && a->scale < 1e30f)) return refuse(op, "scale is no number above 0 and below 1e30");      // a row's maximum is looked for ahead of the scale
   if (a->T > INT_MAX / 8) return refuse(op, "too many rows");
-  // pieces of 16 rows: a request's own, and the groups', whose rows are the step's
-  const long long own = (static_cast<long long>(a->max_rows < a->T ? a->max_rows : a->T) * group + 15) / 16 * a->S, shared = a->G ? (static_cast<long long>(a->T) * group + 15) / 16 + a->G : 0;
-  if ((own + shared) * a->kv_heads > INT_MAX / (a->max_blocks + 2ll * tree::kItem)) return refuse(op, "the pages of all requests pass 32 bits");
+  if (!beam::costs_fit(*a, false) && !beam::costs_fit(*a, true)) return refuse(op, "the pages of all requests pass 32 bits");
   return 0;
 }
 

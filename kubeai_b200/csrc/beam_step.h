@@ -25,6 +25,14 @@ struct Lengths {
   int S, T, G, max_blocks, max_rows;      // G is 0 where starts or group_starts do not ascend
   B200_HD Request request(int s) const { return tree::request_of(starts, ctx, s, T, max_blocks, max_rows, status); }
 };
+// Pieces of 16 rows (token * group + head) of all parts at most: of the requests' own ones by the most rows of each, or where starts ascend (`ordered`) by the step's; and of the groups', which are parts
+// only where starts ascend
+B200_HD long long most_pieces(const b200_shared_attn_args& a, bool ordered) {
+  const long long group = a.q_heads / a.kv_heads, T = a.T, most = a.max_rows < a.T ? a.max_rows : a.T;
+  return (ordered ? T * group / 16 + a.S : (most * group + 15) / 16 * a.S) + (a.G ? (T * group + 15) / 16 + a.G : 0);
+}
+// Whether what they cost fits 32 bits
+B200_HD bool costs_fit(const b200_shared_attn_args& a, bool ordered) { return most_pieces(a, ordered) * a.kv_heads <= INT32_MAX / (a.max_blocks + 2ll * tree::kItem); }
 // Whether every entry i .. of n + 1 values, a step apart, is in order and within 0 .. most
 B200_HD bool ascends(const int* v, int n, int most, int i, int step) {
   bool ok = true;

@@ -528,6 +528,14 @@ shared_attn_join_kernel(const __grid_constant__ b200_shared_attn_args a, const S
   *out = make_uint2(pack_bf16x2(j.y.x * inv, j.y.y * inv), pack_bf16x2(j.y.z * inv, j.y.w * inv));
 }
 
+// Where only the order of `starts` keeps what all parts cost within 32 bits: a copy, in which nobody has rows if they do not ascend
+__global__ void __launch_bounds__(1024)
+ordered_starts_kernel(const int* starts, int S, int T, int* to) {
+  griddep_enter();
+  const bool ordered = __syncthreads_and(beam::ascends(starts, S, T, threadIdx.x, 1024));
+  for (int s = threadIdx.x; s <= S; s += 1024) to[s] = ordered ? starts[s] : 0;
+}
+
 }  // namespace
 
 // How many CTAs may be wide: none where no part can have so many rows, else as many as there are SMs, or as the most work that the call may have feeds
@@ -542,15 +550,25 @@ static int wide_ctas(const b200_shared_attn_args& a) {
 
 static Sizes sizes_of(const b200_shared_attn_args& a) { return {sm_count() * Form<true>::kWarps, wide_ctas(a)}; }
 
+// The copy of `starts`, behind everything else
+static int64_t starts_bytes(const b200_shared_attn_args& a) { return beam::costs_fit(a, false) ? 0 : (a.S + 4ll) / 4 * 16; }
+
 int64_t shared_attention_workspace(const b200_shared_attn_args& a) {
   const Sizes n = sizes_of(a);
   const int64_t T = a.T;
   return 2 * T * a.kv_heads * static_cast<int64_t>(sizeof(Place)) +
-         (2ll * n.warps * kTile16 + 2ll * n.ctas * kWideRows + (a.G ? 2 * T * a.q_heads : 0)) * kLd * static_cast<int64_t>(sizeof(float));
+         (2ll * n.warps * kTile16 + 2ll * n.ctas * kWideRows + (a.G ? 2 * T * a.q_heads : 0)) * kLd * static_cast<int64_t>(sizeof(float)) + starts_bytes(a);
 }
 
-int paged_attention_shared(const b200_shared_attn_args& a, int* error, cudaStream_t st) {
+int paged_attention_shared(const b200_shared_attn_args& args, int* error, cudaStream_t st) {
+  b200_shared_attn_args a = args;
   const Sizes sizes = sizes_of(a);
+  if (const int64_t bytes = starts_bytes(a)) {
+    int* starts = reinterpret_cast<int*>(static_cast<uint8_t*>(a.workspace) + shared_attention_workspace(a) - bytes);
+    launch_pdl(ordered_starts_kernel, dim3(1), dim3(1024), 0, st, a.starts, a.S, a.T, starts);
+    if (cudaGetLastError() != cudaSuccess) return -2;
+    a.starts = starts;
+  }
   const int group = a.q_heads / a.kv_heads;
   CUtensorMap tm_kv, tm_q;
   if (int rc = tmap_encode_bf16_2d(&tm_kv, a.kv_layer, static_cast<uint64_t>(a.num_pages) * 2 * a.kv_heads * 16, kD, kD, 16, 64, 1)) return rc;

@@ -234,3 +234,23 @@ def test_a_scaling_may_say_what_the_call_says():
     plain = ops.rotary(64, 1e6, device="cpu")
     same = ops.rotary(64, 1e6, dict(rope_type="default", rope_theta=1e6, partial_rotary_factor=0.5, original_max_position_embeddings=4096, factor=None), device="cpu")
     assert torch.equal(plain.freqs, same.freqs) and plain.gain == same.gain
+
+
+def test_costs_stay_within_their_bound(tmp_path):
+    exe = tmp_path / "beam_costs_check"
+    subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-I", str(ROOT / "kubeai_b200" / "csrc"),
+                    str(ROOT / "tests" / "native" / "beam_costs_check.cc"), "-o", str(exe)], check=True, capture_output=True, text=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "ok", r.stdout + r.stderr
+
+
+LONG = dict(S=256, T=768, G=32, q_heads=32, kv_heads=8, ldq=6144, ldo=4096, max_blocks=8192, ld_tables=8192, max_rows=512, num_pages=100)
+
+
+def test_one_long_portion_among_many_requests_is_taken():
+    """256 requests with 768 rows, 512 of them one's: 448 pieces of 16 rows in all where starts ascend, not 128 for each."""
+    from kubeai_b200 import lib
+    small = lib().b200_op_paged_attn_shared_workspace(C.byref(attn(**LONG | dict(S=254))))
+    assert small > 0 and lib().b200_op_paged_attn_shared_workspace(C.byref(attn(**LONG))) == small + 260 * 4      # the starts' copy
+    refused("b200_op_paged_attn_shared", attn(**LONG | dict(workspace_bytes=small)), "workspace")
+    refused("b200_op_paged_attn_shared", attn(**LONG | dict(max_blocks=1 << 22, ld_tables=1 << 22)), "the pages of all requests")

@@ -170,3 +170,36 @@ def test_the_same_bits_in_a_graph_and_on_two_streams(kind):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(y, f) for y, f in zip(kept, first))
+
+
+# 256 requests of 768 rows, of which one has 512: most rows times requests would pass 32 bits
+def portion(ctx, own, seed, groups=8):
+    rows = [512] + [2] * 128 + [0] * 127
+    return Batch([(32, ctx)] * groups, [own + n + s % 9 for s, n in enumerate(rows)], rows, 8, 4, seed=seed, width=8192)
+
+
+def test_one_long_portion_among_many_requests():
+    b = portion(32, 3, 11)
+    want, size = b.want()
+    near_attention(b.call(), want, size)
+    graph, out = torch.cuda.CUDAGraph(), torch.empty_like(b.q)
+    from kubeai_b200 import ops
+    maps = [dev(v) for v in (b.tables, b.starts, b.ctx, b.group_starts, b.shared)]
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        ops.paged_attn_shared(b.q, b.kv, *maps, b.heads, b.kvh, 512, out=out)
+    for _ in range(2):
+        out.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        near_attention(out, want, size)
+    # no groups
+    near_attention(b.call(group_starts=dev([0]), shared=dev(np.zeros(0))), want, size)
+
+
+@pytest.mark.parametrize("starts", [[0, 512] * 128 + [0], [768] + [0] * 256, [0, 512, 511] + [768] * 254, [-1] + [768] * 256, [0] * 256 + [769]])
+def test_a_long_portion_without_order_is_nobodys(starts):
+    b = portion(32, 3, 12)
+    assert not b.call(starts=dev(starts)).any()
+    kept = torch.full_like(b.q, 7.0)
+    assert (b.call(starts=dev(starts), out=kept) == 7).all()
