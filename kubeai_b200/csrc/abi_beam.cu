@@ -33,7 +33,7 @@ int b200_op_norm_rope_kvwrite(const b200_norm_rope_args* a, void* stream) {
   if (!a->qkv || !a->positions || !a->slots || (a->dims && !a->freqs) || (a->q_heads && !a->out) || (a->kv_heads && a->num_pages && !a->kv_layer)) return refuse(op, "a buffer is missing");
   if (!aligned(a->qkv, 16) || !aligned(a->out, 16) || !aligned(a->kv_layer, 16) || !aligned(a->q_norm, a->norm_f32 ? 16 : 8) || !aligned(a->k_norm, a->norm_f32 ? 16 : 8))
     return refuse(op, "qkv, out, the cache and fp32 norms are 16-byte aligned, bf16 norms 8-byte");
-  if (a->out == a->qkv && a->ldo != a->ldx) return refuse(op, "queries kept in place have the rows of qkv");
+  if (a->out == a->qkv && a->ldo != a->ldx && a->T > 1) return refuse(op, "queries kept in place have the rows of qkv");
   if (int rc = require_device()) return rc;
   return launched(op, norm_rope_kv_write(*a, static_cast<cudaStream_t>(stream)));
 }

@@ -500,6 +500,8 @@ def norm_rope_kvwrite(qkv, positions, slots, kv_layer, q_heads, kv_heads, freqs,
         ldo = _rows(at, out, _BF16, "out", columns=q_heads * 128)
         if out.shape[0] < T:
             raise _refused(f"out has {out.shape[0]} rows, not {T}")
+    if T == 1:      # any distance will do for a row alone, also where a view's width is no multiple of 8
+        ldx, ldo = width, q_heads * 128
     if (T | ldx | ldo) >> 31:
         raise _refused(_WIDE)
     a = NormRopeArgs(T, q_heads, kv_heads, ldx, ldo, 2 * freqs.numel(), bool(interleaved), max(ldq, 0), max(ldk, 0), f32, eps, gain, kv_layer.shape[0],
@@ -533,6 +535,8 @@ def paged_attn_shared(qkv, kv_layer, block_tables, starts, ctx_lens, group_start
             raise _refused(f"out has {out.shape[0]} rows, not {T}")
         if ldo >> 31:
             raise _refused(_WIDE)
+    if T == 1:
+        ldq = ldo = q_heads * 128
     a = SharedAttnArgs(S, T, G, q_heads, kv_heads, ldq, ldo, block_tables.shape[1], ld, max_rows, max_ctx, fresh, scale, kv_layer.shape[0], qkv.data_ptr(), out.data_ptr(),
                        kv_layer.data_ptr(), block_tables.data_ptr(), starts.data_ptr(), ctx_lens.data_ptr(), group_starts.data_ptr(), shared_lens.data_ptr(), _ptr(status))
     a.workspace_bytes = check(lib().b200_op_paged_attn_shared_workspace(C.byref(a)))

@@ -579,3 +579,24 @@ def test_pages_behind_the_first_four_gigabytes():
 def test_rotation_of_one_or_two_heads(T, heads, kvh, dims, interleaved):
     """The first warps alone have heads, and all pairs' angles are wanted."""
     turned(T, heads, kvh, dims, interleaved, "one", 4000, seed=heads + dims)
+
+
+@pytest.mark.parametrize("spare", [0, 2, 8, 100])
+def test_a_row_alone_has_any_distance(spare):
+    """A row alone of a wider buffer, and its queries in place as a view of their columns, as several rows may have them."""
+    from kubeai_b200 import ops
+    gen = torch.Generator(device="cuda").manual_seed(spare)
+    big = torch.randn(2, 16 * D + 104, generator=gen, device="cuda").bfloat16()
+    kv, f = torch.randn(5, 2, 2, PAGE, D, generator=gen, device="cuda").bfloat16(), ops.rotary().freqs
+    want_kv = kv.clone()
+    want = ops.norm_rope_kvwrite(big[:, :12 * D].contiguous(), dev([7, 9]), dev([3, 20]), want_kv, 8, 2, f)
+    for rows in (1, 2):
+        x, mine = big.clone(), kv.clone()
+        view = x[:rows, :12 * D + spare]
+        got = ops.norm_rope_kvwrite(view, dev([7, 9][:rows]), dev([3, 20][:rows]), mine, 8, 2, f, out=view[:, :8 * D])
+        assert got.data_ptr() == x.data_ptr() and torch.equal(got, want[:rows]) and torch.equal(x[:, 8 * D:], big[:, 8 * D:]) and torch.equal(x[rows:], big[rows:])
+        assert torch.equal(mine[0], want_kv[0]) and torch.equal(mine[1], (want_kv if rows == 2 else kv)[1])
+        queries, out = x[:rows, :8 * D + spare], torch.zeros(2, 8 * D + 104, device="cuda").bfloat16()
+        args = (want_kv, dev([[0], [1]][:rows]), dev([0, 1, 2][:rows + 1]), dev([3, 4][:rows]), dev([0]), dev([]), 8, 2, 1)
+        y = ops.paged_attn_shared(queries, *args, out=out[:rows, :8 * D + spare])
+        assert torch.equal(y[:, :8 * D], ops.paged_attn_shared(want[:rows].contiguous(), *args)) and not out[:, 8 * D:].any() and not out[rows:].any()
