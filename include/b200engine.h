@@ -637,8 +637,9 @@ typedef struct {
 int64_t b200_op_paged_attn_shared_workspace(const b200_shared_attn_args* a);
 int b200_op_paged_attn_shared(const b200_shared_attn_args* a, void* stream);
 /* The k best candidates over a request's beams and the vocabulary, and the beams that go on.  logits [S * beams, V], rows ld apart, bf16 or fp32 (logits_f32), scores fp32 [S, beams]:
- *   c(b, v) = scores[b] + x(b, v) - log(sum over w of exp(x(b, w)))   in 64 bits
- * in descending order, equal ones by the lower beam; a beam's own by the larger logit, equal ones by the lower token.  NaN among logits or scores counts as -inf, and what is -inf is no candidate;
+ *   c(b, v) = scores[b] + x(b, v) - log(sum over w of exp(x(b, w)))
+ * in 64 bits but for the terms of the sum besides a row's largest, which are fp32: the logarithm is off by less than 2^-18 (2^-16 where hundreds of values tie for a last place; measured 2^-22.5),
+ * the same for equal rows wherever they lie, and beams whose candidates lie closer than that may change places.  In descending order, equal ones by the lower beam; a beam's own by the larger logit, equal ones by the lower token.  NaN among logits or scores counts as -inf, and what is -inf is no candidate;
  * +inf logits of a row share its probability.  Out: found_parents, found_tokens, found_scores [S, k] (-1, -1, -inf behind the last); parents, tokens, scores [S, beams]: the first beams of them whose
  * token is none of ends [num_ends] (the same fillers).  beams <= 32, k <= 64, V <= 393216, num_ends <= 1024, rows of logits aligned as their type. */
 typedef struct {

@@ -600,3 +600,62 @@ def test_a_row_alone_has_any_distance(spare):
         args = (want_kv, dev([[0], [1]][:rows]), dev([0, 1, 2][:rows + 1]), dev([3, 4][:rows]), dev([0]), dev([]), 8, 2, 1)
         y = ops.paged_attn_shared(queries, *args, out=out[:rows, :8 * D + spare])
         assert torch.equal(y[:, :8 * D], ops.paged_attn_shared(want[:rows].contiguous(), *args)) and not out[:, 8 * D:].any() and not out[rows:].any()
+
+
+# ------------------------------------------------------------------ the logarithm of a row's sum
+LOG_SUM, LOG_SUM_TIES = 2.0 ** -18, 2.0 ** -16
+# Terms besides a part's largest ones are fp32.  A term's exponent t is rounded by |t| ln 2 2^-24 of the term, and terms of t < -19 are too small to matter: 2^-20; its exponential is off by 2^-22; log2 e in
+# fp32 by 2^-22; a thread adds 32 terms one by one and those of three others: 2^-19 and 2^-23.  In all less than 2^-18.  Where more than 256 values of a part tie for the last place a thread adds 128 terms, whose
+# differences from the largest are rounded too: 2^-17, 2^-19 and the others, less than 2^-16.
+
+
+def shares(rows, dtype):
+    """For rows of logits the score beside which the best candidate's own share is next to nothing, so that fp32 holds what is left of it: what the kernel says, and what it is."""
+    from kubeai_b200 import ops
+    x = torch.tensor(rows, dtype=torch.float64).to(dtype)
+    v = x.double().numpy()
+    top = v.max(1)
+    share = -np.log(np.exp(v - top[:, None]).sum(1))
+    score = (-share).astype(np.float32)
+    got = ops.beam_select(x.cuda(), torch.tensor(score).view(-1, 1).cuda(), 1)
+    return got.found_scores[:, 0].double().cpu().numpy(), score.astype(np.float64) + share
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [1100, 9999, 128256, 393216])
+def test_the_log_of_a_flat_rows_sum(dtype, V):
+    rng = np.random.default_rng(V)
+    rows = [rng.normal(m, s, V) for m, s in ((0, 0.25), (0, 1), (0, 3), (40, 1), (-1000, 2), (3e5, 4))]
+    rows += [np.where(np.arange(V) % 97 == 5, 0.0, -9.0 - rng.random(V)), np.linspace(-13, 0, V)]
+    got, want = shares(np.stack(rows), dtype)
+    assert (np.abs(got - want) <= (LOG_SUM if dtype == torch.float32 else LOG_SUM_TIES)).all(), np.abs(got - want)      # (bf16 values are few far from zero, and tie)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [1, 2, 300, 500, 9999, 128256])
+def test_the_log_of_equal_values_sum(dtype, V):
+    rows = np.full((4, V), -3.0)
+    rows[1] = np.where(np.arange(V) % 2, 1.0, -0.5)
+    rows[2, V // 2] = 8.0
+    rows[3, : V // 2] = -15.0
+    got, want = shares(rows, dtype)
+    assert (np.abs(got - want) <= LOG_SUM_TIES).all(), np.abs(got - want)
+
+
+@pytest.mark.parametrize("V", [5003, 128256])
+def test_close_candidates_of_different_flat_rows_keep_their_order(V):
+    """Their shares lie 2^-17 apart, twice what the logarithms are off by."""
+    from kubeai_b200 import ops
+    rng = np.random.default_rng(V)
+    for _ in range(4):
+        x = rng.normal(0, 1, (8, V)).astype(np.float32)
+        v = x.astype(np.float64)
+        share = -np.log(np.exp(v - v.max(1, keepdims=True)).sum(1))
+        order = rng.permutation(8)
+        score = (order * 2.125 * 2.0 ** -17 - share).astype(np.float32)
+        c = score + share
+        assert (np.diff(np.sort(c)) > 2.0 ** -17).all()
+        got = ops.beam_select(torch.tensor(x).cuda(), torch.tensor(score).view(1, 8).cuda(), 8)
+        want = np.argsort(-c)
+        place = {int(p): i for i, p in reversed(list(enumerate(got.found_parents[0].tolist())))}
+        assert sorted(place, key=place.get) == [int(p) for p in want][:len(place)]
