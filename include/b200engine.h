@@ -592,8 +592,9 @@ int b200_op_tree_accept(const b200_tree_accept_args* a, void* stream);
 /* Norms and rotary positions of queries and keys, and keys and values into the paged cache, in one pass over qkv [T, (q_heads + 2 kv_heads) * 128] bf16, rows ldx apart.
  * For each head of q and k, in fp32 and rounded once:  y = x w / sqrt(mean(x^2) + eps)  (q_norm, k_norm: 128 weights, or 128 for each head where q_norm_ld, k_norm_ld are 128; bf16 or
  * fp32 (norm_f32); NULL: y = x), then the first dims values as pairs (d, d + dims / 2), or with interleaved (2 d, 2 d + 1), turned by positions[t] * freqs[d] (fp64 radians a
- * position, d < dims / 2) and multiplied by gain; the others are y.  The angle is reduced to a part of a turn in integers, so far positions lose nothing.
- * q goes to out [T, q_heads * 128], rows ldo apart (it may be qkv itself, with ldo == ldx where there are several rows, and otherwise shares nothing with it), k and v to the token's slot (page * 16 + offset) of kv_layer [num_pages][2][kv_heads][16][128];
+ * position, d < dims / 2) and multiplied by gain; the others are y.  The angle is reduced to a part of a turn in integers: one of N turns is off by N 2^-52 + 2^-26 of a turn.
+ * q goes to out [T, q_heads * 128], rows ldo apart (it may be qkv itself, with ldo == ldx where there are several rows, and otherwise shares nothing with it), k and v to the token's
+ * slot (page * 16 + offset) of kv_layer [num_pages][2][kv_heads][16][128];
  * a slot that the cache does not have is written nowhere, and slots are distinct.  dims even, 0 to 128; ldx, ldo multiples of 8; qkv, out, kv_layer 16-byte aligned. */
 typedef struct {
   int32_t T, q_heads, kv_heads, ldx, ldo, dims, interleaved, q_norm_ld, k_norm_ld, norm_f32;

@@ -3,8 +3,8 @@
 //   y = x w / sqrt(mean(x^2) + eps);   (y_a, y_b) -> gain (y_a cos - y_b sin, y_b cos + y_a sin),  angle = position * freq
 //
 // Everything between the loads and the stores is fp32 and rounded once to bf16 (the norm's result is not rounded ahead of the rotation).  An angle of a far position
-// has many turns: the frequency becomes a 64-bit part of a turn, the product with the position drops whole turns by itself, and what is left is exact to 2^-33 of a turn; an fp32
-// product would be off by 0.06 radians at position 10^6.
+// has many turns: the frequency becomes a 64-bit part of a turn, and the product with the position drops whole turns by itself.  An angle of N turns is then off by N 2^-52 (the frequency in
+// turns, in fp64: 2^-35 of a turn at position 10^6, 2^-23.6 at 2^31) and, as what is left of a turn goes to the sine in fp32, 2^-26 of a turn; an fp32 product would be off by 0.06 radians at position 10^6.
 // A CTA has a token; its first threads make the token's cosines and sines while the heads are on their way.  Sixteen lanes have a head, eight values each in two
 // pieces of four that hold both values of their pairs: (j, j + n / 4) where halves pair up, (2 j, 2 j + 1) where neighbours do.  Halves of a number of pairs that four does not
 // divide go through shared memory.

@@ -659,3 +659,33 @@ def test_close_candidates_of_different_flat_rows_keep_their_order(V):
         want = np.argsort(-c)
         place = {int(p): i for i, p in reversed(list(enumerate(got.found_parents[0].tolist())))}
         assert sorted(place, key=place.get) == [int(p) for p in want][:len(place)]
+
+
+# ------------------------------------------------------------------ angles with more digits than fp64 has
+TURN = "0.15915494309189533576888376337251436203445964574045644874766734405889679763"      # of a radian: 1 / (2 pi)
+
+
+@pytest.mark.parametrize("position", [1, 1000, 10 ** 6, 2 ** 24 + 1, 2 ** 30 - 1, 2 ** 31 - 1])
+@pytest.mark.parametrize("base", [10000.0, 500000.0])
+def test_angles_against_more_digits(position, base):
+    """An angle of N turns: its frequency in turns has two roundings to fp64, N 2^-52; the position's product is exact but for 2^-65 of a turn a position; what is left of a turn goes through fp32, 2^-26,
+    and a sine and cosine of 2 ulp, 2^-22, are multiplied and added with three roundings of 2^-24.  Values of a pair are chosen that nearly cancel, so that the one rounding to bf16 hides little."""
+    from fractions import Fraction
+
+    from kubeai_b200 import ops
+    freqs = ops.rotary(128, base, device="cpu").freqs
+    whole = [Fraction(float(f)) * position * Fraction(TURN) for f in freqs]
+    angle = np.array([float((n - round(n)) * 2) * math.pi for n in whole])
+    cos, sin = np.cos(angle), np.sin(angle)
+    # of 128 first values each pair's own with the second one that cancels best
+    a = 1 + np.arange(128) / 128
+    b = torch.tensor(a[:, None] * cos / np.where(np.abs(sin) < 2.0 ** -30, 1, sin)).clamp(-2.0 ** 40, 2.0 ** 40).bfloat16().double().numpy()
+    best = np.abs(a[:, None] * cos - b * sin).argmin(0)
+    x = np.zeros((1, 128))
+    x[0, :64], x[0, 64:] = a[best], b[best, np.arange(64)]
+    q = ops.norm_rope_kvwrite(torch.tensor(x).bfloat16().cuda(), dev([position]), dev([-1]), torch.zeros(1, 2, 0, PAGE, D).bfloat16().cuda(), 1, 0, freqs.cuda())
+    got = q.double().cpu().numpy()[0]
+    first, second = x[0, :64], x[0, 64:]
+    want, size = np.concatenate([first * cos - second * sin, second * cos + first * sin]), np.tile(np.abs(first) + np.abs(second), 2)
+    off = 2 * math.pi * (np.array([float(n) for n in whole]) * 2.0 ** -52 + position * 2.0 ** -65 + 2.0 ** -26) + 2.0 ** -22 + 3 * 2.0 ** -24
+    assert (np.abs(got - want) <= BF16 * np.abs(want) + np.tile(off, 2) * size).all(), (np.abs(got - want) - BF16 * np.abs(want)).max()
