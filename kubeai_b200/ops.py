@@ -432,9 +432,9 @@ def rotary(dims=128, base=10000.0, scaling=None, device="cuda") -> Rotary:
     unknown = sorted(set(scaling) - _SCALING_KEYS - _SCALING_KEYS_OF[kind])
     if unknown:
         raise _refused(f"rope scaling {kind!r} with {', '.join(map(repr, unknown))} is not supported")
-    if scaling.get("rope_theta", base) != base or int(128 * scaling.get("partial_rotary_factor", dims / 128)) != dims:
-        raise _refused(f"rope scaling {scaling} says otherwise than a base of {base} and {dims} of 128 values")
     try:
+        if float(scaling.get("rope_theta", base)) != base or int(128 * float(scaling.get("partial_rotary_factor", dims / 128))) != dims:
+            raise _refused(f"rope scaling {scaling} says otherwise than a base of {base} and {dims} of 128 values")
         if kind != "default":
             factor = float(scaling["factor"])
             if not factor > 0:

@@ -254,3 +254,10 @@ def test_one_long_portion_among_many_requests_is_taken():
     assert small > 0 and lib().b200_op_paged_attn_shared_workspace(C.byref(attn(**LONG))) == small + 260 * 4      # the starts' copy
     refused("b200_op_paged_attn_shared", attn(**LONG | dict(workspace_bytes=small)), "workspace")
     refused("b200_op_paged_attn_shared", attn(**LONG | dict(max_blocks=1 << 22, ld_tables=1 << 22)), "the pages of all requests")
+
+
+@pytest.mark.parametrize("scaling", [dict(rope_theta="x"), dict(partial_rotary_factor="half"), dict(partial_rotary_factor=float("nan")), dict(partial_rotary_factor=float("inf"))])
+def test_scalings_without_numbers_are_refused(scaling):
+    from kubeai_b200 import B200Error, ops
+    with pytest.raises(B200Error, match="cannot be made of"):
+        ops.rotary(64, 1e4, scaling, device="cpu")
