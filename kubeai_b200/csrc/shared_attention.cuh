@@ -14,7 +14,7 @@ using beam::Part;
 typedef __nv_bfloat16 bf16;
 constexpr int kD = 128, kTile16 = 16, kNarrow = 2 * kTile16;
 // kNarrow: rows (token * group + head) of a part that go to narrow CTAs, whose warps have tiles of 16.  64 groups of 32 rows behind up to 450 tokens take 62.9 us there and 82.7 in wide CTAs, 8 behind up to
-// 4000 40.2 and 39.3; of 48 rows, in teams of four warps, 114 us behind 4000 and 42 in wide CTAs, 64 groups behind 450 137 and 113.
+// 4000 40.2 and 39.3; of 48 rows, in teams of four warps, 114 us behind 4000 and 43 in wide CTAs, 64 groups behind 450 137 and 101.
 constexpr int kLd = kD + 4;                // floats from row to row of the workspace: output, maximum, sum
 constexpr int kWaitLimit = 1 << 22;
 

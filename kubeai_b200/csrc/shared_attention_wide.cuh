@@ -14,9 +14,10 @@
 // Only steps that reach behind what every row sees are masked.  There the products' warp also clears what must not meet a weight of zero: values behind the last key, and infinities and NaN
 // among values that some row does not see, which the rows that see them add at the end by themselves.
 // Every wait has a limit; a CTA that gives up sets an error mark and still meets at the end.
-// 2 x 24 questions of up to 32 tokens about 16001, 211 GFLOP: 265 us, 0.80 PFLOP/s, 50 % of what a large product reaches.  A step of two tiles takes 4900 cycles: the exponentials' unit is busy for 42 %,
-// issue slots for 37 %.  What bounds it is a tile's chain (scores, load, maximum, 128 exponentials a thread, weights out, products): without loads it takes 221 us, without the softmax 219.  Half tiles of
-// 64 keys with scores ahead of them 300, sixteen softmax warps 287, another order of the exponentials' instructions the same.
+// 2 x 24 questions of up to 32 tokens about 16001, 211 GFLOP: 265 us (285 under the power cap), 0.80 PFLOP/s, 50 % of what a large product reaches.  A CTA has some 95 steps of two tiles in 391,000 cycles,
+// 4100 a step: tensor cores and the exponentials' unit are busy for 45 %, issue slots for 42 %.  What bounds it is a tile's chain (scores, load, maximum, 128 exponentials a thread, weights out, products):
+// with the sum of the unrounded weights, 255 us, it took 221 without loads and 219 without the softmax; half tiles of 64 keys with scores ahead of them 300, sixteen softmax warps 287, another order of the
+// exponentials' instructions the same.  The sum behind the weights' way out, under the products, is no faster (265).
 #pragma once
 #include "shared_attention.cuh"
 
